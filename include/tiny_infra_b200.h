@@ -349,6 +349,80 @@ int ti_kv_scatter(void* k_cache, void* v_cache, const void* k, int64_t k_tok_str
                   int64_t num_blocks, int num_kv_heads, int head_dim, int block_size, int dtype,
                   void* stream);
 
+/* ---- KV cache in 4 bits --------------------------------------------------------------------
+ * No counterpart in the reference.  The pool of one layer is [num_blocks, num_kv_heads, tile]
+ * bytes, tile = ti_kv4_tile_bytes(head_dim) = 18 * head_dim (head_dim 64 or 128, 0 otherwise),
+ * 16-byte aligned, block_size 16, with the block tables and slots of the 16-bit pool.  A tile
+ * holds K codes [16, D/2], V codes [16, D/2], K scales [D/16, 16], V scales [D/16, 16]: two e2m1
+ * codes per byte (lower dim in the low half), one scale byte b per 16 dims of a token = the
+ * half-precision number with bits b << 7.  value = code * scale, exact in bf16 and fp16; scale =
+ * amax / 6 rounded to 4 significant bits, at most 10240; code = value / scale rounded to nearest
+ * even, saturating.  A group of 16 dims with a NaN or an infinity is held as NaN.  A table entry
+ * that is negative or >= num_blocks holds no tokens.
+ *
+ * ti_kv4_append: k / v element (t, h, d) at t*tok_stride + h*head_stride + d (16-byte aligned
+ * rows) into slot_mapping[t] (< 0: skipped; outside the pool: not written, TI_DEVERR_BAD_INPUT;
+ * distinct).  weights (float32 [num_blocks, num_kv_heads, 16] or NULL): set to 0 for the new tokens. */
+size_t ti_kv4_tile_bytes(int head_dim);
+int ti_kv4_append(void* pool, float* weights, const void* k, int64_t k_tok_stride,
+                  int64_t k_head_stride, const void* v, int64_t v_tok_stride,
+                  int64_t v_head_stride, const int64_t* slot_mapping, int num_tokens,
+                  int64_t num_blocks, int num_kv_heads, int head_dim, int block_size, int dtype,
+                  void* stream);
+
+/* Read the first lens[r] tokens of table row row_index[r] (NULL: r) back as 16-bit values: block j
+ * goes to block out_tables[r][j] of k_out / v_out [out_blocks, num_kv_heads, 16, head_dim] (< 0:
+ * skipped; >= out_blocks: not written, TI_DEVERR_BAD_INPUT), zeros behind the length and where the
+ * source entry holds no block.  block_tables and out_tables have at least max_blocks columns. */
+int ti_kv4_dequantize(void* k_out, void* v_out, int64_t out_blocks, const void* pool,
+                      int64_t num_blocks, const int32_t* block_tables, int64_t bt_stride,
+                      const int32_t* row_index, const int32_t* lens, const int32_t* out_tables,
+                      int64_t ot_stride, int rows, int max_blocks, int num_kv_heads, int head_dim,
+                      int block_size, int dtype, void* stream);
+
+/* Decode attention over the 4-bit pool: out / q [batch, num_heads, head_dim] (row strides in
+ * elements, multiples of 8, 16-byte aligned), at most 16 query heads per kv head, batch <= 4096.
+ * lse (float32 [batch, num_heads] or NULL) = ln of the row's sum of exp(q.k / sqrt(head_dim)).
+ * context_lens 0 leaves the rows of out and lse untouched; a sequence without a block gets NaN and
+ * lse -inf.  The workspace (ti_kv4_attention_workspace_bytes, 16-byte aligned) must be zero before
+ * its first call, and every call leaves its counters zero; calls that share it must not overlap on
+ * the GPU. */
+size_t ti_kv4_attention_workspace_bytes(int batch, int num_heads, int num_kv_heads, int head_dim,
+                                        int max_blocks_per_seq);
+int ti_kv4_attention_decode(void* out, int64_t out_seq_stride, float* lse, const void* q,
+                            int64_t q_seq_stride, const void* pool, int64_t num_blocks,
+                            const int32_t* block_tables, int64_t bt_stride,
+                            const int32_t* row_index, const int32_t* context_lens, int batch,
+                            int num_heads, int num_kv_heads, int head_dim, int block_size,
+                            int max_blocks_per_seq, int dtype, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
+/* weights_out = weights + sum over the kv head's query heads of exp(q.k / sqrt(head_dim) - lse), for
+ * each cached token of the batch (float32 [num_blocks, num_kv_heads, 16]; weights_out may be
+ * weights; other tokens are neither read nor written).  lse as ti_kv4_attention_decode gives it for
+ * the same arguments.  The sequences of a call share no block. */
+int ti_kv4_accumulate_weights(float* weights_out, const float* weights, const void* q,
+                              int64_t q_seq_stride, const float* lse, const void* pool,
+                              int64_t num_blocks, const int32_t* block_tables, int64_t bt_stride,
+                              const int32_t* row_index, const int32_t* context_lens, int batch,
+                              int num_heads, int num_kv_heads, int head_dim, int block_size,
+                              int max_blocks_per_seq, int dtype, void* stream);
+
+/* Eviction, per layer, sequence and kv head (pool [num_layers, num_blocks, num_kv_heads, tile],
+ * weights float32 [num_layers, num_blocks, num_kv_heads, 16]): a sequence of more than `keep`
+ * tokens keeps its last `recent` ones and the keep - recent heaviest older ones (equal weights: the
+ * earlier; NaN: the heaviest), in order, moved with their weights to positions 0 .. keep-1 of the
+ * blocks in out_tables' row (the same table: in place; otherwise blocks holding none of the call's
+ * tokens).  kept (int32 [num_layers, batch, num_kv_heads, kept_stride >= keep] or NULL) receives the
+ * survivors' old positions.  1 <= keep, 0 <= recent <= keep.  A sequence with a needed entry outside
+ * the pool or the tables is left as it is (TI_DEVERR_BAD_INPUT).  Sequences share no block. */
+int ti_kv4_evict(void* pool, float* weights, int num_layers, int64_t num_blocks,
+                 const int32_t* block_tables, int64_t bt_stride, const int32_t* out_tables,
+                 int64_t ot_stride, const int32_t* row_index, const int32_t* context_lens,
+                 int batch, int max_blocks_per_seq, int out_max_blocks, int keep, int recent,
+                 int32_t* kept, int64_t kept_stride, int num_kv_heads, int head_dim,
+                 int block_size, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

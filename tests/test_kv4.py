@@ -1,0 +1,168 @@
+"""The 4-bit KV cache on the CPU: the oracle's format against a search over all its values, the
+prefill plan's layout, and the C ABI's refusals (checked before any CUDA call)."""
+import os
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import kv4 as OK
+
+
+@pytest.fixture(scope="module")
+def native():
+    from tiny_infra_b200 import _native
+    if not os.path.exists(_native.LIB_PATH):
+        from tiny_infra_b200 import build
+        build.build()
+    return _native
+
+
+def test_format_is_exact_in_16_bits():
+    """Every code times every finite scale is a bf16 and an fp16 number."""
+    codes, scales = np.arange(16, dtype=np.uint8), np.arange(0xA8 + 1, dtype=np.uint8)
+    assert OK.scale_values(scales[-1:])[0] >= 8.0
+    sb = np.arange(256, dtype=np.uint8)
+    sb = sb[OK.scale_values(sb) <= 10240.0]
+    v = OK.values(np.tile(codes, len(sb)).reshape(len(sb), 16), sb[:, None])
+    t = torch.from_numpy(v)
+    for dt in (torch.bfloat16, torch.float16):
+        assert torch.equal(t.to(dt).double(), t)
+
+
+def test_quantize_takes_the_nearest_value():
+    """Scale: amax / 6 to 4 significant bits; code: no magnitude is nearer, ties to the even code."""
+    rng = np.random.default_rng(0)
+    x = rng.standard_normal((500, 64)) * np.exp2(rng.integers(-20, 15, (500, 1)))
+    x[7], x[8, :16], x[9, 3] = 0.0, 65504.0, np.nan
+    x = torch.from_numpy(x).to(torch.float16).double().numpy()
+    code, sb = OK.quantize(x)
+    s = OK.scale_values(sb)
+    assert (sb[9, 0] == 0xFF) and not np.isfinite(s[9, 0])
+    ok = np.isfinite(s)
+    a = np.abs(np.where(np.isnan(x), 0, x).reshape(500, 4, 16)).max(-1) / 6
+    lim = np.minimum(a, 10240)
+    assert (np.abs(s - lim) <= np.maximum(lim * 2.0 ** -4, 2.0 ** -18))[ok].all()
+    v = OK.values(code, sb).reshape(500, 4, 16)
+    g = x.reshape(500, 4, 16)
+    dist = np.abs(np.abs(g)[..., None] - OK.MAGNITUDES * s[..., None, None])
+    got = np.abs(np.abs(g) - np.abs(v))
+    live = ok & (s > 0)
+    assert (got[live] == dist[live].min(-1)).all()
+    tie = (dist[live] == dist[live].min(-1, keepdims=True)).sum(-1) > 1
+    assert tie.any() and (code.reshape(500, 4, 16)[live][tie] % 2 == 0).all()
+
+
+def test_survivors_rule():
+    w = np.array([1.0, 5.0, 5.0, np.nan, 0.0, 5.0, 9.0, 2.0], np.float32)
+    np.testing.assert_array_equal(OK.survivors(w, 4, 2), [1, 3, 6, 7])
+    np.testing.assert_array_equal(OK.survivors(w, 5, 2), [1, 2, 3, 6, 7])
+    np.testing.assert_array_equal(OK.survivors(w, 8, 0), np.arange(8))
+    np.testing.assert_array_equal(OK.survivors(w, 3, 3), [5, 6, 7])
+    np.testing.assert_array_equal(OK.survivors(w, 1, 0), [3])
+
+
+def test_prefill_plan_layout():
+    from tiny_infra_b200.kv4 import PrefillPlan
+    p = PrefillPlan([0, 511, 100, 7], [1, 33, 130, 0], device="cpu")
+    assert (p.num_seqs, p.num_tokens, p.num_tiles) == (4, 164, 1 + 3 + 9)
+    assert p.lens.tolist() == [1, 544, 230, 0]
+    assert p.scratch_blocks == 1 + 34 + 15 and p.max_blocks == 34
+    t = p.tables.numpy()
+    used = t[t >= 0]
+    assert sorted(used.tolist()) == list(range(50))
+    assert (t[0] >= 0).sum() == 1 and (t[1] >= 0).sum() == 34 and (t[3] >= 0).sum() == 0
+    tiles = list(zip(p.tile_seq.tolist(), p.tile_q0.tolist()))
+    assert sorted(tiles) == sorted([(0, 0)] + [(1, 16 * i) for i in range(3)] +
+                                   [(2, 16 * i) for i in range(9)])
+    ends = [[0, 511, 100][s] + min(q + 16, [1, 33, 130][s]) for s, q in tiles]
+    assert ends == sorted(ends, reverse=True)
+    assert PrefillPlan([], [], device="cpu").num_tiles == 0
+    for bad in (([0], [1, 2]), ([-1], [3]), ([0], [-3])):
+        with pytest.raises(RuntimeError):
+            PrefillPlan(*bad, device="cpu")
+
+
+def test_module_refuses_host_tensors():
+    from tiny_infra_b200 import kv4
+    z = torch.zeros(4, 2, 18 * 64, dtype=torch.uint8)
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        kv4.append(z, torch.zeros(1, 2, 64).bfloat16(), torch.zeros(1, 2, 64).bfloat16(),
+                   torch.zeros(1, dtype=torch.int64))
+    with pytest.raises(RuntimeError, match="head_dim"):
+        kv4.tile_bytes(96)
+    assert kv4.tile_bytes(64) == 1152 and kv4.tile_bytes(128) == 2304
+
+
+FAKE = 1 << 20          # a 16-byte aligned address that is never dereferenced
+
+
+def test_c_abi_refusals(native):
+    lib = native.lib()
+
+    def refused(rc, code, text):
+        assert rc == code and text in lib.ti_last_error(), (rc, lib.ti_last_error())
+
+    def append(pool=FAKE, k=FAKE, stride=128, n=4, nb=8, kvh=2, d=64, bs=16, dt=0):
+        return lib.ti_kv4_append(pool, None, k, stride, 64, FAKE, 128, 64, FAKE, n, nb, kvh, d, bs,
+                                 dt, None)
+    assert append(n=0) == 0
+    refused(append(pool=None), 1, b"null")
+    refused(append(n=-1), 1, b"negative")
+    refused(append(nb=0), 1, b"empty pool")
+    refused(append(d=96), 2, b"head_dim")
+    refused(append(bs=32), 2, b"block_size")
+    refused(append(dt=2), 2, b"dtype")
+    refused(append(stride=132), 1, b"aligned")
+    refused(append(k=FAKE + 2), 1, b"aligned")
+
+    def deq(out=FAKE, rows=2, mb=3, nb=8, ob=8, d=64, bs=16, dt=0):
+        return lib.ti_kv4_dequantize(out, FAKE, ob, FAKE, nb, FAKE, 3, None, FAKE, FAKE, 3, rows,
+                                     mb, 2, d, bs, dt, None)
+    assert deq(rows=0) == 0
+    refused(deq(out=None), 1, b"null")
+    refused(deq(rows=-1), 1, b"negative")
+    refused(deq(ob=0), 1, b"empty pool")
+    refused(deq(d=80), 2, b"head_dim")
+    refused(deq(dt=2), 2, b"dtype")
+    refused(deq(out=FAKE + 8), 1, b"aligned")
+
+    def att(out=FAKE, q=FAKE, qs=14 * 64, b=2, nh=14, kvh=2, d=64, bs=16, mb=4, nb=8, dt=0):
+        need = lib.ti_kv4_attention_workspace_bytes(max(b, 1), nh, max(kvh, 1), d, max(mb, 1))
+        return lib.ti_kv4_attention_decode(out, 14 * 64, None, q, qs, FAKE, nb, FAKE, 4, None,
+                                           FAKE, b, nh, kvh, d, bs, mb, dt, FAKE, need, None)
+    assert att(b=0) == 0
+    refused(att(out=None), 1, b"null")
+    refused(att(b=-1), 1, b"batch")
+    refused(att(nh=15), 1, b"multiple")
+    refused(att(kvh=0), 1, b"head counts")
+    refused(att(nh=34), 2, b"16 query heads")
+    refused(att(d=32), 2, b"head_dim")
+    refused(att(bs=8), 2, b"block_size")
+    refused(att(dt=2), 2, b"dtype")
+    refused(att(b=5000), 2, b"4096")
+    refused(att(qs=14 * 64 + 4), 1, b"aligned")
+    refused(att(q=FAKE + 4), 1, b"aligned")
+
+    def acc(w=FAKE, b=2, nh=14, d=64, q=FAKE):
+        return lib.ti_kv4_accumulate_weights(FAKE, w, q, 14 * 64, FAKE, FAKE, 8, FAKE, 4, None,
+                                             FAKE, b, nh, 2, d, 16, 4, 0, None)
+    assert acc(b=0) == 0
+    refused(acc(w=None), 1, b"null")
+    refused(acc(nh=13), 1, b"multiple")
+    refused(acc(d=256), 2, b"head_dim")
+    refused(acc(q=FAKE + 4), 1, b"aligned")
+
+    def ev(pool=FAKE, layers=1, b=2, keep=4, recent=2, kept=None, ks=0, d=64, bs=16):
+        return lib.ti_kv4_evict(pool, FAKE, layers, 8, FAKE, 4, FAKE, 4, None, FAKE, b, 4, 4, keep,
+                                recent, kept, ks, 2, d, bs, None)
+    assert ev(b=0) == 0 and ev(layers=0) == 0
+    refused(ev(pool=None), 1, b"null")
+    refused(ev(keep=0, recent=0), 1, b"keep")
+    refused(ev(recent=5), 1, b"recent")
+    refused(ev(recent=-1), 1, b"recent")
+    refused(ev(kept=FAKE, ks=3), 1, b"kept")
+    refused(ev(d=32), 2, b"head_dim")
+    refused(ev(bs=32), 2, b"block_size")
+    refused(ev(pool=FAKE + 8), 1, b"aligned")
+    refused(ev(layers=70000), 2, b"65535")

@@ -57,6 +57,17 @@ SIGNATURES: dict[str, tuple] = {
     "ti_paged_attention_decode_planned_ex": (I32, [P, I64, P, I64, P, P, I64, P, I64, P, P, I32,
                                                    I32, I32, I32, I32, I32, I32, P, SZ, P, I32,
                                                    P]),
+    "ti_kv4_tile_bytes": (SZ, [I32]),
+    "ti_kv4_append": (I32, [P, P, P, I64, I64, P, I64, I64, P, I32, I64, I32, I32, I32, I32, P]),
+    "ti_kv4_dequantize": (I32, [P, P, I64, P, I64, P, I64, P, P, P, I64, I32, I32, I32, I32, I32,
+                                I32, P]),
+    "ti_kv4_attention_workspace_bytes": (SZ, [I32, I32, I32, I32, I32]),
+    "ti_kv4_attention_decode": (I32, [P, I64, P, P, I64, P, I64, P, I64, P, P, I32, I32, I32, I32,
+                                      I32, I32, I32, P, SZ, P]),
+    "ti_kv4_accumulate_weights": (I32, [P, P, P, I64, P, P, I64, P, I64, P, P, I32, I32, I32, I32,
+                                        I32, I32, I32, P]),
+    "ti_kv4_evict": (I32, [P, P, I32, I64, P, I64, P, I64, P, P, I32, I32, I32, I32, I32, P, I64,
+                           I32, I32, I32, P]),
 }
 
 TI_EPI_STORE, TI_EPI_SWIGLU, TI_EPI_RESIDUAL, TI_EPI_ARGMAX = 0, 1, 2, 3
