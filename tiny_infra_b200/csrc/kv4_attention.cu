@@ -1,6 +1,7 @@
 // Decode attention over the 4-bit paged KV cache, and the attention-weight totals that eviction
 // ranks tokens by.  Format: kv4.cuh.
 #include <algorithm>
+#include <atomic>
 
 #include "capi_internal.h"
 #include "common.cuh"
@@ -9,6 +10,33 @@
 namespace ti {
 namespace kv4 {
 
+// ---- decode attention ------------------------------------------------------------------------------
+// out = softmax(q K^T / sqrt(D)) V for one query token of each sequence, from the codes: per
+// (block, kv head) tile 18 * D bytes are read once for all query heads of the kv head, so the floor is
+// those bytes at HBM speed, 23 bytes per clock and SM.
+//
+// Work split.  A unit is (sequence, kv head, group of at most 8 query heads); all units' tiles form
+// one stream (units in order, a unit's tiles in order) that is cut evenly over the CTAs and, inside a
+// CTA, over its 16 warps, so ragged lengths balance.  A warp keeps the running max and sum of its
+// current unit in registers; units cut by a warp boundary are joined in shared memory by the CTA,
+// those cut by a CTA boundary through the workspace by the CTA that arrives last (pieces in order:
+// the same bits on every run).  One launch.
+//
+// A warp's step is 64 tokens (D = 64; 32 for D = 128): its 4608 bytes come through a private ring of
+// two stages by 16-byte asynchronous copies, 9 per lane, issued a step ahead.
+//
+// Mathematics of a step, tokens as the matrix instruction's M dimension, heads as N:
+//   S^T = K q^T   A = K: lane (g, t) holds tokens g and g+8 and one or two whole scale groups of
+//                 each (dims D/4 * t ...), so it needs one scale per 16 dims; the order of the dims
+//                 in the sum is free, q is laid out to match.
+//   O^T += V^T P^T  A = V^T: lane (g, t) holds dims D/8 * g ... of tokens 2t, 2t+1, 2t+8, 2t+9; the
+//                 codes of two tokens are interleaved as half-bytes, so one conversion gives the
+//                 pair; P^T comes from S^T by an 8x8 transpose between lanes.
+// Codes become half precision by the hardware conversion and are multiplied by their scale: exact, so
+// both types run on half-precision operands.  bf16 queries are scaled by a power of two that brings
+// the row's largest magnitude to 2^14 (elements below 2^-28 of it lose bits: 2^-39 of the largest);
+// the scores' factor takes it back.  Weights are held as 2^14 p in half precision: 2^-11 relative
+// (the 16-bit outputs round by as much) down to p = 2^-28; their sum is taken before that rounding.
 struct DecodeParams {
   void* out;
   float* lse;                        // [batch, NH] or null
@@ -17,8 +45,627 @@ struct DecodeParams {
   int64_t out_stride, q_stride, num_blocks, bt_stride;
   const int32_t *tables, *row_index, *ctx;
   int batch, NH, KVH, group, max_blocks;
-  float scale;
+  int subs;                          // groups of at most 8 query heads per kv head
+  int unit_mode;                     // one CTA per unit instead of the even cut
+  float scale_log2;
+  uint32_t* counters;                // [gridDim.x], zero between calls
+  float* parts;                      // [gridDim.x][2] pieces
 };
+
+constexpr int kMaxBatch = 4096;
+constexpr int kWarps = 16;
+constexpr int kStages = 2;
+constexpr int kStepBytes = 4608;                 // 64 (D = 64) or 32 tokens of one kv head
+constexpr float kPScale = 14.f;                  // weights are held as 2^14 p
+
+template <int HD>
+struct Shape {
+  static constexpr int kTiles = kStepBytes / Tile<HD>::kBytes;   // tiles of a step
+  static constexpr int kLanes = 32 / kTiles;                     // lanes that copy one tile
+  static constexpr int kPiece = 8 * HD + 16;                     // floats: O, m[8], l[8]
+  static constexpr int kRing = kWarps * kStages * kStepBytes;
+  static constexpr int kPark = kWarps * kPiece * 4;
+  static size_t smem(int batch) { return kRing + kPark + ((size_t)batch + 1) * 4; }
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ void lds64(uint32_t a, uint32_t& x, uint32_t& y) {
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(x), "=r"(y) : "r"(a));
+}
+__device__ __forceinline__ void lds128(uint32_t a, uint32_t (&v)[4]) {
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+               : "r"(a));
+}
+__device__ __forceinline__ uint32_t lds8(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds16(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+
+// Where a warp stands in the stream of tiles.
+struct Cursor {
+  int b, hv, blk, n;                 // sequence, unit within it, tile of the unit, tiles of a unit
+  int64_t left;                      // tiles left in the warp's range
+  __device__ __forceinline__ int step(int most) const {
+    return (int)min((int64_t)min(most, n - blk), left);
+  }
+  // Past k tiles; pref[b] = tiles of one unit of the sequences before b.
+  __device__ __forceinline__ void advance(int k, int units, const uint32_t* pref, int batch) {
+    blk += k;
+    left -= k;
+    if (blk < n || left == 0) return;
+    blk = 0;
+    if (++hv < units) return;
+    hv = 0;
+    do ++b; while (b < batch && pref[b + 1] == pref[b]);
+    if (b < batch) n = (int)(pref[b + 1] - pref[b]);
+  }
+};
+
+// Query rows of a unit as the B operand: q[s][0..1] hold dims D/4 * t + 4 s + {0,1,2,3} of head g.
+// Returns the factor that the rows of heads 2t and 2t+1 were multiplied by, inverted.
+template <typename T, int HD>
+__device__ __forceinline__ float2 load_query(const T* q, int heads, int g, int t,
+                                             uint32_t (&f)[HD / 16][2]) {
+  constexpr int N = HD / 4;                      // dims of a lane
+  uint32_t raw[N / 2];
+#pragma unroll
+  for (int i = 0; i < N / 8; ++i) {
+    uint4 u = make_uint4(0u, 0u, 0u, 0u);
+    if (g < heads) u = *reinterpret_cast<const uint4*>(q + (int64_t)g * HD + t * N + i * 8);
+    raw[4 * i] = u.x;
+    raw[4 * i + 1] = u.y;
+    raw[4 * i + 2] = u.z;
+    raw[4 * i + 3] = u.w;
+  }
+  float inv = 1.f;
+  if constexpr (std::is_same<T, __half>::value) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) f[i / 2][i % 2] = raw[i];
+  } else {
+    uint32_t top = 0;                            // largest magnitude's bits (as bf16)
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) top = max(top, max(raw[i] & 0x7FFFu, (raw[i] >> 16) & 0x7FFFu));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    // exponent field of the largest, between what keeps both factors normal numbers
+    const int e = min(max((int)(top >> 7), 15), 254);
+    const float mul = __uint_as_float((uint32_t)(254 + 14 - e) << 23);   // 2^(14 - (e - 127))
+    inv = __uint_as_float((uint32_t)(e - 14) << 23);
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      const float2 v = Elem<T>::unpack2(raw[i]);
+      f[i / 2][i % 2] = Elem<__half>::pack2(v.x * mul, v.y * mul);
+    }
+  }
+  return make_float2(__shfl_sync(0xffffffffu, inv, 8 * t), __shfl_sync(0xffffffffu, inv, 8 * t + 4));
+}
+
+// The scores of one tile's 16 tokens: c[0], c[1] = token g, heads 2t, 2t+1; c[2], c[3] = token g+8.
+template <int HD>
+__device__ __forceinline__ void tile_scores(uint32_t codes, uint32_t scales, int g, int t,
+                                            const uint32_t (&q)[HD / 16][2], float (&c)[4]) {
+  constexpr int W = HD / 32;                     // words of a lane's dims
+  uint32_t w[2][W];
+  uint32_t sc[2][HD / 64];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const uint32_t a = codes + (g + 8 * r) * (HD / 2) + t * (HD / 8);
+    if constexpr (HD == 64) lds64(a, w[r][0], w[r][1]);
+    else lds128(a, w[r]);
+#pragma unroll
+    for (int u = 0; u < HD / 64; ++u)
+      sc[r][u] = lds8(scales + (t * (HD / 64) + u) * kBlock + g + 8 * r) * 0x00800080u;
+  }
+  c[0] = c[1] = c[2] = c[3] = 0.f;
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
+    uint32_t a[2][4];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      codes_to_half2(w[r][i], a[r]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) a[r][j] = hmul2(a[r][j], sc[r][i / 2]);
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint32_t frag[4] = {a[0][2 * j], a[1][2 * j], a[0][2 * j + 1], a[1][2 * j + 1]};
+      Mma<__half>::run(c, frag, q[2 * i + j][0], q[2 * i + j][1]);
+    }
+  }
+}
+
+// Row of a V code row in shared memory: tokens 0, 2, 4, 6 (and 1, 3, 5, 7) in rows that differ modulo
+// 4, so the lanes of one load cover all banks.
+__device__ __forceinline__ int v_row(int tok) {
+  return (tok & 8) | ((tok & 1) << 2) | ((tok >> 1) & 3);
+}
+
+// O^T += V^T P^T for one tile: o[m][0..1] = dim D/8 * g + 2m, heads 2t, 2t+1; o[m][2..3] = the dim
+// after it.  `live`: tokens of the tile that exist (the others' scales count as zero).
+template <int HD>
+__device__ __forceinline__ void tile_values(uint32_t codes, uint32_t scales, int g, int t, int live,
+                                            const uint32_t (&p)[2], float (&o)[HD / 16][4]) {
+  constexpr int W = HD / 64;                     // words of a lane's dims, per token
+#pragma unroll
+  for (int r = 0; r < 1; ++r) {
+    uint32_t w[4][W], sc[2];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int tok = 2 * t + (k & 1) + 8 * (k >> 1), row = v_row(tok);
+      if constexpr (HD == 64) {
+        w[k][0] = lds32(codes + row * 32 + g * 4);
+      } else {
+        // 64-byte rows: the halves of rows 2 and 3 (modulo 4) change places, see copy_tile
+        lds64(codes + row * 64 + ((g * 8) ^ ((row & 2) << 4)), w[k][0], w[k][1]);
+      }
+    }
+    const int grp = HD == 64 ? g >> 1 : g;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      uint32_t b2 = lds16(scales + grp * kBlock + 2 * t + 8 * k);
+      const int n = live - (2 * t + 8 * k);
+      if (n < 2) b2 = n == 1 ? (b2 & 0xFFu) : 0u;
+      sc[k] = __byte_perm(b2, 0, 0x1404) >> 1;   // bytes to the halves' tops, then << 7 in all
+    }
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      uint32_t ev[2][4], od[2][4];               // dims 2m and 2m+1, token pairs
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint32_t x = w[2 * k][i], y = w[2 * k + 1][i];
+        codes_to_half2((x & 0x0F0F0F0Fu) | ((y << 4) & 0xF0F0F0F0u), ev[k]);
+        codes_to_half2(((x >> 4) & 0x0F0F0F0Fu) | (y & 0xF0F0F0F0u), od[k]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          ev[k][j] = hmul2(ev[k][j], sc[k]);
+          od[k][j] = hmul2(od[k][j], sc[k]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t frag[4] = {ev[0][j], od[0][j], ev[1][j], od[1][j]};
+        Mma<__half>::run(o[4 * i + j], frag, p[0], p[1]);
+      }
+    }
+  }
+}
+
+// This lane's 9 copies of a step: the lanes of one tile take neighbouring 16-byte chunks, the V
+// code rows land permuted (v_row, and for 64-byte rows with the halves of rows 2 and 3 exchanged).
+template <int HD>
+__device__ __forceinline__ void copy_tile(uint32_t dst, const uint8_t* src, int l) {
+  using S = Shape<HD>;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) cp_async16(dst + (l + S::kLanes * i) * 16, src + (l + S::kLanes * i) * 16);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int c = l + S::kLanes * i;             // chunk of the V codes
+    constexpr int kPer = HD / 32;                // chunks of a row
+    const int row = v_row(c / kPer);
+    const int x = HD == 64 ? c % kPer : (c % kPer) ^ (row & 2);
+    cp_async16(dst + Tile<HD>::kV + (row * kPer + x) * 16, src + Tile<HD>::kV + c * 16);
+  }
+  cp_async16(dst + Tile<HD>::kKs + l * 16, src + Tile<HD>::kKs + l * 16);
+}
+
+// Write a unit's finished rows: heads 2t and 2t+1, this lane's D/8 dims.
+template <typename T, int HD>
+__device__ __forceinline__ void store_rows(const DecodeParams& p, int b, int h0, int heads, int g,
+                                           int t, const float (&o)[HD / 16][4], const float (&m)[2],
+                                           const float (&l)[2]) {
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int h = 2 * t + x;
+    if (h >= heads) continue;
+    const float r = 1.f / l[x];
+    T* out = (T*)p.out + b * p.out_stride + (int64_t)(h0 + h) * HD + g * (HD / 8);
+#pragma unroll
+    for (int i = 0; i < HD / 64; ++i) {
+      uint4 u;
+      u.x = Elem<T>::pack2(o[4 * i][x] * r, o[4 * i][2 + x] * r);
+      u.y = Elem<T>::pack2(o[4 * i + 1][x] * r, o[4 * i + 1][2 + x] * r);
+      u.z = Elem<T>::pack2(o[4 * i + 2][x] * r, o[4 * i + 2][2 + x] * r);
+      u.w = Elem<T>::pack2(o[4 * i + 3][x] * r, o[4 * i + 3][2 + x] * r);
+      *reinterpret_cast<uint4*>(out + i * 8) = u;
+    }
+    if (p.lse && g == 0)
+      p.lse[(int64_t)b * p.NH + h0 + h] = (m[x] == -INFINITY ? 0.f : m[x] - kPScale) * 0.6931471805599453f + logf(l[x]);
+  }
+}
+
+// A piece of a unit: O [8][HD], m[8], l[8] (m in the exponent's units, l and O times 2^14).
+template <int HD>
+__device__ __forceinline__ void store_piece(float* dst, int g, int t, const float (&o)[HD / 16][4],
+                                            const float (&m)[2], const float (&l)[2]) {
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    float* row = dst + (2 * t + x) * HD + g * (HD / 8);
+#pragma unroll
+    for (int i = 0; i < HD / 32; ++i)
+      *reinterpret_cast<float4*>(row + 4 * i) =
+          make_float4(o[2 * i][x], o[2 * i][2 + x], o[2 * i + 1][x], o[2 * i + 1][2 + x]);
+    if (g == 0) {
+      dst[8 * HD + 2 * t + x] = m[x];
+      dst[8 * HD + 8 + 2 * t + x] = l[x];
+    }
+  }
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(DecodeParams p) {
+  using S = Shape<HD>;
+  using L = Tile<HD>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  float* park = reinterpret_cast<float*>(smem + S::kRing);
+  uint32_t* pref = reinterpret_cast<uint32_t*>(smem + S::kRing + S::kPark);   // [batch + 1]
+  __shared__ uint32_t s_scan[kWarps + 1];
+  __shared__ int s_last[2], s_start[kWarps + 1];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int units = p.KVH * p.subs;
+  pdl_wait();
+  pdl_launch_dependents();
+
+  // pref[b] = tiles of one unit of the sequences before b (in unit mode: only this CTA's sequence)
+  const int64_t cap = (int64_t)p.max_blocks * kBlock;
+  auto tiles_of = [&](int b) {
+    const int64_t n = min((int64_t)p.ctx[b], cap);
+    return n > 0 ? (uint32_t)((n - 1) / kBlock + 1) : 0u;
+  };
+  int64_t total;
+  int ctas;
+  if (p.unit_mode) {
+    ctas = 1;
+    total = tiles_of(blockIdx.x / units);
+  } else {
+    uint32_t carry = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += kWarps * 32) {
+      const int b = b0 + tid;
+      const uint32_t n = b < p.batch ? tiles_of(b) : 0u;
+      uint32_t x = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      if (lane == 31) s_scan[warp] = x;
+      __syncthreads();
+      uint32_t before = carry, all = 0;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) before += s_scan[w];
+        all += s_scan[w];
+      }
+      if (b < p.batch) pref[b + 1] = before + x;
+      carry += all;
+      __syncthreads();
+    }
+    if (tid == 0) pref[0] = 0;
+    __syncthreads();
+    total = (int64_t)carry * units;
+    // at least two tiles per warp: fewer CTAs for little work, and fewer units cut
+    ctas = (int)min((int64_t)gridDim.x, (total + 2 * kWarps - 1) / (2 * kWarps));
+  }
+  const int cta = p.unit_mode ? 0 : blockIdx.x;
+  if (total == 0 || cta >= ctas) return;
+  const int64_t nw = (int64_t)ctas * kWarps;
+  auto start_of = [&](int64_t w) { return w * total / nw; };     // first tile of warp w (of all CTAs)
+  const int64_t w_begin = start_of((int64_t)cta * kWarps + warp);
+  const int64_t w_end = start_of((int64_t)cta * kWarps + warp + 1);
+
+  Cursor cur;
+  cur.left = w_end - w_begin;
+  if (p.unit_mode) {
+    cur.b = blockIdx.x / units;
+    cur.hv = blockIdx.x % units;
+    cur.n = (int)total;
+    cur.blk = (int)w_begin;
+  } else {
+    int lo = 0, hi = p.batch;                      // last b with pref[b] * units <= w_begin
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if ((int64_t)pref[mid] * units <= w_begin) lo = mid; else hi = mid;
+    }
+    cur.b = lo;
+    cur.n = (int)(pref[lo + 1] - pref[lo]);
+    const int64_t r = w_begin - (int64_t)pref[lo] * units;
+    cur.hv = cur.n ? (int)(r / cur.n) : 0;
+    cur.blk = cur.n ? (int)(r % cur.n) : 0;
+  }
+
+  float o[HD / 16][4], m[2], l[2];
+  bool tail = false;                               // a piece is left in registers after the loop
+  const bool head_cut = cur.blk > 0;               // the first unit began before this warp
+  if (cur.left > 0) {
+    const uint32_t ring = smem_u32(smem) + warp * (kStages * kStepBytes);
+    const int j = lane / S::kLanes, cl = lane % S::kLanes;
+    Cursor ld = cur;
+    uint32_t have = 0;                             // S::kTiles bits per step in flight: blocks that exist
+    int issued = 0;
+    auto next_id = [&]() -> int {
+      if (j >= ld.step(S::kTiles)) return -1;
+      const int row = p.row_index ? p.row_index[ld.b] : ld.b;
+      return p.tables[(int64_t)row * p.bt_stride + ld.blk + j];
+    };
+    int id = next_id();
+    auto issue = [&]() {
+      const bool ok = id >= 0 && id < p.num_blocks;
+      if (ok) {
+        const int kvh = p.subs == 1 ? ld.hv : ld.hv / p.subs;
+        copy_tile<HD>(ring + (issued % kStages) * kStepBytes + j * L::kBytes,
+                      p.pool + ((int64_t)id * p.KVH + kvh) * L::kBytes, cl);
+      }
+      cp_commit();
+      const uint32_t bal = __ballot_sync(0xffffffffu, ok && cl == 0);
+      uint32_t bits = 0;
+#pragma unroll
+      for (int k = 0; k < S::kTiles; ++k) bits |= ((bal >> (k * S::kLanes)) & 1u) << k;
+      have |= bits << ((issued % kStages) * S::kTiles);
+      ++issued;
+      if (ld.left > 0) {
+        ld.advance(ld.step(S::kTiles), units, pref, p.batch);
+        id = ld.left > 0 ? next_id() : -1;
+      }
+    };
+    uint32_t qf[HD / 16][2];
+    float2 sc = make_float2(0.f, 0.f);
+    int ctx = 0, heads = 0, h0 = 0;
+    auto open_unit = [&]() {
+      const int kvh = cur.hv / p.subs, sub = cur.hv % p.subs;
+      h0 = kvh * p.group + sub * 8;
+      heads = min(8, p.group - sub * 8);
+      ctx = (int)min((int64_t)p.ctx[cur.b], cap);
+      const float2 inv = load_query<T, HD>((const T*)p.q + cur.b * p.q_stride + (int64_t)h0 * HD, heads, g, t, qf);
+      sc = make_float2(inv.x * p.scale_log2, inv.y * p.scale_log2);
+#pragma unroll
+      for (int i = 0; i < HD / 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+      m[0] = m[1] = -INFINITY;
+      l[0] = l[1] = 0.f;
+    };
+    issue();
+    open_unit();
+    bool first = true;
+    for (int it = 0;; ++it) {
+      issue();                                     // (an empty group when nothing is left)
+      cp_wait<kStages - 1>();
+      __syncwarp();
+      const int k = cur.step(S::kTiles);
+      const uint32_t st = ring + (it % kStages) * kStepBytes;
+      const uint32_t ok = (have >> ((it % kStages) * S::kTiles)) & ((1u << S::kTiles) - 1u);
+      have &= ~(((1u << S::kTiles) - 1u) << ((it % kStages) * S::kTiles));
+      const int live = ctx - cur.blk * kBlock;     // tokens from this step's first on
+      float s[S::kTiles][4];
+      float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+      for (int x = 0; x < S::kTiles; ++x) {
+        if ((ok >> x) & 1u) {
+          tile_scores<HD>(st + x * L::kBytes + L::kK, st + x * L::kBytes + L::kKs, g, t, qf, s[x]);
+          const int n = live - x * kBlock;
+          if (n < kBlock) {
+            if (g >= n) s[x][0] = s[x][1] = -INFINITY;
+            if (g + 8 >= n) s[x][2] = s[x][3] = -INFINITY;
+          }
+        } else {
+          s[x][0] = s[x][1] = s[x][2] = s[x][3] = -INFINITY;
+        }
+        mx0 = fmaxf(mx0, fmaxf(s[x][0], s[x][2]));
+        mx1 = fmaxf(mx1, fmaxf(s[x][1], s[x][3]));
+      }
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) {
+        mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, d));
+        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, d));
+      }
+      const float n0 = fmaxf(m[0], mx0 * sc.x), n1 = fmaxf(m[1], mx1 * sc.y);
+      if (__any_sync(0xffffffffu, n0 != m[0] || n1 != m[1])) {
+        // (a row that had no token yet: its sums are zero, and stay so)
+        const float a0 = m[0] == -INFINITY ? 0.f : fast_exp2(m[0] - n0);
+        const float a1 = m[1] == -INFINITY ? 0.f : fast_exp2(m[1] - n1);
+        l[0] *= a0;
+        l[1] *= a1;
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i) {
+          o[i][0] *= a0;
+          o[i][1] *= a1;
+          o[i][2] *= a0;
+          o[i][3] *= a1;
+        }
+        m[0] = n0;
+        m[1] = n1;
+      }
+      const float f0 = kPScale - (n0 == -INFINITY ? 0.f : n0), f1 = kPScale - (n1 == -INFINITY ? 0.f : n1);
+#pragma unroll
+      for (int x = 0; x < S::kTiles; ++x) {
+        if (!((ok >> x) & 1u)) continue;
+        const float e0 = fast_exp2(fmaf(s[x][0], sc.x, f0)), e1 = fast_exp2(fmaf(s[x][1], sc.y, f1));
+        const float e2 = fast_exp2(fmaf(s[x][2], sc.x, f0)), e3 = fast_exp2(fmaf(s[x][3], sc.y, f1));
+        l[0] += e0 + e2;
+        l[1] += e1 + e3;
+        const uint32_t pt[2] = {transpose8x8(Elem<__half>::pack2(e0, e1)),
+                                transpose8x8(Elem<__half>::pack2(e2, e3))};
+        tile_values<HD>(st + x * L::kBytes + L::kV, st + x * L::kBytes + L::kVs, g, t,
+                        live - x * kBlock, pt, o);
+      }
+      __syncwarp();                                // the stage is free for the copies after next
+      const int ub = cur.b;
+      const bool done = cur.blk + k == cur.n;      // the unit's last tile
+      cur.advance(k, units, pref, p.batch);
+      if (done || cur.left == 0) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) {
+          l[0] += __shfl_xor_sync(0xffffffffu, l[0], d);
+          l[1] += __shfl_xor_sync(0xffffffffu, l[1], d);
+        }
+        const bool cut = first && head_cut;
+        if (done && !cut) {
+          store_rows<T, HD>(p, ub, h0, heads, g, t, o, m, l);
+        } else if (cut) {
+          store_piece<HD>(park + warp * S::kPiece, g, t, o, m, l);
+        } else {
+          tail = true;
+        }
+        first = false;
+        if (cur.left == 0) break;
+        open_unit();
+      }
+    }
+    cp_wait<0>();
+  }
+  // first tile of every warp, counted from the CTA's
+  const int64_t c_begin = start_of((int64_t)cta * kWarps);
+  if (lane == 0) {
+    s_start[warp] = (int)(w_begin - c_begin);
+    if (warp == kWarps - 1) s_start[kWarps] = (int)(w_end - c_begin);
+  }
+  __syncthreads();
+  // the rings are free: pieces that are still in registers go there
+  float* tails = reinterpret_cast<float*>(smem);
+  if (tail) store_piece<HD>(tails + warp * S::kPiece, g, t, o, m, l);
+  __syncthreads();
+
+  // join the cut units of this CTA; piece of unit [s, e) in warp w: parked when the unit began before
+  // the warp's range, else left in the ring
+  const int64_t c_end = c_begin + s_start[kWarps];
+  auto cta_of = [&](int64_t pos) {                 // the CTA whose range holds tile pos
+    return (int)((((pos + 1) * nw - 1) / total) / kWarps);
+  };
+  auto unit_at = [&](int64_t pos, int& b, int& hv, int64_t& s, int64_t& e) {
+    if (p.unit_mode) {
+      b = blockIdx.x / units;
+      hv = blockIdx.x % units;
+      s = 0;
+      e = total;
+      return;
+    }
+    int lo = 0, hi = p.batch;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if ((int64_t)pref[mid] * units <= pos) lo = mid; else hi = mid;
+    }
+    b = lo;
+    const int64_t n = pref[lo + 1] - pref[lo], base = (int64_t)pref[lo] * units;
+    hv = (int)((pos - base) / n);
+    s = base + hv * n;
+    e = s + n;
+  };
+  auto weight = [](float mi, float mm) { return mi == -INFINITY ? 0.f : fast_exp2(mi - mm); };
+  int n_cross = 0;
+  int64_t cross_s[2], cross_e[2];
+  int cross_b[2], cross_hv[2];
+  for (int64_t pos = c_begin; pos < c_end;) {
+    int b, hv;
+    int64_t s, e;
+    unit_at(pos, b, hv, s, e);
+    pos = e;
+    const bool inside = s >= c_begin && e <= c_end;
+    const int s0 = (int)(max(s, c_begin - 1) - c_begin), e0 = (int)(min(e, c_end) - c_begin);
+    int wa = 0, wb = kWarps - 1;                   // its first and last warp here
+    while (s_start[wa + 1] <= s0) ++wa;
+    while (s_start[wb] >= e0) --wb;
+    if (inside && wa == wb) continue;              // written by its warp
+    const int sub = hv % p.subs, h0 = (hv / p.subs) * p.group + sub * 8;
+    const int heads = min(8, p.group - sub * 8);
+    float* ws = inside ? nullptr : p.parts + ((int64_t)cta * 2 + (s < c_begin ? 0 : 1)) * S::kPiece;
+    for (int i = tid; i < 8 * HD; i += kWarps * 32) {
+      const int h = i / HD;
+      if (h >= heads) break;
+      float mm = -INFINITY, ll = 0.f, oo = 0.f;
+      auto piece = [&](int w) { return (s0 < s_start[w] ? park : tails) + w * S::kPiece; };
+      for (int w = wa; w <= wb; ++w)
+        if (s_start[w] < s_start[w + 1]) mm = fmaxf(mm, piece(w)[8 * HD + h]);
+      for (int w = wa; w <= wb; ++w) {
+        if (s_start[w] == s_start[w + 1]) continue;               // an empty range
+        const float* src = piece(w);
+        const float c = weight(src[8 * HD + h], mm);
+        // (a NaN sum has to stay one whatever its max)
+        ll += src[8 * HD + h] == -INFINITY ? src[8 * HD + 8 + h] : c * src[8 * HD + 8 + h];
+        oo += src[8 * HD + h] == -INFINITY ? src[i] : c * src[i];
+      }
+      if (inside) {
+        ((T*)p.out)[b * p.out_stride + (int64_t)(h0 + h) * HD + i % HD] = Elem<T>::from_f(oo / ll);
+        if (p.lse && i % HD == 0)
+          p.lse[(int64_t)b * p.NH + h0 + h] = (mm == -INFINITY ? 0.f : mm - kPScale) * 0.6931471805599453f + logf(ll);
+      } else {
+        ws[i] = oo;
+        if (i % HD == 0) {
+          ws[8 * HD + h] = mm;
+          ws[8 * HD + 8 + h] = ll;
+        }
+      }
+    }
+    if (!inside) {
+      cross_s[n_cross] = s;
+      cross_e[n_cross] = e;
+      cross_b[n_cross] = b;
+      cross_hv[n_cross++] = hv;
+    }
+  }
+  if (n_cross == 0) return;
+  __threadfence();
+  __syncthreads();
+  if (tid < n_cross) {
+    const int64_t s = tid ? cross_s[1] : cross_s[0], e = tid ? cross_e[1] : cross_e[0];
+    const int fst = cta_of(s), lst = cta_of(e - 1);
+    const uint32_t old = atomicAdd(p.counters + fst, 1u);
+    s_last[tid] = old == (uint32_t)(lst - fst);
+    if (s_last[tid]) p.counters[fst] = 0;          // zero again for the next call
+    __threadfence();
+  }
+  __syncthreads();
+  for (int x = 0; x < n_cross; ++x) {
+    if (!s_last[x]) continue;
+    const int64_t s = cross_s[x], e = cross_e[x];
+    const int fst = cta_of(s), lst = cta_of(e - 1);
+    const int sub = cross_hv[x] % p.subs, h0 = (cross_hv[x] / p.subs) * p.group + sub * 8;
+    const int heads = min(8, p.group - sub * 8), b = cross_b[x];
+    for (int i = tid; i < 8 * HD; i += kWarps * 32) {
+      const int h = i / HD;
+      if (h >= heads) break;
+      float mm = -INFINITY, ll = 0.f, oo = 0.f;
+      auto part = [&](int c) { return p.parts + ((int64_t)c * 2 + (c == fst ? 1 : 0)) * S::kPiece; };
+#pragma unroll 4
+      for (int c = fst; c <= lst; ++c) mm = fmaxf(mm, __ldcg(part(c) + 8 * HD + h));
+#pragma unroll 4
+      for (int c = fst; c <= lst; ++c) {
+        const float mi = __ldcg(part(c) + 8 * HD + h);
+        const float f = mi == -INFINITY ? 1.f : fast_exp2(mi - mm);
+        ll += f * __ldcg(part(c) + 8 * HD + 8 + h);
+        oo += f * __ldcg(part(c) + i);
+      }
+      ((T*)p.out)[b * p.out_stride + (int64_t)(h0 + h) * HD + i % HD] = Elem<T>::from_f(oo / ll);
+      if (p.lse && i % HD == 0)
+        p.lse[(int64_t)b * p.NH + h0 + h] = (mm == -INFINITY ? 0.f : mm - kPScale) * 0.6931471805599453f + logf(ll);
+    }
+  }
+}
 
 // The HD/32 dims lane `lane` holds of one token's codes (a 32-bit word serves 256 / HD lanes).
 template <int HD>
@@ -34,64 +681,6 @@ __device__ __forceinline__ void lane_values(const uint8_t* row, int lane, float 
     f[2 * u] = v.x * s;
     f[2 * u + 1] = v.y * s;
   }
-}
-
-// One CTA per (sequence, query head); warps take every 4th token, lanes HD/32 dims each.
-template <typename T, int HD>
-__global__ void __launch_bounds__(128) decode_kernel(DecodeParams p) {
-  pdl_wait();
-  pdl_launch_dependents();
-  using L = Tile<HD>;
-  constexpr int PL = HD / 64;                      // bytes (dim pairs) of a lane
-  const int h = blockIdx.x, b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n = p.ctx[b];
-  if (n <= 0) return;
-  const int32_t* table = p.tables + (int64_t)(p.row_index ? p.row_index[b] : b) * p.bt_stride;
-  const int kvh = h / p.group;
-  const T* q = (const T*)p.q + b * p.q_stride + (int64_t)h * HD;
-  float qf[2 * PL], o[2 * PL];
-  for (int u = 0; u < 2 * PL; ++u) {
-    qf[u] = Elem<T>::to_f(q[lane * 2 * PL + u]) * p.scale;
-    o[u] = 0.f;
-  }
-  float m = -INFINITY;
-  double l = 0.;                   // a long flat tail is many small terms beside a large one
-  const int n_max = min((int64_t)n, (int64_t)p.max_blocks * kBlock);
-  for (int i = warp; i < n_max; i += 4) {
-    const int32_t blk = table[i / kBlock];
-    if (blk < 0 || blk >= p.num_blocks) continue;
-    const uint8_t* tile = p.pool + ((int64_t)blk * p.KVH + kvh) * L::kBytes;
-    const int off = i % kBlock, g = lane * 2 * PL / kGroup;
-    const float ks = scale_value(tile[L::kKs + g * kBlock + off]);
-    const float vs = scale_value(tile[L::kVs + g * kBlock + off]);
-    float s = 0.f, k[2 * PL], v[2 * PL];
-    lane_values<HD>(tile + L::kK + off * L::kRow, lane, ks, k);
-    lane_values<HD>(tile + L::kV + off * L::kRow, lane, vs, v);
-    for (int u = 0; u < 2 * PL; ++u) s += qf[u] * k[u];
-    s = warp_sum(s);
-    const float m2 = fmaxf(m, s), ref = m2 == -INFINITY ? 0.f : m2;
-    const float c = expf(m - ref), e = expf(s - ref);
-    l = l * c + e;
-    for (int u = 0; u < 2 * PL; ++u) o[u] = o[u] * c + e * v[u];
-    m = m2;
-  }
-  __shared__ float sm[4], so[4][HD];
-  __shared__ double sl[4];
-  if (lane == 0) { sm[warp] = m; sl[warp] = l; }
-  for (int u = 0; u < 2 * PL; ++u) so[warp][lane * 2 * PL + u] = o[u];
-  __syncthreads();
-  if (threadIdx.x >= HD) return;
-  float mm = -INFINITY, oo = 0.f;
-  double ll = 0.;
-  for (int w = 0; w < 4; ++w) mm = fmaxf(mm, sm[w]);
-  const float ref = mm == -INFINITY ? 0.f : mm;
-  for (int w = 0; w < 4; ++w) {
-    const float c = expf(sm[w] - ref);
-    ll += sl[w] * c;
-    oo += so[w][threadIdx.x] * c;
-  }
-  ((T*)p.out)[b * p.out_stride + (int64_t)h * HD + threadIdx.x] = Elem<T>::from_f(oo / (float)ll);
-  if (p.lse && threadIdx.x == 0) p.lse[(int64_t)b * p.NH + h] = ref + logf((float)ll);
 }
 
 struct WeightParams {
@@ -137,9 +726,43 @@ __global__ void __launch_bounds__(256) weights_kernel(WeightParams p) {
   }
 }
 
-static int check_shape(const char* what, int batch, int NH, int KVH, int HD, int block_size,
+constexpr int kMaxCtas = 256;
+constexpr size_t kCounterBytes = kMaxCtas * 4;
+constexpr int kUnitBlocks = 64;                  // widest table that runs one CTA per unit
+
+// One CTA per SM of the current device (its ring fills the shared memory).
+static int decode_ctas() {
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0) {
+    (void)cudaGetLastError();
+    sms = 148;
+  }
+  return std::min(sms, kMaxCtas);
+}
+
+template <typename T, int HD>
+static int launch_decode(const DecodeParams& p, dim3 grid, cudaStream_t s) {
+  static std::atomic<uint64_t> ready{0};         // devices whose limit has been raised
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(ready.load(std::memory_order_acquire) & bit)) {
+    cudaError_t e = cudaFuncSetAttribute(decode_kernel<T, HD>,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)Shape<HD>::smem(kMaxBatch));
+    if (e != cudaSuccess) {
+      (void)cudaGetLastError();
+      return set_cuda_error(e, "cudaFuncSetAttribute(kv4 attention)");
+    }
+    ready.fetch_or(bit, std::memory_order_release);
+  }
+  return launch_kernel("kv4 attention launch", decode_kernel<T, HD>, grid, dim3(kWarps * 32),
+                       Shape<HD>::smem(p.unit_mode ? 0 : p.batch), s, 1, p);
+}
+
+static int check_shape(int batch, int NH, int KVH, int HD, int block_size,
                        int max_blocks, int64_t num_blocks, int dtype) {
-  (void)what;
   if (batch < 0 || max_blocks <= 0 || num_blocks <= 0 || KVH <= 0 || NH <= 0 || NH % KVH)
     return set_error(TI_ERR_INVALID_ARGUMENT,
                      "kv4: bad batch, table width, pool size or head counts (num_heads must be a multiple of num_kv_heads)");
@@ -148,7 +771,9 @@ static int check_shape(const char* what, int batch, int NH, int KVH, int HD, int
   if (NH / KVH > 16) return set_error(TI_ERR_UNSUPPORTED, "kv4: at most 16 query heads per kv head");
   if (dtype != TI_DTYPE_BF16 && dtype != TI_DTYPE_FP16)
     return set_error(TI_ERR_UNSUPPORTED, "kv4: dtype must be bf16 or fp16");
-  if (batch > 4096) return set_error(TI_ERR_UNSUPPORTED, "kv4: at most 4096 sequences per call");
+  if (batch > kMaxBatch) return set_error(TI_ERR_UNSUPPORTED, "kv4: at most 4096 sequences per call");
+  if ((int64_t)batch * max_blocks >= (int64_t)1 << 31)
+    return set_error(TI_ERR_UNSUPPORTED, "kv4: batch times table width must be below 2^31");
   return TI_OK;
 }
 
@@ -159,8 +784,8 @@ using namespace ti;
 
 extern "C" size_t ti_kv4_attention_workspace_bytes(int batch, int num_heads, int num_kv_heads,
                                                    int head_dim, int max_blocks_per_seq) {
-  (void)batch; (void)num_heads; (void)num_kv_heads; (void)head_dim; (void)max_blocks_per_seq;
-  return 16;
+  (void)batch; (void)num_heads; (void)num_kv_heads; (void)max_blocks_per_seq;
+  return kv4::kCounterBytes + (size_t)kv4::decode_ctas() * 2 * (8 * (size_t)head_dim + 16) * 4;
 }
 
 extern "C" int ti_kv4_attention_decode(void* out, int64_t out_seq_stride, float* lse,
@@ -173,27 +798,34 @@ extern "C" int ti_kv4_attention_decode(void* out, int64_t out_seq_stride, float*
                                        size_t workspace_bytes, void* stream) {
   clear_error();
   if (batch == 0) return TI_OK;
-  if (!out || !q || !pool || !block_tables || !context_lens)
+  if (!out || !q || !pool || !block_tables || !context_lens || !workspace)
     return set_error(TI_ERR_INVALID_ARGUMENT, "kv4 attention: null pointer");
-  if (int rc = kv4::check_shape("kv4 attention", batch, num_heads, num_kv_heads, head_dim,
-                                block_size, max_blocks_per_seq, num_blocks, dtype))
+  if (int rc = kv4::check_shape(batch, num_heads, num_kv_heads, head_dim, block_size,
+                                max_blocks_per_seq, num_blocks, dtype))
     return rc;
   if (((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(q) |
-        reinterpret_cast<uintptr_t>(pool)) & 15) || (out_seq_stride % 8) || (q_seq_stride % 8))
+        reinterpret_cast<uintptr_t>(pool) | reinterpret_cast<uintptr_t>(workspace)) & 15) ||
+      (out_seq_stride % 8) || (q_seq_stride % 8))
     return set_error(TI_ERR_INVALID_ARGUMENT, "kv4 attention: tensors must be 16-byte aligned");
-  (void)workspace; (void)workspace_bytes;
+  if (workspace_bytes < ti_kv4_attention_workspace_bytes(batch, num_heads, num_kv_heads, head_dim,
+                                                         max_blocks_per_seq))
+    return set_error(TI_ERR_WORKSPACE, "kv4 attention: workspace too small");
+  const int group = num_heads / num_kv_heads, subs = (group + 7) / 8;
+  const int ctas = kv4::decode_ctas();
+  const int64_t units = (int64_t)batch * num_kv_heads * subs;
+  const bool unit_mode = units <= ctas && max_blocks_per_seq <= kv4::kUnitBlocks;
   kv4::DecodeParams p{out, lse, q, (const uint8_t*)pool, out_seq_stride, q_seq_stride, num_blocks,
                       bt_stride, block_tables, row_index, context_lens, batch, num_heads,
-                      num_kv_heads, num_heads / num_kv_heads, max_blocks_per_seq,
-                      1.0f / sqrtf((float)head_dim)};
+                      num_kv_heads, group, max_blocks_per_seq, subs, unit_mode,
+                      1.4426950408889634f / sqrtf((float)head_dim), (uint32_t*)workspace,
+                      (float*)((uint8_t*)workspace + kv4::kCounterBytes)};
+  const dim3 grid(unit_mode ? (unsigned)units : (unsigned)ctas);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  auto go = [&](auto kern) {
-    return launch_kernel("kv4 attention launch", kern, dim3(num_heads, batch), dim3(128), 0, s, 1, p);
-  };
   if (dtype == TI_DTYPE_BF16)
-    return head_dim == 64 ? go(kv4::decode_kernel<__nv_bfloat16, 64>)
-                          : go(kv4::decode_kernel<__nv_bfloat16, 128>);
-  return head_dim == 64 ? go(kv4::decode_kernel<__half, 64>) : go(kv4::decode_kernel<__half, 128>);
+    return head_dim == 64 ? kv4::launch_decode<__nv_bfloat16, 64>(p, grid, s)
+                          : kv4::launch_decode<__nv_bfloat16, 128>(p, grid, s);
+  return head_dim == 64 ? kv4::launch_decode<__half, 64>(p, grid, s)
+                        : kv4::launch_decode<__half, 128>(p, grid, s);
 }
 
 extern "C" int ti_kv4_accumulate_weights(float* weights_out, const float* weights, const void* q,
@@ -207,7 +839,7 @@ extern "C" int ti_kv4_accumulate_weights(float* weights_out, const float* weight
   if (batch == 0) return TI_OK;
   if (!weights_out || !weights || !q || !lse || !pool || !block_tables || !context_lens)
     return set_error(TI_ERR_INVALID_ARGUMENT, "kv4 weights: null pointer");
-  if (int rc = kv4::check_shape("kv4 weights", batch, num_heads, num_kv_heads, head_dim,
+  if (int rc = kv4::check_shape(batch, num_heads, num_kv_heads, head_dim,
                                 block_size, max_blocks_per_seq, num_blocks, dtype))
     return rc;
   if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(pool)) & 15) ||
