@@ -62,6 +62,7 @@ template <int HD>
 struct Shape {
   static constexpr int kTiles = kStepBytes / Tile<HD>::kBytes;   // tiles of a step
   static constexpr int kLanes = 32 / kTiles;                     // lanes that copy one tile
+  static constexpr uint32_t kFirsts = kTiles == 4 ? 0x01010101u : 0x00010001u;
   static constexpr int kPiece = 8 * HD + 16;                     // floats: O, m[8], l[8]
   static constexpr int kRing = kWarps * kStages * kStepBytes;
   static constexpr int kPark = kWarps * kPiece * 4;
@@ -113,10 +114,8 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
 // Where a warp stands in the stream of tiles.
 struct Cursor {
   int b, hv, blk, n;                 // sequence, unit within it, tile of the unit, tiles of a unit
-  int64_t left;                      // tiles left in the warp's range
-  __device__ __forceinline__ int step(int most) const {
-    return (int)min((int64_t)min(most, n - blk), left);
-  }
+  int left;                          // tiles left in the warp's range
+  __device__ __forceinline__ int step(int most) const { return min(min(most, n - blk), left); }
   // Past k tiles; pref[b] = tiles of one unit of the sequences before b.
   __device__ __forceinline__ void advance(int k, int units, const uint32_t* pref, int batch) {
     blk += k;
@@ -127,6 +126,17 @@ struct Cursor {
     hv = 0;
     do ++b; while (b < batch && pref[b + 1] == pref[b]);
     if (b < batch) n = (int)(pref[b + 1] - pref[b]);
+  }
+};
+
+// An even cut of `total` tiles over `n` warps: the first `rem` warps take one tile more.
+struct Cut {
+  uint32_t quot, rem;
+  __device__ __forceinline__ Cut(uint32_t total, uint32_t n) : quot(total / n), rem(total % n) {}
+  __device__ __forceinline__ uint32_t start(uint32_t w) const { return w * quot + min(w, rem); }
+  __device__ __forceinline__ uint32_t owner(uint32_t tile) const {
+    const uint32_t big = rem * (quot + 1);
+    return tile < big ? tile / (quot + 1) : rem + (tile - big) / quot;
   }
 };
 
@@ -211,12 +221,11 @@ __device__ __forceinline__ int v_row(int tok) {
 
 // O^T += V^T P^T for one tile: o[m][0..1] = dim D/8 * g + 2m, heads 2t, 2t+1; o[m][2..3] = the dim
 // after it.  `live`: tokens of the tile that exist (the others' scales count as zero).
-template <int HD>
+template <int HD, bool FULL>
 __device__ __forceinline__ void tile_values(uint32_t codes, uint32_t scales, int g, int t, int live,
                                             const uint32_t (&p)[2], float (&o)[HD / 16][4]) {
   constexpr int W = HD / 64;                     // words of a lane's dims, per token
-#pragma unroll
-  for (int r = 0; r < 1; ++r) {
+  {
     uint32_t w[4][W], sc[2];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -232,8 +241,10 @@ __device__ __forceinline__ void tile_values(uint32_t codes, uint32_t scales, int
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       uint32_t b2 = lds16(scales + grp * kBlock + 2 * t + 8 * k);
-      const int n = live - (2 * t + 8 * k);
-      if (n < 2) b2 = n == 1 ? (b2 & 0xFFu) : 0u;
+      if constexpr (!FULL) {
+        const int n = live - (2 * t + 8 * k);
+        if (n < 2) b2 = n == 1 ? (b2 & 0xFFu) : 0u;
+      }
       sc[k] = __byte_perm(b2, 0, 0x1404) >> 1;   // bytes to the halves' tops, then << 7 in all
     }
 #pragma unroll
@@ -259,23 +270,33 @@ __device__ __forceinline__ void tile_values(uint32_t codes, uint32_t scales, int
   }
 }
 
-// This lane's 9 copies of a step: the lanes of one tile take neighbouring 16-byte chunks, the V
-// code rows land permuted (v_row, and for 64-byte rows with the halves of rows 2 and 3 exchanged).
+// This lane's 9 copies of a step: the lanes of one tile take neighbouring 16-byte chunks, the V code
+// rows land permuted (v_row, and for 64-byte rows with the halves of rows 2 and 3 exchanged).  A
+// lane's chunk l + kLanes * i lies in row 4 i + (l / chunks of a row), whose place is a constant of i
+// plus one of the lane: `even` and `odd` are the lane's parts for even and odd i.
 template <int HD>
-__device__ __forceinline__ void copy_tile(uint32_t dst, const uint8_t* src, int l) {
-  using S = Shape<HD>;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) cp_async16(dst + (l + S::kLanes * i) * 16, src + (l + S::kLanes * i) * 16);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int c = l + S::kLanes * i;             // chunk of the V codes
-    constexpr int kPer = HD / 32;                // chunks of a row
-    const int row = v_row(c / kPer);
-    const int x = HD == 64 ? c % kPer : (c % kPer) ^ (row & 2);
-    cp_async16(dst + Tile<HD>::kV + (row * kPer + x) * 16, src + Tile<HD>::kV + c * 16);
+struct CopyLane {
+  uint32_t k, even, odd;
+  __device__ __forceinline__ explicit CopyLane(int l) {
+    constexpr int kPer = HD / 32;                // chunks of a row of codes
+    const int r = l / kPer, c = l % kPer;
+    const uint32_t row = ((r & 1) * 4 + (r >> 1)) * kPer * 16;
+    k = l * 16;
+    even = Tile<HD>::kV + row + c * 16;
+    odd = Tile<HD>::kV + row + (HD == 64 ? c : c ^ 2) * 16;
   }
-  cp_async16(dst + Tile<HD>::kKs + l * 16, src + Tile<HD>::kKs + l * 16);
-}
+  __device__ __forceinline__ void copy(uint32_t dst, const uint8_t* src) const {
+    constexpr int kStep = Shape<HD>::kLanes * 16, kRowBytes = Tile<HD>::kRow;
+    const uint8_t* p = src + k;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) cp_async16(dst + k + i * kStep, p + i * kStep);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      cp_async16(dst + ((i & 1) ? odd : even) + ((i >> 1) * 8 + (i & 1) * 2) * kRowBytes,
+                 p + Tile<HD>::kV + i * kStep);
+    cp_async16(dst + k + Tile<HD>::kKs, p + Tile<HD>::kKs);
+  }
+};
 
 // Write a unit's finished rows: heads 2t and 2t+1, this lane's D/8 dims.
 template <typename T, int HD>
@@ -329,18 +350,19 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(DecodeParams p) 
   uint32_t* pref = reinterpret_cast<uint32_t*>(smem + S::kRing + S::kPark);   // [batch + 1]
   __shared__ uint32_t s_scan[kWarps + 1];
   __shared__ int s_last[2], s_start[kWarps + 1];
+  __shared__ int4 s_first;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int units = p.KVH * p.subs;
   pdl_wait();
   pdl_launch_dependents();
 
   // pref[b] = tiles of one unit of the sequences before b (in unit mode: only this CTA's sequence)
-  const int64_t cap = (int64_t)p.max_blocks * kBlock;
+  const int cap = (int)min((int64_t)p.max_blocks * kBlock, (int64_t)0x7FFFFFFF);
   auto tiles_of = [&](int b) {
-    const int64_t n = min((int64_t)p.ctx[b], cap);
+    const int n = min(p.ctx[b], cap);
     return n > 0 ? (uint32_t)((n - 1) / kBlock + 1) : 0u;
   };
-  int64_t total;
+  uint32_t total;
   int ctas;
   if (p.unit_mode) {
     ctas = 1;
@@ -349,12 +371,11 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(DecodeParams p) 
     uint32_t carry = 0;
     for (int b0 = 0; b0 < p.batch; b0 += kWarps * 32) {
       const int b = b0 + tid;
-      const uint32_t n = b < p.batch ? tiles_of(b) : 0u;
-      uint32_t x = n;
+      uint32_t x = b < p.batch ? tiles_of(b) : 0u;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
+      for (int d = 1; d < 32; d <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, x, d);
+        if (lane >= d) x += y;
       }
       if (lane == 31) s_scan[warp] = x;
       __syncthreads();
@@ -370,35 +391,44 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(DecodeParams p) 
     }
     if (tid == 0) pref[0] = 0;
     __syncthreads();
-    total = (int64_t)carry * units;
+    total = carry * (uint32_t)units;
     // at least two tiles per warp: fewer CTAs for little work, and fewer units cut
-    ctas = (int)min((int64_t)gridDim.x, (total + 2 * kWarps - 1) / (2 * kWarps));
+    ctas = min((int)gridDim.x, (int)((total + 2 * kWarps - 1) / (2 * kWarps)));
   }
   const int cta = p.unit_mode ? 0 : blockIdx.x;
   if (total == 0 || cta >= ctas) return;
-  const int64_t nw = (int64_t)ctas * kWarps;
-  auto start_of = [&](int64_t w) { return w * total / nw; };     // first tile of warp w (of all CTAs)
-  const int64_t w_begin = start_of((int64_t)cta * kWarps + warp);
-  const int64_t w_end = start_of((int64_t)cta * kWarps + warp + 1);
+  const Cut cut_of(total, (uint32_t)ctas * kWarps);
+  const uint32_t c_begin = cut_of.start(cta * kWarps);
+  const uint32_t w_begin = cut_of.start(cta * kWarps + warp);
 
   Cursor cur;
-  cur.left = w_end - w_begin;
+  cur.left = (int)(cut_of.start(cta * kWarps + warp + 1) - w_begin);
   if (p.unit_mode) {
     cur.b = blockIdx.x / units;
     cur.hv = blockIdx.x % units;
     cur.n = (int)total;
     cur.blk = (int)w_begin;
   } else {
-    int lo = 0, hi = p.batch;                      // last b with pref[b] * units <= w_begin
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if ((int64_t)pref[mid] * units <= w_begin) lo = mid; else hi = mid;
+    // last b with pref[b] * units <= w_begin: 32 probes at a time
+    const uint32_t at = w_begin / (uint32_t)units;
+    int lo = 0, len = p.batch;                     // the answer is in [lo, lo + len)
+    while (len > 1) {
+      const int step = (len + 31) / 32, probe = lo + lane * step;
+      const uint32_t ok = __ballot_sync(0xffffffffu, lane * step < len && pref[min(probe, p.batch)] <= at);
+      const int k = 31 - __clz(ok);
+      lo += k * step;
+      len = min(step, len - k * step);
     }
     cur.b = lo;
     cur.n = (int)(pref[lo + 1] - pref[lo]);
-    const int64_t r = w_begin - (int64_t)pref[lo] * units;
-    cur.hv = cur.n ? (int)(r / cur.n) : 0;
-    cur.blk = cur.n ? (int)(r % cur.n) : 0;
+    const uint32_t r = w_begin - pref[lo] * (uint32_t)units, n = max(cur.n, 1);
+    cur.hv = (int)(r / n);
+    cur.blk = (int)(r % n);
+  }
+  if (lane == 0) {
+    s_start[warp] = (int)(w_begin - c_begin);
+    if (warp == kWarps - 1) s_start[kWarps] = (int)(w_begin - c_begin) + cur.left;
+    if (warp == 0) s_first = make_int4(cur.b, cur.hv, cur.blk, cur.n);
   }
 
   float o[HD / 16][4], m[2], l[2];
@@ -406,9 +436,10 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(DecodeParams p) 
   const bool head_cut = cur.blk > 0;               // the first unit began before this warp
   if (cur.left > 0) {
     const uint32_t ring = smem_u32(smem) + warp * (kStages * kStepBytes);
-    const int j = lane / S::kLanes, cl = lane % S::kLanes;
+    const int j = lane / S::kLanes;
+    const CopyLane<HD> mine(lane % S::kLanes);
     Cursor ld = cur;
-    uint32_t have = 0;                             // S::kTiles bits per step in flight: blocks that exist
+    uint32_t have = 0;                             // which tiles of the steps in flight exist
     int issued = 0;
     auto next_id = [&]() -> int {
       if (j >= ld.step(S::kTiles)) return -1;
@@ -420,15 +451,13 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(DecodeParams p) 
       const bool ok = id >= 0 && id < p.num_blocks;
       if (ok) {
         const int kvh = p.subs == 1 ? ld.hv : ld.hv / p.subs;
-        copy_tile<HD>(ring + (issued % kStages) * kStepBytes + j * L::kBytes,
-                      p.pool + ((int64_t)id * p.KVH + kvh) * L::kBytes, cl);
+        mine.copy(ring + (issued & (kStages - 1)) * kStepBytes + j * L::kBytes,
+                  p.pool + ((int64_t)id * p.KVH + kvh) * L::kBytes);
       }
       cp_commit();
-      const uint32_t bal = __ballot_sync(0xffffffffu, ok && cl == 0);
-      uint32_t bits = 0;
-#pragma unroll
-      for (int k = 0; k < S::kTiles; ++k) bits |= ((bal >> (k * S::kLanes)) & 1u) << k;
-      have |= bits << ((issued % kStages) * S::kTiles);
+      // one bit per tile at its first lane's place; a step's bits in the half it was issued to
+      const uint32_t bal = __ballot_sync(0xffffffffu, ok) & S::kFirsts;
+      have = (issued & 1) ? (have & S::kFirsts) | (bal << 1) : (have & (S::kFirsts << 1)) | bal;
       ++issued;
       if (ld.left > 0) {
         ld.advance(ld.step(S::kTiles), units, pref, p.batch);
@@ -442,7 +471,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(DecodeParams p) 
       const int kvh = cur.hv / p.subs, sub = cur.hv % p.subs;
       h0 = kvh * p.group + sub * 8;
       heads = min(8, p.group - sub * 8);
-      ctx = (int)min((int64_t)p.ctx[cur.b], cap);
+      ctx = min(p.ctx[cur.b], cap);
       const float2 inv = load_query<T, HD>((const T*)p.q + cur.b * p.q_stride + (int64_t)h0 * HD, heads, g, t, qf);
       sc = make_float2(inv.x * p.scale_log2, inv.y * p.scale_log2);
 #pragma unroll
@@ -453,23 +482,17 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(DecodeParams p) 
     issue();
     open_unit();
     bool first = true;
-    for (int it = 0;; ++it) {
-      issue();                                     // (an empty group when nothing is left)
-      cp_wait<kStages - 1>();
-      __syncwarp();
-      const int k = cur.step(S::kTiles);
-      const uint32_t st = ring + (it % kStages) * kStepBytes;
-      const uint32_t ok = (have >> ((it % kStages) * S::kTiles)) & ((1u << S::kTiles) - 1u);
-      have &= ~(((1u << S::kTiles) - 1u) << ((it % kStages) * S::kTiles));
-      const int live = ctx - cur.blk * kBlock;     // tokens from this step's first on
+    // one step: full = all tiles exist and all their tokens are within the length
+    auto run_step = [&](auto full_t, uint32_t st, uint32_t ok, int live) {
+      constexpr bool FULL = decltype(full_t)::value;
       float s[S::kTiles][4];
       float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
       for (int x = 0; x < S::kTiles; ++x) {
-        if ((ok >> x) & 1u) {
+        if (FULL || ((ok >> (x * S::kLanes)) & 1u)) {
           tile_scores<HD>(st + x * L::kBytes + L::kK, st + x * L::kBytes + L::kKs, g, t, qf, s[x]);
-          const int n = live - x * kBlock;
-          if (n < kBlock) {
+          if constexpr (!FULL) {
+            const int n = live - x * kBlock;
             if (g >= n) s[x][0] = s[x][1] = -INFINITY;
             if (g + 8 >= n) s[x][2] = s[x][3] = -INFINITY;
           }
@@ -504,16 +527,27 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(DecodeParams p) 
       const float f0 = kPScale - (n0 == -INFINITY ? 0.f : n0), f1 = kPScale - (n1 == -INFINITY ? 0.f : n1);
 #pragma unroll
       for (int x = 0; x < S::kTiles; ++x) {
-        if (!((ok >> x) & 1u)) continue;
+        if (!FULL && !((ok >> (x * S::kLanes)) & 1u)) continue;
         const float e0 = fast_exp2(fmaf(s[x][0], sc.x, f0)), e1 = fast_exp2(fmaf(s[x][1], sc.y, f1));
         const float e2 = fast_exp2(fmaf(s[x][2], sc.x, f0)), e3 = fast_exp2(fmaf(s[x][3], sc.y, f1));
         l[0] += e0 + e2;
         l[1] += e1 + e3;
         const uint32_t pt[2] = {transpose8x8(Elem<__half>::pack2(e0, e1)),
                                 transpose8x8(Elem<__half>::pack2(e2, e3))};
-        tile_values<HD>(st + x * L::kBytes + L::kV, st + x * L::kBytes + L::kVs, g, t,
-                        live - x * kBlock, pt, o);
+        tile_values<HD, FULL>(st + x * L::kBytes + L::kV, st + x * L::kBytes + L::kVs, g, t,
+                              live - x * kBlock, pt, o);
       }
+    };
+    for (int it = 0;; ++it) {
+      issue();                                     // (an empty group when nothing is left)
+      cp_wait<kStages - 1>();
+      __syncwarp();
+      const int k = cur.step(S::kTiles);
+      const uint32_t st = ring + (it & (kStages - 1)) * kStepBytes;
+      const uint32_t ok = ((it & 1) ? have >> 1 : have) & S::kFirsts;
+      const int live = ctx - cur.blk * kBlock;     // tokens from this step's first on
+      if (ok == S::kFirsts && live >= S::kTiles * kBlock) run_step(std::true_type{}, st, ok, live);
+      else run_step(std::false_type{}, st, ok, live);
       __syncwarp();                                // the stage is free for the copies after next
       const int ub = cur.b;
       const bool done = cur.blk + k == cur.n;      // the unit's last tile
@@ -539,12 +573,6 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(DecodeParams p) 
     }
     cp_wait<0>();
   }
-  // first tile of every warp, counted from the CTA's
-  const int64_t c_begin = start_of((int64_t)cta * kWarps);
-  if (lane == 0) {
-    s_start[warp] = (int)(w_begin - c_begin);
-    if (warp == kWarps - 1) s_start[kWarps] = (int)(w_end - c_begin);
-  }
   __syncthreads();
   // the rings are free: pieces that are still in registers go there
   float* tails = reinterpret_cast<float*>(smem);
@@ -553,52 +581,34 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(DecodeParams p) 
 
   // join the cut units of this CTA; piece of unit [s, e) in warp w: parked when the unit began before
   // the warp's range, else left in the ring
-  const int64_t c_end = c_begin + s_start[kWarps];
-  auto cta_of = [&](int64_t pos) {                 // the CTA whose range holds tile pos
-    return (int)((((pos + 1) * nw - 1) / total) / kWarps);
-  };
-  auto unit_at = [&](int64_t pos, int& b, int& hv, int64_t& s, int64_t& e) {
-    if (p.unit_mode) {
-      b = blockIdx.x / units;
-      hv = blockIdx.x % units;
-      s = 0;
-      e = total;
-      return;
-    }
-    int lo = 0, hi = p.batch;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if ((int64_t)pref[mid] * units <= pos) lo = mid; else hi = mid;
-    }
-    b = lo;
-    const int64_t n = pref[lo + 1] - pref[lo], base = (int64_t)pref[lo] * units;
-    hv = (int)((pos - base) / n);
-    s = base + hv * n;
-    e = s + n;
-  };
+  // (positions below count from the CTA's first tile; the unit that began before it has s < 0)
+  const int c_len = s_start[kWarps];
   auto weight = [](float mi, float mm) { return mi == -INFINITY ? 0.f : fast_exp2(mi - mm); };
-  int n_cross = 0;
-  int64_t cross_s[2], cross_e[2];
-  int cross_b[2], cross_hv[2];
-  for (int64_t pos = c_begin; pos < c_end;) {
-    int b, hv;
-    int64_t s, e;
-    unit_at(pos, b, hv, s, e);
-    pos = e;
-    const bool inside = s >= c_begin && e <= c_end;
-    const int s0 = (int)(max(s, c_begin - 1) - c_begin), e0 = (int)(min(e, c_end) - c_begin);
+  int n_cross = 0, cross_s[2], cross_n[2], cross_b[2], cross_hv[2];
+  int b = s_first.x, hv = s_first.y, n_unit = s_first.w;
+  for (int s = -s_first.z; s < c_len;) {
+    const int e = s + n_unit, ub = b, uh = hv, us = s;
+    s = e;                                         // the next unit
+    if (++hv == units) {
+      hv = 0;
+      if (!p.unit_mode && s < c_len) {
+        do ++b; while (pref[b + 1] == pref[b]);
+        n_unit = (int)(pref[b + 1] - pref[b]);
+      }
+    }
+    const bool inside = us >= 0 && e <= c_len;
     int wa = 0, wb = kWarps - 1;                   // its first and last warp here
-    while (s_start[wa + 1] <= s0) ++wa;
-    while (s_start[wb] >= e0) --wb;
+    while (s_start[wa + 1] <= us) ++wa;
+    while (s_start[wb] >= e) --wb;
     if (inside && wa == wb) continue;              // written by its warp
-    const int sub = hv % p.subs, h0 = (hv / p.subs) * p.group + sub * 8;
+    const int sub = uh % p.subs, h0 = (uh / p.subs) * p.group + sub * 8;
     const int heads = min(8, p.group - sub * 8);
-    float* ws = inside ? nullptr : p.parts + ((int64_t)cta * 2 + (s < c_begin ? 0 : 1)) * S::kPiece;
+    float* ws = inside ? nullptr : p.parts + ((int64_t)cta * 2 + (us < 0 ? 0 : 1)) * S::kPiece;
     for (int i = tid; i < 8 * HD; i += kWarps * 32) {
       const int h = i / HD;
       if (h >= heads) break;
       float mm = -INFINITY, ll = 0.f, oo = 0.f;
-      auto piece = [&](int w) { return (s0 < s_start[w] ? park : tails) + w * S::kPiece; };
+      auto piece = [&](int w) { return (us < s_start[w] ? park : tails) + w * S::kPiece; };
       for (int w = wa; w <= wb; ++w)
         if (s_start[w] < s_start[w + 1]) mm = fmaxf(mm, piece(w)[8 * HD + h]);
       for (int w = wa; w <= wb; ++w) {
@@ -610,9 +620,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(DecodeParams p) 
         oo += src[8 * HD + h] == -INFINITY ? src[i] : c * src[i];
       }
       if (inside) {
-        ((T*)p.out)[b * p.out_stride + (int64_t)(h0 + h) * HD + i % HD] = Elem<T>::from_f(oo / ll);
+        ((T*)p.out)[ub * p.out_stride + (int64_t)(h0 + h) * HD + i % HD] = Elem<T>::from_f(oo / ll);
         if (p.lse && i % HD == 0)
-          p.lse[(int64_t)b * p.NH + h0 + h] = (mm == -INFINITY ? 0.f : mm - kPScale) * 0.6931471805599453f + logf(ll);
+          p.lse[(int64_t)ub * p.NH + h0 + h] = (mm == -INFINITY ? 0.f : mm - kPScale) * 0.6931471805599453f + logf(ll);
       } else {
         ws[i] = oo;
         if (i % HD == 0) {
@@ -622,18 +632,18 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(DecodeParams p) 
       }
     }
     if (!inside) {
-      cross_s[n_cross] = s;
-      cross_e[n_cross] = e;
-      cross_b[n_cross] = b;
-      cross_hv[n_cross++] = hv;
+      cross_s[n_cross] = us;
+      cross_n[n_cross] = e - us;
+      cross_b[n_cross] = ub;
+      cross_hv[n_cross++] = uh;
     }
   }
   if (n_cross == 0) return;
   __threadfence();
   __syncthreads();
   if (tid < n_cross) {
-    const int64_t s = tid ? cross_s[1] : cross_s[0], e = tid ? cross_e[1] : cross_e[0];
-    const int fst = cta_of(s), lst = cta_of(e - 1);
+    const uint32_t s = c_begin + (tid ? cross_s[1] : cross_s[0]), n = tid ? cross_n[1] : cross_n[0];
+    const int fst = cut_of.owner(s) / kWarps, lst = cut_of.owner(s + n - 1) / kWarps;
     const uint32_t old = atomicAdd(p.counters + fst, 1u);
     s_last[tid] = old == (uint32_t)(lst - fst);
     if (s_last[tid]) p.counters[fst] = 0;          // zero again for the next call
@@ -642,10 +652,10 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(DecodeParams p) 
   __syncthreads();
   for (int x = 0; x < n_cross; ++x) {
     if (!s_last[x]) continue;
-    const int64_t s = cross_s[x], e = cross_e[x];
-    const int fst = cta_of(s), lst = cta_of(e - 1);
+    const uint32_t s = c_begin + cross_s[x];
+    const int fst = cut_of.owner(s) / kWarps, lst = cut_of.owner(s + cross_n[x] - 1) / kWarps;
     const int sub = cross_hv[x] % p.subs, h0 = (cross_hv[x] / p.subs) * p.group + sub * 8;
-    const int heads = min(8, p.group - sub * 8), b = cross_b[x];
+    const int heads = min(8, p.group - sub * 8), ub = cross_b[x];
     for (int i = tid; i < 8 * HD; i += kWarps * 32) {
       const int h = i / HD;
       if (h >= heads) break;
@@ -660,9 +670,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(DecodeParams p) 
         ll += f * __ldcg(part(c) + 8 * HD + 8 + h);
         oo += f * __ldcg(part(c) + i);
       }
-      ((T*)p.out)[b * p.out_stride + (int64_t)(h0 + h) * HD + i % HD] = Elem<T>::from_f(oo / ll);
+      ((T*)p.out)[ub * p.out_stride + (int64_t)(h0 + h) * HD + i % HD] = Elem<T>::from_f(oo / ll);
       if (p.lse && i % HD == 0)
-        p.lse[(int64_t)b * p.NH + h0 + h] = (mm == -INFINITY ? 0.f : mm - kPScale) * 0.6931471805599453f + logf(ll);
+        p.lse[(int64_t)ub * p.NH + h0 + h] = (mm == -INFINITY ? 0.f : mm - kPScale) * 0.6931471805599453f + logf(ll);
     }
   }
 }
@@ -772,8 +782,9 @@ static int check_shape(int batch, int NH, int KVH, int HD, int block_size,
   if (dtype != TI_DTYPE_BF16 && dtype != TI_DTYPE_FP16)
     return set_error(TI_ERR_UNSUPPORTED, "kv4: dtype must be bf16 or fp16");
   if (batch > kMaxBatch) return set_error(TI_ERR_UNSUPPORTED, "kv4: at most 4096 sequences per call");
-  if ((int64_t)batch * max_blocks >= (int64_t)1 << 31)
-    return set_error(TI_ERR_UNSUPPORTED, "kv4: batch times table width must be below 2^31");
+  if ((int64_t)batch * max_blocks * KVH * ((NH / KVH + 7) / 8) >= (int64_t)1 << 31)
+    return set_error(TI_ERR_UNSUPPORTED,
+                     "kv4: batch * table width * kv heads (twice beyond 8 query heads each) must be below 2^31");
   return TI_OK;
 }
 
