@@ -132,7 +132,7 @@ struct Cursor {
 // An even cut of `total` tiles over `n` warps: the first `rem` warps take one tile more.
 struct Cut {
   uint32_t quot, rem;
-  __device__ __forceinline__ Cut(uint32_t total, uint32_t n) : quot(total / n), rem(total % n) {}
+  __device__ __forceinline__ Cut(uint32_t total, uint32_t n) : quot(total / n), rem(total - quot * n) {}
   __device__ __forceinline__ uint32_t start(uint32_t w) const { return w * quot + min(w, rem); }
   __device__ __forceinline__ uint32_t owner(uint32_t tile) const {
     const uint32_t big = rem * (quot + 1);
@@ -298,6 +298,13 @@ struct CopyLane {
   }
 };
 
+// ln of the sum: m in units of the exponent, l times 2^14 (lg2.approx: off by 2^-22).
+__device__ __forceinline__ float row_lse(float m, float l) {
+  float g;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(g) : "f"(l));
+  return ((m == -INFINITY ? 0.f : m - kPScale) + g) * 0.6931471805599453f;
+}
+
 // Write a unit's finished rows: heads 2t and 2t+1, this lane's D/8 dims.
 template <typename T, int HD>
 __device__ __forceinline__ void store_rows(const DecodeParams& p, int b, int h0, int heads, int g,
@@ -319,7 +326,7 @@ __device__ __forceinline__ void store_rows(const DecodeParams& p, int b, int h0,
       *reinterpret_cast<uint4*>(out + i * 8) = u;
     }
     if (p.lse && g == 0)
-      p.lse[(int64_t)b * p.NH + h0 + h] = (m[x] == -INFINITY ? 0.f : m[x] - kPScale) * 0.6931471805599453f + logf(l[x]);
+      p.lse[(int64_t)b * p.NH + h0 + h] = row_lse(m[x], l[x]);
   }
 }
 
@@ -341,6 +348,19 @@ __device__ __forceinline__ void store_piece(float* dst, int g, int t, const floa
   }
 }
 
+// A joined row: HD/32 dims per lane.
+template <typename T, int HD>
+__device__ __forceinline__ void store_joined(const DecodeParams& p, int b, int h, int lane,
+                                             const float (&o)[HD / 32], float m, float l) {
+  T* out = (T*)p.out + b * p.out_stride + (int64_t)h * HD + lane * (HD / 32);
+  const float r = 1.f / l;
+#pragma unroll
+  for (int i = 0; i < HD / 64; ++i)
+    reinterpret_cast<uint32_t*>(out)[i] = Elem<T>::pack2(o[2 * i] * r, o[2 * i + 1] * r);
+  if (p.lse && lane == 0)
+    p.lse[(int64_t)b * p.NH + h] = row_lse(m, l);
+}
+
 template <typename T, int HD>
 __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(DecodeParams p) {
   using S = Shape<HD>;
@@ -350,7 +370,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(DecodeParams p) 
   uint32_t* pref = reinterpret_cast<uint32_t*>(smem + S::kRing + S::kPark);   // [batch + 1]
   __shared__ uint32_t s_scan[kWarps + 1];
   __shared__ int s_last[2], s_start[kWarps + 1];
-  __shared__ int4 s_first;
+  // cut units by where their first piece in this CTA is: tail of warp i, or (16) head of warp 0;
+  // x = first tile counted from the CTA's, y = tiles (0: none), z = sequence, w = unit of it
+  __shared__ int4 s_cut[kWarps + 1];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int units = p.KVH * p.subs;
   pdl_wait();
@@ -410,11 +432,10 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(DecodeParams p) 
     cur.blk = (int)w_begin;
   } else {
     // last b with pref[b] * units <= w_begin: 32 probes at a time
-    const uint32_t at = w_begin / (uint32_t)units;
     int lo = 0, len = p.batch;                     // the answer is in [lo, lo + len)
     while (len > 1) {
       const int step = (len + 31) / 32, probe = lo + lane * step;
-      const uint32_t ok = __ballot_sync(0xffffffffu, lane * step < len && pref[min(probe, p.batch)] <= at);
+      const uint32_t ok = __ballot_sync(0xffffffffu, lane * step < len && pref[min(probe, p.batch)] * (uint32_t)units <= w_begin);
       const int k = 31 - __clz(ok);
       lo += k * step;
       len = min(step, len - k * step);
@@ -423,12 +444,13 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(DecodeParams p) 
     cur.n = (int)(pref[lo + 1] - pref[lo]);
     const uint32_t r = w_begin - pref[lo] * (uint32_t)units, n = max(cur.n, 1);
     cur.hv = (int)(r / n);
-    cur.blk = (int)(r % n);
+    cur.blk = (int)(r - cur.hv * n);
   }
   if (lane == 0) {
     s_start[warp] = (int)(w_begin - c_begin);
     if (warp == kWarps - 1) s_start[kWarps] = (int)(w_begin - c_begin) + cur.left;
-    if (warp == 0) s_first = make_int4(cur.b, cur.hv, cur.blk, cur.n);
+    s_cut[warp] = make_int4(0, 0, 0, 0);
+    if (warp == 0) s_cut[kWarps] = make_int4(0, 0, 0, 0);
   }
 
   float o[HD / 16][4], m[2], l[2];
@@ -479,8 +501,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(DecodeParams p) 
       m[0] = m[1] = -INFINITY;
       l[0] = l[1] = 0.f;
     };
+    open_unit();                                   // (its loads and the first block id's overlap)
     issue();
-    open_unit();
+    const int total_left = cur.left;
     bool first = true;
     // one step: full = all tiles exist and all their tokens are within the length
     auto run_step = [&](auto full_t, uint32_t st, uint32_t ok, int live) {
@@ -549,7 +572,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(DecodeParams p) 
       if (ok == S::kFirsts && live >= S::kTiles * kBlock) run_step(std::true_type{}, st, ok, live);
       else run_step(std::false_type{}, st, ok, live);
       __syncwarp();                                // the stage is free for the copies after next
-      const int ub = cur.b;
+      const int ub = cur.b, uhv = cur.hv, ublk = cur.blk, un = cur.n;
+      const int at = total_left - cur.left;        // this step's place in the warp's range
       const bool done = cur.blk + k == cur.n;      // the unit's last tile
       cur.advance(k, units, pref, p.batch);
       if (done || cur.left == 0) {
@@ -561,10 +585,12 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(DecodeParams p) 
         const bool cut = first && head_cut;
         if (done && !cut) {
           store_rows<T, HD>(p, ub, h0, heads, g, t, o, m, l);
-        } else if (cut) {
-          store_piece<HD>(park + warp * S::kPiece, g, t, o, m, l);
         } else {
-          tail = true;
+          if (cut) store_piece<HD>(park + warp * S::kPiece, g, t, o, m, l);
+          else tail = true;
+          if (lane == 0 && (!cut || warp == 0))
+            s_cut[cut ? kWarps : warp] =
+                make_int4((int)(w_begin - c_begin) + at - ublk, un, ub, uhv);
         }
         first = false;
         if (cur.left == 0) break;
@@ -579,71 +605,63 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(DecodeParams p) 
   if (tail) store_piece<HD>(tails + warp * S::kPiece, g, t, o, m, l);
   __syncthreads();
 
-  // join the cut units of this CTA; piece of unit [s, e) in warp w: parked when the unit began before
-  // the warp's range, else left in the ring
-  // (positions below count from the CTA's first tile; the unit that began before it has s < 0)
+  // Join the cut units of this CTA, one warp per (unit, head).  The piece of a unit in warp w is parked
+  // when the unit began before the warp's range, else it was left in the ring.  Positions count from
+  // the CTA's first tile; a unit that began before it has a negative one.
   const int c_len = s_start[kWarps];
-  auto weight = [](float mi, float mm) { return mi == -INFINITY ? 0.f : fast_exp2(mi - mm); };
-  int n_cross = 0, cross_s[2], cross_n[2], cross_b[2], cross_hv[2];
-  int b = s_first.x, hv = s_first.y, n_unit = s_first.w;
-  for (int s = -s_first.z; s < c_len;) {
-    const int e = s + n_unit, ub = b, uh = hv, us = s;
-    s = e;                                         // the next unit
-    if (++hv == units) {
-      hv = 0;
-      if (!p.unit_mode && s < c_len) {
-        do ++b; while (pref[b + 1] == pref[b]);
-        n_unit = (int)(pref[b + 1] - pref[b]);
-      }
+  const int my_start = lane < kWarps ? s_start[lane] : 0;
+  const int my_end = lane < kWarps ? s_start[lane + 1] : 0;       // (other lanes: an empty range)
+  const int4 mine = lane <= kWarps ? s_cut[lane] : make_int4(0, 0, 0, 0);
+  uint32_t cuts = __ballot_sync(0xffffffffu, mine.y > 0);
+  const uint32_t cross = __ballot_sync(0xffffffffu, mine.y > 0 && (mine.x < 0 || mine.x + mine.y > c_len));
+  for (int i = 0; cuts; ++i, cuts &= cuts - 1) {
+    if ((i & (kWarps / 8 - 1)) != warp >> 3) continue;            // 8 warps per unit
+    const int4 u = s_cut[__ffs(cuts) - 1];
+    const int sub = p.subs == 1 ? 0 : u.w % p.subs, kvh = p.subs == 1 ? u.w : u.w / p.subs;
+    const int h = warp & 7, h0 = kvh * p.group + sub * 8;
+    if (h >= min(8, p.group - sub * 8)) continue;
+    const int us = u.x, e = u.x + u.y;
+    const bool has = my_start < my_end && my_start < e && my_end > us;
+    const uint32_t pieces = __ballot_sync(0xffffffffu, has);
+    const float* src = (us < my_start ? park : tails) + lane * S::kPiece;
+    const float mi = has ? src[8 * HD + h] : -INFINITY;
+    const float li = has ? src[8 * HD + 8 + h] : 0.f;
+    const int wa = __ffs(pieces) - 1, wb = 31 - __clz(pieces);
+    const bool first_parked = us < s_start[wa];
+    const float mm = warp_max(mi);
+    // (a piece without a finite score keeps its sum: zero, or NaN)
+    const float c = mi == -INFINITY ? 1.f : fast_exp2(mi - mm);
+    const float ll = warp_sum(c * li);
+    float acc[HD / 32] = {};
+#pragma unroll 4
+    for (int w = wa; w <= wb; ++w) {
+      const float cw = __shfl_sync(0xffffffffu, c, w);
+      // only its first piece can be a tail: the unit reaches into every later warp from the left
+      const float* o_w = (w == wa && !first_parked ? tails : park) + w * S::kPiece + h * HD + lane * (HD / 32);
+#pragma unroll
+      for (int k = 0; k < HD / 32; ++k)
+        if ((pieces >> w) & 1u) acc[k] += cw * o_w[k];
     }
-    const bool inside = us >= 0 && e <= c_len;
-    int wa = 0, wb = kWarps - 1;                   // its first and last warp here
-    while (s_start[wa + 1] <= us) ++wa;
-    while (s_start[wb] >= e) --wb;
-    if (inside && wa == wb) continue;              // written by its warp
-    const int sub = uh % p.subs, h0 = (uh / p.subs) * p.group + sub * 8;
-    const int heads = min(8, p.group - sub * 8);
-    float* ws = inside ? nullptr : p.parts + ((int64_t)cta * 2 + (us < 0 ? 0 : 1)) * S::kPiece;
-    for (int i = tid; i < 8 * HD; i += kWarps * 32) {
-      const int h = i / HD;
-      if (h >= heads) break;
-      float mm = -INFINITY, ll = 0.f, oo = 0.f;
-      auto piece = [&](int w) { return (us < s_start[w] ? park : tails) + w * S::kPiece; };
-      for (int w = wa; w <= wb; ++w)
-        if (s_start[w] < s_start[w + 1]) mm = fmaxf(mm, piece(w)[8 * HD + h]);
-      for (int w = wa; w <= wb; ++w) {
-        if (s_start[w] == s_start[w + 1]) continue;               // an empty range
-        const float* src = piece(w);
-        const float c = weight(src[8 * HD + h], mm);
-        // (a NaN sum has to stay one whatever its max)
-        ll += src[8 * HD + h] == -INFINITY ? src[8 * HD + 8 + h] : c * src[8 * HD + 8 + h];
-        oo += src[8 * HD + h] == -INFINITY ? src[i] : c * src[i];
+    if (us >= 0 && e <= c_len) {
+      store_joined<T, HD>(p, u.z, h0 + h, lane, acc, mm, ll);
+    } else {
+      float* ws = p.parts + ((int64_t)cta * 2 + (us < 0 ? 0 : 1)) * S::kPiece;
+#pragma unroll
+      for (int k = 0; k < HD / 32; ++k) ws[h * HD + lane * (HD / 32) + k] = acc[k];
+      if (lane == 0) {
+        ws[8 * HD + h] = mm;
+        ws[8 * HD + 8 + h] = ll;
       }
-      if (inside) {
-        ((T*)p.out)[ub * p.out_stride + (int64_t)(h0 + h) * HD + i % HD] = Elem<T>::from_f(oo / ll);
-        if (p.lse && i % HD == 0)
-          p.lse[(int64_t)ub * p.NH + h0 + h] = (mm == -INFINITY ? 0.f : mm - kPScale) * 0.6931471805599453f + logf(ll);
-      } else {
-        ws[i] = oo;
-        if (i % HD == 0) {
-          ws[8 * HD + h] = mm;
-          ws[8 * HD + 8 + h] = ll;
-        }
-      }
-    }
-    if (!inside) {
-      cross_s[n_cross] = us;
-      cross_n[n_cross] = e - us;
-      cross_b[n_cross] = ub;
-      cross_hv[n_cross++] = uh;
     }
   }
-  if (n_cross == 0) return;
-  __threadfence();
+  if (cross == 0) return;
   __syncthreads();
+  const int x0 = __ffs(cross) - 1, x1 = 31 - __clz(cross), n_cross = __popc(cross);
   if (tid < n_cross) {
-    const uint32_t s = c_begin + (tid ? cross_s[1] : cross_s[0]), n = tid ? cross_n[1] : cross_n[0];
-    const int fst = cut_of.owner(s) / kWarps, lst = cut_of.owner(s + n - 1) / kWarps;
+    __threadfence();                               // the CTA's pieces before the arrival
+    const int4 u = s_cut[tid ? x1 : x0];
+    const uint32_t s = c_begin + u.x;
+    const int fst = cut_of.owner(s) / kWarps, lst = cut_of.owner(s + u.y - 1) / kWarps;
     const uint32_t old = atomicAdd(p.counters + fst, 1u);
     s_last[tid] = old == (uint32_t)(lst - fst);
     if (s_last[tid]) p.counters[fst] = 0;          // zero again for the next call
@@ -652,27 +670,47 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(DecodeParams p) 
   __syncthreads();
   for (int x = 0; x < n_cross; ++x) {
     if (!s_last[x]) continue;
-    const uint32_t s = c_begin + cross_s[x];
-    const int fst = cut_of.owner(s) / kWarps, lst = cut_of.owner(s + cross_n[x] - 1) / kWarps;
-    const int sub = cross_hv[x] % p.subs, h0 = (cross_hv[x] / p.subs) * p.group + sub * 8;
-    const int heads = min(8, p.group - sub * 8), ub = cross_b[x];
-    for (int i = tid; i < 8 * HD; i += kWarps * 32) {
-      const int h = i / HD;
-      if (h >= heads) break;
-      float mm = -INFINITY, ll = 0.f, oo = 0.f;
-      auto part = [&](int c) { return p.parts + ((int64_t)c * 2 + (c == fst ? 1 : 0)) * S::kPiece; };
+    const int4 u = s_cut[x ? x1 : x0];
+    const uint32_t s = c_begin + u.x;
+    const int fst = cut_of.owner(s) / kWarps, lst = cut_of.owner(s + u.y - 1) / kWarps;
+    const int sub = u.w % p.subs, h0 = (u.w / p.subs) * p.group + sub * 8;
+    const int heads = min(8, p.group - sub * 8);
+    auto part = [&](int c) { return p.parts + ((int64_t)c * 2 + (c == fst ? 1 : 0)) * S::kPiece; };
+    for (int h = warp; h < heads; h += kWarps) {
+      float mm = -INFINITY, ll = 0.f, acc[HD / 32] = {};
+      for (int c0 = fst; c0 <= lst; c0 += 32) {    // rounds of 32 pieces, rescaled between them
+        const bool in = c0 + lane <= lst;
+        const float mi = in ? __ldcg(part(c0 + lane) + 8 * HD + h) : -INFINITY;
+        const float li = in ? __ldcg(part(c0 + lane) + 8 * HD + 8 + h) : 0.f;
+        const int n = min(32, lst - c0 + 1);
+        float first4[4][HD / 32];                  // the first four pieces load beside their sums
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int i = 0; i < HD / 32; ++i)
+            first4[k][i] = k < n ? __ldcg(part(c0 + k) + h * HD + lane * (HD / 32) + i) : 0.f;
+        const float m2 = fmaxf(mm, warp_max(mi));
+        const float a = mm == -INFINITY ? 1.f : fast_exp2(mm - m2);
+        const float f = mi == -INFINITY ? 1.f : fast_exp2(mi - m2);
+        mm = m2;
+        ll = ll * a + warp_sum(f * li);
+#pragma unroll
+        for (int i = 0; i < HD / 32; ++i) acc[i] *= a;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float fk = __shfl_sync(0xffffffffu, f, k);
+#pragma unroll
+          for (int i = 0; i < HD / 32; ++i) acc[i] += fk * first4[k][i];
+        }
 #pragma unroll 4
-      for (int c = fst; c <= lst; ++c) mm = fmaxf(mm, __ldcg(part(c) + 8 * HD + h));
-#pragma unroll 4
-      for (int c = fst; c <= lst; ++c) {
-        const float mi = __ldcg(part(c) + 8 * HD + h);
-        const float f = mi == -INFINITY ? 1.f : fast_exp2(mi - mm);
-        ll += f * __ldcg(part(c) + 8 * HD + 8 + h);
-        oo += f * __ldcg(part(c) + i);
+        for (int k = 4; k < n; ++k) {
+          const float fk = __shfl_sync(0xffffffffu, f, k);
+          const float* o_k = part(c0 + k) + h * HD + lane * (HD / 32);
+#pragma unroll
+          for (int i = 0; i < HD / 32; ++i) acc[i] += fk * __ldcg(o_k + i);
+        }
       }
-      ((T*)p.out)[ub * p.out_stride + (int64_t)(h0 + h) * HD + i % HD] = Elem<T>::from_f(oo / ll);
-      if (p.lse && i % HD == 0)
-        p.lse[(int64_t)ub * p.NH + h0 + h] = (mm == -INFINITY ? 0.f : mm - kPScale) * 0.6931471805599453f + logf(ll);
+      store_joined<T, HD>(p, u.z, h0 + h, lane, acc, mm, ll);
     }
   }
 }
