@@ -58,6 +58,16 @@ constexpr int kStages = 2;
 constexpr int kStepBytes = 4608;                 // 64 (D = 64) or 32 tokens of one kv head
 constexpr float kPScale = 14.f;                  // weights are held as 2^14 p
 
+// What the warps of a CTA tell one another.
+struct Shared {
+  uint32_t scan[kWarps];
+  int start[kWarps + 1];             // first tile of every warp, counted from the CTA's
+  // cut units by where their first piece in this CTA is: tail of warp i, or (16) head of warp 0;
+  // x = first tile counted from the CTA's, y = tiles (0: none), z = sequence, w = unit of it
+  int4 cut[kWarps + 1];
+  int2 last[2];                      // first and last CTA of a unit that this CTA joins
+};
+
 template <int HD>
 struct Shape {
   static constexpr int kTiles = kStepBytes / Tile<HD>::kBytes;   // tiles of a step
@@ -66,7 +76,9 @@ struct Shape {
   static constexpr int kPiece = 8 * HD + 16;                     // floats: O, m[8], l[8]
   static constexpr int kRing = kWarps * kStages * kStepBytes;
   static constexpr int kPark = kWarps * kPiece * 4;
-  static size_t smem(int batch) { return kRing + kPark + ((size_t)batch + 1) * 4; }
+  // All of it dynamic, so that the rings begin on a 128-byte line: copies of 8 lanes' 16-byte chunks
+  // that straddle lines cost 165 -> 228 us at 256 x U[8192, 32768].
+  static size_t smem(int batch) { return kRing + kPark + sizeof(Shared) + ((size_t)batch + 1) * 4; }
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
@@ -348,31 +360,164 @@ __device__ __forceinline__ void store_piece(float* dst, int g, int t, const floa
   }
 }
 
-// A joined row: HD/32 dims per lane.
+// Joining pieces takes HD/4 lanes a row, 4 dims each: half a warp or a warp per (unit, head).
+template <int HD>
+struct Row {
+  static constexpr int kLanes = HD / 4, kWarpsPerUnit = 8 * kLanes / 32;
+  int h, j, at;                      // head of the unit, lane of the row, its place in a piece
+  __device__ __forceinline__ Row(int warp, int lane)
+      : h((warp % kWarpsPerUnit) * (32 / kLanes) + lane / kLanes), j(lane % kLanes), at(h * HD + j * 4) {}
+};
+__device__ __forceinline__ void fma4(float4& acc, float c, const float4 v) {
+  acc.x += c * v.x;
+  acc.y += c * v.y;
+  acc.z += c * v.z;
+  acc.w += c * v.w;
+}
 template <typename T, int HD>
-__device__ __forceinline__ void store_joined(const DecodeParams& p, int b, int h, int lane,
-                                             const float (&o)[HD / 32], float m, float l) {
-  T* out = (T*)p.out + b * p.out_stride + (int64_t)h * HD + lane * (HD / 32);
+__device__ __forceinline__ void store_joined(const DecodeParams& p, int b, int h, int j,
+                                             const float4 o, float m, float l) {
   const float r = 1.f / l;
+  *reinterpret_cast<uint2*>((T*)p.out + b * p.out_stride + (int64_t)h * HD + j * 4) =
+      make_uint2(Elem<T>::pack2(o.x * r, o.y * r), Elem<T>::pack2(o.z * r, o.w * r));
+  if (p.lse && j == 0) p.lse[(int64_t)b * p.NH + h] = row_lse(m, l);
+}
+
+// Add to a counter, after this thread's (and, behind a barrier, its CTA's) writes, before its reads.
+__device__ __forceinline__ uint32_t arrive(uint32_t* counter) {
+  uint32_t old;
+  asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(old) : "l"(counter) : "memory");
+  return old;
+}
+
+// Units cut between the warps of this CTA.  Returns the bits of the entries of sh.cut that other CTAs
+// share.  (Out of line: it runs once, and the main loop keeps its registers.)
+template <typename T, int HD>
+__device__ __noinline__ uint32_t join_warps(const DecodeParams& p, Shared& sh, const float* park,
+                                            const float* tails, int cta) {
+  using S = Shape<HD>;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // Lane i (modulo 16) stands for warp i's piece of a unit: parked when the unit began before the
+  // warp's range, else left in the ring.  Positions count from the CTA's first tile; a unit that began
+  // before it has a negative one.
+  static_assert(kWarps == 16, "a piece per lane of half a warp");
+  const Row<HD> row(warp, lane);
+  const int hl = lane & 15, c_len = sh.start[kWarps];
+  const int my_start = sh.start[hl], my_end = sh.start[hl + 1];
+  const int4 entry = lane <= kWarps ? sh.cut[lane] : make_int4(0, 0, 0, 0);
+  uint32_t cuts = __ballot_sync(0xffffffffu, entry.y > 0);
+  const uint32_t cross = __ballot_sync(0xffffffffu, entry.y > 0 && (entry.x < 0 || entry.x + entry.y > c_len));
+  constexpr int kAtOnce = kWarps / Row<HD>::kWarpsPerUnit;
+  for (int i = 0; cuts; ++i, cuts &= cuts - 1) {
+    if (i % kAtOnce != warp / Row<HD>::kWarpsPerUnit) continue;
+    const int4 u = sh.cut[__ffs(cuts) - 1];
+    const int sub = p.subs == 1 ? 0 : u.w % p.subs, kvh = p.subs == 1 ? u.w : u.w / p.subs;
+    const int h0 = kvh * p.group + sub * 8, us = u.x, e = u.x + u.y;
+    const bool has = my_start < my_end && my_start < e && my_end > us;
+    const uint32_t pieces = __ballot_sync(0xffffffffu, has) & 0xFFFFu;
+    const int wa = __ffs(pieces) - 1, wb = 31 - __clz(pieces);
+    // only its first piece can be a tail: the unit reaches into every later warp from the left
+    const float* first = (us < sh.start[wa] ? park : tails) + wa * S::kPiece;
+    const float* src = hl == wa ? first : park + hl * S::kPiece;
+    const float mi = has ? src[8 * HD + row.h] : -INFINITY;
+    const float li = has ? src[8 * HD + 8 + row.h] : 0.f;
+    float mm = mi;
 #pragma unroll
-  for (int i = 0; i < HD / 64; ++i)
-    reinterpret_cast<uint32_t*>(out)[i] = Elem<T>::pack2(o[2 * i] * r, o[2 * i + 1] * r);
-  if (p.lse && lane == 0)
-    p.lse[(int64_t)b * p.NH + h] = row_lse(m, l);
+    for (int d = 8; d > 0; d >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
+    // (a piece without a finite score keeps its sum: zero, or NaN)
+    const float c = mi == -INFINITY ? 1.f : fast_exp2(mi - mm);
+    float ll = c * li;
+#pragma unroll
+    for (int d = 8; d > 0; d >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, d);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int w = wa; w <= wb; ++w) {
+      const float cw = __shfl_sync(0xffffffffu, c, w, 16);
+      if ((pieces >> w) & 1u)                      // (else an empty range)
+        fma4(acc, cw, *reinterpret_cast<const float4*>((w == wa ? first : park + w * S::kPiece) + row.at));
+    }
+    if (row.h >= p.group - sub * 8) continue;
+    if (us >= 0 && e <= c_len) {
+      store_joined<T, HD>(p, u.z, h0 + row.h, row.j, acc, mm, ll);
+    } else {
+      float* ws = p.parts + ((int64_t)cta * 2 + (us < 0 ? 0 : 1)) * S::kPiece;
+      *reinterpret_cast<float4*>(ws + row.at) = acc;
+      if (row.j == 0) {
+        ws[8 * HD + row.h] = mm;
+        ws[8 * HD + 8 + row.h] = ll;
+      }
+    }
+  }
+  return cross;
+}
+
+// Units that other CTAs share: announce this CTA's pieces; the CTA that is the last of a unit joins
+// them, in order.  cross: bits of the entries of sh.cut concerned (one or two).
+template <typename T, int HD>
+__device__ __noinline__ void join_ctas(const DecodeParams& p, Shared& sh, uint32_t cross,
+                                       uint32_t c_begin, Cut cut_of) {
+  using S = Shape<HD>;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hl = lane & 15;
+  __syncthreads();
+  const int x0 = __ffs(cross) - 1, x1 = 31 - __clz(cross), n_cross = __popc(cross);
+  if (tid < n_cross) {
+    const int4 u = sh.cut[tid ? x1 : x0];
+    const uint32_t s = c_begin + u.x;
+    const int fst = cut_of.owner(s) / kWarps, lst = cut_of.owner(s + u.y - 1) / kWarps;
+    const bool last = arrive(p.counters + fst) == (uint32_t)(lst - fst);
+    if (last) p.counters[fst] = 0;                 // zero again for the next call
+    sh.last[tid] = last ? make_int2(fst, lst) : make_int2(-1, -1);
+  }
+  __syncthreads();
+  // the pieces of a unit from all its CTAs, in order
+  const Row<HD> row(warp, lane);
+  const int x = warp / Row<HD>::kWarpsPerUnit;
+  if (x >= n_cross || sh.last[x].x < 0) return;
+  const int4 u = sh.cut[x ? x1 : x0];
+  const int fst = sh.last[x].x, n = sh.last[x].y - fst + 1;
+  const int sub = u.w % p.subs, h0 = (u.w / p.subs) * p.group + sub * 8;
+  // (rows of heads beyond the group were not written: their values are loaded, not used)
+  auto part = [&](int c) { return p.parts + ((int64_t)(fst + c) * 2 + (c == 0 ? 1 : 0)) * S::kPiece; };
+  auto value = [&](int c) { return __ldcg(reinterpret_cast<const float4*>(part(c) + row.at)); };
+  float mm = -INFINITY, ll = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int c0 = 0; c0 < n; c0 += 16) {             // rounds of 16 pieces, rescaled between them
+    const bool in = c0 + hl < n;
+    const float mi = in ? __ldcg(part(c0 + hl) + 8 * HD + row.h) : -INFINITY;
+    const float li = in ? __ldcg(part(c0 + hl) + 8 * HD + 8 + row.h) : 0.f;
+    const int k_n = min(16, n - c0);
+    constexpr int kAhead = 4;                      // pieces whose values load beside the sums
+    float4 v[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) v[k] = k < k_n ? value(c0 + k) : make_float4(0.f, 0.f, 0.f, 0.f);
+    float m2 = mi;
+#pragma unroll
+    for (int d = 8; d > 0; d >>= 1) m2 = fmaxf(m2, __shfl_xor_sync(0xffffffffu, m2, d));
+    m2 = fmaxf(mm, m2);
+    const float a = mm == -INFINITY ? 1.f : fast_exp2(mm - m2);
+    const float f = mi == -INFINITY ? 1.f : fast_exp2(mi - m2);
+    float sum = f * li;
+#pragma unroll
+    for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    mm = m2;
+    ll = ll * a + sum;
+    acc = make_float4(acc.x * a, acc.y * a, acc.z * a, acc.w * a);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) fma4(acc, __shfl_sync(0xffffffffu, f, k, 16), v[k]);
+#pragma unroll 4
+    for (int k = kAhead; k < k_n; ++k) fma4(acc, __shfl_sync(0xffffffffu, f, k, 16), value(c0 + k));
+  }
+  if (row.h < p.group - sub * 8) store_joined<T, HD>(p, u.z, h0 + row.h, row.j, acc, mm, ll);
 }
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(DecodeParams p) {
+__global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const __grid_constant__ DecodeParams p) {
   using S = Shape<HD>;
   using L = Tile<HD>;
   extern __shared__ __align__(128) uint8_t smem[];
   float* park = reinterpret_cast<float*>(smem + S::kRing);
-  uint32_t* pref = reinterpret_cast<uint32_t*>(smem + S::kRing + S::kPark);   // [batch + 1]
-  __shared__ uint32_t s_scan[kWarps + 1];
-  __shared__ int s_last[2], s_start[kWarps + 1];
-  // cut units by where their first piece in this CTA is: tail of warp i, or (16) head of warp 0;
-  // x = first tile counted from the CTA's, y = tiles (0: none), z = sequence, w = unit of it
-  __shared__ int4 s_cut[kWarps + 1];
+  Shared& sh = *reinterpret_cast<Shared*>(smem + S::kRing + S::kPark);
+  uint32_t* pref = reinterpret_cast<uint32_t*>(&sh + 1);                      // [batch + 1]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int units = p.KVH * p.subs;
   pdl_wait();
@@ -399,13 +544,13 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(DecodeParams p) 
         const uint32_t y = __shfl_up_sync(0xffffffffu, x, d);
         if (lane >= d) x += y;
       }
-      if (lane == 31) s_scan[warp] = x;
+      if (lane == 31) sh.scan[warp] = x;
       __syncthreads();
       uint32_t before = carry, all = 0;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) before += s_scan[w];
-        all += s_scan[w];
+        if (w < warp) before += sh.scan[w];
+        all += sh.scan[w];
       }
       if (b < p.batch) pref[b + 1] = before + x;
       carry += all;
@@ -447,10 +592,10 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(DecodeParams p) 
     cur.blk = (int)(r - cur.hv * n);
   }
   if (lane == 0) {
-    s_start[warp] = (int)(w_begin - c_begin);
-    if (warp == kWarps - 1) s_start[kWarps] = (int)(w_begin - c_begin) + cur.left;
-    s_cut[warp] = make_int4(0, 0, 0, 0);
-    if (warp == 0) s_cut[kWarps] = make_int4(0, 0, 0, 0);
+    sh.start[warp] = (int)(w_begin - c_begin);
+    if (warp == kWarps - 1) sh.start[kWarps] = (int)(w_begin - c_begin) + cur.left;
+    sh.cut[warp] = make_int4(0, 0, 0, 0);
+    if (warp == 0) sh.cut[kWarps] = make_int4(0, 0, 0, 0);
   }
 
   float o[HD / 16][4], m[2], l[2];
@@ -589,7 +734,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(DecodeParams p) 
           if (cut) store_piece<HD>(park + warp * S::kPiece, g, t, o, m, l);
           else tail = true;
           if (lane == 0 && (!cut || warp == 0))
-            s_cut[cut ? kWarps : warp] =
+            sh.cut[cut ? kWarps : warp] =
                 make_int4((int)(w_begin - c_begin) + at - ublk, un, ub, uhv);
         }
         first = false;
@@ -605,114 +750,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(DecodeParams p) 
   if (tail) store_piece<HD>(tails + warp * S::kPiece, g, t, o, m, l);
   __syncthreads();
 
-  // Join the cut units of this CTA, one warp per (unit, head).  The piece of a unit in warp w is parked
-  // when the unit began before the warp's range, else it was left in the ring.  Positions count from
-  // the CTA's first tile; a unit that began before it has a negative one.
-  const int c_len = s_start[kWarps];
-  const int my_start = lane < kWarps ? s_start[lane] : 0;
-  const int my_end = lane < kWarps ? s_start[lane + 1] : 0;       // (other lanes: an empty range)
-  const int4 mine = lane <= kWarps ? s_cut[lane] : make_int4(0, 0, 0, 0);
-  uint32_t cuts = __ballot_sync(0xffffffffu, mine.y > 0);
-  const uint32_t cross = __ballot_sync(0xffffffffu, mine.y > 0 && (mine.x < 0 || mine.x + mine.y > c_len));
-  for (int i = 0; cuts; ++i, cuts &= cuts - 1) {
-    if ((i & (kWarps / 8 - 1)) != warp >> 3) continue;            // 8 warps per unit
-    const int4 u = s_cut[__ffs(cuts) - 1];
-    const int sub = p.subs == 1 ? 0 : u.w % p.subs, kvh = p.subs == 1 ? u.w : u.w / p.subs;
-    const int h = warp & 7, h0 = kvh * p.group + sub * 8;
-    if (h >= min(8, p.group - sub * 8)) continue;
-    const int us = u.x, e = u.x + u.y;
-    const bool has = my_start < my_end && my_start < e && my_end > us;
-    const uint32_t pieces = __ballot_sync(0xffffffffu, has);
-    const float* src = (us < my_start ? park : tails) + lane * S::kPiece;
-    const float mi = has ? src[8 * HD + h] : -INFINITY;
-    const float li = has ? src[8 * HD + 8 + h] : 0.f;
-    const int wa = __ffs(pieces) - 1, wb = 31 - __clz(pieces);
-    const bool first_parked = us < s_start[wa];
-    const float mm = warp_max(mi);
-    // (a piece without a finite score keeps its sum: zero, or NaN)
-    const float c = mi == -INFINITY ? 1.f : fast_exp2(mi - mm);
-    const float ll = warp_sum(c * li);
-    float acc[HD / 32] = {};
-#pragma unroll 4
-    for (int w = wa; w <= wb; ++w) {
-      const float cw = __shfl_sync(0xffffffffu, c, w);
-      // only its first piece can be a tail: the unit reaches into every later warp from the left
-      const float* o_w = (w == wa && !first_parked ? tails : park) + w * S::kPiece + h * HD + lane * (HD / 32);
-#pragma unroll
-      for (int k = 0; k < HD / 32; ++k)
-        if ((pieces >> w) & 1u) acc[k] += cw * o_w[k];
-    }
-    if (us >= 0 && e <= c_len) {
-      store_joined<T, HD>(p, u.z, h0 + h, lane, acc, mm, ll);
-    } else {
-      float* ws = p.parts + ((int64_t)cta * 2 + (us < 0 ? 0 : 1)) * S::kPiece;
-#pragma unroll
-      for (int k = 0; k < HD / 32; ++k) ws[h * HD + lane * (HD / 32) + k] = acc[k];
-      if (lane == 0) {
-        ws[8 * HD + h] = mm;
-        ws[8 * HD + 8 + h] = ll;
-      }
-    }
-  }
-  if (cross == 0) return;
-  __syncthreads();
-  const int x0 = __ffs(cross) - 1, x1 = 31 - __clz(cross), n_cross = __popc(cross);
-  if (tid < n_cross) {
-    __threadfence();                               // the CTA's pieces before the arrival
-    const int4 u = s_cut[tid ? x1 : x0];
-    const uint32_t s = c_begin + u.x;
-    const int fst = cut_of.owner(s) / kWarps, lst = cut_of.owner(s + u.y - 1) / kWarps;
-    const uint32_t old = atomicAdd(p.counters + fst, 1u);
-    s_last[tid] = old == (uint32_t)(lst - fst);
-    if (s_last[tid]) p.counters[fst] = 0;          // zero again for the next call
-    __threadfence();
-  }
-  __syncthreads();
-  for (int x = 0; x < n_cross; ++x) {
-    if (!s_last[x]) continue;
-    const int4 u = s_cut[x ? x1 : x0];
-    const uint32_t s = c_begin + u.x;
-    const int fst = cut_of.owner(s) / kWarps, lst = cut_of.owner(s + u.y - 1) / kWarps;
-    const int sub = u.w % p.subs, h0 = (u.w / p.subs) * p.group + sub * 8;
-    const int heads = min(8, p.group - sub * 8);
-    auto part = [&](int c) { return p.parts + ((int64_t)c * 2 + (c == fst ? 1 : 0)) * S::kPiece; };
-    for (int h = warp; h < heads; h += kWarps) {
-      float mm = -INFINITY, ll = 0.f, acc[HD / 32] = {};
-      for (int c0 = fst; c0 <= lst; c0 += 32) {    // rounds of 32 pieces, rescaled between them
-        const bool in = c0 + lane <= lst;
-        const float mi = in ? __ldcg(part(c0 + lane) + 8 * HD + h) : -INFINITY;
-        const float li = in ? __ldcg(part(c0 + lane) + 8 * HD + 8 + h) : 0.f;
-        const int n = min(32, lst - c0 + 1);
-        float first4[4][HD / 32];                  // the first four pieces load beside their sums
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-#pragma unroll
-          for (int i = 0; i < HD / 32; ++i)
-            first4[k][i] = k < n ? __ldcg(part(c0 + k) + h * HD + lane * (HD / 32) + i) : 0.f;
-        const float m2 = fmaxf(mm, warp_max(mi));
-        const float a = mm == -INFINITY ? 1.f : fast_exp2(mm - m2);
-        const float f = mi == -INFINITY ? 1.f : fast_exp2(mi - m2);
-        mm = m2;
-        ll = ll * a + warp_sum(f * li);
-#pragma unroll
-        for (int i = 0; i < HD / 32; ++i) acc[i] *= a;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float fk = __shfl_sync(0xffffffffu, f, k);
-#pragma unroll
-          for (int i = 0; i < HD / 32; ++i) acc[i] += fk * first4[k][i];
-        }
-#pragma unroll 4
-        for (int k = 4; k < n; ++k) {
-          const float fk = __shfl_sync(0xffffffffu, f, k);
-          const float* o_k = part(c0 + k) + h * HD + lane * (HD / 32);
-#pragma unroll
-          for (int i = 0; i < HD / 32; ++i) acc[i] += fk * __ldcg(o_k + i);
-        }
-      }
-      store_joined<T, HD>(p, u.z, h0 + h, lane, acc, mm, ll);
-    }
-  }
+  const uint32_t cross = join_warps<T, HD>(p, sh, park, tails, cta);
+  if (cross) join_ctas<T, HD>(p, sh, cross, c_begin, cut_of);
 }
 
 // The HD/32 dims lane `lane` holds of one token's codes (a 32-bit word serves 256 / HD lanes).
