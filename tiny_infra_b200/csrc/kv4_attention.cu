@@ -54,7 +54,7 @@ struct DecodeParams {
 
 constexpr int kMaxBatch = 4096;
 constexpr int kWarps = 16;
-constexpr int kStages = 2;
+constexpr int kStages = 2;                       // (the code below counts on two)
 constexpr int kStepBytes = 4608;                 // 64 (D = 64) or 32 tokens of one kv head
 constexpr float kPScale = 14.f;                  // weights are held as 2^14 p
 
@@ -123,16 +123,15 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
   return d;
 }
 
-// Where a warp stands in the stream of tiles.
+// Where a warp stands in the stream of tiles: at tile blk of unit hv of sequence b, whose units have n
+// tiles; `left` more tiles are its own.
 struct Cursor {
-  int b, hv, blk, n;                 // sequence, unit within it, tile of the unit, tiles of a unit
-  int left;                          // tiles left in the warp's range
-  __device__ __forceinline__ int step(int most) const { return min(min(most, n - blk), left); }
-  // Past k tiles; pref[b] = tiles of one unit of the sequences before b.
-  __device__ __forceinline__ void advance(int k, int units, const uint32_t* pref, int batch) {
-    blk += k;
-    left -= k;
-    if (blk < n || left == 0) return;
+  int b, hv, blk, n, left;
+  __device__ __forceinline__ int piece() const { return min(n - blk, left); }
+  // To the next unit; pref[b] = tiles of one unit of the sequences before b.
+  __device__ __forceinline__ void next_unit(int units, const uint32_t* pref, int batch) {
+    left -= piece();
+    if (left == 0) return;
     blk = 0;
     if (++hv < units) return;
     hv = 0;
@@ -391,9 +390,9 @@ __device__ __forceinline__ uint32_t arrive(uint32_t* counter) {
 }
 
 // Units cut between the warps of this CTA.  Returns the bits of the entries of sh.cut that other CTAs
-// share.  (Out of line: it runs once, and the main loop keeps its registers.)
+// share.
 template <typename T, int HD>
-__device__ __noinline__ uint32_t join_warps(const DecodeParams& p, Shared& sh, const float* park,
+__device__ __forceinline__ uint32_t join_warps(const DecodeParams& p, Shared& sh, const float* park,
                                             const float* tails, int cta) {
   using S = Shape<HD>;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -454,7 +453,7 @@ __device__ __noinline__ uint32_t join_warps(const DecodeParams& p, Shared& sh, c
 // Units that other CTAs share: announce this CTA's pieces; the CTA that is the last of a unit joins
 // them, in order.  cross: bits of the entries of sh.cut concerned (one or two).
 template <typename T, int HD>
-__device__ __noinline__ void join_ctas(const DecodeParams& p, Shared& sh, uint32_t cross,
+__device__ __forceinline__ void join_ctas(const DecodeParams& p, Shared& sh, uint32_t cross,
                                        uint32_t c_begin, Cut cut_of) {
   using S = Shape<HD>;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hl = lane & 15;
@@ -603,33 +602,38 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const __grid_con
   const bool head_cut = cur.blk > 0;               // the first unit began before this warp
   if (cur.left > 0) {
     const uint32_t ring = smem_u32(smem) + warp * (kStages * kStepBytes);
+    // copies run one step ahead of the arithmetic, the block ids one step ahead of the copies
     const int j = lane / S::kLanes;
     const CopyLane<HD> mine(lane % S::kLanes);
+    const uint32_t my_tile = ring + j * L::kBytes;
+    const uint32_t num_blocks = (uint32_t)min(p.num_blocks, (int64_t)0x7FFFFFFF);
+    const int64_t block_bytes = (int64_t)p.KVH * L::kBytes;
     Cursor ld = cur;
-    uint32_t have = 0;                             // which tiles of the steps in flight exist
-    int issued = 0;
-    auto next_id = [&]() -> int {
-      if (j >= ld.step(S::kTiles)) return -1;
+    int ld_left = 0, ld_stage = 0, id = -1;
+    const int32_t* ids = nullptr;
+    const uint8_t* pool_h = nullptr;
+    auto open_loads = [&]() {
       const int row = p.row_index ? p.row_index[ld.b] : ld.b;
-      return p.tables[(int64_t)row * p.bt_stride + ld.blk + j];
+      ids = p.tables + (int64_t)row * p.bt_stride + ld.blk + j;
+      pool_h = p.pool + (int64_t)(p.subs == 1 ? ld.hv : ld.hv / p.subs) * L::kBytes;
+      ld_left = ld.piece();
     };
-    int id = next_id();
-    auto issue = [&]() {
-      const bool ok = id >= 0 && id < p.num_blocks;
-      if (ok) {
-        const int kvh = p.subs == 1 ? ld.hv : ld.hv / p.subs;
-        mine.copy(ring + (issued & (kStages - 1)) * kStepBytes + j * L::kBytes,
-                  p.pool + ((int64_t)id * p.KVH + kvh) * L::kBytes);
-      }
+    open_loads();
+    id = j < ld_left ? *ids : -1;
+    // start the next step's copies; returns which of its tiles exist (bits of S::kFirsts)
+    auto issue = [&]() -> uint32_t {
+      const bool ok = (uint32_t)id < num_blocks;
+      if (ok) mine.copy(my_tile + ld_stage, pool_h + id * block_bytes);
       cp_commit();
-      // one bit per tile at its first lane's place; a step's bits in the half it was issued to
-      const uint32_t bal = __ballot_sync(0xffffffffu, ok) & S::kFirsts;
-      have = (issued & 1) ? (have & S::kFirsts) | (bal << 1) : (have & (S::kFirsts << 1)) | bal;
-      ++issued;
-      if (ld.left > 0) {
-        ld.advance(ld.step(S::kTiles), units, pref, p.batch);
-        id = ld.left > 0 ? next_id() : -1;
+      ld_stage = kStepBytes - ld_stage;
+      ids += S::kTiles;
+      ld_left -= S::kTiles;
+      if (ld_left <= 0 && ld.left > 0) {
+        ld.next_unit(units, pref, p.batch);
+        if (ld.left > 0) open_loads();
       }
+      id = j < ld_left ? *ids : -1;
+      return __ballot_sync(0xffffffffu, ok) & S::kFirsts;
     };
     uint32_t qf[HD / 16][2];
     float2 sc = make_float2(0.f, 0.f);
@@ -647,7 +651,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const __grid_con
       l[0] = l[1] = 0.f;
     };
     open_unit();                                   // (its loads and the first block id's overlap)
-    issue();
+    uint32_t ok_next = issue();
     const int total_left = cur.left;
     bool first = true;
     // one step: full = all tiles exist and all their tokens are within the length
@@ -706,41 +710,37 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const __grid_con
                               live - x * kBlock, pt, o);
       }
     };
-    for (int it = 0;; ++it) {
-      issue();                                     // (an empty group when nothing is left)
-      cp_wait<kStages - 1>();
-      __syncwarp();
-      const int k = cur.step(S::kTiles);
-      const uint32_t st = ring + (it & (kStages - 1)) * kStepBytes;
-      const uint32_t ok = ((it & 1) ? have >> 1 : have) & S::kFirsts;
-      const int live = ctx - cur.blk * kBlock;     // tokens from this step's first on
-      if (ok == S::kFirsts && live >= S::kTiles * kBlock) run_step(std::true_type{}, st, ok, live);
-      else run_step(std::false_type{}, st, ok, live);
-      __syncwarp();                                // the stage is free for the copies after next
-      const int ub = cur.b, uhv = cur.hv, ublk = cur.blk, un = cur.n;
-      const int at = total_left - cur.left;        // this step's place in the warp's range
-      const bool done = cur.blk + k == cur.n;      // the unit's last tile
-      cur.advance(k, units, pref, p.batch);
-      if (done || cur.left == 0) {
-#pragma unroll
-        for (int d = 4; d < 32; d <<= 1) {
-          l[0] += __shfl_xor_sync(0xffffffffu, l[0], d);
-          l[1] += __shfl_xor_sync(0xffffffffu, l[1], d);
-        }
-        const bool cut = first && head_cut;
-        if (done && !cut) {
-          store_rows<T, HD>(p, ub, h0, heads, g, t, o, m, l);
-        } else {
-          if (cut) store_piece<HD>(park + warp * S::kPiece, g, t, o, m, l);
-          else tail = true;
-          if (lane == 0 && (!cut || warp == 0))
-            sh.cut[cut ? kWarps : warp] =
-                make_int4((int)(w_begin - c_begin) + at - ublk, un, ub, uhv);
-        }
-        first = false;
-        if (cur.left == 0) break;
-        open_unit();
+    for (uint32_t st = ring;;) {                   // one unit's tiles
+      int live = ctx - cur.blk * kBlock;           // its tokens from the step's first on
+      for (int rem = cur.piece(); rem > 0; rem -= S::kTiles, live -= S::kTiles * kBlock) {
+        const uint32_t ok = ok_next;
+        ok_next = issue();                         // (an empty group when nothing is left)
+        cp_wait<1>();
+        __syncwarp();
+        if (ok == S::kFirsts && live >= S::kTiles * kBlock) run_step(std::true_type{}, st, ok, live);
+        else run_step(std::false_type{}, st, ok, live);
+        __syncwarp();                              // the stage is free for the copies after next
+        st = 2 * ring + kStepBytes - st;
       }
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) {
+        l[0] += __shfl_xor_sync(0xffffffffu, l[0], d);
+        l[1] += __shfl_xor_sync(0xffffffffu, l[1], d);
+      }
+      const bool cut = first && head_cut;
+      if (cur.n - cur.blk <= cur.left && !cut) {   // the unit whole
+        store_rows<T, HD>(p, cur.b, h0, heads, g, t, o, m, l);
+      } else {
+        if (cut) store_piece<HD>(park + warp * S::kPiece, g, t, o, m, l);
+        else tail = true;
+        if (lane == 0 && (!cut || warp == 0))
+          sh.cut[cut ? kWarps : warp] = make_int4(
+              (int)(w_begin - c_begin) + total_left - cur.left - cur.blk, cur.n, cur.b, cur.hv);
+      }
+      first = false;
+      cur.next_unit(units, pref, p.batch);
+      if (cur.left == 0) break;
+      open_unit();
     }
     cp_wait<0>();
   }
