@@ -46,7 +46,6 @@ struct DecodeParams {
   const int32_t *tables, *row_index, *ctx;
   int batch, NH, KVH, group, max_blocks;
   int subs;                          // groups of at most 8 query heads per kv head
-  int unit_mode;                     // one CTA per unit instead of the even cut
   float scale_log2;
   uint32_t* counters;                // [gridDim.x], zero between calls
   float* parts;                      // [gridDim.x][2] pieces
@@ -61,9 +60,9 @@ constexpr float kPScale = 14.f;                  // weights are held as 2^14 p
 // What the warps of a CTA tell one another.
 struct Shared {
   uint32_t scan[kWarps];
-  int start[kWarps + 1];             // first tile of every warp, counted from the CTA's
+  int start[kWarps + 1];             // first grain of every warp, counted from the CTA's
   // cut units by where their first piece in this CTA is: tail of warp i, or (16) head of warp 0;
-  // x = first tile counted from the CTA's, y = tiles (0: none), z = sequence, w = unit of it
+  // x = first grain counted from the CTA's, y = grains (0: none), z = sequence, w = unit of it
   int4 cut[kWarps + 1];
   int2 last[2];                      // first and last CTA of a unit that this CTA joins
 };
@@ -123,69 +122,86 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
   return d;
 }
 
-// Where a warp stands in the stream of tiles: at tile blk of unit hv of sequence b, whose units have n
-// tiles; `left` more tiles are its own.
+// Where a warp stands in the stream.  The stream is cut at grains: whole steps (the last one of a unit
+// may be short), or tiles where a CTA has one unit.  A warp is at grain `at` of unit hv of sequence b,
+// whose units have n grains, the last one of `tail` tiles; `left` more grains are its own.
 struct Cursor {
-  int b, hv, blk, n, left;
-  __device__ __forceinline__ int piece() const { return min(n - blk, left); }
-  // To the next unit; pref[b] = tiles of one unit of the sequences before b.
+  int b, hv, at, n, tail, left;
+  __device__ __forceinline__ int piece() const { return min(n - at, left); }
+  __device__ __forceinline__ int piece_tiles(int grain) const {
+    const int k = piece();
+    return at + k == n ? (k - 1) * grain + tail : k * grain;
+  }
+  // Grains of a unit of sequence b; pref[b] = those of the sequences before b, times 4, plus tail - 1.
+  __device__ __forceinline__ void look_up(const uint32_t* pref) {
+    n = (int)((pref[b + 1] >> 2) - (pref[b] >> 2));
+    tail = (int)(pref[b] & 3u) + 1;
+  }
   __device__ __forceinline__ void next_unit(int units, const uint32_t* pref, int batch) {
     left -= piece();
     if (left == 0) return;
-    blk = 0;
+    at = 0;
     if (++hv < units) return;
     hv = 0;
-    do ++b; while (b < batch && pref[b + 1] == pref[b]);
-    if (b < batch) n = (int)(pref[b + 1] - pref[b]);
+    do {
+      ++b;
+      look_up(pref);
+    } while (n == 0 && b < batch - 1);
   }
 };
 
-// An even cut of `total` tiles over `n` warps: the first `rem` warps take one tile more.
+// An even cut of `total` grains over `n` warps: the first `rem` warps take one more.
 struct Cut {
   uint32_t quot, rem;
   __device__ __forceinline__ Cut(uint32_t total, uint32_t n) : quot(total / n), rem(total - quot * n) {}
   __device__ __forceinline__ uint32_t start(uint32_t w) const { return w * quot + min(w, rem); }
-  __device__ __forceinline__ uint32_t owner(uint32_t tile) const {
+  __device__ __forceinline__ uint32_t owner(uint32_t pos) const {
     const uint32_t big = rem * (quot + 1);
-    return tile < big ? tile / (quot + 1) : rem + (tile - big) / quot;
+    return pos < big ? pos / (quot + 1) : rem + (pos - big) / quot;
   }
 };
 
-// Query rows of a unit as the B operand: q[s][0..1] hold dims D/4 * t + 4 s + {0,1,2,3} of head g.
-// Returns the factor that the rows of heads 2t and 2t+1 were multiplied by, inverted.
+// Query rows of a unit: lane (g, t) holds dims D/4 * t ... of head g (zeros beyond the unit's heads).
 template <typename T, int HD>
-__device__ __forceinline__ float2 load_query(const T* q, int heads, int g, int t,
-                                             uint32_t (&f)[HD / 16][2]) {
+__device__ __forceinline__ void load_query(const T* q, int heads, int g, int t, uint4 (&raw)[HD / 32]) {
   constexpr int N = HD / 4;                      // dims of a lane
+#pragma unroll
+  for (int i = 0; i < N / 8; ++i) {
+    raw[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (g < heads) raw[i] = *reinterpret_cast<const uint4*>(q + (int64_t)g * HD + t * N + i * 8);
+  }
+}
+// ... as the B operand: f[s][0..1] hold dims D/4 * t + 4 s + {0,1,2,3} of head g.  Returns the factor
+// that the rows of heads 2t and 2t+1 were multiplied by, inverted.
+template <typename T, int HD>
+__device__ __forceinline__ float2 convert_query(const uint4 (&raw4)[HD / 32], int t, uint32_t (&f)[HD / 16][2]) {
+  constexpr int N = HD / 4;
   uint32_t raw[N / 2];
 #pragma unroll
   for (int i = 0; i < N / 8; ++i) {
-    uint4 u = make_uint4(0u, 0u, 0u, 0u);
-    if (g < heads) u = *reinterpret_cast<const uint4*>(q + (int64_t)g * HD + t * N + i * 8);
-    raw[4 * i] = u.x;
-    raw[4 * i + 1] = u.y;
-    raw[4 * i + 2] = u.z;
-    raw[4 * i + 3] = u.w;
+    raw[4 * i] = raw4[i].x;
+    raw[4 * i + 1] = raw4[i].y;
+    raw[4 * i + 2] = raw4[i].z;
+    raw[4 * i + 3] = raw4[i].w;
   }
-  float inv = 1.f;
   if constexpr (std::is_same<T, __half>::value) {
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) f[i / 2][i % 2] = raw[i];
-  } else {
-    uint32_t top = 0;                            // largest magnitude's bits (as bf16)
+    return make_float2(1.f, 1.f);
+  }
+  uint32_t top = 0;                              // largest magnitude's bits (as bf16)
 #pragma unroll
-    for (int i = 0; i < N / 2; ++i) top = max(top, max(raw[i] & 0x7FFFu, (raw[i] >> 16) & 0x7FFFu));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    // exponent field of the largest, between what keeps both factors normal numbers
-    const int e = min(max((int)(top >> 7), 15), 254);
-    const float mul = __uint_as_float((uint32_t)(254 + 14 - e) << 23);   // 2^(14 - (e - 127))
-    inv = __uint_as_float((uint32_t)(e - 14) << 23);
+  for (int i = 0; i < N / 2; ++i) top = max(top, max(raw[i] & 0x7FFFu, (raw[i] >> 16) & 0x7FFFu));
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  // exponent field of the largest, between what keeps both factors normal numbers
+  const int e = min(max((int)(top >> 7), 15), 254);
+  const float mul = __uint_as_float((uint32_t)(254 + 14 - e) << 23);   // 2^(14 - (e - 127))
+  const float inv = __uint_as_float((uint32_t)(e - 14) << 23);
 #pragma unroll
-    for (int i = 0; i < N / 2; ++i) {
-      const float2 v = Elem<T>::unpack2(raw[i]);
-      f[i / 2][i % 2] = Elem<__half>::pack2(v.x * mul, v.y * mul);
-    }
+  for (int i = 0; i < N / 2; ++i) {
+    const float2 v = Elem<T>::unpack2(raw[i]);
+    f[i / 2][i % 2] = Elem<__half>::pack2(v.x * mul, v.y * mul);
   }
   return make_float2(__shfl_sync(0xffffffffu, inv, 8 * t), __shfl_sync(0xffffffffu, inv, 8 * t + 4));
 }
@@ -509,7 +525,8 @@ __device__ __forceinline__ void join_ctas(const DecodeParams& p, Shared& sh, uin
   if (row.h < p.group - sub * 8) store_joined<T, HD>(p, u.z, h0 + row.h, row.j, acc, mm, ll);
 }
 
-template <typename T, int HD>
+// UNIT: one CTA per unit instead of the even cut.
+template <typename T, int HD, bool UNIT>
 __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const __grid_constant__ DecodeParams p) {
   using S = Shape<HD>;
   using L = Tile<HD>;
@@ -522,22 +539,25 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const __grid_con
   pdl_wait();
   pdl_launch_dependents();
 
-  // pref[b] = tiles of one unit of the sequences before b (in unit mode: only this CTA's sequence)
+  // the grains of the batch (in unit mode: of this CTA's sequence)
   const int cap = (int)min((int64_t)p.max_blocks * kBlock, (int64_t)0x7FFFFFFF);
+  constexpr int grain = UNIT ? 1 : S::kTiles;      // tiles
   auto tiles_of = [&](int b) {
     const int n = min(p.ctx[b], cap);
-    return n > 0 ? (uint32_t)((n - 1) / kBlock + 1) : 0u;
+    return n > 0 ? (n - 1) / kBlock + 1 : 0;
   };
   uint32_t total;
   int ctas;
-  if (p.unit_mode) {
+  if constexpr (UNIT) {
     ctas = 1;
     total = tiles_of(blockIdx.x / units);
   } else {
     uint32_t carry = 0;
     for (int b0 = 0; b0 < p.batch; b0 += kWarps * 32) {
       const int b = b0 + tid;
-      uint32_t x = b < p.batch ? tiles_of(b) : 0u;
+      const int tiles = b < p.batch ? tiles_of(b) : 0;
+      const uint32_t n = (tiles + S::kTiles - 1) / S::kTiles;
+      uint32_t x = n;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
         const uint32_t y = __shfl_up_sync(0xffffffffu, x, d);
@@ -551,17 +571,16 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const __grid_con
         if (w < warp) before += sh.scan[w];
         all += sh.scan[w];
       }
-      if (b < p.batch) pref[b + 1] = before + x;
+      if (b < p.batch) pref[b] = (before + x - n) * 4u + (uint32_t)(tiles + S::kTiles - 1) % S::kTiles;
       carry += all;
+      if (tid == 0) pref[p.batch] = carry * 4u;
       __syncthreads();
     }
-    if (tid == 0) pref[0] = 0;
-    __syncthreads();
     total = carry * (uint32_t)units;
-    // at least two tiles per warp: fewer CTAs for little work, and fewer units cut
-    ctas = min((int)gridDim.x, (int)((total + 2 * kWarps - 1) / (2 * kWarps)));
+    // at least one step per warp: fewer CTAs for little work
+    ctas = min((int)gridDim.x, (int)((total + kWarps - 1) / kWarps));
   }
-  const int cta = p.unit_mode ? 0 : blockIdx.x;
+  const int cta = UNIT ? 0 : blockIdx.x;
   if (total == 0 || cta >= ctas) return;
   const Cut cut_of(total, (uint32_t)ctas * kWarps);
   const uint32_t c_begin = cut_of.start(cta * kWarps);
@@ -569,26 +588,27 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const __grid_con
 
   Cursor cur;
   cur.left = (int)(cut_of.start(cta * kWarps + warp + 1) - w_begin);
-  if (p.unit_mode) {
+  if constexpr (UNIT) {
     cur.b = blockIdx.x / units;
     cur.hv = blockIdx.x % units;
     cur.n = (int)total;
-    cur.blk = (int)w_begin;
+    cur.tail = 1;
+    cur.at = (int)w_begin;
   } else {
-    // last b with pref[b] * units <= w_begin: 32 probes at a time
+    // last b with (grains before b) * units <= w_begin: 32 probes at a time
     int lo = 0, len = p.batch;                     // the answer is in [lo, lo + len)
     while (len > 1) {
       const int step = (len + 31) / 32, probe = lo + lane * step;
-      const uint32_t ok = __ballot_sync(0xffffffffu, lane * step < len && pref[min(probe, p.batch)] * (uint32_t)units <= w_begin);
+      const uint32_t ok = __ballot_sync(0xffffffffu, lane * step < len && (pref[min(probe, p.batch)] >> 2) * (uint32_t)units <= w_begin);
       const int k = 31 - __clz(ok);
       lo += k * step;
       len = min(step, len - k * step);
     }
     cur.b = lo;
-    cur.n = (int)(pref[lo + 1] - pref[lo]);
-    const uint32_t r = w_begin - pref[lo] * (uint32_t)units, n = max(cur.n, 1);
+    cur.look_up(pref);
+    const uint32_t r = w_begin - (pref[lo] >> 2) * (uint32_t)units, n = max(cur.n, 1);
     cur.hv = (int)(r / n);
-    cur.blk = (int)(r - cur.hv * n);
+    cur.at = (int)(r - cur.hv * n);
   }
   if (lane == 0) {
     sh.start[warp] = (int)(w_begin - c_begin);
@@ -599,7 +619,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const __grid_con
 
   float o[HD / 16][4], m[2], l[2];
   bool tail = false;                               // a piece is left in registers after the loop
-  const bool head_cut = cur.blk > 0;               // the first unit began before this warp
+  const bool head_cut = cur.at > 0;               // the first unit began before this warp
   if (cur.left > 0) {
     const uint32_t ring = smem_u32(smem) + warp * (kStages * kStepBytes);
     // copies run one step ahead of the arithmetic, the block ids one step ahead of the copies
@@ -614,9 +634,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const __grid_con
     const uint8_t* pool_h = nullptr;
     auto open_loads = [&]() {
       const int row = p.row_index ? p.row_index[ld.b] : ld.b;
-      ids = p.tables + (int64_t)row * p.bt_stride + ld.blk + j;
+      ids = p.tables + (int64_t)row * p.bt_stride + (int64_t)ld.at * grain + j;
       pool_h = p.pool + (int64_t)(p.subs == 1 ? ld.hv : ld.hv / p.subs) * L::kBytes;
-      ld_left = ld.piece();
+      ld_left = ld.piece_tiles(grain);
     };
     open_loads();
     id = j < ld_left ? *ids : -1;
@@ -628,7 +648,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const __grid_con
       ld_stage = kStepBytes - ld_stage;
       ids += S::kTiles;
       ld_left -= S::kTiles;
-      if (ld_left <= 0 && ld.left > 0) {
+      if (!UNIT && ld_left <= 0 && ld.left > 0) {
         ld.next_unit(units, pref, p.batch);
         if (ld.left > 0) open_loads();
       }
@@ -638,20 +658,25 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const __grid_con
     uint32_t qf[HD / 16][2];
     float2 sc = make_float2(0.f, 0.f);
     int ctx = 0, heads = 0, h0 = 0;
-    auto open_unit = [&]() {
+    uint4 raw[HD / 32];
+    auto load_unit = [&]() {
       const int kvh = cur.hv / p.subs, sub = cur.hv % p.subs;
       h0 = kvh * p.group + sub * 8;
       heads = min(8, p.group - sub * 8);
       ctx = min(p.ctx[cur.b], cap);
-      const float2 inv = load_query<T, HD>((const T*)p.q + cur.b * p.q_stride + (int64_t)h0 * HD, heads, g, t, qf);
+      load_query<T, HD>((const T*)p.q + cur.b * p.q_stride + (int64_t)h0 * HD, heads, g, t, raw);
+    };
+    auto open_unit = [&]() {
+      const float2 inv = convert_query<T, HD>(raw, t, qf);
       sc = make_float2(inv.x * p.scale_log2, inv.y * p.scale_log2);
 #pragma unroll
       for (int i = 0; i < HD / 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
       m[0] = m[1] = -INFINITY;
       l[0] = l[1] = 0.f;
     };
-    open_unit();                                   // (its loads and the first block id's overlap)
+    load_unit();                                   // (in flight beside the first block ids)
     uint32_t ok_next = issue();
+    open_unit();
     const int total_left = cur.left;
     bool first = true;
     // one step: full = all tiles exist and all their tokens are within the length
@@ -711,8 +736,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const __grid_con
       }
     };
     for (uint32_t st = ring;;) {                   // one unit's tiles
-      int live = ctx - cur.blk * kBlock;           // its tokens from the step's first on
-      for (int rem = cur.piece(); rem > 0; rem -= S::kTiles, live -= S::kTiles * kBlock) {
+      int live = ctx - cur.at * grain * kBlock;    // its tokens from the step's first on
+      for (int rem = cur.piece_tiles(grain); rem > 0; rem -= S::kTiles, live -= S::kTiles * kBlock) {
         const uint32_t ok = ok_next;
         ok_next = issue();                         // (an empty group when nothing is left)
         cp_wait<1>();
@@ -728,18 +753,20 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const __grid_con
         l[1] += __shfl_xor_sync(0xffffffffu, l[1], d);
       }
       const bool cut = first && head_cut;
-      if (cur.n - cur.blk <= cur.left && !cut) {   // the unit whole
+      if (cur.n - cur.at <= cur.left && !cut) {   // the unit whole
         store_rows<T, HD>(p, cur.b, h0, heads, g, t, o, m, l);
       } else {
         if (cut) store_piece<HD>(park + warp * S::kPiece, g, t, o, m, l);
         else tail = true;
         if (lane == 0 && (!cut || warp == 0))
           sh.cut[cut ? kWarps : warp] = make_int4(
-              (int)(w_begin - c_begin) + total_left - cur.left - cur.blk, cur.n, cur.b, cur.hv);
+              (int)(w_begin - c_begin) + total_left - cur.left - cur.at, cur.n, cur.b, cur.hv);
       }
       first = false;
+      if constexpr (UNIT) break;
       cur.next_unit(units, pref, p.batch);
       if (cur.left == 0) break;
+      load_unit();
       open_unit();
     }
     cp_wait<0>();
@@ -751,7 +778,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const __grid_con
   __syncthreads();
 
   const uint32_t cross = join_warps<T, HD>(p, sh, park, tails, cta);
-  if (cross) join_ctas<T, HD>(p, sh, cross, c_begin, cut_of);
+  if constexpr (!UNIT)
+    if (cross) join_ctas<T, HD>(p, sh, cross, c_begin, cut_of);
 }
 
 // The HD/32 dims lane `lane` holds of one token's codes (a 32-bit word serves 256 / HD lanes).
@@ -828,14 +856,14 @@ static int decode_ctas() {
   return std::min(sms, kMaxCtas);
 }
 
-template <typename T, int HD>
+template <typename T, int HD, bool UNIT>
 static int launch_decode(const DecodeParams& p, dim3 grid, cudaStream_t s) {
   static std::atomic<uint64_t> ready{0};         // devices whose limit has been raised
   int dev = 0;
   cudaGetDevice(&dev);
   const uint64_t bit = 1ull << (dev & 63);
   if (!(ready.load(std::memory_order_acquire) & bit)) {
-    cudaError_t e = cudaFuncSetAttribute(decode_kernel<T, HD>,
+    cudaError_t e = cudaFuncSetAttribute(decode_kernel<T, HD, UNIT>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          (int)Shape<HD>::smem(kMaxBatch));
     if (e != cudaSuccess) {
@@ -844,8 +872,8 @@ static int launch_decode(const DecodeParams& p, dim3 grid, cudaStream_t s) {
     }
     ready.fetch_or(bit, std::memory_order_release);
   }
-  return launch_kernel("kv4 attention launch", decode_kernel<T, HD>, grid, dim3(kWarps * 32),
-                       Shape<HD>::smem(p.unit_mode ? 0 : p.batch), s, 1, p);
+  return launch_kernel("kv4 attention launch", decode_kernel<T, HD, UNIT>, grid, dim3(kWarps * 32),
+                       Shape<HD>::smem(UNIT ? 0 : p.batch), s, 1, p);
 }
 
 static int check_shape(int batch, int NH, int KVH, int HD, int block_size,
@@ -904,16 +932,22 @@ extern "C" int ti_kv4_attention_decode(void* out, int64_t out_seq_stride, float*
   const bool unit_mode = units <= ctas && max_blocks_per_seq <= kv4::kUnitBlocks;
   kv4::DecodeParams p{out, lse, q, (const uint8_t*)pool, out_seq_stride, q_seq_stride, num_blocks,
                       bt_stride, block_tables, row_index, context_lens, batch, num_heads,
-                      num_kv_heads, group, max_blocks_per_seq, subs, unit_mode,
+                      num_kv_heads, group, max_blocks_per_seq, subs,
                       1.4426950408889634f / sqrtf((float)head_dim), (uint32_t*)workspace,
                       (float*)((uint8_t*)workspace + kv4::kCounterBytes)};
   const dim3 grid(unit_mode ? (unsigned)units : (unsigned)ctas);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == TI_DTYPE_BF16)
-    return head_dim == 64 ? kv4::launch_decode<__nv_bfloat16, 64>(p, grid, s)
-                          : kv4::launch_decode<__nv_bfloat16, 128>(p, grid, s);
-  return head_dim == 64 ? kv4::launch_decode<__half, 64>(p, grid, s)
-                        : kv4::launch_decode<__half, 128>(p, grid, s);
+  auto go = [&](auto t, auto hd) {
+    using T = decltype(t);
+    constexpr int HD = decltype(hd)::value;
+    return unit_mode ? kv4::launch_decode<T, HD, true>(p, grid, s)
+                     : kv4::launch_decode<T, HD, false>(p, grid, s);
+  };
+  auto go_dim = [&](auto t) {
+    return head_dim == 64 ? go(t, std::integral_constant<int, 64>{})
+                          : go(t, std::integral_constant<int, 128>{});
+  };
+  return dtype == TI_DTYPE_BF16 ? go_dim(__nv_bfloat16{}) : go_dim(__half{});
 }
 
 extern "C" int ti_kv4_accumulate_weights(float* weights_out, const float* weights, const void* q,
