@@ -132,10 +132,10 @@ struct Cursor {
     const int k = piece();
     return at + k == n ? (k - 1) * grain + tail : k * grain;
   }
-  // Grains of a unit of sequence b; pref[b] = those of the sequences before b, times 4, plus tail - 1.
+  // Grains of a unit of sequence b; pref[b] = those of the sequences before b, times 8, plus tail - 1.
   __device__ __forceinline__ void look_up(const uint32_t* pref) {
-    n = (int)((pref[b + 1] >> 2) - (pref[b] >> 2));
-    tail = (int)(pref[b] & 3u) + 1;
+    n = (int)((pref[b + 1] >> 3) - (pref[b] >> 3));
+    tail = (int)(pref[b] & 7u) + 1;
   }
   __device__ __forceinline__ void next_unit(int units, const uint32_t* pref, int batch) {
     left -= piece();
@@ -160,6 +160,65 @@ struct Cut {
     return pos < big ? pos / (quot + 1) : rem + (pos - big) / quot;
   }
 };
+
+// The batch's stream in grains of KT tiles, cut evenly over the warps of (at most) gridDim.x CTAs: at
+// least one grain per warp, so little work takes fewer CTAs.  All threads call it; pref [batch + 1]
+// and scan [kWarps] are shared memory.  With total == 0 or a CTA index >= ctas there is no work here.
+struct Place {
+  uint32_t total;
+  int ctas;
+};
+template <int KT>
+__device__ __forceinline__ Place scan_batch(const int32_t* ctx, int batch, int cap, int units,
+                                            uint32_t* pref, uint32_t* scan) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  uint32_t carry = 0;
+  for (int b0 = 0; b0 < batch; b0 += kWarps * 32) {
+    const int b = b0 + tid;
+    const int len = b < batch ? min(ctx[b], cap) : 0;
+    const int tiles = len > 0 ? (len - 1) / kBlock + 1 : 0;
+    const uint32_t n = (tiles + KT - 1) / KT;
+    uint32_t x = n;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const uint32_t y = __shfl_up_sync(0xffffffffu, x, d);
+      if (lane >= d) x += y;
+    }
+    if (lane == 31) scan[warp] = x;
+    __syncthreads();
+    uint32_t before = carry, all = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += scan[w];
+      all += scan[w];
+    }
+    if (b < batch) pref[b] = (before + x - n) * 8u + (uint32_t)(tiles + KT - 1) % KT;
+    carry += all;
+    if (tid == 0) pref[batch] = carry * 8u;
+    __syncthreads();
+  }
+  const uint32_t total = carry * (uint32_t)units;
+  return {total, min((int)gridDim.x, (int)((total + kWarps - 1) / kWarps))};
+}
+// Where grain `pos` of the stream is; all lanes of a warp call it.
+__device__ __forceinline__ void find_place(uint32_t pos, int batch, int units, const uint32_t* pref,
+                                           int lane, Cursor& cur) {
+  // last b with (grains before b) * units <= pos: 32 probes at a time
+  int lo = 0, len = batch;                         // the answer is in [lo, lo + len)
+  while (len > 1) {
+    const int step = (len + 31) / 32, probe = lo + lane * step;
+    const uint32_t ok = __ballot_sync(0xffffffffu, lane * step < len &&
+                                      (pref[min(probe, batch)] >> 3) * (uint32_t)units <= pos);
+    const int k = 31 - __clz(ok);
+    lo += k * step;
+    len = min(step, len - k * step);
+  }
+  cur.b = lo;
+  cur.look_up(pref);
+  const uint32_t r = pos - (pref[lo] >> 3) * (uint32_t)units, n = max(cur.n, 1);
+  cur.hv = (int)(r / n);
+  cur.at = (int)(r - cur.hv * n);
+}
 
 // Query rows of a unit: lane (g, t) holds dims D/4 * t ... of head g (zeros beyond the unit's heads).
 template <typename T, int HD>
@@ -542,43 +601,16 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const __grid_con
   // the grains of the batch (in unit mode: of this CTA's sequence)
   const int cap = (int)min((int64_t)p.max_blocks * kBlock, (int64_t)0x7FFFFFFF);
   constexpr int grain = UNIT ? 1 : S::kTiles;      // tiles
-  auto tiles_of = [&](int b) {
-    const int n = min(p.ctx[b], cap);
-    return n > 0 ? (n - 1) / kBlock + 1 : 0;
-  };
   uint32_t total;
   int ctas;
   if constexpr (UNIT) {
+    const int len = min(p.ctx[blockIdx.x / units], cap);
     ctas = 1;
-    total = tiles_of(blockIdx.x / units);
+    total = len > 0 ? (len - 1) / kBlock + 1 : 0;
   } else {
-    uint32_t carry = 0;
-    for (int b0 = 0; b0 < p.batch; b0 += kWarps * 32) {
-      const int b = b0 + tid;
-      const int tiles = b < p.batch ? tiles_of(b) : 0;
-      const uint32_t n = (tiles + S::kTiles - 1) / S::kTiles;
-      uint32_t x = n;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const uint32_t y = __shfl_up_sync(0xffffffffu, x, d);
-        if (lane >= d) x += y;
-      }
-      if (lane == 31) sh.scan[warp] = x;
-      __syncthreads();
-      uint32_t before = carry, all = 0;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) before += sh.scan[w];
-        all += sh.scan[w];
-      }
-      if (b < p.batch) pref[b] = (before + x - n) * 4u + (uint32_t)(tiles + S::kTiles - 1) % S::kTiles;
-      carry += all;
-      if (tid == 0) pref[p.batch] = carry * 4u;
-      __syncthreads();
-    }
-    total = carry * (uint32_t)units;
-    // at least one step per warp: fewer CTAs for little work
-    ctas = min((int)gridDim.x, (int)((total + kWarps - 1) / kWarps));
+    const Place pl = scan_batch<S::kTiles>(p.ctx, p.batch, cap, units, pref, sh.scan);
+    total = pl.total;
+    ctas = pl.ctas;
   }
   const int cta = UNIT ? 0 : blockIdx.x;
   if (total == 0 || cta >= ctas) return;
@@ -595,20 +627,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const __grid_con
     cur.tail = 1;
     cur.at = (int)w_begin;
   } else {
-    // last b with (grains before b) * units <= w_begin: 32 probes at a time
-    int lo = 0, len = p.batch;                     // the answer is in [lo, lo + len)
-    while (len > 1) {
-      const int step = (len + 31) / 32, probe = lo + lane * step;
-      const uint32_t ok = __ballot_sync(0xffffffffu, lane * step < len && (pref[min(probe, p.batch)] >> 2) * (uint32_t)units <= w_begin);
-      const int k = 31 - __clz(ok);
-      lo += k * step;
-      len = min(step, len - k * step);
-    }
-    cur.b = lo;
-    cur.look_up(pref);
-    const uint32_t r = w_begin - (pref[lo] >> 2) * (uint32_t)units, n = max(cur.n, 1);
-    cur.hv = (int)(r / n);
-    cur.at = (int)(r - cur.hv * n);
+    find_place(w_begin, p.batch, units, pref, lane, cur);
   }
   if (lane == 0) {
     sh.start[warp] = (int)(w_begin - c_begin);
@@ -782,22 +801,14 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const __grid_con
     if (cross) join_ctas<T, HD>(p, sh, cross, c_begin, cut_of);
 }
 
-// The HD/32 dims lane `lane` holds of one token's codes (a 32-bit word serves 256 / HD lanes).
-template <int HD>
-__device__ __forceinline__ void lane_values(const uint8_t* row, int lane, float s,
-                                            float (&f)[HD / 32]) {
-  constexpr int PL = HD / 64;                      // bytes (dim pairs) of a lane
-  uint32_t h[4];
-  codes_to_half2(*reinterpret_cast<const uint32_t*>(row + ((lane * PL) & ~3)), h);
-#pragma unroll
-  for (int u = 0; u < PL; ++u) {
-    const int j = (lane * PL + u) & 3;
-    const float2 v = Elem<__half>::unpack2(j == 0 ? h[0] : j == 1 ? h[1] : j == 2 ? h[2] : h[3]);
-    f[2 * u] = v.x * s;
-    f[2 * u + 1] = v.y * s;
-  }
-}
-
+// ---- attention-weight totals ------------------------------------------------------------------------
+// weights += sum over the kv head's query heads of exp(q.k / sqrt(D) - lse), a read of the K half of the
+// cache (9/16 D bytes a token and kv head) and 8 bytes of totals.  The same stream, cut, scores and
+// two-stage ring as the decode kernel, without anything to join: a token belongs to one warp.  A step
+// is 8 tiles (D = 64; 4 for D = 128).  Heads are the columns of the scores, so a token's total is the sum
+// of two columns over four lanes; a step's totals are brought together by a reduce-scatter (12
+// shuffles for 8 tiles instead of 32) and go through shared memory to the lanes that hold the old
+// totals, four tokens each, loaded a step ahead.
 struct WeightParams {
   float* out;
   const float* in;
@@ -807,38 +818,166 @@ struct WeightParams {
   int64_t q_stride, num_blocks, bt_stride;
   const int32_t *tables, *row_index, *ctx;
   int batch, NH, KVH, group, max_blocks;
-  float scale;
+  float scale_log2;
 };
 
-// One warp per (sequence, kv head, token): the weights of the group's heads, summed in head order.
-template <typename T, int HD>
-__global__ void __launch_bounds__(256) weights_kernel(WeightParams p) {
+template <int HD>
+struct WShape {
+  static constexpr int kTileBytes = 9 * HD;                      // K codes, K scales
+  static constexpr int kTiles = kStepBytes / kTileBytes;
+  static constexpr int kLanes = 32 / kTiles;
+  static constexpr int kRing = kWarps * 2 * kStepBytes;
+  static constexpr int kSums = kWarps * kTiles * kBlock * 4;
+  static size_t smem(int batch) { return kRing + kSums + kWarps * 4 + ((size_t)batch + 1) * 4; }
+};
+
+// NS: groups of at most 8 query heads per kv head.
+template <typename T, int HD, int NS>
+__global__ void __launch_bounds__(kWarps * 32, 1) weights_kernel(const __grid_constant__ WeightParams p) {
+  using S = WShape<HD>;
+  using L = Tile<HD>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  float* sums = reinterpret_cast<float*>(smem + S::kRing) + warp * S::kTiles * kBlock;
+  uint32_t* scan = reinterpret_cast<uint32_t*>(smem + S::kRing + S::kSums);
+  uint32_t* pref = scan + kWarps;
   pdl_wait();
   pdl_launch_dependents();
-  using L = Tile<HD>;
-  constexpr int PL = HD / 64;
-  const int kvh = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31;
-  const int n = (int)min((int64_t)p.ctx[b], (int64_t)p.max_blocks * kBlock);
-  const int32_t* table = p.tables + (int64_t)(p.row_index ? p.row_index[b] : b) * p.bt_stride;
-  for (int i = blockIdx.x * 8 + (threadIdx.x >> 5); i < n; i += gridDim.x * 8) {
-    const int32_t blk = table[i / kBlock];
-    if (blk < 0 || blk >= p.num_blocks) continue;
-    const int64_t tile_i = (int64_t)blk * p.KVH + kvh;
-    const uint8_t* tile = p.pool + tile_i * L::kBytes;
-    const int off = i % kBlock, g = lane * 2 * PL / kGroup;
-    const float ks = scale_value(tile[L::kKs + g * kBlock + off]);
-    float k[2 * PL];
-    lane_values<HD>(tile + L::kK + off * L::kRow, lane, ks, k);
-    float w = 0.f;
-    for (int hg = 0; hg < p.group; ++hg) {
-      const int h = kvh * p.group + hg;
-      const T* q = (const T*)p.q + b * p.q_stride + (int64_t)h * HD + lane * 2 * PL;
-      float s = 0.f;
-      for (int u = 0; u < 2 * PL; ++u) s += Elem<T>::to_f(q[u]) * k[u];
-      w += expf(warp_sum(s) * p.scale - p.lse[(int64_t)b * p.NH + h]);
+  const int cap = (int)min((int64_t)p.max_blocks * kBlock, (int64_t)0x7FFFFFFF);
+  const Place pl = scan_batch<S::kTiles>(p.ctx, p.batch, cap, p.KVH, pref, scan);
+  if (pl.total == 0 || (int)blockIdx.x >= pl.ctas) return;
+  const Cut cut_of(pl.total, (uint32_t)pl.ctas * kWarps);
+  const uint32_t w_begin = cut_of.start(blockIdx.x * kWarps + warp);
+  Cursor cur;
+  cur.left = (int)(cut_of.start(blockIdx.x * kWarps + warp + 1) - w_begin);
+  if (cur.left == 0) return;
+  find_place(w_begin, p.batch, p.KVH, pref, lane, cur);
+
+  const uint32_t ring = smem_u32(smem) + warp * (2 * kStepBytes);
+  const int j = lane / S::kLanes, cl = lane % S::kLanes;
+  const uint32_t my_tile = ring + j * S::kTileBytes + cl * 16;
+  const uint32_t num_blocks = (uint32_t)min(p.num_blocks, (int64_t)0x7FFFFFFF);
+  Cursor ld = cur;
+  int ld_left = 0, ld_stage = 0, id = -1;
+  const int32_t* ids = nullptr;
+  auto open_loads = [&]() {
+    const int row = p.row_index ? p.row_index[ld.b] : ld.b;
+    ids = p.tables + (int64_t)row * p.bt_stride + (int64_t)ld.at * S::kTiles + j;
+    ld_left = ld.piece_tiles(S::kTiles);
+  };
+  open_loads();
+  id = j < ld_left ? *ids : -1;
+  // old totals of the next step: lane (tile j, quarter cl) holds tokens 4 cl .. 4 cl + 3
+  float4 w_next = make_float4(0.f, 0.f, 0.f, 0.f);
+  int64_t at_next = -1;
+  auto issue = [&]() {
+    const bool ok = (uint32_t)id < num_blocks;
+    at_next = -1;
+    if (ok) {
+      const int64_t tile = (int64_t)id * p.KVH + ld.hv;
+      const uint8_t* src = p.pool + tile * L::kBytes + cl * 16;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) cp_async16(my_tile + ld_stage + i * S::kLanes * 16, src + i * S::kLanes * 16);
+      cp_async16(my_tile + ld_stage + 8 * HD, src + L::kKs);
+      if (cl < 4) {
+        at_next = tile * kBlock + cl * 4;
+        w_next = *reinterpret_cast<const float4*>(p.in + at_next);
+      }
     }
-    if (lane == 0) p.out[tile_i * kBlock + off] = p.in[tile_i * kBlock + off] + w;
+    cp_commit();
+    ld_stage = kStepBytes - ld_stage;
+    ids += S::kTiles;
+    ld_left -= S::kTiles;
+    if (ld_left <= 0 && ld.left > 0) {
+      ld.next_unit(p.KVH, pref, p.batch);
+      if (ld.left > 0) open_loads();
+    }
+    id = j < ld_left ? *ids : -1;
+  };
+
+  uint32_t qf[NS][HD / 16][2];
+  float2 sc[NS], off[NS];
+  int ctx = 0;
+  auto open_unit = [&](bool start) {
+    uint4 raw[NS][HD / 32];
+#pragma unroll
+    for (int u = 0; u < NS; ++u)
+      load_query<T, HD>((const T*)p.q + cur.b * p.q_stride + ((int64_t)cur.hv * p.group + u * 8) * HD,
+                        min(8, p.group - u * 8), g, t, raw[u]);
+    ctx = min(p.ctx[cur.b], cap);
+    const float* lse = p.lse + (int64_t)cur.b * p.NH + cur.hv * p.group;
+#pragma unroll
+    for (int u = 0; u < NS; ++u) {
+      // heads beyond the group weigh nothing: 2^(0 - inf)
+      const int h = u * 8 + 2 * t;
+      off[u].x = h < p.group ? -1.4426950408889634f * lse[h] : -INFINITY;
+      off[u].y = h + 1 < p.group ? -1.4426950408889634f * lse[h + 1] : -INFINITY;
+    }
+    if (start) issue();
+#pragma unroll
+    for (int u = 0; u < NS; ++u) {
+      const float2 inv = convert_query<T, HD>(raw[u], t, qf[u]);
+      sc[u] = make_float2(inv.x * p.scale_log2, inv.y * p.scale_log2);
+    }
+  };
+  open_unit(true);
+  for (uint32_t st = ring;;) {
+    int live = ctx - cur.at * (S::kTiles * kBlock);
+    for (int rem = cur.piece_tiles(S::kTiles); rem > 0; rem -= S::kTiles, live -= S::kTiles * kBlock) {
+      const float4 w = w_next;
+      const int64_t at = at_next;
+      issue();                                     // (an empty group when nothing is left)
+      cp_wait<1>();
+      __syncwarp();
+      float v[S::kTiles * 2];                      // [tile][token g, token g + 8], two heads summed
+#pragma unroll
+      for (int x = 0; x < S::kTiles; ++x) {
+        v[2 * x] = v[2 * x + 1] = 0.f;
+        if (x >= rem) continue;
+#pragma unroll
+        for (int u = 0; u < NS; ++u) {
+          float c[4];
+          tile_scores<HD>(st + x * S::kTileBytes, st + x * S::kTileBytes + 8 * HD, g, t, qf[u], c);
+          v[2 * x] += fast_exp2(fmaf(c[0], sc[u].x, off[u].x)) + fast_exp2(fmaf(c[1], sc[u].y, off[u].y));
+          v[2 * x + 1] += fast_exp2(fmaf(c[2], sc[u].x, off[u].x)) + fast_exp2(fmaf(c[3], sc[u].y, off[u].y));
+        }
+      }
+      // sum over the four lanes of a token; lane t keeps tiles t and t + 4
+      float h1[S::kTiles], h2[S::kTiles / 2];
+#pragma unroll
+      for (int k = 0; k < S::kTiles; ++k) {        // k = 2 * (tile / 2) + row: tiles of this lane's parity
+        const float even = v[4 * (k / 2) + k % 2], odd = v[4 * (k / 2) + 2 + k % 2];
+        h1[k] = ((t & 1) ? odd : even) + __shfl_xor_sync(0xffffffffu, (t & 1) ? even : odd, 1);
+      }
+#pragma unroll
+      for (int k = 0; k < S::kTiles / 2; ++k) {
+        const float lo = h1[4 * (k / 2) + k % 2], hi = h1[4 * (k / 2) + 2 + k % 2];
+        h2[k] = ((t & 2) ? hi : lo) + __shfl_xor_sync(0xffffffffu, (t & 2) ? lo : hi, 2);
+      }
+#pragma unroll
+      for (int k = 0; k < S::kTiles / 2; ++k)
+        sums[(4 * (k / 2) + t) * kBlock + g + 8 * (k % 2)] = h2[k];
+      __syncwarp();
+      if (at >= 0) {
+        const float4 n = *reinterpret_cast<const float4*>(sums + j * kBlock + cl * 4);
+        const int left = live - j * kBlock - cl * 4;
+        float* out = p.out + at;
+        if (left >= 4) {
+          *reinterpret_cast<float4*>(out) = make_float4(w.x + n.x, w.y + n.y, w.z + n.z, w.w + n.w);
+        } else {
+          if (left > 0) out[0] = w.x + n.x;
+          if (left > 1) out[1] = w.y + n.y;
+          if (left > 2) out[2] = w.z + n.z;
+        }
+      }
+      __syncwarp();                                // the stage and the sums are free again
+      st = 2 * ring + kStepBytes - st;
+    }
+    cur.next_unit(p.KVH, pref, p.batch);
+    if (cur.left == 0) break;
+    open_unit(false);
   }
+  cp_wait<0>();
 }
 
 constexpr int kMaxCtas = 256;
@@ -856,22 +995,34 @@ static int decode_ctas() {
   return std::min(sms, kMaxCtas);
 }
 
-template <typename T, int HD, bool UNIT>
-static int launch_decode(const DecodeParams& p, dim3 grid, cudaStream_t s) {
-  static std::atomic<uint64_t> ready{0};         // devices whose limit has been raised
+// Raise a kernel's shared-memory limit, once per device (bits of `ready`).
+template <typename K>
+static int allow_smem(K kern, size_t bytes, std::atomic<uint64_t>& ready) {
   int dev = 0;
   cudaGetDevice(&dev);
   const uint64_t bit = 1ull << (dev & 63);
-  if (!(ready.load(std::memory_order_acquire) & bit)) {
-    cudaError_t e = cudaFuncSetAttribute(decode_kernel<T, HD, UNIT>,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)Shape<HD>::smem(kMaxBatch));
-    if (e != cudaSuccess) {
-      (void)cudaGetLastError();
-      return set_cuda_error(e, "cudaFuncSetAttribute(kv4 attention)");
-    }
-    ready.fetch_or(bit, std::memory_order_release);
+  if (ready.load(std::memory_order_acquire) & bit) return TI_OK;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e != cudaSuccess) {
+    (void)cudaGetLastError();
+    return set_cuda_error(e, "cudaFuncSetAttribute(kv4)");
   }
+  ready.fetch_or(bit, std::memory_order_release);
+  return TI_OK;
+}
+
+template <typename T, int HD, int NS>
+static int launch_weights(const WeightParams& p, dim3 grid, cudaStream_t s) {
+  static std::atomic<uint64_t> ready{0};
+  if (int rc = allow_smem(weights_kernel<T, HD, NS>, WShape<HD>::smem(kMaxBatch), ready)) return rc;
+  return launch_kernel("kv4 weights launch", weights_kernel<T, HD, NS>, grid, dim3(kWarps * 32),
+                       WShape<HD>::smem(p.batch), s, 1, p);
+}
+
+template <typename T, int HD, bool UNIT>
+static int launch_decode(const DecodeParams& p, dim3 grid, cudaStream_t s) {
+  static std::atomic<uint64_t> ready{0};
+  if (int rc = allow_smem(decode_kernel<T, HD, UNIT>, Shape<HD>::smem(kMaxBatch), ready)) return rc;
   return launch_kernel("kv4 attention launch", decode_kernel<T, HD, UNIT>, grid, dim3(kWarps * 32),
                        Shape<HD>::smem(UNIT ? 0 : p.batch), s, 1, p);
 }
@@ -887,9 +1038,9 @@ static int check_shape(int batch, int NH, int KVH, int HD, int block_size,
   if (dtype != TI_DTYPE_BF16 && dtype != TI_DTYPE_FP16)
     return set_error(TI_ERR_UNSUPPORTED, "kv4: dtype must be bf16 or fp16");
   if (batch > kMaxBatch) return set_error(TI_ERR_UNSUPPORTED, "kv4: at most 4096 sequences per call");
-  if ((int64_t)batch * max_blocks * KVH * ((NH / KVH + 7) / 8) >= (int64_t)1 << 31)
+  if ((int64_t)batch * max_blocks * KVH * ((NH / KVH + 7) / 8) >= (int64_t)1 << 29)
     return set_error(TI_ERR_UNSUPPORTED,
-                     "kv4: batch * table width * kv heads (twice beyond 8 query heads each) must be below 2^31");
+                     "kv4: batch * table width * kv heads (twice beyond 8 query heads each) must be below 2^29");
   return TI_OK;
 }
 
@@ -964,21 +1115,24 @@ extern "C" int ti_kv4_accumulate_weights(float* weights_out, const float* weight
   if (int rc = kv4::check_shape(batch, num_heads, num_kv_heads, head_dim,
                                 block_size, max_blocks_per_seq, num_blocks, dtype))
     return rc;
-  if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(pool)) & 15) ||
+  if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(pool) |
+        reinterpret_cast<uintptr_t>(weights) | reinterpret_cast<uintptr_t>(weights_out)) & 15) ||
       (q_seq_stride % 8))
     return set_error(TI_ERR_INVALID_ARGUMENT, "kv4 weights: tensors must be 16-byte aligned");
   kv4::WeightParams p{weights_out, weights, q, lse, (const uint8_t*)pool, q_seq_stride, num_blocks,
                       bt_stride, block_tables, row_index, context_lens, batch, num_heads,
                       num_kv_heads, num_heads / num_kv_heads, max_blocks_per_seq,
-                      1.0f / sqrtf((float)head_dim)};
+                      1.4426950408889634f / sqrtf((float)head_dim)};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const dim3 grid(std::min(max_blocks_per_seq, 64), num_kv_heads, batch);
-  auto go = [&](auto kern) {
-    return launch_kernel("kv4 weights launch", kern, grid, dim3(256), 0, s, 1, p);
+  const dim3 grid(kv4::decode_ctas());
+  auto go = [&](auto t, auto hd) {
+    using T = decltype(t);
+    constexpr int HD = decltype(hd)::value;
+    return p.group <= 8 ? kv4::launch_weights<T, HD, 1>(p, grid, s) : kv4::launch_weights<T, HD, 2>(p, grid, s);
   };
-  if (dtype == TI_DTYPE_BF16)
-    return head_dim == 64 ? go(kv4::weights_kernel<__nv_bfloat16, 64>)
-                          : go(kv4::weights_kernel<__nv_bfloat16, 128>);
-  return head_dim == 64 ? go(kv4::weights_kernel<__half, 64>)
-                        : go(kv4::weights_kernel<__half, 128>);
+  auto go_dim = [&](auto t) {
+    return head_dim == 64 ? go(t, std::integral_constant<int, 64>{})
+                          : go(t, std::integral_constant<int, 128>{});
+  };
+  return dtype == TI_DTYPE_BF16 ? go_dim(__nv_bfloat16{}) : go_dim(__half{});
 }

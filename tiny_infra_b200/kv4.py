@@ -26,62 +26,109 @@ import torch
 from . import _native as N
 
 BLOCK = 16
+_HALF = (torch.bfloat16, torch.float16)
 _ws = N.Workspace()
 
 
-def _check(cond: bool, msg: str) -> None:
-    if not cond:
-        raise RuntimeError(msg)
+# The checks below run on every call, in front of kernels of a few microseconds: plain conditions
+# on cheap attributes, messages built only when they fail.
+def _fail(msg: str) -> None:
+    raise RuntimeError(msg)
 
 
-def _cuda(**tensors) -> None:
-    dev = None
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        _check(isinstance(t, torch.Tensor) and t.is_cuda, f"{name} must be a CUDA tensor")
-        dev = t.device if dev is None else dev
-        _check(t.device == dev, f"{name} is on {t.device}, other tensors on {dev}")
+def _device(*tensors) -> int:
+    """The CUDA device index that all the tensors (None: absent) are on."""
+    dev = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            _fail(f"all tensors must be on one CUDA device, not {t.device} and {tensors[0].device}")
+    if dev < 0:
+        _fail("pool and the other arguments must be CUDA tensors")
+    return dev
 
 
-def _on(t: torch.Tensor):
+def _on(dev: int):
     """Launches go to the current device: make it the tensors' one."""
-    if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+    return _HERE if dev == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
-def _pool_shape(pool: torch.Tensor, head_dim: int | None = None):
-    _check(pool.dtype == torch.uint8 and pool.dim() == 3 and pool.is_contiguous(),
-           "pool must be a contiguous uint8 [num_blocks, num_kv_heads, 18 * head_dim] tensor")
+_HERE = contextlib.nullcontext()
+
+
+def _stream(dev: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(dev)
+
+
+def _pool_shape(pool: torch.Tensor):
+    if pool.dtype != torch.uint8 or pool.dim() != 3 or not pool.is_contiguous():
+        _fail("pool must be a contiguous uint8 [num_blocks, num_kv_heads, 18 * head_dim] tensor")
     nb, kvh, tile = pool.shape
-    d = tile // 18
-    _check(tile in (18 * 64, 18 * 128), "pool tiles must be 18 * head_dim bytes, head_dim 64 or 128")
-    _check(head_dim is None or d == head_dim, "head_dim does not match the pool's tiles")
-    _check(nb > 0 and kvh > 0, "the pool is empty")
-    return nb, kvh, d
+    if tile != 1152 and tile != 2304:
+        _fail("pool tiles must be 18 * head_dim bytes, head_dim 64 or 128")
+    if nb <= 0 or kvh <= 0:
+        _fail("the pool is empty")
+    return nb, kvh, tile // 18
 
 
 def _index(name: str, t: torch.Tensor | None, numel: int | None = None) -> None:
     if t is None:
         return
-    _check(t.dtype == torch.int32 and t.is_contiguous(), f"{name} must be contiguous int32")
-    _check(numel is None or t.numel() == numel, f"{name} must have {numel} entries")
+    if t.dtype != torch.int32 or not t.is_contiguous():
+        _fail(f"{name} must be contiguous int32")
+    if numel is not None and t.numel() != numel:
+        _fail(f"{name} must have {numel} entries")
 
 
-def _table(name: str, t: torch.Tensor, rows: int | None) -> None:
-    _check(t.dtype == torch.int32 and t.dim() == 2 and (t.shape[1] <= 1 or t.stride(1) == 1),
-           f"{name} must be int32 [rows, max_blocks] with contiguous rows")
-    _check(t.shape[1] > 0, f"{name} has no columns")
-    _check(rows is None or t.shape[0] >= rows, f"{name} has fewer rows than the batch")
+def _table(name: str, t: torch.Tensor, rows: int | None):
+    """(row stride, columns) of a block table."""
+    if t.dtype != torch.int32 or t.dim() != 2:
+        _fail(f"{name} must be int32 [rows, max_blocks]")
+    n, cols = t.shape
+    if cols <= 0:
+        _fail(f"{name} has no columns")
+    stride, inner = t.stride()
+    if inner != 1 and cols > 1:
+        _fail(f"{name} must have contiguous rows")
+    if rows is not None and n < rows:
+        _fail(f"{name} has fewer rows than the batch")
+    return stride, cols
 
 
-def _rows(name: str, t: torch.Tensor) -> None:
-    """[T, heads, D] of a 16-bit type, each token's heads contiguous."""
-    _check(t.dim() == 3 and t.dtype in (torch.bfloat16, torch.float16),
-           f"{name} must be bf16 or fp16 [tokens, heads, head_dim]")
-    _check(t.numel() == 0 or (t.stride(2) == 1 and t.stride(1) == t.shape[2]),
-           f"{name} must have contiguous [heads, head_dim] rows")
+def _rows(name: str, t: torch.Tensor):
+    """Shape and token stride of a [T, heads, D] tensor of a 16-bit type whose tokens' heads are
+    contiguous."""
+    if t.dim() != 3 or t.dtype not in _HALF:
+        _fail(f"{name} must be bf16 or fp16 [tokens, heads, head_dim]")
+    T, heads, d = t.shape
+    tok, head, inner = t.stride()
+    if t.numel() and (inner != 1 or (head != d and heads > 1)):
+        _fail(f"{name} must have contiguous [heads, head_dim] rows")
+    return T, heads, d, tok
+
+
+def _attention(q, pool, block_tables, context_lens, row_index):
+    """Checks shared by the calls that take one query token per sequence."""
+    nb, kvh, d = _pool_shape(pool)
+    B, NH, dq, q_stride = _rows("q", q)
+    if dq != d:
+        _fail("head_dim does not match the pool's tiles")
+    if NH <= 0 or NH % kvh or NH > 16 * kvh:
+        _fail("query heads must be a multiple of the kv heads, at most 16 per kv head")
+    _index("context_lens", context_lens, B)
+    _index("row_index", row_index, B)
+    bt_stride, cols = _table("block_tables", block_tables, B if row_index is None else None)
+    return B, NH, nb, kvh, d, q_stride, bt_stride, cols
+
+
+def _head_sums(name: str, t: torch.Tensor, B: int, NH: int) -> None:
+    if t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != B * NH:
+        _fail(f"{name} must be contiguous float32 [batch, heads]")
+
+
+def _totals(name: str, w: torch.Tensor | None, nb: int, kvh: int) -> None:
+    if w is not None and (w.dtype != torch.float32 or not w.is_contiguous() or
+                          w.shape != (nb, kvh, BLOCK)):
+        _fail(f"{name} must be contiguous float32 [num_blocks, num_kv_heads, 16]")
 
 
 def _ptr(t: torch.Tensor | None):
@@ -91,7 +138,8 @@ def _ptr(t: torch.Tensor | None):
 def tile_bytes(head_dim: int) -> int:
     """Bytes of one (block, kv head): 16 tokens' K and V codes and scales."""
     n = int(N.lib().ti_kv4_tile_bytes(int(head_dim)))
-    _check(n > 0, "head_dim must be 64 or 128")
+    if n <= 0:
+        _fail("head_dim must be 64 or 128")
     return n
 
 
@@ -111,30 +159,28 @@ def append(pool: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slot_mapping: t
     slots of a call are distinct.  With ``weights`` (float32 [num_blocks, KVH, 16]) the new tokens'
     attention-weight totals become zero.  A group of 16 dims with a NaN or an infinity becomes NaN;
     magnitudes above 61440 saturate."""
-    _cuda(pool=pool, k=k, v=v, slot_mapping=slot_mapping, weights=weights)
-    _check(k.dim() == 3 and v.shape == k.shape and k.dtype == v.dtype and
-           k.dtype in (torch.bfloat16, torch.float16),
-           "k and v must be [tokens, num_kv_heads, head_dim] of the same 16-bit dtype")
-    nb, kvh, d = _pool_shape(pool, k.shape[2])
-    _check(k.shape[1] == kvh, "k and v do not have the pool's kv heads")
-    _check(slot_mapping.dtype == torch.int64 and slot_mapping.is_contiguous() and
-           slot_mapping.numel() == k.shape[0], "slot_mapping must be contiguous int64 [tokens]")
-    _weights("weights", weights, nb, kvh)
-    if k.shape[0] == 0:
+    dev = _device(pool, k, v, slot_mapping, weights)
+    nb, kvh, d = _pool_shape(pool)
+    if k.dim() != 3 or v.shape != k.shape or k.dtype != v.dtype or k.dtype not in _HALF:
+        _fail("k and v must be [tokens, num_kv_heads, head_dim] of the same 16-bit dtype")
+    T, heads, dk = k.shape
+    if heads != kvh or dk != d:
+        _fail("k and v do not have the pool's kv heads and head_dim")
+    if slot_mapping.dtype != torch.int64 or not slot_mapping.is_contiguous() or \
+            slot_mapping.numel() != T:
+        _fail("slot_mapping must be contiguous int64 [tokens]")
+    _totals("weights", weights, nb, kvh)
+    if T == 0:
         return
-    _check(k.stride(2) == 1 and v.stride(2) == 1, "k and v must have contiguous head_dim")
-    with _on(pool):
+    k_tok, k_head, k_in = k.stride()
+    v_tok, v_head, v_in = v.stride()
+    if k_in != 1 or v_in != 1:
+        _fail("k and v must have contiguous head_dim")
+    with _on(dev):
         N.check(N.lib().ti_kv4_append(
-            pool.data_ptr(), _ptr(weights), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
-            v.stride(0), v.stride(1), slot_mapping.data_ptr(), k.shape[0], nb, kvh, d, BLOCK,
-            N.dtype_code(k.dtype), N.stream_of(pool)))
-
-
-def _weights(name: str, w: torch.Tensor | None, nb: int, kvh: int) -> None:
-    if w is not None:
-        _check(w.dtype == torch.float32 and w.is_contiguous() and
-               tuple(w.shape) == (nb, kvh, BLOCK),
-               f"{name} must be contiguous float32 [num_blocks, num_kv_heads, 16]")
+            pool.data_ptr(), _ptr(weights), k.data_ptr(), k_tok, k_head, v.data_ptr(), v_tok,
+            v_head, slot_mapping.data_ptr(), T, nb, kvh, d, BLOCK, N.dtype_code(k.dtype),
+            _stream(dev)))
 
 
 def dequantize(pool: torch.Tensor, block_tables: torch.Tensor, lens: torch.Tensor,
@@ -144,47 +190,35 @@ def dequantize(pool: torch.Tensor, block_tables: torch.Tensor, lens: torch.Tenso
     ``v_out`` [out_blocks, KVH, 16, D]: block j of row r goes to block ``out_tables[r, j]`` (a
     negative entry skips it), zeros behind the row's length and where the source entry holds no
     block.  ``row_index`` selects the rows of ``block_tables``.  The target blocks are distinct."""
-    _cuda(pool=pool, block_tables=block_tables, lens=lens, out_tables=out_tables, k_out=k_out,
-          v_out=v_out, row_index=row_index)
+    dev = _device(pool, block_tables, lens, out_tables, k_out, v_out, row_index)
     nb, kvh, d = _pool_shape(pool)
-    _check(k_out.dim() == 4 and k_out.shape == v_out.shape and k_out.dtype == v_out.dtype and
-           k_out.dtype in (torch.bfloat16, torch.float16) and k_out.is_contiguous() and
-           v_out.is_contiguous() and tuple(k_out.shape[1:]) == (kvh, BLOCK, d),
-           "k_out and v_out must be contiguous 16-bit [out_blocks, num_kv_heads, 16, head_dim]")
+    if k_out.dim() != 4 or k_out.shape != v_out.shape or k_out.dtype != v_out.dtype or \
+            k_out.dtype not in _HALF or not k_out.is_contiguous() or \
+            not v_out.is_contiguous() or k_out.shape[1:] != (kvh, BLOCK, d):
+        _fail("k_out and v_out must be contiguous 16-bit [out_blocks, num_kv_heads, 16, head_dim]")
     rows = lens.numel()
     _index("lens", lens)
     _index("row_index", row_index, rows)
-    _table("out_tables", out_tables, rows)
-    _table("block_tables", block_tables, rows if row_index is None else None)
-    _check(block_tables.shape[1] >= out_tables.shape[1], "block_tables is narrower than out_tables")
+    ot_stride, cols = _table("out_tables", out_tables, rows)
+    bt_stride, width = _table("block_tables", block_tables, rows if row_index is None else None)
+    if width < cols:
+        _fail("block_tables is narrower than out_tables")
     if rows == 0 or k_out.shape[0] == 0:
         return
-    with _on(pool):
+    with _on(dev):
         N.check(N.lib().ti_kv4_dequantize(
             k_out.data_ptr(), v_out.data_ptr(), k_out.shape[0], pool.data_ptr(), nb,
-            block_tables.data_ptr(), block_tables.stride(0), _ptr(row_index), lens.data_ptr(),
-            out_tables.data_ptr(), out_tables.stride(0), rows, out_tables.shape[1], kvh, d, BLOCK,
-            N.dtype_code(k_out.dtype), N.stream_of(pool)))
+            block_tables.data_ptr(), bt_stride, _ptr(row_index), lens.data_ptr(),
+            out_tables.data_ptr(), ot_stride, rows, cols, kvh, d, BLOCK,
+            N.dtype_code(k_out.dtype), _stream(dev)))
 
 
-def _workspace(device: torch.device, nbytes: int, stream: int) -> torch.Tensor:
+def _workspace(dev: int, nbytes: int, stream: int) -> torch.Tensor:
     """Zeroed scratch, one per (device, stream); inside a stream capture one of the graph's own
     (so graphs that replay at the same time do not share it), zeroed by the graph itself."""
     if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(nbytes, dtype=torch.uint8, device=device)
-    return _ws.get(device, nbytes, stream)
-
-
-def _batch(q, pool, block_tables, context_lens, row_index):
-    _rows("q", q)
-    nb, kvh, d = _pool_shape(pool, q.shape[2])
-    B, NH, _ = q.shape
-    _check(NH > 0 and NH % kvh == 0 and NH // kvh <= 16,
-           "query heads must be a multiple of the kv heads, at most 16 per kv head")
-    _index("context_lens", context_lens, B)
-    _index("row_index", row_index, B)
-    _table("block_tables", block_tables, B if row_index is None else None)
-    return B, NH, nb, kvh, d
+        return torch.zeros(nbytes, dtype=torch.uint8, device=torch.device("cuda", dev))
+    return _ws.get(torch.device("cuda", dev), nbytes, stream)
 
 
 def decode_attention(out: torch.Tensor, q: torch.Tensor, pool: torch.Tensor,
@@ -199,26 +233,25 @@ def decode_attention(out: torch.Tensor, q: torch.Tensor, pool: torch.Tensor,
     length 0 leaves its rows of ``out`` and ``lse`` as they were; one whose table holds no block
     gets NaN, and -inf in ``lse``.  One launch; results do not depend on the batch's other rows'
     contents and are the same on every run."""
-    _cuda(out=out, q=q, pool=pool, block_tables=block_tables, context_lens=context_lens,
-          row_index=row_index, lse=lse)
-    B, NH, nb, kvh, d = _batch(q, pool, block_tables, context_lens, row_index)
-    _rows("out", out)
-    _check(out.shape == q.shape and out.dtype == q.dtype, "out must have q's shape and dtype")
+    dev = _device(pool, out, q, block_tables, context_lens, row_index, lse)
+    B, NH, nb, kvh, d, q_stride, bt_stride, cols = _attention(q, pool, block_tables, context_lens,
+                                                              row_index)
+    _, _, _, out_stride = _rows("out", out)
+    if out.shape != q.shape or out.dtype != q.dtype:
+        _fail("out must have q's shape and dtype")
     if lse is not None:
-        _check(lse.dtype == torch.float32 and lse.is_contiguous() and lse.numel() == B * NH,
-               "lse must be contiguous float32 [batch, heads]")
+        _head_sums("lse", lse, B, NH)
     if B == 0:
         return
     lib = N.lib()
-    with _on(pool):
-        stream = N.stream_of(pool)
-        need = lib.ti_kv4_attention_workspace_bytes(B, NH, kvh, d, block_tables.shape[1])
-        ws = _workspace(pool.device, need, stream)
+    with _on(dev):
+        stream = _stream(dev)
+        need = lib.ti_kv4_attention_workspace_bytes(B, NH, kvh, d, cols)
+        ws = _workspace(dev, need, stream)
         N.check(lib.ti_kv4_attention_decode(
-            out.data_ptr(), out.stride(0), _ptr(lse), q.data_ptr(), q.stride(0), pool.data_ptr(),
-            nb, block_tables.data_ptr(), block_tables.stride(0), _ptr(row_index),
-            context_lens.data_ptr(), B, NH, kvh, d, BLOCK, block_tables.shape[1],
-            N.dtype_code(q.dtype), ws.data_ptr(), ws.numel(), stream))
+            out.data_ptr(), out_stride, _ptr(lse), q.data_ptr(), q_stride, pool.data_ptr(), nb,
+            block_tables.data_ptr(), bt_stride, _ptr(row_index), context_lens.data_ptr(), B, NH,
+            kvh, d, BLOCK, cols, N.dtype_code(q.dtype), ws.data_ptr(), ws.numel(), stream))
 
 
 def accumulate_weights(weights: torch.Tensor, q: torch.Tensor, lse: torch.Tensor,
@@ -231,22 +264,21 @@ def accumulate_weights(weights: torch.Tensor, q: torch.Tensor, lse: torch.Tensor
     ``lse`` float32 [B, NH] as ``decode_attention`` gives it for the same arguments; weights and
     out (default: weights itself) float32 [num_blocks, KVH, 16], of which only the sequences' own
     tokens are read and written.  The sequences of a call share no block."""
-    _cuda(weights=weights, q=q, lse=lse, pool=pool, block_tables=block_tables,
-          context_lens=context_lens, row_index=row_index, out=out)
     out = weights if out is None else out
-    B, NH, nb, kvh, d = _batch(q, pool, block_tables, context_lens, row_index)
-    _weights("weights", weights, nb, kvh)
-    _weights("out", out, nb, kvh)
-    _check(lse.dtype == torch.float32 and lse.is_contiguous() and lse.numel() == B * NH,
-           "lse must be contiguous float32 [batch, heads]")
+    dev = _device(pool, weights, q, lse, block_tables, context_lens, row_index, out)
+    B, NH, nb, kvh, d, q_stride, bt_stride, cols = _attention(q, pool, block_tables, context_lens,
+                                                              row_index)
+    _totals("weights", weights, nb, kvh)
+    _totals("out", out, nb, kvh)
+    _head_sums("lse", lse, B, NH)
     if B == 0:
         return
-    with _on(pool):
+    with _on(dev):
         N.check(N.lib().ti_kv4_accumulate_weights(
-            out.data_ptr(), weights.data_ptr(), q.data_ptr(), q.stride(0), lse.data_ptr(),
-            pool.data_ptr(), nb, block_tables.data_ptr(), block_tables.stride(0), _ptr(row_index),
-            context_lens.data_ptr(), B, NH, kvh, d, BLOCK, block_tables.shape[1],
-            N.dtype_code(q.dtype), N.stream_of(pool)))
+            out.data_ptr(), weights.data_ptr(), q.data_ptr(), q_stride, lse.data_ptr(),
+            pool.data_ptr(), nb, block_tables.data_ptr(), bt_stride, _ptr(row_index),
+            context_lens.data_ptr(), B, NH, kvh, d, BLOCK, cols, N.dtype_code(q.dtype),
+            _stream(dev)))
 
 
 class PrefillPlan:
@@ -257,12 +289,14 @@ class PrefillPlan:
 
     def __init__(self, starts, counts, device="cuda") -> None:
         starts, counts = np.asarray(starts, np.int64), np.asarray(counts, np.int64)
-        _check(starts.ndim == 1 and starts.shape == counts.shape, "starts and counts must match")
-        _check(bool((starts >= 0).all() and (counts >= 0).all()), "starts and counts must be >= 0")
+        if starts.ndim != 1 or starts.shape != counts.shape:
+            _fail("starts and counts must be lists of the same length")
+        if not ((starts >= 0).all() and (counts >= 0).all()):
+            _fail("starts and counts must be >= 0")
         lens = np.where(counts > 0, starts + counts, 0)
         blocks = -(-lens // BLOCK)
-        _check(int(lens.max(initial=0)) < 2 ** 31 and int(blocks.sum()) < 2 ** 31,
-               "prefill too long")
+        if int(lens.max(initial=0)) >= 2 ** 31 or int(blocks.sum()) >= 2 ** 31:
+            _fail("prefill too long")
         self.num_seqs, self.num_tokens = len(starts), int(counts.sum())
         self.max_blocks = int(blocks.max(initial=0))
         self.scratch_blocks = int(blocks.sum())
@@ -297,32 +331,41 @@ def prefill_attention(out: torch.Tensor, q: torch.Tensor, pool: torch.Tensor,
     The cached values are exact in 16 bits, so they are read back once (``dequantize``, 2 *
     scratch_blocks * KVH * 16 * D values of scratch) and the 16-bit pool's tensor-core prefill
     kernel runs on them; the read-back is a few per cent of a chunk's attention."""
-    _cuda(out=out, q=q, pool=pool, block_tables=block_tables, start_pos=plan.start_pos,
-          row_index=row_index)
-    _rows("q", q)
-    _rows("out", out)
-    nb, kvh, d = _pool_shape(pool, q.shape[2])
-    T, NH, _ = q.shape
-    _check(out.shape == q.shape and out.dtype == q.dtype, "out must have q's shape and dtype")
-    _check(NH > 0 and NH % kvh == 0 and NH // kvh <= 16,
-           "query heads must be a multiple of the kv heads, at most 16 per kv head")
-    _check(T == plan.num_tokens, "q does not have the plan's tokens")
+    dev = _device(pool, out, q, block_tables, plan.start_pos, row_index)
+    nb, kvh, d = _pool_shape(pool)
+    T, NH, dq, q_stride = _rows("q", q)
+    _, _, _, out_stride = _rows("out", out)
+    if dq != d:
+        _fail("head_dim does not match the pool's tiles")
+    if out.shape != q.shape or out.dtype != q.dtype:
+        _fail("out must have q's shape and dtype")
+    if NH <= 0 or NH % kvh or NH > 16 * kvh:
+        _fail("query heads must be a multiple of the kv heads, at most 16 per kv head")
+    if T != plan.num_tokens:
+        _fail("q does not have the plan's tokens")
     _index("row_index", row_index, plan.num_seqs)
-    _table("block_tables", block_tables, plan.num_seqs if row_index is None else None)
-    _check(block_tables.shape[1] >= plan.max_blocks, "block_tables is too narrow for the plan")
+    bt_stride, cols = _table("block_tables", block_tables, plan.num_seqs if row_index is None else None)
+    if cols < plan.max_blocks:
+        _fail("block_tables is too narrow for the plan")
     if plan.num_tiles == 0:
         return
-    shape = (plan.scratch_blocks, kvh, BLOCK, d)
-    with _on(pool):
-        k = torch.empty(shape, dtype=q.dtype, device=pool.device)
-        v = torch.empty(shape, dtype=q.dtype, device=pool.device)
-        dequantize(pool, block_tables, plan.lens, plan.tables, k, v, row_index=row_index)
-        N.check(N.lib().ti_paged_prefill_attention(
-            out.data_ptr(), out.stride(0), q.data_ptr(), q.stride(0), k.data_ptr(), v.data_ptr(),
-            plan.scratch_blocks, plan.tables.data_ptr(), plan.tables.stride(0),
-            plan.rows.data_ptr(), plan.start_pos.data_ptr(), plan.cu_seqlens.data_ptr(), plan.tile_seq.data_ptr(),
-            plan.tile_q0.data_ptr(), plan.num_tiles, NH, kvh, d, BLOCK, N.dtype_code(q.dtype),
-            N.stream_of(pool)))
+    lib, dt, nblk = N.lib(), N.dtype_code(q.dtype), plan.scratch_blocks
+    half = nblk * kvh * BLOCK * d                       # elements of K, then of V
+    tables, tab_stride = plan.tables.data_ptr(), plan.tables.stride(0)
+    with _on(dev):
+        stream = _stream(dev)
+        scratch = torch.empty(2 * half, dtype=q.dtype, device=pool.device)
+        k = scratch.data_ptr()
+        v = k + 2 * half
+        N.check(lib.ti_kv4_dequantize(
+            k, v, nblk, pool.data_ptr(), nb, block_tables.data_ptr(), bt_stride, _ptr(row_index),
+            plan.lens.data_ptr(), tables, tab_stride, plan.num_seqs, plan.max_blocks, kvh, d,
+            BLOCK, dt, stream))
+        N.check(lib.ti_paged_prefill_attention(
+            out.data_ptr(), out_stride, q.data_ptr(), q_stride, k, v, nblk, tables, tab_stride,
+            plan.rows.data_ptr(), plan.start_pos.data_ptr(), plan.cu_seqlens.data_ptr(),
+            plan.tile_seq.data_ptr(), plan.tile_q0.data_ptr(), plan.num_tiles, NH, kvh, d, BLOCK,
+            dt, stream))
 
 
 def evict(pool: torch.Tensor, weights: torch.Tensor, block_tables: torch.Tensor,
@@ -341,35 +384,36 @@ def evict(pool: torch.Tensor, weights: torch.Tensor, block_tables: torch.Tensor,
     caller shortens the lengths to min(context_lens, keep) and frees the blocks behind.  A sequence
     with a needed table entry outside the pool is left as it is and raises TI_DEVERR_BAD_INPUT.
     The sequences of a call share no block."""
-    _cuda(pool=pool, weights=weights, block_tables=block_tables, context_lens=context_lens,
-          row_index=row_index, out_block_tables=out_block_tables, kept=kept)
-    _check(pool.dim() in (3, 4), "pool must be [num_blocks, KVH, 18 D] or [layers, ...]")
+    dev = _device(pool, weights, block_tables, context_lens, row_index, out_block_tables, kept)
+    if pool.dim() not in (3, 4) or not pool.is_contiguous():
+        _fail("pool must be contiguous [num_blocks, KVH, 18 D] or [layers, num_blocks, KVH, 18 D]")
     layers = pool.shape[0] if pool.dim() == 4 else 1
     if layers == 0:
         return
-    _check(pool.is_contiguous(), "pool must be contiguous")
     nb, kvh, d = _pool_shape(pool[0] if pool.dim() == 4 else pool)
-    _check(weights.dtype == torch.float32 and weights.is_contiguous() and
-           tuple(weights.shape) == (*pool.shape[:-1], BLOCK),
-           "weights must be contiguous float32, the pool's shape with 16 in the last place")
+    if weights.dtype != torch.float32 or not weights.is_contiguous() or \
+            weights.shape != (*pool.shape[:-1], BLOCK):
+        _fail("weights must be contiguous float32, the pool's shape with 16 in the last place")
     keep, recent = int(keep), int(recent)
-    _check(keep >= 1 and 0 <= recent <= keep, "needs keep >= 1 and 0 <= recent <= keep")
+    if keep < 1 or not 0 <= recent <= keep:
+        _fail("needs keep >= 1 and 0 <= recent <= keep")
     B = context_lens.numel()
     _index("context_lens", context_lens)
     _index("row_index", row_index, B)
-    _table("block_tables", block_tables, B if row_index is None else None)
+    rows = B if row_index is None else None
+    bt_stride, cols = _table("block_tables", block_tables, rows)
     to = block_tables if out_block_tables is None else out_block_tables
-    _table("out_block_tables", to, B if row_index is None else block_tables.shape[0])
-    if kept is not None:
-        _check(kept.dtype == torch.int32 and kept.is_contiguous() and kept.dim() == 4 and
-               tuple(kept.shape[:3]) == (layers, B, kvh) and kept.shape[3] >= keep,
-               "kept must be contiguous int32 [layers, batch, num_kv_heads, >= keep]")
+    to_stride, to_cols = _table("out_block_tables", to, rows if rows is not None
+                                else block_tables.shape[0])
+    if kept is not None and (kept.dtype != torch.int32 or not kept.is_contiguous() or
+                             kept.dim() != 4 or kept.shape[:3] != (layers, B, kvh) or
+                             kept.shape[3] < keep):
+        _fail("kept must be contiguous int32 [layers, batch, num_kv_heads, >= keep]")
     if B == 0:
         return
-    with _on(pool):
+    with _on(dev):
         N.check(N.lib().ti_kv4_evict(
-            pool.data_ptr(), weights.data_ptr(), layers, nb, block_tables.data_ptr(),
-            block_tables.stride(0), to.data_ptr(), to.stride(0), _ptr(row_index),
-            context_lens.data_ptr(), B, block_tables.shape[1], to.shape[1], keep, recent,
-            _ptr(kept), kept.shape[3] if kept is not None else 0, kvh, d, BLOCK,
-            N.stream_of(pool)))
+            pool.data_ptr(), weights.data_ptr(), layers, nb, block_tables.data_ptr(), bt_stride,
+            to.data_ptr(), to_stride, _ptr(row_index), context_lens.data_ptr(), B, cols, to_cols,
+            keep, recent, _ptr(kept), kept.shape[3] if kept is not None else 0, kvh, d, BLOCK,
+            _stream(dev)))
