@@ -426,10 +426,13 @@ def test_prefill(kv4, nh, kvh, d, dtn, starts, counts):
 ])
 @pytest.mark.parametrize("kind", ["random", "ties", "odd"])
 @pytest.mark.parametrize("in_place", [True, False])
-def test_evict(kv4, d, kvh, layers, lens, keep, recent, kind, in_place):
+@pytest.mark.parametrize("wide", [False, True])
+def test_evict(kv4, d, kvh, layers, lens, keep, recent, kind, in_place, wide):
+    """wide: a table of more than 48 * 1024 tokens, which the kernel for long sequences serves."""
     rng = np.random.default_rng(keep)
     lens = np.array(lens, np.int32)
-    tables, nb = tables_for(rng, lens, spare=sum(-(-min(n, keep) // 16) for n in lens) + 3)
+    tables, nb = tables_for(rng, lens, spare=sum(-(-min(n, keep) // 16) for n in lens) + 3,
+                            width=3100 if wide else None)
     pool = rng.integers(0, 256, (layers, nb, kvh, 18 * d), dtype=np.uint8)
     w = (rng.random((layers, nb, kvh, 16)) ** 4).astype(np.float32)
     if kind == "ties":

@@ -91,7 +91,7 @@ __device__ __forceinline__ uint2 quantize16(const float (&f)[16], uint32_t& scal
   const float r = __frcp_rn(s);
   float y[16];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) y[i] = __fsub_rn(__fadd_rn(__fmul_rn(f[i], r), 384.f), 384.f);
+  for (int i = 0; i < 16; ++i) y[i] = __fsub_rn(__fmaf_rn(f[i], r, 384.f), 384.f);
   return make_uint2(floats_to_codes(y), floats_to_codes(y + 8));
 }
 

@@ -1,6 +1,7 @@
 // The 4-bit KV cache's writes and moves: quantise-and-append (with or without RoPE), read back as
 // 16-bit values, and eviction by accumulated attention weight.  Format: kv4.cuh.
 #include <algorithm>
+#include <atomic>
 
 #include "capi_internal.h"
 #include "common.cuh"
@@ -34,9 +35,9 @@ __device__ __forceinline__ void store_group(uint8_t* tile, bool is_v, int off, i
 }
 
 // ---- append -------------------------------------------------------------------------------------
-// One thread per (token, K or V of a head, group of 16 dims): 32 bytes in, 9 bytes out.  The
-// groups of a token run over neighbouring lanes and then the tokens, so a warp writes whole
-// 32-byte rows of codes and runs of scale bytes.
+// One thread per (token, group of 16 dims), grid.y over K and V of the heads: 32 bytes in, 9 bytes
+// out.  The groups of a token run over neighbouring lanes and then the tokens, so a warp reads whole
+// lines and writes whole 32-byte rows of codes and runs of scale bytes.
 struct AppendParams {
   uint8_t* pool;
   float* weights;                    // attention-weight totals to clear for the new tokens, or null
@@ -52,22 +53,22 @@ __global__ void append_kernel(AppendParams p) {
   pdl_wait();
   pdl_launch_dependents();
   using L = Tile<HD>;
-  const int64_t per = (int64_t)p.tokens * L::kGroups, total = per * 2 * p.KVH;
+  const int h = blockIdx.y >> 1;
+  const bool is_v = blockIdx.y & 1;
+  const T* base = is_v ? (const T*)p.v + h * p.v_head : (const T*)p.k + h * p.k_head;
+  const int64_t stride = is_v ? p.v_tok : p.k_tok;
+  const int64_t total = (int64_t)p.tokens * L::kGroups;
   for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total;
        i += (int64_t)gridDim.x * blockDim.x) {
-    const int hv = (int)(i / per), h = hv >> 1, g = (int)(i % L::kGroups);
-    const int t = (int)((i % per) / L::kGroups);
-    const bool is_v = hv & 1;
+    const int t = (int)(i / L::kGroups), g = (int)(i % L::kGroups);
     const int64_t slot = p.slots[t];
+    float f[16];
+    load16(base + t * stride + g * kGroup, f);
     if (slot < 0) continue;
     if (slot >= p.pool_slots) {
-      if (hv == 0 && g == 0) raise_device_error(TI_DEVERR_BAD_INPUT);
+      if (blockIdx.y == 0 && g == 0) raise_device_error(TI_DEVERR_BAD_INPUT);
       continue;
     }
-    const T* src = is_v ? (const T*)p.v + t * p.v_tok + h * p.v_head
-                        : (const T*)p.k + t * p.k_tok + h * p.k_head;
-    float f[16];
-    load16(src + g * kGroup, f);
     const int64_t tile = (slot / kBlock) * p.KVH + h;
     const int off = (int)(slot % kBlock);
     store_group<HD>(p.pool + tile * L::kBytes, is_v, off, g, f);
@@ -77,7 +78,7 @@ __global__ void append_kernel(AppendParams p) {
 
 // ---- read back ------------------------------------------------------------------------------------
 // One thread per (table entry, head, K or V, token, group): 9 bytes in, 32 bytes out; zeros behind
-// the row's length.
+// the row's length.  A CTA of 256 threads takes one or two whole tiles at a time.
 struct DequantParams {
   void *k_out, *v_out;
   int64_t out_blocks;
@@ -92,35 +93,35 @@ struct DequantParams {
   int rows, max_blocks, KVH;
 };
 
+constexpr int kDequantThreads = 256;
+
 template <typename T, int HD>
-__global__ void dequantize_kernel(DequantParams p) {
+__global__ void __launch_bounds__(kDequantThreads) dequantize_kernel(DequantParams p) {
   pdl_wait();
   pdl_launch_dependents();
   using L = Tile<HD>;
   constexpr int kPerTile = 2 * kBlock * L::kGroups;
-  const int64_t entries = (int64_t)p.rows * p.max_blocks;
-  const int64_t total = entries * p.KVH * kPerTile;
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total;
-       i += (int64_t)gridDim.x * blockDim.x) {
-    const int w = (int)(i % kPerTile);
-    const int64_t eh = i / kPerTile;
-    const int h = (int)(eh % p.KVH);
-    const int64_t entry = eh / p.KVH;
-    const int r = (int)(entry / p.max_blocks), j = (int)(entry % p.max_blocks);
+  const int w = threadIdx.x % kPerTile;
+  const int64_t tiles = (int64_t)p.rows * p.max_blocks * p.KVH;
+  constexpr int kAtOnce = kDequantThreads / kPerTile;
+  for (int64_t i = (int64_t)blockIdx.x * kAtOnce + threadIdx.x / kPerTile; i < tiles;
+       i += (int64_t)gridDim.x * kAtOnce) {
+    // (a batch has fewer than 2^32 tiles: 32-bit divisions)
+    const uint32_t entry = (uint32_t)i / (uint32_t)p.KVH, h = (uint32_t)i - entry * p.KVH;
+    const uint32_t r = entry / (uint32_t)p.max_blocks, j = entry - r * p.max_blocks;
     const int len = p.lens[r];
-    if ((int64_t)j * kBlock >= len) continue;
     const int32_t dst = p.out_tables[r * p.ot_stride + j];
-    if (dst < 0) continue;
+    if ((int64_t)j * kBlock >= len || dst < 0) continue;
     if (dst >= p.out_blocks) {
       if (w == 0 && h == 0) raise_device_error(TI_DEVERR_BAD_INPUT);
       continue;
     }
-    const int32_t src = p.tables[(p.row_index ? p.row_index[r] : r) * p.bt_stride + j];
+    const int32_t src = p.tables[(p.row_index ? p.row_index[r] : (int)r) * p.bt_stride + j];
     const bool is_v = w >= kPerTile / 2;
     const int off = (w / L::kGroups) % kBlock, g = w % L::kGroups;
     Vec8<T> lo, hi;
     lo.raw = hi.raw = make_uint4(0u, 0u, 0u, 0u);
-    if (src >= 0 && src < p.num_blocks && j * kBlock + off < len) {
+    if (src >= 0 && src < p.num_blocks && (int)j * kBlock + off < len) {
       const uint8_t* tile = p.pool + ((int64_t)src * p.KVH + h) * L::kBytes;
       const uint2 c = *reinterpret_cast<const uint2*>(tile + (is_v ? L::kV : L::kK) +
                                                       off * L::kRow + g * 8);
@@ -150,10 +151,18 @@ __global__ void dequantize_kernel(DequantParams p) {
 // ---- eviction -------------------------------------------------------------------------------------
 // One CTA per (layer, sequence, kv head).  With n cached tokens and n > keep it keeps the last
 // `recent` and the keep - recent heaviest of the older ones (ties: the earlier token), in order.
-// The weight of the lightest kept token is found by a radix select over order-preserving 32-bit
-// keys (4 passes of 8 bits); then the tokens are scanned in order and each kept one's codes, scales
-// and weight move to the next place in front.  A place is never behind its token, and a round
-// reads all of its tokens before it writes any, so the move may be in place.
+//
+// evict_kernel: the weights become order-preserving 32-bit keys in shared memory, read once.  The
+// lightest kept key is found bit by bit from the top (how many keys are at least the trial value?),
+// leaving out the bits that all keys share and stopping as soon as the count is exact, which for
+// distinct weights is after about log2(n) bits.  Ranks come from one scan of (heavier, equal) counts;
+// the survivors' slots replace the keys in shared memory (a rank is never behind its token), then a
+// warp per block of 16 survivors moves their codes, scales and weights.  A survivor's place is never
+// behind its old one and a round reads all of its tokens before it writes any, so the move may be in
+// place.  Bound: HBM for a large batch, the chain of barriers for one sequence.
+//
+// evict_long_kernel: the same for sequences whose keys exceed shared memory, the weights read again
+// in each pass.
 struct EvictParams {
   uint8_t* pool;
   float* weights;
@@ -169,7 +178,10 @@ struct EvictParams {
   int batch, KVH, max_blocks, out_max_blocks, keep, recent;
 };
 
-constexpr int kEvictThreads = 256;
+constexpr int kEvictThreads = 512;
+constexpr int kEvictWarps = kEvictThreads / 32;
+constexpr int kEvictMaxTokens = 48 * 1024;       // keys of the longest sequence: 192 KB
+constexpr int kEvictLongThreads = 256;
 
 // Larger weight, larger key; NaN counts as the largest, -0 as 0.
 __device__ __forceinline__ uint32_t weight_key(float w) {
@@ -178,8 +190,207 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
+// The sequence's length if every block of it, and every block that its survivors go to, is in the
+// pool and the tables; else 0 (and the error bit, once).  All threads of the CTA call it.
+__device__ __forceinline__ int checked_length(const EvictParams& p, int row, int n, int threads) {
+  if (n <= 0) return 0;
+  const int32_t* src = p.tables + (int64_t)row * p.bt_stride;
+  const int32_t* dst = p.out_tables + (int64_t)row * p.ot_stride;
+  const int nb = (n - 1) / kBlock + 1, mb = (min(n, p.keep) - 1) / kBlock + 1;
+  bool bad = nb > p.max_blocks || mb > p.out_max_blocks;
+  if (!bad) {
+    for (int j = threadIdx.x; j < nb; j += threads) {
+      bad |= (uint32_t)src[j] >= (uint64_t)p.num_blocks;
+      if (j < mb) bad |= (uint32_t)dst[j] >= (uint64_t)p.num_blocks;
+    }
+  }
+  if (!__syncthreads_or(bad)) return n;
+  if (threadIdx.x == 0) raise_device_error(TI_DEVERR_BAD_INPUT);
+  return 0;
+}
+
 template <int HD>
 __global__ void __launch_bounds__(kEvictThreads) evict_kernel(EvictParams p) {
+  using L = Tile<HD>;
+  extern __shared__ __align__(16) uint32_t keys[];             // then the survivors' slots
+  __shared__ __align__(16) uint32_t s_count[2][kEvictWarps];
+  __shared__ uint32_t s_and, s_or;
+  const int h = blockIdx.x, b = blockIdx.y, layer = blockIdx.z;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int row = p.row_index ? p.row_index[b] : b;
+  const int n = checked_length(p, row, p.ctx[b], kEvictThreads);
+  if (n == 0) return;
+  const int32_t* src_row = p.tables + (int64_t)row * p.bt_stride;
+  const int32_t* dst_row = p.out_tables + (int64_t)row * p.ot_stride;
+  int32_t* kept = p.kept ? p.kept + ((int64_t)(layer * p.batch + b) * p.KVH + h) * p.kept_stride
+                         : nullptr;
+  uint8_t* pool = p.pool + (int64_t)layer * p.num_blocks * p.KVH * L::kBytes;
+  float* weights = p.weights + (int64_t)layer * p.num_blocks * p.KVH * kBlock;
+  const int m = min(n, p.keep);
+  const int old = n - p.recent;                   // candidates: positions 0 .. old-1
+  const int want = p.keep - p.recent;             // how many of them stay (when n > keep)
+  const bool all = n <= p.keep;
+  uint32_t bound = 0xFFFFFFFFu, ties = 0;         // keys above bound stay, and `ties` of those at it
+  if (!all && want > 0) {
+    if (tid == 0) { s_and = 0xFFFFFFFFu; s_or = 0; }
+    __syncthreads();
+    uint32_t both = 0xFFFFFFFFu, any = 0;
+    for (int i = tid * 4; i < old; i += kEvictThreads * 4) {    // four tokens of one block
+      const float4 w = *reinterpret_cast<const float4*>(
+          weights + ((int64_t)src_row[i / kBlock] * p.KVH + h) * kBlock + i % kBlock);
+      const float f[4] = {w.x, w.y, w.z, w.w};
+      uint32_t k[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        k[u] = weight_key(f[u]);
+        if (i + u < old) {
+          both &= k[u];
+          any |= k[u];
+        } else {
+          k[u] = 0;                               // below every trial value
+        }
+      }
+      *reinterpret_cast<uint4*>(keys + i) = make_uint4(k[0], k[1], k[2], k[3]);
+    }
+    both = __reduce_and_sync(0xffffffffu, both);
+    any = __reduce_or_sync(0xffffffffu, any);
+    if (lane == 0) {
+      atomicAnd(&s_and, both);
+      atomicOr(&s_or, any);
+    }
+    __syncthreads();
+    const uint32_t differ = s_and ^ s_or;
+    uint32_t low = s_and;                         // at least `want` keys are >= low
+    if (differ) low &= ~((2u << (31 - __clz(differ))) - 1u);
+    bool exact = false;
+    int pass = 0;
+    for (uint32_t bit = differ ? 1u << (31 - __clz(differ)) : 0u; bit && !exact; bit >>= 1, pass ^= 1) {
+      const uint32_t trial = low | bit;
+      uint32_t c = 0;
+      for (int i = tid * 4; i < old; i += kEvictThreads * 4) {
+        const uint4 k = *reinterpret_cast<const uint4*>(keys + i);
+        c += (k.x >= trial) + (k.y >= trial) + (k.z >= trial) + (k.w >= trial);
+      }
+      c = __reduce_add_sync(0xffffffffu, c);
+      if (lane == 0) s_count[pass][warp] = c;
+      __syncthreads();
+      c = __reduce_add_sync(0xffffffffu, lane < kEvictWarps ? s_count[pass][lane] : 0u);
+      if (c >= (uint32_t)want) low = trial;
+      exact = c == (uint32_t)want;
+    }
+    if (exact) {
+      bound = low - 1u;                           // keys >= low are exactly the wanted ones
+    } else {
+      // low is the key of the lightest kept token; the earliest ones of that key fill up
+      uint32_t c = 0;
+      for (int i = tid * 4; i < old; i += kEvictThreads * 4) {
+        const uint4 k = *reinterpret_cast<const uint4*>(keys + i);
+        c += (k.x > low) + (k.y > low) + (k.z > low) + (k.w > low);
+      }
+      c = __reduce_add_sync(0xffffffffu, c);
+      if (lane == 0) s_count[pass][warp] = c;
+      __syncthreads();
+      c = __reduce_add_sync(0xffffffffu, lane < kEvictWarps ? s_count[pass][lane] : 0u);
+      bound = low;
+      ties = (uint32_t)want - c;
+    }
+    __syncthreads();                              // s_count is used again below
+  }
+  // ranks: tokens above the bound and tokens at it before each token (16 bits each: 2048 a round)
+  uint32_t above = 0, at = 0;
+  for (int i0 = 0, pass = 0; i0 < n; i0 += kEvictThreads * 4, pass ^= 1) {
+    const int i = i0 + tid * 4;
+    uint32_t gt = 0, eq = 0;                      // bits of this thread's four tokens
+    if (i < n) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (i + u >= n) break;
+        if (all || i + u >= old) {
+          gt |= 1u << u;
+        } else if (want > 0) {
+          const uint32_t k = keys[i + u];
+          if (k > bound) gt |= 1u << u;
+          else if (k == bound) eq |= 1u << u;
+        }
+      }
+    }
+    const uint32_t mine = (uint32_t)__popc(gt) | ((uint32_t)__popc(eq) << 16);
+    uint32_t x = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const uint32_t y = __shfl_up_sync(0xffffffffu, x, d);
+      if (lane >= d) x += y;
+    }
+    if (lane == 31) s_count[pass][warp] = x;
+    __syncthreads();                              // (also: the round's keys have been read)
+    const uint32_t other = lane < kEvictWarps ? s_count[pass][lane] : 0u;
+    const uint32_t before = __reduce_add_sync(0xffffffffu, lane < warp ? other : 0u) + x - mine;
+    uint32_t r_gt = above + (before & 0xFFFFu), r_eq = at + (before >> 16);
+    const uint32_t round = __reduce_add_sync(0xffffffffu, other);
+    above += round & 0xFFFFu;
+    at += round >> 16;
+    if (gt | eq) {
+      const uint32_t slot = (uint32_t)src_row[i / kBlock] * kBlock + i % kBlock;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const bool is_eq = (eq >> u) & 1u, stay = ((gt >> u) & 1u) || (is_eq && r_eq < ties);
+        if (stay) {
+          const uint32_t rank = r_gt + min(r_eq, ties);
+          keys[rank] = slot + u;
+          if (kept) kept[rank] = i + u;
+        }
+        r_gt += (gt >> u) & 1u;
+        r_eq += is_eq;
+      }
+    }
+  }
+  __syncthreads();
+  // move: lane = (token of the block, K or V); kAtOnce blocks of a warp in flight
+  constexpr int kChunks = HD / 32, kBytes = HD / 16;             // 16-byte chunks, scale bytes
+  constexpr int kAtOnce = HD == 64 ? 4 : 2;
+  const int tok = lane & 15, part = lane >> 4, blocks = (m - 1) / kBlock + 1;
+  for (int j0 = 0; j0 < blocks; j0 += kEvictWarps * kAtOnce) {
+    uint4 c[kAtOnce][kChunks];
+    uint8_t sc[kAtOnce][kBytes];
+    float w[kAtOnce];
+    int32_t dst[kAtOnce];
+#pragma unroll
+    for (int a = 0; a < kAtOnce; ++a) {
+      const int j = j0 + a * kEvictWarps + warp;
+      dst[a] = -1;
+      if (j * kBlock + tok >= m) continue;
+      dst[a] = dst_row[j];
+      const uint32_t slot = keys[j * kBlock + tok];
+      const int64_t tile = (int64_t)(slot / kBlock) * p.KVH + h;
+      const int off = (int)(slot % kBlock);
+      const uint8_t* src = pool + tile * L::kBytes;
+#pragma unroll
+      for (int u = 0; u < kChunks; ++u)
+        c[a][u] = *reinterpret_cast<const uint4*>(src + (part ? L::kV : L::kK) + off * L::kRow + u * 16);
+#pragma unroll
+      for (int u = 0; u < kBytes; ++u) sc[a][u] = src[(part ? L::kVs : L::kKs) + u * kBlock + off];
+      if (part == 0) w[a] = weights[tile * kBlock + off];
+    }
+    __syncthreads();                              // the round's tokens have been read
+#pragma unroll
+    for (int a = 0; a < kAtOnce; ++a) {
+      if (dst[a] < 0) continue;
+      const int64_t tile = (int64_t)dst[a] * p.KVH + h;
+      uint8_t* to = pool + tile * L::kBytes;
+#pragma unroll
+      for (int u = 0; u < kChunks; ++u)
+        *reinterpret_cast<uint4*>(to + (part ? L::kV : L::kK) + tok * L::kRow + u * 16) = c[a][u];
+#pragma unroll
+      for (int u = 0; u < kBytes; ++u) to[(part ? L::kVs : L::kKs) + u * kBlock + tok] = sc[a][u];
+      if (part == 0) weights[tile * kBlock + tok] = w[a];
+    }
+  }
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kEvictLongThreads) evict_long_kernel(EvictParams p) {
   pdl_wait();
   pdl_launch_dependents();
   using L = Tile<HD>;
@@ -187,32 +398,14 @@ __global__ void __launch_bounds__(kEvictThreads) evict_kernel(EvictParams p) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   __shared__ uint32_t hist[256];
   __shared__ uint32_t s_prefix, s_left;
-  __shared__ int s_bad, s_warp[kEvictThreads / 32];
+  __shared__ int s_warp[kEvictLongThreads / 32];
   const int row = p.row_index ? p.row_index[b] : b;
-  const int n = p.ctx[b];
-  if (n <= 0) return;
+  const int n = checked_length(p, row, p.ctx[b], kEvictLongThreads);
+  if (n == 0) return;
   int32_t* kept = p.kept ? p.kept + ((int64_t)(layer * p.batch + b) * p.KVH + h) * p.kept_stride
                          : nullptr;
   const int32_t* src_row = p.tables + (int64_t)row * p.bt_stride;
   const int32_t* dst_row = p.out_tables + (int64_t)row * p.ot_stride;
-  const int m = min(n, p.keep);
-  // every block of the sequence, and every block that the survivors go to, has to be in the pool
-  const int nb = (n - 1) / kBlock + 1, mb = (m - 1) / kBlock + 1;
-  if (tid == 0) s_bad = (nb > p.max_blocks || mb > p.out_max_blocks);
-  __syncthreads();
-  if (!s_bad) {
-    bool bad = false;
-    for (int j = tid; j < nb; j += kEvictThreads) {
-      bad |= (uint32_t)src_row[j] >= (uint64_t)p.num_blocks;
-      if (j < mb) bad |= (uint32_t)dst_row[j] >= (uint64_t)p.num_blocks;
-    }
-    if (bad) s_bad = 1;
-  }
-  __syncthreads();
-  if (s_bad) {
-    if (tid == 0) raise_device_error(TI_DEVERR_BAD_INPUT);
-    return;
-  }
   uint8_t* pool = p.pool + (int64_t)layer * p.num_blocks * p.KVH * L::kBytes;
   float* weights = p.weights + (int64_t)layer * p.num_blocks * p.KVH * kBlock;
   auto tile_of = [&](const int32_t* r, int i) { return (int64_t)r[i / kBlock] * p.KVH + h; };
@@ -225,7 +418,7 @@ __global__ void __launch_bounds__(kEvictThreads) evict_kernel(EvictParams p) {
       hist[tid] = 0;
       __syncthreads();
       const uint32_t prefix = s_prefix;
-      for (int i = tid; i < old; i += kEvictThreads) {
+      for (int i = tid; i < old; i += kEvictLongThreads) {
         const uint32_t key = weight_key(weights[tile_of(src_row, i) * kBlock + i % kBlock]);
         if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8)))
           atomicAdd(&hist[(key >> shift) & 255u], 1u);
@@ -245,7 +438,7 @@ __global__ void __launch_bounds__(kEvictThreads) evict_kernel(EvictParams p) {
   }
   int placed = 0;
   uint32_t tied = 0;
-  for (int i0 = 0; i0 < n; i0 += kEvictThreads) {
+  for (int i0 = 0; i0 < n; i0 += kEvictLongThreads) {
     const int i = i0 + tid;
     uint32_t key = 0;
     bool in = i < n, gt = false, eq = false;
@@ -269,7 +462,7 @@ __global__ void __launch_bounds__(kEvictThreads) evict_kernel(EvictParams p) {
       __syncthreads();
       int before = 0;
       total = 0;
-      for (int k = 0; k < kEvictThreads / 32; ++k) {
+      for (int k = 0; k < kEvictLongThreads / 32; ++k) {
         if (k < warp) before += s_warp[k];
         total += s_warp[k];
       }
@@ -358,9 +551,13 @@ extern "C" int ti_kv4_append(void* pool, float* weights, const void* k, int64_t 
   kv4::AppendParams p{(uint8_t*)pool, weights, k, v, k_tok_stride, k_head_stride, v_tok_stride,
                       v_head_stride, slot_mapping, num_blocks * kv4::kBlock, num_tokens,
                       num_kv_heads};
-  const dim3 grid(kv4::grid_for((int64_t)num_tokens * num_kv_heads * (head_dim / 8), 256));
+  if (num_kv_heads > 32767)
+    return set_error(TI_ERR_UNSUPPORTED, "kv4_append: at most 32767 kv heads");
+  // few tokens in small blocks, so that they spread over the SMs
+  const int threads = num_tokens <= 1024 ? 64 : 256;
+  const dim3 grid(kv4::grid_for((int64_t)num_tokens * (head_dim / 16), threads), 2 * num_kv_heads);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  auto go = [&](auto kern) { return launch_kernel("kv4_append launch", kern, grid, dim3(256), 0, s, 1, p); };
+  auto go = [&](auto kern) { return launch_kernel("kv4_append launch", kern, grid, dim3(threads), 0, s, 1, p); };
   if (dtype == TI_DTYPE_BF16)
     return head_dim == 64 ? go(kv4::append_kernel<__nv_bfloat16, 64>)
                           : go(kv4::append_kernel<__nv_bfloat16, 128>);
@@ -388,7 +585,10 @@ extern "C" int ti_kv4_dequantize(void* k_out, void* v_out, int64_t out_blocks, c
   kv4::DequantParams p{k_out, v_out, out_blocks, (const uint8_t*)pool, num_blocks, block_tables,
                        bt_stride, row_index, lens, out_tables, ot_stride, rows, max_blocks,
                        num_kv_heads};
-  const dim3 grid(kv4::grid_for((int64_t)rows * max_blocks * num_kv_heads * 2 * head_dim, 256));
+  if ((int64_t)rows * max_blocks * num_kv_heads >= (int64_t)1 << 32)
+    return set_error(TI_ERR_UNSUPPORTED, "kv4_dequantize: rows * max_blocks * kv heads must be below 2^32");
+  const dim3 grid(kv4::grid_for((int64_t)rows * max_blocks * num_kv_heads * 2 * head_dim,
+                                kv4::kDequantThreads));
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   auto go = [&](auto kern) { return launch_kernel("kv4_dequantize launch", kern, grid, dim3(256), 0, s, 1, p); };
   if (dtype == TI_DTYPE_BF16)
@@ -417,8 +617,8 @@ extern "C" int ti_kv4_evict(void* pool, float* weights, int num_layers, int64_t 
     return set_error(TI_ERR_INVALID_ARGUMENT, "kv4_evict: needs 1 <= keep and 0 <= recent <= keep");
   if (kept && kept_stride < keep)
     return set_error(TI_ERR_INVALID_ARGUMENT, "kv4_evict: kept rows are shorter than keep");
-  if (reinterpret_cast<uintptr_t>(pool) & 15)
-    return set_error(TI_ERR_INVALID_ARGUMENT, "kv4_evict: the pool must be 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(pool) | reinterpret_cast<uintptr_t>(weights)) & 15)
+    return set_error(TI_ERR_INVALID_ARGUMENT, "kv4_evict: pool and weights must be 16-byte aligned");
   if (batch > 65535 || num_layers > 65535)
     return set_error(TI_ERR_UNSUPPORTED, "kv4_evict: at most 65535 sequences and layers");
   kv4::EvictParams p{(uint8_t*)pool, weights, num_blocks, block_tables, bt_stride, out_tables,
@@ -426,6 +626,27 @@ extern "C" int ti_kv4_evict(void* pool, float* weights, int num_layers, int64_t 
                      max_blocks_per_seq, out_max_blocks, keep, recent};
   const dim3 grid(num_kv_heads, batch, num_layers);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return launch_kernel("kv4_evict launch", head_dim == 64 ? kv4::evict_kernel<64> : kv4::evict_kernel<128>,
-                       grid, dim3(kv4::kEvictThreads), 0, s, 1, p);
+  // the widest table bounds the sequences' lengths; slots are 32 bits in shared memory
+  const int64_t tokens = (int64_t)max_blocks_per_seq * kv4::kBlock;
+  if (tokens > kv4::kEvictMaxTokens || num_blocks > (int64_t)1 << 28)
+    return launch_kernel("kv4_evict launch", head_dim == 64 ? kv4::evict_long_kernel<64> : kv4::evict_long_kernel<128>,
+                         grid, dim3(kv4::kEvictLongThreads), 0, s, 1, p);
+  auto go = [&](auto kern, std::atomic<uint64_t>& ready) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const uint64_t bit = 1ull << (dev & 63);
+    if (!(ready.load(std::memory_order_acquire) & bit)) {
+      cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           kv4::kEvictMaxTokens * 4);
+      if (e != cudaSuccess) {
+        (void)cudaGetLastError();
+        return set_cuda_error(e, "cudaFuncSetAttribute(kv4_evict)");
+      }
+      ready.fetch_or(bit, std::memory_order_release);
+    }
+    return launch_kernel("kv4_evict launch", kern, grid, dim3(kv4::kEvictThreads),
+                         (size_t)tokens * 4, s, 1, p);
+  };
+  static std::atomic<uint64_t> ready64{0}, ready128{0};
+  return head_dim == 64 ? go(kv4::evict_kernel<64>, ready64) : go(kv4::evict_kernel<128>, ready128);
 }
