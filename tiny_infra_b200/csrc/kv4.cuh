@@ -13,8 +13,11 @@
 // contiguous over the tokens, so a tile's 16 tokens take one or two bytes per lane.
 #pragma once
 
+#include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <stdint.h>
+
+#include <type_traits>
 
 namespace ti {
 namespace kv4 {
@@ -63,36 +66,51 @@ __device__ __forceinline__ uint32_t floats_to_codes(const float* f) {
   return w;
 }
 
-// Quantise one group of 16 values (of a 16-bit type, held in fp32): 8 bytes of codes and the
-// scale byte.  scale = amax / 6 rounded to 4 significant bits (ties to even, steps of 2^-17 below
-// 2^-14), at most 10240; code = x / scale rounded to e2m1 (ties to even), saturating.  A group with
-// a NaN or an infinity becomes NaN as a whole (scale 0xFF); a group whose scale rounds to zero
-// (amax below 2^-18 * 6) becomes zero.
+// Quantise one group of 16 values (of a 16-bit type, held in fp32; `top` = the fp32 bits of their
+// largest magnitude): 8 bytes of codes and the scale byte.  scale = amax / 6 rounded to 4 significant
+// bits (ties to even, steps of 2^-17 below 2^-14), at most 10240; code = x / scale rounded to e2m1
+// (ties to even), saturating.  A group with a NaN or an infinity becomes NaN as a whole (scale 0xFF);
+// a group whose scale rounds to zero (amax at most 6 * 2^-18) becomes zero.
 //
-// x / scale is formed as x * rn(1 / scale), off by less than 2^-20, then rounded to a multiple of
-// 2^-15: x has at most 11 significant bits and a midpoint of two codes times the scale at most 7,
-// so an x that is not on a midpoint is at least 2^-13 away from it after the division, and one
-// that is on it lands on it exactly.  The codes are therefore those of the exact quotient.
-__device__ __forceinline__ uint2 quantize16(const float (&f)[16], uint32_t& scale_byte) {
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(f[i]) & 0x7FFFFFFFu);
-  const float a = __fdiv_rn(__uint_as_float(top), 6.0f);
+// Both quotients are products with an approximate reciprocal, off by less than 2^-19 where they are
+// rounded, and are first rounded to a multiple of 2^-15 (the sum with 384): x and amax have at most 11
+// significant bits and a midpoint of two codes times the scale, or of two scales times 6, at most 7,
+// so a quotient that is not a midpoint is at least 2^-13 away from one (2^-8 for the scale's 8 .. 16),
+// and one that is lands on it exactly.  The results are therefore those of the exact quotients.
+__device__ __forceinline__ uint2 quantize16(const float (&f)[16], uint32_t top, uint32_t& scale_byte) {
+  const float a = __uint_as_float(top) * (1.0f / 6.0f);
   const int e = max((int)(__float_as_uint(a) >> 23) - 127, -14);
   const float inv_step = __uint_as_float((uint32_t)(127 + 3 - e) << 23);
   const float step = __uint_as_float((uint32_t)(127 - 3 + e) << 23);
-  const float s = fminf(rintf(a * inv_step) * step, kMaxScale);
+  const float s = fminf(rintf(__fsub_rn(__fmaf_rn(a, inv_step, 384.f), 384.f)) * step, kMaxScale);
   scale_byte = (uint32_t)__half_as_ushort(__float2half_rn(s)) >> 7;
   if (top >= 0x7F800000u) {
     scale_byte = kNanScale;
     return make_uint2(0u, 0u);
   }
   if (s == 0.f) return make_uint2(0u, 0u);
-  const float r = __frcp_rn(s);
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
   float y[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) y[i] = __fsub_rn(__fmaf_rn(f[i], r, 384.f), 384.f);
   return make_uint2(floats_to_codes(y), floats_to_codes(y + 8));
+}
+
+// fp32 bits of the largest magnitude of 16 values of a 16-bit type, two at a time (a NaN among them
+// comes through as one: at least the bits of infinity).
+template <typename T>
+__device__ __forceinline__ uint32_t largest16(const uint32_t (&w)[8]) {
+  using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+  T2 top;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t u = w[i] & 0x7FFF7FFFu;
+    const T2 v = *reinterpret_cast<const T2*>(&u);
+    top = i == 0 ? v : __hmax2_nan(top, v);
+  }
+  const float a = Elem<T>::to_f(top.x), b = Elem<T>::to_f(top.y);
+  return max(__float_as_uint(a), __float_as_uint(b));             // (both are >= 0, or NaN)
 }
 
 }  // namespace kv4

@@ -13,23 +13,21 @@ namespace kv4 {
 
 using ew::Vec8;
 
-// 16 consecutive elements of a 16-bit type as floats (two 16-byte loads).
-template <typename T>
-__device__ __forceinline__ void load16(const T* p, float (&f)[16]) {
-  Vec8<T> a, b;
-  a.load(p);
-  b.load(p + 8);
-  a.to_float(f);
-  b.to_float(f + 8);
-}
-
-// Store one quantised group of token `off` of a tile.
-template <int HD>
+// One quantised group of token `off` of a tile, from 16 elements of a 16-bit type.
+template <typename T, int HD>
 __device__ __forceinline__ void store_group(uint8_t* tile, bool is_v, int off, int g,
-                                            const float (&f)[16]) {
+                                            const uint4 lo, const uint4 hi) {
   using L = Tile<HD>;
+  const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+  float f[16];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float2 v = Elem<T>::unpack2(w[i]);
+    f[2 * i] = v.x;
+    f[2 * i + 1] = v.y;
+  }
   uint32_t sb;
-  const uint2 c = quantize16(f, sb);
+  const uint2 c = quantize16(f, largest16<T>(w), sb);
   *reinterpret_cast<uint2*>(tile + (is_v ? L::kV : L::kK) + off * L::kRow + g * 8) = c;
   tile[(is_v ? L::kVs : L::kKs) + g * kBlock + off] = (uint8_t)sb;
 }
@@ -62,23 +60,25 @@ __global__ void append_kernel(AppendParams p) {
        i += (int64_t)gridDim.x * blockDim.x) {
     const int t = (int)(i / L::kGroups), g = (int)(i % L::kGroups);
     const int64_t slot = p.slots[t];
-    float f[16];
-    load16(base + t * stride + g * kGroup, f);
+    const uint4* src = reinterpret_cast<const uint4*>(base + t * stride + g * kGroup);
+    const uint4 lo = src[0], hi = src[1];
     if (slot < 0) continue;
     if (slot >= p.pool_slots) {
       if (blockIdx.y == 0 && g == 0) raise_device_error(TI_DEVERR_BAD_INPUT);
       continue;
     }
-    const int64_t tile = (slot / kBlock) * p.KVH + h;
-    const int off = (int)(slot % kBlock);
-    store_group<HD>(p.pool + tile * L::kBytes, is_v, off, g, f);
+    const int64_t tile = (int64_t)((uint64_t)slot / kBlock) * p.KVH + h;
+    const int off = (int)slot & (kBlock - 1);
+    store_group<T, HD>(p.pool + tile * L::kBytes, is_v, off, g, lo, hi);
     if (p.weights && !is_v && g == 0) p.weights[tile * kBlock + off] = 0.f;
   }
 }
 
 // ---- read back ------------------------------------------------------------------------------------
-// One thread per (table entry, head, K or V, token, group): 9 bytes in, 32 bytes out; zeros behind
-// the row's length.  A CTA of 256 threads takes one or two whole tiles at a time.
+// One thread per (table entry, head, token, 8 dims), K and V both: 8 bytes of codes and 2 scales in,
+// 32 bytes out, the lanes of a warp on neighbouring 16 bytes (with 16 dims per thread the 16-byte
+// stores took half a sector each: 122 us instead of @@ for 393 MB); zeros behind the row's length.
+// grid = (runs of a row's blocks, head, row).
 struct DequantParams {
   void *k_out, *v_out;
   int64_t out_blocks;
@@ -94,57 +94,63 @@ struct DequantParams {
 };
 
 constexpr int kDequantThreads = 256;
+constexpr int kDequantUnroll = 2;                // tiles per thread
+
+// 8 values in a 16-bit type.
+template <typename T>
+__device__ __forceinline__ uint4 values8(uint32_t codes, uint32_t scale_byte) {
+  uint32_t h[4], w[4];
+  codes_to_half2(codes, h);
+  const float s = scale_value(scale_byte);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 v = Elem<__half>::unpack2(h[i]);
+    w[i] = Elem<T>::pack2(v.x * s, v.y * s);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(kDequantThreads) dequantize_kernel(DequantParams p) {
+  using L = Tile<HD>;
+  constexpr int kPer = HD / 8, kPerTile = kBlock * kPer, kTiles = kDequantThreads / kPerTile;
+  const int w = threadIdx.x % kPerTile, off = w / kPer, c = w % kPer, h = blockIdx.y;
+  const int code = off * L::kRow + c * 4, scale = (c / 2) * kBlock + off;
+  const int64_t j0 = (int64_t)blockIdx.x * (kTiles * kDequantUnroll) + threadIdx.x / kPerTile;
   pdl_wait();
   pdl_launch_dependents();
-  using L = Tile<HD>;
-  constexpr int kPerTile = 2 * kBlock * L::kGroups;
-  const int w = threadIdx.x % kPerTile;
-  const int64_t tiles = (int64_t)p.rows * p.max_blocks * p.KVH;
-  constexpr int kAtOnce = kDequantThreads / kPerTile;
-  for (int64_t i = (int64_t)blockIdx.x * kAtOnce + threadIdx.x / kPerTile; i < tiles;
-       i += (int64_t)gridDim.x * kAtOnce) {
-    // (a batch has fewer than 2^32 tiles: 32-bit divisions)
-    const uint32_t entry = (uint32_t)i / (uint32_t)p.KVH, h = (uint32_t)i - entry * p.KVH;
-    const uint32_t r = entry / (uint32_t)p.max_blocks, j = entry - r * p.max_blocks;
-    const int len = p.lens[r];
-    const int32_t dst = p.out_tables[r * p.ot_stride + j];
-    if ((int64_t)j * kBlock >= len || dst < 0) continue;
-    if (dst >= p.out_blocks) {
-      if (w == 0 && h == 0) raise_device_error(TI_DEVERR_BAD_INPUT);
-      continue;
-    }
-    const int32_t src = p.tables[(p.row_index ? p.row_index[r] : (int)r) * p.bt_stride + j];
-    const bool is_v = w >= kPerTile / 2;
-    const int off = (w / L::kGroups) % kBlock, g = w % L::kGroups;
-    Vec8<T> lo, hi;
-    lo.raw = hi.raw = make_uint4(0u, 0u, 0u, 0u);
-    if (src >= 0 && src < p.num_blocks && (int)j * kBlock + off < len) {
+  for (int r = blockIdx.z; r < p.rows; r += gridDim.z) {
+    const int64_t len = p.lens[r];
+    const int32_t* srcs = p.tables + (p.row_index ? p.row_index[r] : r) * p.bt_stride;
+    const int32_t* dsts = p.out_tables + r * p.ot_stride;
+    uint32_t kc[kDequantUnroll], vc[kDequantUnroll], ks[kDequantUnroll], vs[kDequantUnroll];
+    int32_t dst[kDequantUnroll];
+#pragma unroll
+    for (int u = 0; u < kDequantUnroll; ++u) {
+      const int64_t j = j0 + u * kTiles, left = len - j * kBlock;   // the row's tokens from block j on
+      kc[u] = vc[u] = ks[u] = vs[u] = 0u;
+      dst[u] = -1;
+      if (j >= p.max_blocks || left <= 0) continue;
+      dst[u] = dsts[j];
+      const int32_t src = srcs[j];
+      if (src < 0 || src >= p.num_blocks || off >= left) continue;
       const uint8_t* tile = p.pool + ((int64_t)src * p.KVH + h) * L::kBytes;
-      const uint2 c = *reinterpret_cast<const uint2*>(tile + (is_v ? L::kV : L::kK) +
-                                                      off * L::kRow + g * 8);
-      const float s = scale_value(tile[(is_v ? L::kVs : L::kKs) + g * kBlock + off]);
-      uint32_t h4[4];
-      float f[16];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        codes_to_half2(u ? c.y : c.x, h4);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float2 v = Elem<__half>::unpack2(h4[q]);
-          f[u * 8 + 2 * q] = v.x * s;
-          f[u * 8 + 2 * q + 1] = v.y * s;
-        }
-      }
-      lo.from_float(f);
-      hi.from_float(f + 8);
+      kc[u] = *reinterpret_cast<const uint32_t*>(tile + L::kK + code);
+      vc[u] = *reinterpret_cast<const uint32_t*>(tile + L::kV + code);
+      ks[u] = tile[L::kKs + scale];
+      vs[u] = tile[L::kVs + scale];
     }
-    T* out = (T*)(is_v ? p.v_out : p.k_out) +
-             (((int64_t)dst * p.KVH + h) * kBlock + off) * HD + g * kGroup;
-    lo.store(out);
-    hi.store(out + 8);
+#pragma unroll
+    for (int u = 0; u < kDequantUnroll; ++u) {
+      if (dst[u] < 0) continue;
+      if (dst[u] >= p.out_blocks) {
+        if (w == 0 && h == 0) raise_device_error(TI_DEVERR_BAD_INPUT);
+        continue;
+      }
+      const int64_t at = (((int64_t)dst[u] * p.KVH + h) * kBlock + off) * HD + c * 8;
+      *reinterpret_cast<uint4*>((T*)p.k_out + at) = values8<T>(kc[u], ks[u]);
+      *reinterpret_cast<uint4*>((T*)p.v_out + at) = values8<T>(vc[u], vs[u]);
+    }
   }
 }
 
@@ -210,7 +216,7 @@ __device__ __forceinline__ int checked_length(const EvictParams& p, int row, int
 }
 
 template <int HD>
-__global__ void __launch_bounds__(kEvictThreads) evict_kernel(EvictParams p) {
+__global__ void __launch_bounds__(kEvictThreads, 3) evict_kernel(EvictParams p) {
   using L = Tile<HD>;
   extern __shared__ __align__(16) uint32_t keys[];             // then the survivors' slots
   __shared__ __align__(16) uint32_t s_count[2][kEvictWarps];
@@ -347,44 +353,41 @@ __global__ void __launch_bounds__(kEvictThreads) evict_kernel(EvictParams p) {
     }
   }
   __syncthreads();
-  // move: lane = (token of the block, K or V); kAtOnce blocks of a warp in flight
-  constexpr int kChunks = HD / 32, kBytes = HD / 16;             // 16-byte chunks, scale bytes
-  constexpr int kAtOnce = HD == 64 ? 4 : 2;
-  const int tok = lane & 15, part = lane >> 4, blocks = (m - 1) / kBlock + 1;
-  for (int j0 = 0; j0 < blocks; j0 += kEvictWarps * kAtOnce) {
-    uint4 c[kAtOnce][kChunks];
-    uint8_t sc[kAtOnce][kBytes];
+  // move: HD/16 lanes a token, each 16 bytes of its K or V codes and two of their scales, so a warp
+  // reads and writes whole rows; kAtOnce groups of tokens of a warp in flight
+  constexpr int kLanes = HD / 16, kTok = 32 / kLanes, kAtOnce = 4;
+  const int part = (lane % kLanes) / (kLanes / 2), chunk = lane % (kLanes / 2);
+  const int code = (part ? L::kV : L::kK) + chunk * 16;
+  const int scale = (part ? L::kVs : L::kKs) + 2 * chunk * kBlock;
+  const bool has_weight = lane % kLanes == 0;
+  for (int j0 = 0; j0 < m; j0 += kEvictWarps * kAtOnce * kTok) {
+    uint4 c[kAtOnce];
+    uint32_t sc[kAtOnce];
     float w[kAtOnce];
-    int32_t dst[kAtOnce];
 #pragma unroll
     for (int a = 0; a < kAtOnce; ++a) {
-      const int j = j0 + a * kEvictWarps + warp;
-      dst[a] = -1;
-      if (j * kBlock + tok >= m) continue;
-      dst[a] = dst_row[j];
-      const uint32_t slot = keys[j * kBlock + tok];
+      const int to = j0 + (a * kEvictWarps + warp) * kTok + lane / kLanes;
+      if (to >= m) continue;
+      const uint32_t slot = keys[to];
       const int64_t tile = (int64_t)(slot / kBlock) * p.KVH + h;
       const int off = (int)(slot % kBlock);
       const uint8_t* src = pool + tile * L::kBytes;
-#pragma unroll
-      for (int u = 0; u < kChunks; ++u)
-        c[a][u] = *reinterpret_cast<const uint4*>(src + (part ? L::kV : L::kK) + off * L::kRow + u * 16);
-#pragma unroll
-      for (int u = 0; u < kBytes; ++u) sc[a][u] = src[(part ? L::kVs : L::kKs) + u * kBlock + off];
-      if (part == 0) w[a] = weights[tile * kBlock + off];
+      c[a] = *reinterpret_cast<const uint4*>(src + code + off * L::kRow);
+      sc[a] = src[scale + off] | ((uint32_t)src[scale + kBlock + off] << 8);
+      if (has_weight) w[a] = weights[tile * kBlock + off];
     }
     __syncthreads();                              // the round's tokens have been read
 #pragma unroll
     for (int a = 0; a < kAtOnce; ++a) {
-      if (dst[a] < 0) continue;
-      const int64_t tile = (int64_t)dst[a] * p.KVH + h;
-      uint8_t* to = pool + tile * L::kBytes;
-#pragma unroll
-      for (int u = 0; u < kChunks; ++u)
-        *reinterpret_cast<uint4*>(to + (part ? L::kV : L::kK) + tok * L::kRow + u * 16) = c[a][u];
-#pragma unroll
-      for (int u = 0; u < kBytes; ++u) to[(part ? L::kVs : L::kKs) + u * kBlock + tok] = sc[a][u];
-      if (part == 0) weights[tile * kBlock + tok] = w[a];
+      const int to = j0 + (a * kEvictWarps + warp) * kTok + lane / kLanes;
+      if (to >= m) continue;
+      const int64_t tile = (int64_t)dst_row[to / kBlock] * p.KVH + h;
+      const int off = to % kBlock;
+      uint8_t* dst = pool + tile * L::kBytes;
+      *reinterpret_cast<uint4*>(dst + code + off * L::kRow) = c[a];
+      dst[scale + off] = (uint8_t)sc[a];
+      dst[scale + kBlock + off] = (uint8_t)(sc[a] >> 8);
+      if (has_weight) weights[tile * kBlock + off] = w[a];
     }
   }
 }
@@ -585,12 +588,13 @@ extern "C" int ti_kv4_dequantize(void* k_out, void* v_out, int64_t out_blocks, c
   kv4::DequantParams p{k_out, v_out, out_blocks, (const uint8_t*)pool, num_blocks, block_tables,
                        bt_stride, row_index, lens, out_tables, ot_stride, rows, max_blocks,
                        num_kv_heads};
-  if ((int64_t)rows * max_blocks * num_kv_heads >= (int64_t)1 << 32)
-    return set_error(TI_ERR_UNSUPPORTED, "kv4_dequantize: rows * max_blocks * kv heads must be below 2^32");
-  const dim3 grid(kv4::grid_for((int64_t)rows * max_blocks * num_kv_heads * 2 * head_dim,
-                                kv4::kDequantThreads));
+  if (num_kv_heads > 65535)
+    return set_error(TI_ERR_UNSUPPORTED, "kv4_dequantize: at most 65535 kv heads");
+  const int per_cta = kv4::kDequantThreads / (2 * head_dim) * kv4::kDequantUnroll;   // tiles
+  const dim3 grid((unsigned)(((int64_t)max_blocks + per_cta - 1) / per_cta), num_kv_heads,
+                  std::min(rows, 65535));
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  auto go = [&](auto kern) { return launch_kernel("kv4_dequantize launch", kern, grid, dim3(256), 0, s, 1, p); };
+  auto go = [&](auto kern) { return launch_kernel("kv4_dequantize launch", kern, grid, dim3(kv4::kDequantThreads), 0, s, 1, p); };
   if (dtype == TI_DTYPE_BF16)
     return head_dim == 64 ? go(kv4::dequantize_kernel<__nv_bfloat16, 64>)
                           : go(kv4::dequantize_kernel<__nv_bfloat16, 128>);

@@ -59,10 +59,13 @@ def _stream(dev: int) -> int:
     return torch._C._cuda_getCurrentRawStream(dev)
 
 
-def _pool_shape(pool: torch.Tensor):
-    if pool.dtype != torch.uint8 or pool.dim() != 3 or not pool.is_contiguous():
-        _fail("pool must be a contiguous uint8 [num_blocks, num_kv_heads, 18 * head_dim] tensor")
-    nb, kvh, tile = pool.shape
+def _pool_shape(pool: torch.Tensor, layered: bool = False):
+    dims = pool.dim()
+    if pool.dtype != torch.uint8 or not pool.is_contiguous() or \
+            not (dims == 3 or layered and dims == 4):
+        _fail("pool must be a contiguous uint8 [num_blocks, num_kv_heads, 18 * head_dim] tensor"
+              + (" or [layers, ...]" if layered else ""))
+    nb, kvh, tile = pool.shape[-3:]
     if tile != 1152 and tile != 2304:
         _fail("pool tiles must be 18 * head_dim bytes, head_dim 64 or 128")
     if nb <= 0 or kvh <= 0:
@@ -385,12 +388,8 @@ def evict(pool: torch.Tensor, weights: torch.Tensor, block_tables: torch.Tensor,
     with a needed table entry outside the pool is left as it is and raises TI_DEVERR_BAD_INPUT.
     The sequences of a call share no block."""
     dev = _device(pool, weights, block_tables, context_lens, row_index, out_block_tables, kept)
-    if pool.dim() not in (3, 4) or not pool.is_contiguous():
-        _fail("pool must be contiguous [num_blocks, KVH, 18 D] or [layers, num_blocks, KVH, 18 D]")
+    nb, kvh, d = _pool_shape(pool, layered=True)
     layers = pool.shape[0] if pool.dim() == 4 else 1
-    if layers == 0:
-        return
-    nb, kvh, d = _pool_shape(pool[0] if pool.dim() == 4 else pool)
     if weights.dtype != torch.float32 or not weights.is_contiguous() or \
             weights.shape != (*pool.shape[:-1], BLOCK):
         _fail("weights must be contiguous float32, the pool's shape with 16 in the last place")
@@ -409,7 +408,7 @@ def evict(pool: torch.Tensor, weights: torch.Tensor, block_tables: torch.Tensor,
                              kept.dim() != 4 or kept.shape[:3] != (layers, B, kvh) or
                              kept.shape[3] < keep):
         _fail("kept must be contiguous int32 [layers, batch, num_kv_heads, >= keep]")
-    if B == 0:
+    if B == 0 or layers == 0:
         return
     with _on(dev):
         N.check(N.lib().ti_kv4_evict(
