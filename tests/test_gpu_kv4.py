@@ -423,6 +423,8 @@ def test_prefill(kv4, nh, kvh, d, dtn, starts, counts):
     (64, 2, 2, [1000, 1, 16, 2000], 16, 3),
     (64, 2, 1, [3000, 2999], 1500, 100),
     (64, 1, 1, [20000], 9000, 64),
+    (64, 2, 24, [130, 5, 64, 33, 200, 77, 1, 90], 50, 7),     # many units: the small CTAs
+    (128, 3, 30, [40, 120, 80, 300], 64, 0),
 ])
 @pytest.mark.parametrize("kind", ["random", "ties", "odd"])
 @pytest.mark.parametrize("in_place", [True, False])

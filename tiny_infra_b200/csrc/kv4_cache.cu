@@ -77,7 +77,7 @@ __global__ void append_kernel(AppendParams p) {
 // ---- read back ------------------------------------------------------------------------------------
 // One thread per (table entry, head, token, 8 dims), K and V both: 8 bytes of codes and 2 scales in,
 // 32 bytes out, the lanes of a warp on neighbouring 16 bytes (with 16 dims per thread the 16-byte
-// stores took half a sector each: 122 us instead of @@ for 393 MB); zeros behind the row's length.
+// stores took half a sector each: 122 us instead of 105 for 393 MB); zeros behind the row's length.
 // grid = (runs of a row's blocks, head, row).
 struct DequantParams {
   void *k_out, *v_out;
@@ -159,9 +159,9 @@ __global__ void __launch_bounds__(kDequantThreads) dequantize_kernel(DequantPara
 // `recent` and the keep - recent heaviest of the older ones (ties: the earlier token), in order.
 //
 // evict_kernel: the weights become order-preserving 32-bit keys in shared memory, read once.  The
-// lightest kept key is found bit by bit from the top (how many keys are at least the trial value?),
-// leaving out the bits that all keys share and stopping as soon as the count is exact, which for
-// distinct weights is after about log2(n) bits.  Ranks come from one scan of (heavier, equal) counts;
+// lightest kept key is found two bits at a time from the top (how many keys are at least each of the
+// three trial values?), leaving out the bits that all keys share and stopping as soon as a count is
+// exact, which for distinct weights is after about log2(n) bits below the exponent.  Ranks come from one scan of (heavier, equal) counts;
 // the survivors' slots replace the keys in shared memory (a rank is never behind its token), then a
 // warp per block of 16 survivors moves their codes, scales and weights.  A survivor's place is never
 // behind its old one and a round reads all of its tokens before it writes any, so the move may be in
@@ -184,8 +184,6 @@ struct EvictParams {
   int batch, KVH, max_blocks, out_max_blocks, keep, recent;
 };
 
-constexpr int kEvictThreads = 512;
-constexpr int kEvictWarps = kEvictThreads / 32;
 constexpr int kEvictMaxTokens = 48 * 1024;       // keys of the longest sequence: 192 KB
 constexpr int kEvictLongThreads = 256;
 
@@ -196,38 +194,36 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
-// The sequence's length if every block of it, and every block that its survivors go to, is in the
-// pool and the tables; else 0 (and the error bit, once).  All threads of the CTA call it.
-__device__ __forceinline__ int checked_length(const EvictParams& p, int row, int n, int threads) {
-  if (n <= 0) return 0;
-  const int32_t* src = p.tables + (int64_t)row * p.bt_stride;
-  const int32_t* dst = p.out_tables + (int64_t)row * p.ot_stride;
-  const int nb = (n - 1) / kBlock + 1, mb = (min(n, p.keep) - 1) / kBlock + 1;
+// Is any block that the sequence's n tokens or its m survivors need outside the pool or the tables?
+// Thread `tid` of `threads` looks at its share of the entries.
+__device__ __forceinline__ bool bad_entries(const EvictParams& p, const int32_t* src, const int32_t* dst,
+                                            int n, int m, int tid, int threads) {
+  const int nb = (n - 1) / kBlock + 1, mb = (m - 1) / kBlock + 1;
   bool bad = nb > p.max_blocks || mb > p.out_max_blocks;
-  if (!bad) {
-    for (int j = threadIdx.x; j < nb; j += threads) {
+  if (!bad)
+    for (int j = tid; j < nb; j += threads) {
       bad |= (uint32_t)src[j] >= (uint64_t)p.num_blocks;
       if (j < mb) bad |= (uint32_t)dst[j] >= (uint64_t)p.num_blocks;
     }
-  }
-  if (!__syncthreads_or(bad)) return n;
-  if (threadIdx.x == 0) raise_device_error(TI_DEVERR_BAD_INPUT);
-  return 0;
+  return bad;
 }
 
-template <int HD>
-__global__ void __launch_bounds__(kEvictThreads, 3) evict_kernel(EvictParams p) {
+template <int HD, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) evict_kernel(EvictParams p) {
   using L = Tile<HD>;
+  constexpr int kEvictWarps = kThreads / 32;
   extern __shared__ __align__(16) uint32_t keys[];             // then the survivors' slots
-  __shared__ __align__(16) uint32_t s_count[2][kEvictWarps];
+  __shared__ uint2 s_trial[2][kEvictWarps];
+  __shared__ uint32_t s_count[2][kEvictWarps];
   __shared__ uint32_t s_and, s_or;
   const int h = blockIdx.x, b = blockIdx.y, layer = blockIdx.z;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) { s_and = 0xFFFFFFFFu; s_or = 0; }
   pdl_wait();
   pdl_launch_dependents();
+  const int n = p.ctx[b];
+  if (n <= 0) return;
   const int row = p.row_index ? p.row_index[b] : b;
-  const int n = checked_length(p, row, p.ctx[b], kEvictThreads);
-  if (n == 0) return;
   const int32_t* src_row = p.tables + (int64_t)row * p.bt_stride;
   const int32_t* dst_row = p.out_tables + (int64_t)row * p.ot_stride;
   int32_t* kept = p.kept ? p.kept + ((int64_t)(layer * p.batch + b) * p.KVH + h) * p.kept_stride
@@ -237,15 +233,17 @@ __global__ void __launch_bounds__(kEvictThreads, 3) evict_kernel(EvictParams p) 
   const int m = min(n, p.keep);
   const int old = n - p.recent;                   // candidates: positions 0 .. old-1
   const int want = p.keep - p.recent;             // how many of them stay (when n > keep)
-  const bool all = n <= p.keep;
+  const bool all = n <= p.keep, pick = !all && want > 0;
   uint32_t bound = 0xFFFFFFFFu, ties = 0;         // keys above bound stay, and `ties` of those at it
-  if (!all && want > 0) {
-    if (tid == 0) { s_and = 0xFFFFFFFFu; s_or = 0; }
-    __syncthreads();
-    uint32_t both = 0xFFFFFFFFu, any = 0;
-    for (int i = tid * 4; i < old; i += kEvictThreads * 4) {    // four tokens of one block
-      const float4 w = *reinterpret_cast<const float4*>(
-          weights + ((int64_t)src_row[i / kBlock] * p.KVH + h) * kBlock + i % kBlock);
+  __syncthreads();
+  // the keys' loads and the check of the table entries overlap: a bad entry's weights are not read
+  uint32_t both = 0xFFFFFFFFu, any = 0;
+  if (pick && n <= p.max_blocks * (int64_t)kBlock) {
+    for (int i = tid * 4; i < old; i += kThreads * 4) {         // four tokens of one block
+      const uint32_t id = (uint32_t)src_row[i / kBlock];
+      float4 w = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (id < (uint64_t)p.num_blocks)
+        w = *reinterpret_cast<const float4*>(weights + ((int64_t)id * p.KVH + h) * kBlock + i % kBlock);
       const float f[4] = {w.x, w.y, w.z, w.w};
       uint32_t k[4];
 #pragma unroll
@@ -266,47 +264,65 @@ __global__ void __launch_bounds__(kEvictThreads, 3) evict_kernel(EvictParams p) 
       atomicAnd(&s_and, both);
       atomicOr(&s_or, any);
     }
-    __syncthreads();
+  }
+  if (__syncthreads_or(bad_entries(p, src_row, dst_row, n, m, tid, kThreads))) {
+    if (tid == 0) raise_device_error(TI_DEVERR_BAD_INPUT);
+    return;
+  }
+  if (pick) {
     const uint32_t differ = s_and ^ s_or;
+    const int top = differ ? (31 - __clz(differ)) | 1 : -1;      // odd: pairs of bits from here down
     uint32_t low = s_and;                         // at least `want` keys are >= low
-    if (differ) low &= ~((2u << (31 - __clz(differ))) - 1u);
+    if (top >= 0) low &= ~((2u << top) - 1u);
     bool exact = false;
     int pass = 0;
-    for (uint32_t bit = differ ? 1u << (31 - __clz(differ)) : 0u; bit && !exact; bit >>= 1, pass ^= 1) {
-      const uint32_t trial = low | bit;
-      uint32_t c = 0;
-      for (int i = tid * 4; i < old; i += kEvictThreads * 4) {
+    for (int sh = top - 1; sh >= 0 && !exact; sh -= 2, pass ^= 1) {
+      const uint32_t t1 = low | (1u << sh), t2 = low | (2u << sh), t3 = low | (3u << sh);
+      uint32_t c12 = 0, c3 = 0;                   // counts of two trials in 16 bits each
+      for (int i = tid * 4; i < old; i += kThreads * 4) {
         const uint4 k = *reinterpret_cast<const uint4*>(keys + i);
-        c += (k.x >= trial) + (k.y >= trial) + (k.z >= trial) + (k.w >= trial);
+        const uint32_t v[4] = {k.x, k.y, k.z, k.w};
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          c12 += (v[u] >= t1) + ((uint32_t)(v[u] >= t2) << 16);
+          c3 += v[u] >= t3;
+        }
       }
-      c = __reduce_add_sync(0xffffffffu, c);
-      if (lane == 0) s_count[pass][warp] = c;
+      c12 = __reduce_add_sync(0xffffffffu, c12);
+      c3 = __reduce_add_sync(0xffffffffu, c3);
+      if (lane == 0) s_trial[pass][warp] = make_uint2(c12, c3);
       __syncthreads();
-      c = __reduce_add_sync(0xffffffffu, lane < kEvictWarps ? s_count[pass][lane] : 0u);
-      if (c >= (uint32_t)want) low = trial;
-      exact = c == (uint32_t)want;
+      const uint2 part = lane < kEvictWarps ? s_trial[pass][lane] : make_uint2(0u, 0u);
+      c12 = __reduce_add_sync(0xffffffffu, part.x);
+      c3 = __reduce_add_sync(0xffffffffu, part.y);
+      const uint32_t goal = (uint32_t)want, c1 = c12 & 0xFFFFu, c2 = c12 >> 16;
+      const uint32_t c = c3 >= goal ? c3 : c2 >= goal ? c2 : c1;
+      if (c3 >= goal) low = t3;
+      else if (c2 >= goal) low = t2;
+      else if (c1 >= goal) low = t1;
+      exact = c == goal;
     }
     if (exact) {
       bound = low - 1u;                           // keys >= low are exactly the wanted ones
     } else {
       // low is the key of the lightest kept token; the earliest ones of that key fill up
       uint32_t c = 0;
-      for (int i = tid * 4; i < old; i += kEvictThreads * 4) {
+      for (int i = tid * 4; i < old; i += kThreads * 4) {
         const uint4 k = *reinterpret_cast<const uint4*>(keys + i);
         c += (k.x > low) + (k.y > low) + (k.z > low) + (k.w > low);
       }
       c = __reduce_add_sync(0xffffffffu, c);
-      if (lane == 0) s_count[pass][warp] = c;
+      if (lane == 0) s_count[0][warp] = c;
       __syncthreads();
-      c = __reduce_add_sync(0xffffffffu, lane < kEvictWarps ? s_count[pass][lane] : 0u);
+      c = __reduce_add_sync(0xffffffffu, lane < kEvictWarps ? s_count[0][lane] : 0u);
       bound = low;
       ties = (uint32_t)want - c;
+      __syncthreads();                            // s_count is used again below
     }
-    __syncthreads();                              // s_count is used again below
   }
-  // ranks: tokens above the bound and tokens at it before each token (16 bits each: 2048 a round)
+  // ranks: tokens above the bound and tokens at it before each token (16 bits each in a round)
   uint32_t above = 0, at = 0;
-  for (int i0 = 0, pass = 0; i0 < n; i0 += kEvictThreads * 4, pass ^= 1) {
+  for (int i0 = 0, pass = 0; i0 < n; i0 += kThreads * 4, pass ^= 1) {
     const int i = i0 + tid * 4;
     uint32_t gt = 0, eq = 0;                      // bits of this thread's four tokens
     if (i < n) {
@@ -403,12 +419,16 @@ __global__ void __launch_bounds__(kEvictLongThreads) evict_long_kernel(EvictPara
   __shared__ uint32_t s_prefix, s_left;
   __shared__ int s_warp[kEvictLongThreads / 32];
   const int row = p.row_index ? p.row_index[b] : b;
-  const int n = checked_length(p, row, p.ctx[b], kEvictLongThreads);
-  if (n == 0) return;
+  const int n = p.ctx[b];
+  if (n <= 0) return;
   int32_t* kept = p.kept ? p.kept + ((int64_t)(layer * p.batch + b) * p.KVH + h) * p.kept_stride
                          : nullptr;
   const int32_t* src_row = p.tables + (int64_t)row * p.bt_stride;
   const int32_t* dst_row = p.out_tables + (int64_t)row * p.ot_stride;
+  if (__syncthreads_or(bad_entries(p, src_row, dst_row, n, min(n, p.keep), tid, kEvictLongThreads))) {
+    if (tid == 0) raise_device_error(TI_DEVERR_BAD_INPUT);
+    return;
+  }
   uint8_t* pool = p.pool + (int64_t)layer * p.num_blocks * p.KVH * L::kBytes;
   float* weights = p.weights + (int64_t)layer * p.num_blocks * p.KVH * kBlock;
   auto tile_of = [&](const int32_t* r, int i) { return (int64_t)r[i / kBlock] * p.KVH + h; };
@@ -635,22 +655,28 @@ extern "C" int ti_kv4_evict(void* pool, float* weights, int num_layers, int64_t 
   if (tokens > kv4::kEvictMaxTokens || num_blocks > (int64_t)1 << 28)
     return launch_kernel("kv4_evict launch", head_dim == 64 ? kv4::evict_long_kernel<64> : kv4::evict_long_kernel<128>,
                          grid, dim3(kv4::kEvictLongThreads), 0, s, 1, p);
-  auto go = [&](auto kern, std::atomic<uint64_t>& ready) {
+  // Many (layer, sequence, head) units: small CTAs, several per SM; few: wide ones, the chain of one
+  // unit counts.  24 layers x 2 heads, one sequence of 2048: 17 us with 512 threads, 23 with 256; 32
+  // sequences of up to 4096: 111 and 99 (cold caches).
+  auto go = [&](auto hd) {
+    constexpr int HD = decltype(hd)::value;
+    static std::atomic<uint64_t> ready[2];
+    const bool small = (int64_t)num_kv_heads * batch * num_layers > 2 * kv4::sm_count();
+    auto kern = small ? kv4::evict_kernel<HD, 256> : kv4::evict_kernel<HD, 512>;
     int dev = 0;
     cudaGetDevice(&dev);
     const uint64_t bit = 1ull << (dev & 63);
-    if (!(ready.load(std::memory_order_acquire) & bit)) {
+    if (!(ready[small].load(std::memory_order_acquire) & bit)) {
       cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                            kv4::kEvictMaxTokens * 4);
       if (e != cudaSuccess) {
         (void)cudaGetLastError();
         return set_cuda_error(e, "cudaFuncSetAttribute(kv4_evict)");
       }
-      ready.fetch_or(bit, std::memory_order_release);
+      ready[small].fetch_or(bit, std::memory_order_release);
     }
-    return launch_kernel("kv4_evict launch", kern, grid, dim3(kv4::kEvictThreads),
-                         (size_t)tokens * 4, s, 1, p);
+    return launch_kernel("kv4_evict launch", kern, grid, dim3(small ? 256 : 512), (size_t)tokens * 4,
+                         s, 1, p);
   };
-  static std::atomic<uint64_t> ready64{0}, ready128{0};
-  return head_dim == 64 ? go(kv4::evict_kernel<64>, ready64) : go(kv4::evict_kernel<128>, ready128);
+  return head_dim == 64 ? go(std::integral_constant<int, 64>{}) : go(std::integral_constant<int, 128>{});
 }
