@@ -331,6 +331,17 @@ int ti_decode_prepare(const int32_t* tokens, const int32_t* slots, const int32_t
                       int32_t* ctx_lens, float* hidden, const void* embed, int hidden_size,
                       int64_t vocab, int rows, int dtype, void* stream);
 
+/* The same with positions[r] = seq_len[slot] + pos_offset[slot] (NULL: no offset): a sequence whose
+ * cache lost pos_offset[slot] tokens to eviction (ti_kv4_evict) goes on at its own positions.
+ * slot_mapping and ctx_lens follow seq_len, the cached length. */
+int ti_decode_prepare_ex(const int32_t* tokens, const int32_t* slots, const int32_t* new_block,
+                         const int32_t* seq_len, const int32_t* pos_offset, int32_t* block_tables,
+                         int64_t bt_stride, int num_slots, int max_blocks_per_seq,
+                         int64_t num_blocks, int block_size, int32_t* positions,
+                         int64_t* slot_mapping, int32_t* ctx_lens, float* hidden,
+                         const void* embed, int hidden_size, int64_t vocab, int rows, int dtype,
+                         void* stream);
+
 /* Greedy token per row from TI_EPI_ARGMAX partials (largest value, lowest index among equal
  * values; reference engine/scheduler.py:153 uses torch.argmax), written to out_tokens[rows].
  * If seq_len and slots are given, seq_len[slots[r]] += seq_inc for every slot >= 0
@@ -369,6 +380,14 @@ int ti_kv4_append(void* pool, float* weights, const void* k, int64_t k_tok_strid
                   int64_t v_head_stride, const int64_t* slot_mapping, int num_tokens,
                   int64_t num_blocks, int num_kv_heads, int head_dim, int block_size, int dtype,
                   void* stream);
+
+/* ti_rope_kv_append for the 4-bit pool: rows [q | k | v] of T new tokens (ti_rope_kv_append's
+ * layout); q and k are rotated in place, then k and v quantised into slot_mapping[t] as
+ * ti_kv4_append would from the rotated rows. */
+int ti_rope_kv4_append(void* qkv, int64_t qkv_stride, void* pool, float* weights,
+                       const int64_t* slot_mapping, const float* cos, const float* sin,
+                       const int32_t* pos, int num_tokens, int64_t num_blocks, int num_heads,
+                       int num_kv_heads, int head_dim, int block_size, int dtype, void* stream);
 
 /* Read the first lens[r] tokens of table row row_index[r] (NULL: r) back as 16-bit values: block j
  * goes to block out_tables[r][j] of k_out / v_out [out_blocks, num_kv_heads, 16, head_dim] (< 0:

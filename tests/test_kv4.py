@@ -166,3 +166,91 @@ def test_c_abi_refusals(native):
     refused(ev(bs=32), 2, b"block_size")
     refused(ev(pool=FAKE + 8), 1, b"aligned")
     refused(ev(layers=70000), 2, b"65535")
+
+    def rope(qkv=FAKE, stride=18 * 64, n=4, nb=8, d=64, bs=16, dt=0, nh=14):
+        return lib.ti_rope_kv4_append(qkv, stride, FAKE, None, FAKE, FAKE, FAKE, FAKE, n, nb, nh, 2,
+                                      d, bs, dt, None)
+    assert rope(n=0) == 0
+    refused(rope(qkv=None), 1, b"null")
+    refused(rope(nh=0), 1, b"negative size")
+    refused(rope(d=32), 2, b"head_dim")
+    refused(rope(dt=2), 2, b"dtype")
+    refused(rope(stride=18 * 64 + 4), 1, b"aligned")
+
+
+def test_allocator_truncate():
+    from tiny_infra_b200.cache_manager import BlockAllocator
+    a = BlockAllocator(2, 128, 16, 12)
+    a.plan_tokens([0, 1], [100, 40])
+    a.advance([0, 1], [100, 40])
+    row = a.block_tables[0].copy()
+    free = list(a.free_blocks)
+    a.truncate(0, 33)
+    assert (a.seq_len[0], a.pos_offset[0]) == (33, 67)
+    np.testing.assert_array_equal(a.block_tables[0, :3], row[:3])
+    assert (a.block_tables[0, 3:] == -1).all()
+    assert list(a.free_blocks) == free + row[3:7].tolist()        # in logical order, at the back
+    a.plan_tokens([0], [20])
+    a.advance([0], [20])
+    a.truncate(0, 48)
+    assert (a.seq_len[0], a.pos_offset[0]) == (48, 72)
+    a.truncate(0, 48)                                             # nothing to do
+    assert (a.seq_len[0], a.pos_offset[0]) == (48, 72)
+    for bad in (-1, 49):
+        with pytest.raises(ValueError):
+            a.truncate(0, bad)
+    a.truncate(0, 0)
+    assert (a.block_tables[0] == -1).all() and a.seq_len[0] == 0
+    a.free_slot(0)
+    a.free_slot(1)
+    assert a.pos_offset[0] == 0 and sorted(a.free_blocks) == list(range(12))
+
+
+def test_cache_manager_refusals():
+    from tiny_infra_b200.cache_manager import KVCacheManager
+    for kw in (dict(kv_bits=8), dict(track_weights=True), dict(kv_bits=4, block_size=32),
+               dict(max_positions=100)):
+        with pytest.raises(RuntimeError):
+            KVCacheManager(2, 128, 1, 2, 64, **kw)
+    with pytest.raises(RuntimeError):
+        KVCacheManager(2, 128, 1, 2, 96, kv_bits=4)
+
+
+def test_scheduler_evicts_before_decode():
+    """Sequences at evict_above tokens are brought down before the step, and only those."""
+    import asyncio
+
+    from tests.test_scheduler_trace import _HostKV, _StandInBackend
+    from tiny_infra_b200.scheduler import ContinuousBatcher, GenerationRequest
+    kv = _HostKV(dict(max_batch_size=3, max_seq_len=32, block_size=16, head_dim=64))
+    calls = []
+    kv.seq_len_host = lambda s: int(kv.alloc.seq_len[s])
+
+    def evict(slots, keep, recent):
+        calls.append((list(slots), [kv.seq_len_host(s) for s in slots], keep, recent))
+        for s in slots:
+            kv.alloc.truncate(s, keep)
+    kv.evict = evict
+    sched = ContinuousBatcher(None, kv, backend=_StandInBackend(kv, 1000), evict_above=20,
+                              evict_keep=12, evict_recent=5)
+
+    async def run():
+        for n, m in ((18, 30), (5, 9), (19, 2)):
+            sched.requests_queue.put_nowait(GenerationRequest(list(range(n)), m, 0.0))
+        sched._fill_active_slots()
+        reqs = list(sched.active_slots)
+        while sched._has_active_requests():
+            sched._step_generation()
+        return reqs
+    reqs = asyncio.run(run())
+    assert [len(r.generated_tokens) for r in reqs] == [30, 9, 2]
+    assert all(r.error is None for r in reqs)
+    # slot 0 reaches 20 after two steps and then again every 8 tokens
+    assert [c[:2] for c in calls] == [([0], [20])] * len(calls)
+    assert len(calls) == 1 + (29 - 2 - 1) // 8 and all(c[2:] == (12, 5) for c in calls)
+    assert sched.stats()["evictions"] == len(calls)
+    assert sorted(kv.alloc.free_blocks) == list(range(6))
+    for kw in (dict(evict_keep=3), dict(evict_above=20, evict_keep=20),
+               dict(evict_above=20, evict_keep=4, evict_recent=5), dict(evict_above=33)):
+        with pytest.raises(ValueError):
+            ContinuousBatcher(None, kv, backend=object(), **kw)

@@ -14,6 +14,14 @@ per token per layer; here the engine plans a whole step's allocations on host mi
 ``seq_len`` / ``block_tables`` once (not once per layer) and the device tables are updated by
 the step's own kernels.
 
+``kv_bits=4`` keeps the pool in 4 bits instead (``kv4_pool`` uint8 [L, num_blocks, KVH, 18 * D], see
+``kv4``; ``key_cache`` / ``value_cache`` are then None): the same tables, slots and allocation, 9/32 of
+the bytes.  With ``track_weights`` the model adds up each cached token's attention weight
+(``attn_weights`` float32 [L, num_blocks, KVH, block_size]) and ``evict`` brings sequences down to
+their recent and heaviest tokens; a sequence's next position then is ``seq_len + pos_offset``, and
+``max_positions`` (default ``max_seq_len``) bounds that position where ``max_seq_len`` bounds the
+cached tokens.
+
 Differences, by design: the pool lives on a CUDA device only; ``num_blocks`` may be given to
 size the pool independently of max_batch * max_blocks_per_seq (the reference's formula is the
 default); the free list is a deque (``pop(0)`` is O(1)).
@@ -26,6 +34,7 @@ import numpy as np
 import torch
 
 from . import _native as N
+from . import kv4
 
 
 class FreeBlockList(collections.deque):
@@ -58,6 +67,7 @@ class BlockAllocator:
                                       if num_blocks is None else int(num_blocks))
         self.free_blocks = FreeBlockList(range(self.total_physical_blocks))
         self.seq_len = np.zeros(max_batch_size, np.int32)
+        self.pos_offset = np.zeros(max_batch_size, np.int32)     # tokens evicted from each slot
         self.block_tables = np.full((max_batch_size, self.max_blocks_per_seq), -1, np.int32)
 
     def plan_tokens(self, slots, counts, *, strict_len: bool = True):
@@ -149,18 +159,43 @@ class BlockAllocator:
                 self.free_blocks.append(phys)
                 row[lb] = -1
         self.seq_len[batch_idx] = 0
+        self.pos_offset[batch_idx] = 0
+
+    def truncate(self, slot: int, keep: int) -> None:
+        """The slot's cache now holds ``keep`` of its tokens: the blocks behind go to the back of
+        the free list in logical order, and the slot's positions go on where they were."""
+        n = int(self.seq_len[slot])
+        if not 0 <= keep <= n:
+            raise ValueError(f"slot {slot} holds {n} tokens, cannot keep {keep}")
+        row = self.block_tables[slot]
+        for lb in range(-(-keep // self.block_size), self.max_blocks_per_seq):
+            phys = int(row[lb])
+            if phys != -1:
+                self.free_blocks.append(phys)
+                row[lb] = -1
+        self.seq_len[slot] = keep
+        self.pos_offset[slot] += n - keep
 
 
 class KVCacheManager:
     def __init__(self, max_batch_size: int, max_seq_len: int, num_layers: int, num_kv_heads: int,
                  head_dim: int, block_size: int = 16,
                  device: torch.device | str = "cuda", dtype: torch.dtype = torch.bfloat16,
-                 num_blocks: int | None = None) -> None:
+                 num_blocks: int | None = None, *, kv_bits: int = 16, track_weights: bool = False,
+                 max_positions: int | None = None) -> None:
         device = torch.device(device)
         if device.type != "cuda":
             raise RuntimeError("tiny_infra_b200 keeps the KV pool on a CUDA device")
         if dtype not in (torch.bfloat16, torch.float16):
             raise RuntimeError("KV pool dtype must be bfloat16 or float16")
+        if kv_bits not in (16, 4):
+            raise RuntimeError("kv_bits must be 16 or 4")
+        if kv_bits == 4 and (block_size != kv4.BLOCK or head_dim not in (64, 128)):
+            raise RuntimeError("the 4-bit KV pool needs block_size 16 and head_dim 64 or 128")
+        if track_weights and kv_bits != 4:
+            raise RuntimeError("attention weights are tracked for the 4-bit KV pool only")
+        if max_positions is not None and max_positions < max_seq_len:
+            raise RuntimeError("max_positions must be at least max_seq_len")
         self.max_batch_size = max_batch_size
         self.max_seq_len = max_seq_len
         self.num_layers = num_layers
@@ -172,15 +207,26 @@ class KVCacheManager:
         self.alloc = BlockAllocator(max_batch_size, max_seq_len, block_size, num_blocks)
         self.max_blocks_per_seq = self.alloc.max_blocks_per_seq
         self.total_physical_blocks = self.alloc.total_physical_blocks
+        self.kv_bits = kv_bits
+        self.max_positions = int(max_positions or max_seq_len)
         shape = (num_layers, self.total_physical_blocks, num_kv_heads, block_size, head_dim)
-        self.key_cache = torch.zeros(shape, device=device, dtype=dtype)
-        self.value_cache = torch.zeros(shape, device=device, dtype=dtype)
+        self.key_cache = self.value_cache = self.kv4_pool = self.attn_weights = None
+        if kv_bits == 4:
+            self.kv4_pool = kv4.new_pool(self.total_physical_blocks, num_kv_heads, head_dim,
+                                         num_layers=num_layers, device=device)
+            if track_weights:
+                self.attn_weights = torch.zeros(shape[:-1], device=device, dtype=torch.float32)
+        else:
+            self.key_cache = torch.zeros(shape, device=device, dtype=dtype)
+            self.value_cache = torch.zeros(shape, device=device, dtype=dtype)
+        self.pos_offset = torch.zeros(max_batch_size, device=device, dtype=torch.int32)
         self.seq_len = torch.zeros(max_batch_size, device=device, dtype=torch.int32)
         self.block_tables = torch.full((max_batch_size, self.max_blocks_per_seq), -1,
                                        dtype=torch.int32, device=device)
         # host mirrors (the allocator's arrays), authoritative for the engine's step planning
         self._seq_host = self.alloc.seq_len
         self._bt_host = self.alloc.block_tables
+        self._evicted = False            # has any slot's position left its cached length?
 
     @property
     def free_blocks(self) -> FreeBlockList:
@@ -193,13 +239,31 @@ class KVCacheManager:
         scheduler does with ``kv_cache.seq_len[idx] += n``."""
         self._seq_host[:] = self.seq_len.cpu().numpy()
         self._bt_host[:] = self.block_tables.cpu().numpy()
+        self.alloc.pos_offset[:] = self.pos_offset.cpu().numpy()
+        self._evicted = bool(self.alloc.pos_offset.any())
 
     def seq_len_host(self, slot: int) -> int:
         return int(self._seq_host[slot])
 
+    def position_host(self, slot: int) -> int:
+        """Position of the slot's next token: its cached length plus the tokens evicted."""
+        return int(self._seq_host[slot] + self.alloc.pos_offset[slot])
+
+    def _check_positions(self, slots, counts) -> None:
+        """No position beyond the model's (cached lengths are checked by the allocator)."""
+        if not self._evicted:
+            return                       # the allocator's max_seq_len is the tighter bound
+        sl = np.asarray(slots, np.int64)
+        off = self.alloc.pos_offset[sl]
+        over = off + self._seq_host[sl] + np.asarray(counts) > self.max_positions
+        if over.any():
+            raise ValueError(f"Position exceeds the maximum of {self.max_positions} for batch index "
+                             f"{int(sl[np.argmax(over)])}.")
+
     def plan_tokens(self, slots, counts, *, strict_len: bool = True):
         """``BlockAllocator.plan_tokens`` on the host mirror; the new block-table entries are
         pushed to the device table (also those made before an allocation error)."""
+        self._check_positions(slots, counts)
         try:
             out, updates = self.alloc.plan_tokens(slots, counts, strict_len=strict_len)
         except (ValueError, RuntimeError) as e:
@@ -212,6 +276,7 @@ class KVCacheManager:
         """One new token per slot: the block each slot must take from the free list this step,
         or -1.  Same order and checks as :meth:`plan_tokens`; the device block table is written
         by the step's prepare kernel (``ti_decode_prepare``), not here."""
+        self._check_positions(slots, 1)
         return self.alloc.plan_decode(slots)
 
     def _push_updates(self, updates) -> None:
@@ -256,7 +321,12 @@ class KVCacheManager:
         k = new_keys.to(device=self.device, dtype=self.dtype).permute(0, 2, 1, 3).reshape(-1, self.num_kv_heads, self.head_dim).contiguous()
         v = new_values.to(device=self.device, dtype=self.dtype).permute(0, 2, 1, 3).reshape(-1, self.num_kv_heads, self.head_dim).contiguous()
         n = len(mapping)
-        if n:
+        if n and self.kv_bits == 4:
+            m = torch.from_numpy(mapping).to(self.device)
+            kv4.append(self.kv4_pool[layer_idx], k[:n], v[:n], m,
+                       weights=None if self.attn_weights is None else self.attn_weights[layer_idx])
+            torch.cuda.current_stream(self.device).synchronize()
+        elif n:
             m = torch.from_numpy(mapping).to(self.device)
             N.check(N.lib().ti_kv_scatter(
                 self.key_cache[layer_idx].data_ptr(), self.value_cache[layer_idx].data_ptr(),
@@ -291,3 +361,36 @@ class KVCacheManager:
         self.alloc.free_slot(batch_idx)
         self.block_tables[batch_idx].fill_(-1)
         self.seq_len[batch_idx] = 0
+        self.pos_offset[batch_idx] = 0
+
+    # ---- eviction ---------------------------------------------------------------------------
+    def evict(self, slots, keep: int, recent: int) -> list[int]:
+        """Bring each of the slots that holds more than ``keep`` tokens down to ``keep``: in every
+        layer and kv head its last ``recent`` tokens and the ``keep - recent`` older ones of the
+        largest attention weight so far stay, in their order (``kv4.evict``); the blocks behind go
+        back to the pool.  Positions go on where they were.  Returns the slots that shrank.  Needs
+        ``kv_bits=4`` and ``track_weights``; runs on the current stream, between steps."""
+        if self.attn_weights is None:
+            raise RuntimeError("eviction needs a 4-bit KV pool with track_weights")
+        keep, recent = int(keep), int(recent)
+        if keep < 1 or not 0 <= recent <= keep:
+            raise ValueError("eviction needs keep >= 1 and 0 <= recent <= keep")
+        slots = [int(s) for s in slots]
+        if len(set(slots)) != len(slots) or any(not 0 <= s < self.max_batch_size for s in slots):
+            raise ValueError("eviction needs distinct slots of the batch")
+        shrink = [s for s in slots if self.seq_len_host(s) > keep]
+        if not shrink:
+            return shrink
+        host = torch.tensor([shrink, [self.seq_len_host(s) for s in shrink]], dtype=torch.int32)
+        dev = host.to(self.device)
+        rows, lens = dev[0].contiguous(), dev[1].contiguous()
+        kv4.evict(self.kv4_pool, self.attn_weights, self.block_tables, lens, keep, recent,
+                  row_index=rows)
+        idx = rows.long()
+        self.block_tables[idx, -(-keep // self.block_size):] = -1
+        self.seq_len[idx] = keep
+        self.pos_offset[idx] += lens - keep
+        for s in shrink:
+            self.alloc.truncate(s, keep)
+        self._evicted = True
+        return shrink

@@ -17,17 +17,6 @@ constexpr int kThreads = 256;
 constexpr int kRmsSmallRows = 2048;                   // up to here: the small-CTA RMSNorm grid
 constexpr int kRmsSmallThreads = TI_RMS_SMALL_THREADS;
 
-// Rotate 8 dims of the first half (x1) with the matching 8 dims of the second half (x2)
-// (reference src/fused_rope.cu:37-50).
-__device__ __forceinline__ void rotate8(float* x1, float* x2, const float* c, const float* s) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float a = x1[i], b = x2[i];
-    x1[i] = a * c[i] - b * s[i];
-    x2[i] = a * s[i] + b * c[i];
-  }
-}
-
 // ---- in-place RoPE on separate q / k tensors (drop-in for custom_rope.apply_inplace) --------
 template <typename T>
 __global__ void rope_inplace_kernel(T* q, int64_t q_stride, T* k, int64_t k_stride,

@@ -11,6 +11,8 @@
 namespace ti {
 namespace kv4 {
 
+using ew::load8f;
+using ew::rotate8;
 using ew::Vec8;
 
 // One quantised group of token `off` of a tile, from 16 elements of a 16-bit type.
@@ -71,6 +73,77 @@ __global__ void append_kernel(AppendParams p) {
     const int off = (int)slot & (kBlock - 1);
     store_group<T, HD>(p.pool + tile * L::kBytes, is_v, off, g, lo, hi);
     if (p.weights && !is_v && g == 0) p.weights[tile * kBlock + off] = 0.f;
+  }
+}
+
+// ---- RoPE and append ---------------------------------------------------------------------------------
+// The decode and prefill layers' form, on rows [q | k | v] of the fused projection: q and k are rotated
+// in place and rounded to the type, as ti_rope_inplace does, then k and v are quantised from those
+// values.  One thread per 16 dims and their 16 partners of a q or k head, or per 16 dims of v.
+struct RopeAppendParams {
+  void* qkv;
+  int64_t stride;
+  uint8_t* pool;
+  float* weights;
+  const int64_t* slots;
+  int64_t pool_slots;
+  const float *cos, *sin;
+  const int32_t* pos;
+  int tokens, NH, KVH;
+};
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(128) rope_append_kernel(RopeAppendParams p) {
+  using L = Tile<HD>;
+  constexpr int kHalf = HD / 2, kPieces = kHalf / kGroup;        // pieces of a rotated head
+  pdl_wait();
+  pdl_launch_dependents();
+  const int turns = (p.NH + p.KVH) * kPieces, per_tok = turns + p.KVH * L::kGroups;
+  const int64_t total = (int64_t)p.tokens * per_tok;
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total;
+       i += (int64_t)gridDim.x * blockDim.x) {
+    const int t = (int)(i / per_tok), r = (int)(i - (int64_t)t * per_tok);
+    T* row = (T*)p.qkv + t * p.stride;
+    const int64_t slot = p.slots[t];
+    const bool write = slot >= 0 && slot < p.pool_slots;
+    if (slot >= p.pool_slots && r == 0) raise_device_error(TI_DEVERR_BAD_INPUT);
+    const int off = (int)slot & (kBlock - 1);
+    uint8_t* tiles = p.pool + (int64_t)((uint64_t)(write ? slot : 0) / kBlock) * p.KVH * L::kBytes;
+    if (r < turns) {
+      const int h = r / kPieces, piece = r % kPieces, d0 = piece * kGroup;
+      T* base = row + (int64_t)h * HD;             // q heads, then k heads
+      const int64_t tab = (int64_t)p.pos[t] * kHalf + d0;
+      uint4 x[2][2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        Vec8<T> a, b;
+        float c[8], s[8], x1[8], x2[8];
+        load8f(p.cos + tab + 8 * u, c);
+        load8f(p.sin + tab + 8 * u, s);
+        a.load(base + d0 + 8 * u);
+        b.load(base + kHalf + d0 + 8 * u);
+        a.to_float(x1);
+        b.to_float(x2);
+        rotate8(x1, x2, c, s);
+        a.from_float(x1);
+        b.from_float(x2);
+        a.store(base + d0 + 8 * u);
+        b.store(base + kHalf + d0 + 8 * u);
+        x[0][u] = a.raw;
+        x[1][u] = b.raw;
+      }
+      if (h >= p.NH && write) {
+        uint8_t* tile = tiles + (int64_t)(h - p.NH) * L::kBytes;
+        store_group<T, HD>(tile, false, off, piece, x[0][0], x[0][1]);
+        store_group<T, HD>(tile, false, off, piece + kPieces, x[1][0], x[1][1]);
+        if (p.weights && piece == 0)
+          p.weights[((int64_t)((uint64_t)slot / kBlock) * p.KVH + h - p.NH) * kBlock + off] = 0.f;
+      }
+    } else if (write) {
+      const int h = (r - turns) / L::kGroups, g = (r - turns) % L::kGroups;
+      const uint4* src = reinterpret_cast<const uint4*>(row + (int64_t)(p.NH + p.KVH + h) * HD + g * kGroup);
+      store_group<T, HD>(tiles + (int64_t)h * L::kBytes, true, off, g, src[0], src[1]);
+    }
   }
 }
 
@@ -585,6 +658,39 @@ extern "C" int ti_kv4_append(void* pool, float* weights, const void* k, int64_t 
     return head_dim == 64 ? go(kv4::append_kernel<__nv_bfloat16, 64>)
                           : go(kv4::append_kernel<__nv_bfloat16, 128>);
   return head_dim == 64 ? go(kv4::append_kernel<__half, 64>) : go(kv4::append_kernel<__half, 128>);
+}
+
+extern "C" int ti_rope_kv4_append(void* qkv, int64_t qkv_stride, void* pool, float* weights,
+                                  const int64_t* slot_mapping, const float* cos, const float* sin,
+                                  const int32_t* pos, int num_tokens, int64_t num_blocks,
+                                  int num_heads, int num_kv_heads, int head_dim, int block_size,
+                                  int dtype, void* stream) {
+  clear_error();
+  if (num_tokens == 0) return TI_OK;
+  if (!qkv || !pool || !slot_mapping || !cos || !sin || !pos || num_tokens < 0 ||
+      num_blocks <= 0 || num_heads <= 0 || num_kv_heads <= 0)
+    return set_error(TI_ERR_INVALID_ARGUMENT, "rope_kv4_append: null pointer, negative size or empty pool");
+  if ((head_dim != 64 && head_dim != 128) || block_size != kv4::kBlock)
+    return set_error(TI_ERR_UNSUPPORTED, "rope_kv4_append: head_dim must be 64 or 128, block_size 16");
+  if (dtype != TI_DTYPE_BF16 && dtype != TI_DTYPE_FP16)
+    return set_error(TI_ERR_UNSUPPORTED, "rope_kv4_append: dtype must be bf16 or fp16");
+  if ((qkv_stride % 8) ||
+      ((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(pool) |
+        reinterpret_cast<uintptr_t>(cos) | reinterpret_cast<uintptr_t>(sin)) & 15))
+    return set_error(TI_ERR_INVALID_ARGUMENT, "rope_kv4_append: tensors must be 16-byte aligned");
+  kv4::RopeAppendParams p{qkv, qkv_stride, (uint8_t*)pool, weights, slot_mapping,
+                          num_blocks * kv4::kBlock, cos, sin, pos, num_tokens, num_heads,
+                          num_kv_heads};
+  const int64_t work = (int64_t)num_tokens * ((num_heads + num_kv_heads) * (head_dim / 32) +
+                                              num_kv_heads * (head_dim / 16));
+  const dim3 grid(kv4::grid_for(work, 128));
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  auto go = [&](auto kern) { return launch_kernel("rope_kv4_append launch", kern, grid, dim3(128), 0, s, 1, p); };
+  if (dtype == TI_DTYPE_BF16)
+    return head_dim == 64 ? go(kv4::rope_append_kernel<__nv_bfloat16, 64>)
+                          : go(kv4::rope_append_kernel<__nv_bfloat16, 128>);
+  return head_dim == 64 ? go(kv4::rope_append_kernel<__half, 64>)
+                        : go(kv4::rope_append_kernel<__half, 128>);
 }
 
 extern "C" int ti_kv4_dequantize(void* k_out, void* v_out, int64_t out_blocks, const void* pool,

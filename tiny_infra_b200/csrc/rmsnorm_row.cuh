@@ -39,6 +39,17 @@ __device__ __forceinline__ void load8f(const float* p, float* f) {
   f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
 }
 
+// Rotate 8 dims of the first half (x1) with the matching 8 dims of the second half (x2)
+// (reference src/fused_rope.cu:37-50).
+__device__ __forceinline__ void rotate8(float* x1, float* x2, const float* c, const float* s) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float a = x1[i], b = x2[i];
+    x1[i] = a * c[i] - b * s[i];
+    x2[i] = a * s[i] + b * c[i];
+  }
+}
+
 // The norm weight as this lane's NC chunks of 8 floats (static: loadable before any wait).
 template <typename T, int NC>
 __device__ __forceinline__ void rms_load_weight(const T* __restrict__ w, int H, int lane,

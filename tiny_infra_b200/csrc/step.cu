@@ -21,7 +21,8 @@ template <typename T>
 __global__ void decode_prepare_kernel(const int32_t* __restrict__ tokens,
                                       const int32_t* __restrict__ slots,
                                       const int32_t* __restrict__ new_block,
-                                      const int32_t* __restrict__ seq_len, int32_t* block_tables,
+                                      const int32_t* __restrict__ seq_len,
+                                      const int32_t* __restrict__ pos_offset, int32_t* block_tables,
                                       int64_t bt_stride, int num_slots, int max_blocks,
                                       int64_t num_blocks, int bs, int32_t* __restrict__ positions,
                                       int64_t* __restrict__ slot_mapping,
@@ -51,7 +52,7 @@ __global__ void decode_prepare_kernel(const int32_t* __restrict__ tokens,
       if (nb >= num_blocks) raise_device_error(TI_DEVERR_BAD_INPUT);
       else if (nb >= 0) row[pos / bs] = nb;
       const int blk = row[pos / bs];
-      positions[r] = pos;
+      positions[r] = pos + (pos_offset ? pos_offset[slot] : 0);
       // a block id outside the pool gets no KV write (attention treats it as absent too)
       slot_mapping[r] = (blk >= 0 && blk < num_blocks) ? (int64_t)blk * bs + pos % bs : -1;
       ctx_lens[r] = pos + 1;
@@ -146,9 +147,9 @@ __global__ void kv_scatter_kernel(T* k_cache, T* v_cache, const T* __restrict__ 
 
 using namespace ti;
 
-extern "C" int ti_decode_prepare(const int32_t* tokens, const int32_t* slots,
-                                 const int32_t* new_block, const int32_t* seq_len,
-                                 int32_t* block_tables, int64_t bt_stride, int num_slots,
+extern "C" int ti_decode_prepare_ex(const int32_t* tokens, const int32_t* slots,
+                                    const int32_t* new_block, const int32_t* seq_len,
+                                    const int32_t* pos_offset, int32_t* block_tables, int64_t bt_stride, int num_slots,
                                  int max_blocks_per_seq, int64_t num_blocks, int block_size,
                                  int32_t* positions, int64_t* slot_mapping, int32_t* ctx_lens,
                                  float* hidden, const void* embed, int hidden_size, int64_t vocab,
@@ -166,17 +167,30 @@ extern "C" int ti_decode_prepare(const int32_t* tokens, const int32_t* slots,
   if (dtype == TI_DTYPE_BF16)
     return launch_kernel("decode_prepare launch", step::decode_prepare_kernel<__nv_bfloat16>,
                          dim3(rows), dim3(128), 0, s, 1,
-        tokens, slots, new_block, seq_len, block_tables, bt_stride, num_slots, max_blocks_per_seq,
+        tokens, slots, new_block, seq_len, pos_offset, block_tables, bt_stride, num_slots, max_blocks_per_seq,
         num_blocks, block_size, positions, slot_mapping, ctx_lens, hidden,
         (const __nv_bfloat16*)embed, hidden_size, vocab, rows);
   else if (dtype == TI_DTYPE_FP16)
     return launch_kernel("decode_prepare launch", step::decode_prepare_kernel<__half>,
                          dim3(rows), dim3(128), 0, s, 1,
-        tokens, slots, new_block, seq_len, block_tables, bt_stride, num_slots, max_blocks_per_seq,
+        tokens, slots, new_block, seq_len, pos_offset, block_tables, bt_stride, num_slots, max_blocks_per_seq,
         num_blocks, block_size, positions, slot_mapping, ctx_lens, hidden, (const __half*)embed,
         hidden_size, vocab, rows);
   else
     return set_error(TI_ERR_UNSUPPORTED, "decode_prepare: dtype must be bf16 or fp16");
+}
+
+extern "C" int ti_decode_prepare(const int32_t* tokens, const int32_t* slots,
+                                 const int32_t* new_block, const int32_t* seq_len,
+                                 int32_t* block_tables, int64_t bt_stride, int num_slots,
+                                 int max_blocks_per_seq, int64_t num_blocks, int block_size,
+                                 int32_t* positions, int64_t* slot_mapping, int32_t* ctx_lens,
+                                 float* hidden, const void* embed, int hidden_size, int64_t vocab,
+                                 int rows, int dtype, void* stream) {
+  return ti_decode_prepare_ex(tokens, slots, new_block, seq_len, nullptr, block_tables, bt_stride,
+                              num_slots, max_blocks_per_seq, num_blocks, block_size, positions,
+                              slot_mapping, ctx_lens, hidden, embed, hidden_size, vocab, rows,
+                              dtype, stream);
 }
 
 extern "C" int ti_argmax_finish(const float* part_val, const int32_t* part_idx, int ntiles,

@@ -27,7 +27,7 @@ class DecodeEngine:
         self.max_rows = int(max_rows or kv_cache.max_batch_size)
         R = self.max_rows
         self.use_graphs = use_graphs
-        self.cos, self.sin = model.rope_tables(kv_cache.max_seq_len)
+        self.cos, self.sin = model.rope_tables(kv_cache.max_positions)
         # inputs of a step: tokens, slots (-1 = padding row), new block per row (-1 = none)
         self.d_in = torch.zeros(3, R, dtype=torch.int32, device=dev)
         self.h_in = torch.zeros(3, R, dtype=torch.int32).pin_memory()
@@ -43,10 +43,8 @@ class DecodeEngine:
         self.h_out = torch.zeros(R, dtype=torch.int32).pin_memory()
         self.bufs: dict = {}
         model.scratch(R, self.bufs)
-        need = N.lib().ti_paged_attention_workspace_bytes(
-            R, c.num_attention_heads, c.num_key_value_heads, c.head_dim,
-            kv_cache.max_blocks_per_seq, 0)
-        self.ws = torch.zeros(need, dtype=torch.uint8, device=dev)
+        self.ws = torch.zeros(model.attention_workspace_bytes(kv_cache, R), dtype=torch.uint8,
+                              device=dev)
         self.plan = torch.zeros(N.lib().ti_paged_attention_plan_bytes(R), dtype=torch.uint8,
                                 device=dev)
         self.graphs: dict[tuple, torch.cuda.CUDAGraph] = {}
@@ -79,9 +77,9 @@ class DecodeEngine:
         s = torch.cuda.current_stream(m.device).cuda_stream
         dt = N.dtype_code(m.dtype)
         kv = self.kv
-        N.check(lib.ti_decode_prepare(
+        N.check(lib.ti_decode_prepare_ex(
             self.d_in[0].data_ptr(), self.d_in[1].data_ptr(), self.d_in[2].data_ptr(),
-            kv.seq_len.data_ptr(), kv.block_tables.data_ptr(), kv.block_tables.stride(0),
+            kv.seq_len.data_ptr(), kv.pos_offset.data_ptr(), kv.block_tables.data_ptr(), kv.block_tables.stride(0),
             kv.block_tables.shape[0], kv.block_tables.shape[1], kv.total_physical_blocks,
             kv.block_size, self.positions.data_ptr(), self.slot_mapping.data_ptr(),
             self.ctx_lens.data_ptr(), self.hidden.data_ptr(), m.weights["embed"].data_ptr(),

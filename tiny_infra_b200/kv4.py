@@ -6,6 +6,7 @@ head) tile holds K codes, V codes, K scales, V scales; a value is an e2m1 code t
 its 16 dims (an unsigned 8-bit float), exact in bf16 and fp16.  ``head_dim`` is 64 or 128.
 
 * ``append``              quantise new tokens' K and V into their slots
+* ``rope_append``         the same from the fused projection's rows, rotating q and k first
 * ``dequantize``          read cached tokens back as 16-bit values
 * ``decode_attention``    one query token per sequence (out, and log-sum-exp on request)
 * ``prefill_attention``   ragged causal chunks (``PrefillPlan`` holds their layout)
@@ -184,6 +185,36 @@ def append(pool: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slot_mapping: t
             pool.data_ptr(), _ptr(weights), k.data_ptr(), k_tok, k_head, v.data_ptr(), v_tok,
             v_head, slot_mapping.data_ptr(), T, nb, kvh, d, BLOCK, N.dtype_code(k.dtype),
             _stream(dev)))
+
+
+def rope_append(pool: torch.Tensor, qkv: torch.Tensor, num_heads: int,
+                slot_mapping: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                positions: torch.Tensor, *, weights: torch.Tensor | None = None) -> None:
+    """Rows [q | k | v] of the fused projection, ``qkv`` [T, (num_heads + 2 KVH) * D]: rotate q and k
+    in place (rotate-half, tables ``cos`` / ``sin`` float32 [*, D/2], ``positions`` int32 [T]) and
+    ``append`` the rotated k and v."""
+    dev = _device(pool, qkv, slot_mapping, cos, sin, positions, weights)
+    nb, kvh, d = _pool_shape(pool)
+    if qkv.dim() != 2 or qkv.dtype not in _HALF or num_heads <= 0 or \
+            qkv.shape[1] != (num_heads + 2 * kvh) * d or (qkv.numel() and qkv.stride(1) != 1):
+        _fail("qkv must be 16-bit [tokens, (num_heads + 2 * kv heads) * head_dim] rows")
+    T = qkv.shape[0]
+    if slot_mapping.dtype != torch.int64 or not slot_mapping.is_contiguous() or \
+            slot_mapping.numel() != T:
+        _fail("slot_mapping must be contiguous int64 [tokens]")
+    _index("positions", positions, T)
+    for name, t in (("cos", cos), ("sin", sin)):
+        if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] != d // 2 or \
+                not t.is_contiguous():
+            _fail(f"{name} must be contiguous float32 [positions, head_dim / 2]")
+    _totals("weights", weights, nb, kvh)
+    if T == 0:
+        return
+    with _on(dev):
+        N.check(N.lib().ti_rope_kv4_append(
+            qkv.data_ptr(), qkv.stride(0), pool.data_ptr(), _ptr(weights), slot_mapping.data_ptr(),
+            cos.data_ptr(), sin.data_ptr(), positions.data_ptr(), T, nb, num_heads, kvh, d, BLOCK,
+            N.dtype_code(qkv.dtype), _stream(dev)))
 
 
 def dequantize(pool: torch.Tensor, block_tables: torch.Tensor, lens: torch.Tensor,

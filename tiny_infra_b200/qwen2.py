@@ -12,6 +12,11 @@ Per layer the decode forward is 8 kernel launches:
   -> O GEMM (+residual, split-K) -> rmsnorm -> gate/up GEMM (+SwiGLU) -> down GEMM (+residual)
 (no merge when every sequence fits 32 blocks: the attention then finishes each sequence in one
 CTA; prefill: one ragged prefill-attention launch instead of the attention and its merge)
+A cache with ``kv_bits=4`` (``KVCacheManager``) runs the same layers on the 4-bit pool: QKV GEMM
+(+bias) -> RoPE and quantised append -> 4-bit paged attention (prefill: read back, then the ragged
+prefill attention); when the cache tracks attention weights, each decode token, and the last
+``OBSERVE`` tokens of a prefill chunk, add theirs to the cached tokens' totals.
+
 with the residual stream kept in float32 (the reference keeps it in the model dtype; float32
 is closer to the float32 oracle).  The lm_head runs only on the rows whose logits are needed
 and, for greedy decoding, reduces to one token per row inside the GEMM epilogue.
@@ -24,12 +29,14 @@ import numpy as np
 import torch
 
 from . import _native as N
+from . import kv4
 from .config import QwenConfig
 
 GATE_UP_GROUP = 8           # gate/up weight rows interleaved 8 gate, 8 up (TI_EPI_SWIGLU16)
 LM_TILE = 128               # block_n of the lm_head GEMM (argmax partials per 128 columns)
 O_TILE = 64                 # block_n of the o_proj GEMM (+residual, split-K)
 DOWN_TILE = 128             # block_n of the down_proj GEMM (+residual, split-K)
+OBSERVE = 8                 # query tokens of a prefill chunk whose attention weights are added up
 
 
 def _ptr(t: torch.Tensor | None):
@@ -53,6 +60,8 @@ class PackedBatch:
     num_seqs: int
     decode: bool
     last_rows: torch.Tensor        # int64 [nseq] row of each sequence's last token
+    kv4_plan: kv4.PrefillPlan | None = None   # prefill layout on a 4-bit cache
+    observe: tuple | None = None   # rows, slots, lengths of the chunks' last OBSERVE tokens
 
 
 class Qwen2ForCausalLM:
@@ -213,7 +222,9 @@ class Qwen2ForCausalLM:
         cu = np.zeros(nseq + 1, np.int32)
         cu[1:] = np.cumsum(counts)
         T = int(cu[-1])
-        pos = np.concatenate([start[i] + np.arange(counts[i], dtype=np.int32)
+        # positions go on behind evicted tokens; everything else follows the cached lengths
+        first = np.array([kv_cache.position_host(s) for s in slots], np.int32)
+        pos = np.concatenate([first[i] + np.arange(counts[i], dtype=np.int32)
                               for i in range(nseq)]) if T else np.zeros(0, np.int32)
         decode = bool((counts == 1).all())
         tseq, tq0 = None, None
@@ -231,6 +242,11 @@ class Qwen2ForCausalLM:
             tseq = torch.tensor(np.asarray(ts, np.int32)[order], dtype=torch.int32, device=dev)
             tq0 = torch.tensor(np.asarray(tq, np.int32)[order], dtype=torch.int32, device=dev)
         as_dev = lambda a, dt: torch.from_numpy(np.ascontiguousarray(a)).to(dev, dt)  # noqa: E731
+        plan4 = observe = None
+        if kv_cache.kv_bits == 4 and not decode:
+            plan4 = kv4.PrefillPlan(start, counts, device=dev)
+            if kv_cache.attn_weights is not None:
+                observe = self._observed(slots, start, counts, cu, as_dev)
         return PackedBatch(
             input_ids=as_dev(np.asarray(token_ids, np.int32), torch.int32),
             positions=as_dev(pos, torch.int32), slot_mapping=as_dev(mapping, torch.int64),
@@ -238,7 +254,19 @@ class Qwen2ForCausalLM:
             start_pos=as_dev(start, torch.int32), cu_seqlens=as_dev(cu, torch.int32),
             ctx_lens=as_dev(start + counts, torch.int32), tile_seq=tseq, tile_q0=tq0,
             num_tokens=T, num_seqs=nseq, decode=decode,
-            last_rows=as_dev(cu[1:] - 1, torch.int64))
+            last_rows=as_dev(cu[1:] - 1, torch.int64), kv4_plan=plan4, observe=observe)
+
+    @staticmethod
+    def _observed(slots, start, counts, cu, as_dev):
+        """The chunks' last OBSERVE tokens as rows of a decode call, [OBSERVE, nseq]: query row,
+        table row and attended length (0: the chunk is shorter)."""
+        back = np.arange(OBSERVE, dtype=np.int32)[::-1, None]       # last token: 0 back
+        live = back < counts
+        rows = np.where(live, cu[1:] - 1 - back, 0)
+        lens = np.where(live, start + counts - back, 0)
+        table = np.broadcast_to(np.asarray(slots, np.int32), lens.shape)
+        return (as_dev(rows.reshape(-1), torch.int64), as_dev(table.reshape(-1), torch.int32),
+                as_dev(lens.reshape(-1), torch.int32))
 
     # ---- forward -----------------------------------------------------------------------------
     def scratch(self, rows: int, owner: dict | None = None) -> dict:
@@ -250,7 +278,11 @@ class Qwen2ForCausalLM:
         shapes = {"xn": (rows, c.hidden_size), "qkv": (rows, (NH + 2 * KVH) * D),
                   "attn": (rows, NH * D), "act": (rows, c.intermediate_size)}
         if owner is None:
-            return {k: self._buf(k, v, self.dtype) for k, v in shapes.items()}
+            out = {k: self._buf(k, v, self.dtype) for k, v in shapes.items()}
+            out["lse"] = self._buf("lse", (rows, NH), torch.float32)
+            return out
+        if "lse" not in owner:
+            owner["lse"] = torch.empty(rows, NH, dtype=torch.float32, device=self.device)
         for k, v in shapes.items():
             if k not in owner:
                 owner[k] = torch.empty(*v, dtype=self.dtype, device=self.device)
@@ -284,10 +316,12 @@ class Qwen2ForCausalLM:
         nb = kv_cache.total_physical_blocks
         bt = kv_cache.block_tables
         maxb = kv_cache.max_blocks_per_seq
+        four = kv_cache.kv_bits == 4
         if pb.decode and ws is None:
-            need = lib.ti_paged_attention_workspace_bytes(pb.num_seqs, NH, KVH, D, maxb, 0)
-            ws = self._ws.get(self.device, need)
-        if pb.decode:
+            need = self.attention_workspace_bytes(kv_cache, pb.num_seqs)
+            # (the 4-bit attention's counters have to be zero: its own buffer per stream)
+            ws = self._ws.get(self.device, need, stream if four else None)
+        if pb.decode and not four:
             # the batch's attention work split, resolved once for all layers
             if plan is None:
                 plan = self._plan_ws.get(self.device,
@@ -313,32 +347,35 @@ class Qwen2ForCausalLM:
                                    weight.data_ptr(), c.rms_norm_eps, rows, H, dt, stream))
 
         for li in range(first_layer, end):
-            kc, vc = kv_cache.key_cache[li], kv_cache.value_cache[li]
             rmsnorm(xn, W[f"{li}.ln1"], T)
             mark(li, "xn1")
-            N.check(lib.ti_gemm_qkv_rope(
-                xn.data_ptr(), H, W[f"{li}.qkv"].data_ptr(), H, W[f"{li}.qkv_bias"].data_ptr(),
-                T, H, NH, KVH, D, qkv.data_ptr(), QKV, kc.data_ptr(), vc.data_ptr(),
-                pb.slot_mapping.data_ptr(), cos.data_ptr(), sin.data_ptr(),
-                pb.positions.data_ptr(), kv_cache.block_size, dt, stream))
-            mark(li, "qkv")
-            if pb.decode:
-                # the plan and every KV block but each sequence's last (the one the QKV epilogue
-                # appends to) are final before the QKV GEMM starts (the RMSNorm before it lets it
-                # launch only once the plan kernel has completed): the attention streams them
-                # while that GEMM still runs
-                early = self.early_attention
-                N.check(lib.ti_paged_attention_decode_planned_ex(
-                    attn.data_ptr(), NH * D, qkv.data_ptr(), QKV, kc.data_ptr(), vc.data_ptr(), nb,
-                    bt.data_ptr(), bt.stride(0), pb.seq_slots.data_ptr(), pb.ctx_lens.data_ptr(),
-                    pb.num_seqs, NH, KVH, D, kv_cache.block_size, maxb, dt, ws.data_ptr(),
-                    ws.numel(), plan.data_ptr(), N.TI_ATTN_EARLY_KV if early else 0, stream))
+            if four:
+                self._kv4_attention(li, pb, kv_cache, cos, sin, bufs, ws, stream, mark)
             else:
-                N.check(lib.ti_paged_prefill_attention(
-                    attn.data_ptr(), NH * D, qkv.data_ptr(), QKV, kc.data_ptr(), vc.data_ptr(), nb,
-                    bt.data_ptr(), bt.stride(0), pb.seq_slots.data_ptr(), pb.start_pos.data_ptr(),
-                    pb.cu_seqlens.data_ptr(), pb.tile_seq.data_ptr(), pb.tile_q0.data_ptr(),
-                    pb.tile_seq.numel(), NH, KVH, D, kv_cache.block_size, dt, stream))
+                kc, vc = kv_cache.key_cache[li], kv_cache.value_cache[li]
+                N.check(lib.ti_gemm_qkv_rope(
+                    xn.data_ptr(), H, W[f"{li}.qkv"].data_ptr(), H, W[f"{li}.qkv_bias"].data_ptr(),
+                    T, H, NH, KVH, D, qkv.data_ptr(), QKV, kc.data_ptr(), vc.data_ptr(),
+                    pb.slot_mapping.data_ptr(), cos.data_ptr(), sin.data_ptr(),
+                    pb.positions.data_ptr(), kv_cache.block_size, dt, stream))
+                mark(li, "qkv")
+                if pb.decode:
+                    # the plan and every KV block but each sequence's last (the one the QKV epilogue
+                    # appends to) are final before the QKV GEMM starts (the RMSNorm before it lets it
+                    # launch only once the plan kernel has completed): the attention streams them
+                    # while that GEMM still runs
+                    early = self.early_attention
+                    N.check(lib.ti_paged_attention_decode_planned_ex(
+                        attn.data_ptr(), NH * D, qkv.data_ptr(), QKV, kc.data_ptr(), vc.data_ptr(), nb,
+                        bt.data_ptr(), bt.stride(0), pb.seq_slots.data_ptr(), pb.ctx_lens.data_ptr(),
+                        pb.num_seqs, NH, KVH, D, kv_cache.block_size, maxb, dt, ws.data_ptr(),
+                        ws.numel(), plan.data_ptr(), N.TI_ATTN_EARLY_KV if early else 0, stream))
+                else:
+                    N.check(lib.ti_paged_prefill_attention(
+                        attn.data_ptr(), NH * D, qkv.data_ptr(), QKV, kc.data_ptr(), vc.data_ptr(), nb,
+                        bt.data_ptr(), bt.stride(0), pb.seq_slots.data_ptr(), pb.start_pos.data_ptr(),
+                        pb.cu_seqlens.data_ptr(), pb.tile_seq.data_ptr(), pb.tile_q0.data_ptr(),
+                        pb.tile_seq.numel(), NH, KVH, D, kv_cache.block_size, dt, stream))
             mark(li, "attn")
             N.check(lib.ti_gemm(residual, attn.data_ptr(), NH * D, W[f"{li}.o"].data_ptr(),
                                 NH * D, T, H, NH * D, hidden.data_ptr(), H, None, None, None, dt,
@@ -356,6 +393,67 @@ class Qwen2ForCausalLM:
             mark(li, "h_out")
         if final_norm_out is not None and end == c.num_layers:
             rmsnorm(final_norm_out, W["norm"], final_norm_out.shape[0])
+
+    def attention_workspace_bytes(self, kv_cache, num_seqs: int) -> int:
+        """Scratch of one decode attention call over the cache."""
+        c, lib = self.config, N.lib()
+        args = (num_seqs, c.num_attention_heads, c.num_key_value_heads, c.head_dim,
+                kv_cache.max_blocks_per_seq)
+        if kv_cache.kv_bits == 4:
+            return lib.ti_kv4_attention_workspace_bytes(*args)
+        return lib.ti_paged_attention_workspace_bytes(*args, 0)
+
+    def _kv4_attention(self, li: int, pb: PackedBatch, kv_cache, cos, sin, bufs: dict,
+                       ws: torch.Tensor | None, stream: int, mark) -> None:
+        """QKV projection, append and attention of one layer on a 4-bit cache: xn -> attn."""
+        c, W, lib, dt = self.config, self.weights, N.lib(), N.dtype_code(self.dtype)
+        T, H, D = pb.num_tokens, c.hidden_size, c.head_dim
+        NH, KVH = c.num_attention_heads, c.num_key_value_heads
+        QKV = (NH + 2 * KVH) * D
+        xn, qkv, attn, lse = bufs["xn"], bufs["qkv"], bufs["attn"], bufs["lse"]
+        pool = kv_cache.kv4_pool[li]
+        weights = None if kv_cache.attn_weights is None else kv_cache.attn_weights[li]
+        bt = kv_cache.block_tables
+        nb, bs, maxb = (kv_cache.total_physical_blocks, kv_cache.block_size,
+                        kv_cache.max_blocks_per_seq)
+        # decode sizes: narrow tiles and a K split, so that the 18 column tiles cover the GPU
+        N.check(lib.ti_gemm(N.TI_EPI_STORE, xn.data_ptr(), H, W[f"{li}.qkv"].data_ptr(), H, T, QKV,
+                            H, qkv.data_ptr(), QKV, W[f"{li}.qkv_bias"].data_ptr(), None, None, dt,
+                            64 if T <= 512 else 128, 8 if T <= 512 else 1, stream))
+        N.check(lib.ti_rope_kv4_append(
+            qkv.data_ptr(), QKV, pool.data_ptr(), _ptr(weights), pb.slot_mapping.data_ptr(),
+            cos.data_ptr(), sin.data_ptr(), pb.positions.data_ptr(), T, nb, NH, KVH, D, bs, dt,
+            stream))
+        mark(li, "qkv")
+        if pb.decode:
+            N.check(lib.ti_kv4_attention_decode(
+                attn.data_ptr(), NH * D, lse.data_ptr(), qkv.data_ptr(), QKV, pool.data_ptr(), nb,
+                bt.data_ptr(), bt.stride(0), pb.seq_slots.data_ptr(), pb.ctx_lens.data_ptr(),
+                pb.num_seqs, NH, KVH, D, bs, maxb, dt, ws.data_ptr(), ws.numel(), stream))
+            if weights is not None:
+                N.check(lib.ti_kv4_accumulate_weights(
+                    weights.data_ptr(), weights.data_ptr(), qkv.data_ptr(), QKV, lse.data_ptr(),
+                    pool.data_ptr(), nb, bt.data_ptr(), bt.stride(0), pb.seq_slots.data_ptr(),
+                    pb.ctx_lens.data_ptr(), pb.num_seqs, NH, KVH, D, bs, maxb, dt, stream))
+            return
+        q = qkv[:, :NH * D].view(T, NH, D)
+        kv4.prefill_attention(attn.view(T, NH, D), q, pool, bt, pb.kv4_plan,
+                              row_index=pb.seq_slots)
+        if pb.observe is not None:
+            # a decode call over the observed tokens gives their log-sum-exp; their weights are added
+            # one token per sequence at a time (a call's sequences share no block)
+            rows, table, lens = pb.observe
+            obs = q.index_select(0, rows)
+            out, sums = torch.empty_like(obs), torch.empty(len(rows), NH, device=self.device)
+            for r in range(0, len(rows), 4096):
+                e = slice(r, r + 4096)
+                kv4.decode_attention(out[e], obs[e], pool, bt, lens[e], row_index=table[e],
+                                     lse=sums[e])
+            n = pb.num_seqs
+            for k in range(0, len(rows), n):
+                e = slice(k, k + n)
+                kv4.accumulate_weights(weights, obs[e], sums[e], pool, bt, lens[e],
+                                       row_index=table[e])
 
     def _final_norm(self, hidden_rows: torch.Tensor, stream: int) -> torch.Tensor:
         c = self.config

@@ -51,6 +51,7 @@ class SchedulerStats:
     decode_steps: int = 0
     requests_finished: int = 0
     requests_failed: int = 0
+    evictions: int = 0             # sequences brought down to evict_keep
     last_tick_s: float = 0.0
     total_tick_s: float = 0.0
 
@@ -88,12 +89,29 @@ class GenerationRequest:
 
 class ContinuousBatcher:
     def __init__(self, model, kv_cache, eos_token_id: Optional[int] = None, *, backend=None,
-                 prefill_chunk_tokens: Optional[int] = None):
+                 prefill_chunk_tokens: Optional[int] = None, evict_above: Optional[int] = None,
+                 evict_keep: Optional[int] = None, evict_recent: Optional[int] = None):
         """``prefill_chunk_tokens``: at most this many prompt tokens are prefilled per tick
         (chunked prefill interleaved with decode; a request's first token is emitted after its
         last chunk).  None: whole prompts every tick, as the reference (block tables then match
         the reference's bit for bit; with chunking the allocation order interleaves with decode).
+        ``evict_above`` (a cache that tracks attention weights, ``KVCacheManager(kv_bits=4,
+        track_weights=True)``): before a decode step, sequences that hold that many tokens or more
+        are brought down to ``evict_keep`` (default: half), of which ``evict_recent`` (default: a
+        quarter of that) are the latest ones, so generation may run past the cached length, up to
+        the cache's ``max_positions``.
         """
+        if evict_above is not None:
+            evict_keep = evict_above // 2 if evict_keep is None else int(evict_keep)
+            evict_recent = evict_keep // 4 if evict_recent is None else int(evict_recent)
+            if not 1 <= evict_keep < evict_above or not 0 <= evict_recent <= evict_keep:
+                raise ValueError("eviction needs 1 <= evict_keep < evict_above and "
+                                 "0 <= evict_recent <= evict_keep")
+            if evict_above > kv_cache.max_seq_len:
+                raise ValueError("evict_above is beyond the cache's max_seq_len")
+        elif evict_keep is not None or evict_recent is not None:
+            raise ValueError("evict_keep and evict_recent need evict_above")
+        self.evict_above, self.evict_keep, self.evict_recent = evict_above, evict_keep, evict_recent
         self.model = model
         self.prefill_chunk_tokens = prefill_chunk_tokens
         self.kv_cache = kv_cache
@@ -122,8 +140,9 @@ class ContinuousBatcher:
         return d
 
     def _init_rope_cache(self):
-        """cos/sin [max_seq_len, head_dim/2] float32 with base 1e6 (engine/scheduler.py:36-48)."""
-        max_seq_len = self.kv_cache.max_seq_len
+        """cos/sin [max_seq_len, head_dim/2] float32 with base 1e6 (engine/scheduler.py:36-48); as
+        many rows as the cache has positions."""
+        max_seq_len = getattr(self.kv_cache, "max_positions", self.kv_cache.max_seq_len)
         head_dim = self.kv_cache.head_dim
         inv_freq = 1.0 / (1000000.0 ** (torch.arange(0, head_dim, 2, device=self.device).float()
                                         / head_dim))
@@ -267,6 +286,12 @@ class ContinuousBatcher:
 
     def _execute_decode(self, decode_indices: List[int]):
         """One batched decode step (engine/scheduler.py:250-281)."""
+        if self.evict_above is not None:
+            full = [s for s in decode_indices
+                    if self.kv_cache.seq_len_host(s) >= self.evict_above]
+            if full:
+                self.kv_cache.evict(full, self.evict_keep, self.evict_recent)
+                self._stats.evictions += len(full)
         reqs = [self.active_slots[s] for s in decode_indices]
         tokens = self.backend.decode(decode_indices, reqs)
         self._stats.decode_steps += 1
