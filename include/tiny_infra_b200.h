@@ -416,6 +416,28 @@ int ti_kv4_attention_decode(void* out, int64_t out_seq_stride, float* lse, const
                             int max_blocks_per_seq, int dtype, void* workspace,
                             size_t workspace_bytes, void* stream);
 
+/* Ragged causal prefill attention over the 4-bit pool: query rows cu_seqlens[i] ..
+ * cu_seqlens[i+1]-1 of q / out ([rows, num_heads, head_dim], token strides in elements) at positions
+ * start_pos[i] + j, whose K and V are in the pool; each attends to positions 0 .. its own of table
+ * row row_index[i] (NULL: i).  At most 16 query heads per kv head.  The caller lays out the work: a
+ * tile is 128 / slots tokens, slots = the query heads per kv head rounded up to a power of two; an
+ * item (6 int32: sequence, first token of two neighbouring tiles within the chunk, first key, end of
+ * the keys, part or -1, 0) is two tiles over keys [first, end), first a multiple of 64.  Items of one
+ * pair that cover its keys 0 .. last query position in several ranges name consecutive parts
+ * (0 .. num_parts-1, their partial results in the workspace), and a merge (4 int32: sequence, first
+ * token, first part, parts) joins them; a single item has part -1.  Every pair of tiles is covered.
+ * tiny_infra_b200.kv4.PrefillPlan builds both lists. */
+size_t ti_kv4_prefill_workspace_bytes(int num_parts, int num_kv_heads, int head_dim);
+int ti_kv4_prefill_attention(void* out, int64_t out_tok_stride, const void* q,
+                             int64_t q_tok_stride, const void* pool, int64_t num_blocks,
+                             const int32_t* block_tables, int64_t bt_stride,
+                             int max_blocks_per_seq, const int32_t* row_index,
+                             const int32_t* start_pos, const int32_t* cu_seqlens,
+                             const int32_t* items, int num_items, const int32_t* merges,
+                             int num_merges, int num_parts, int num_heads, int num_kv_heads,
+                             int head_dim, int block_size, int dtype, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
 /* weights_out = weights + sum over the kv head's query heads of exp(q.k / sqrt(head_dim) - lse), for
  * each cached token of the batch (float32 [num_blocks, num_kv_heads, 16]; weights_out may be
  * weights; other tokens are neither read nor written).  lse as ti_kv4_attention_decode gives it for

@@ -13,8 +13,9 @@ where tiny is the type's smallest normal number: outputs below it are multiples 
 2^-24), so rounding moves them by up to u tiny whatever their size.
   |lse - exact| <= ds + 2^-20 + 2^-22 |lse|
 A total of attention weight adds, per head, p * (ds + (1 + |s| + |lse|) 2^-20) and one rounding
-2^-23 of the total.  Prefill runs the 16-bit pool's tensor-core kernel: the same, its weights
-half precision of at most 1 (steps of 2^-24: 2^-25 F) or bf16 in two parts.
+2^-23 of the total.  Prefill: the same with p = 1 held as 2^7 (its running maximum may trail the
+row's by 2^8): weights below 2^-21 are multiples of 2^-31, each off by at most 2^-32, against the
+running maximum up to 2^8 times less: 2^-31 F covers what is left of them at the row's end.
 """
 import numpy as np
 import pytest
@@ -385,11 +386,18 @@ def test_decode_large_batch_and_pool_offsets(kv4):
 # ---- prefill ----------------------------------------------------------------------------------------
 @pytest.mark.parametrize("nh,kvh,d,dtn,starts,counts", [
     (14, 2, 64, "bf16", [0], [1]),
+    (14, 2, 64, "bf16", [63, 64, 127], [1, 1, 2]),
     (14, 2, 64, "bf16", [511, 0, 100], [1, 37, 130]),
-    (14, 2, 64, "fp16", [15, 16, 17, 0], [16, 17, 1, 0]),
+    (14, 2, 64, "fp16", [15, 16, 17, 0, 5], [16, 17, 1, 0, 33]),
     (9, 3, 128, "bf16", [0, 70], [33, 20]),
     (32, 8, 128, "fp16", [250], [9]),
     (16, 1, 64, "bf16", [31], [40]),
+    (12, 1, 128, "fp16", [3], [70]),
+    (4, 4, 64, "fp16", [5], [300]),
+    (2, 1, 128, "bf16", [0], [260]),
+    (4, 1, 64, "bf16", [40, 0], [65, 64]),
+    (14, 2, 64, "bf16", [5000, 2000], [3, 20]),        # cut along the keys, and joined
+    (8, 1, 128, "fp16", [3000], [33]),
 ])
 def test_prefill(kv4, nh, kvh, d, dtn, starts, counts):
     rng = np.random.default_rng(sum(counts))
@@ -401,16 +409,80 @@ def test_prefill(kv4, nh, kvh, d, dtn, starts, counts):
     T = sum(counts)
     q = rounded(rng.standard_normal((T, nh, d)), dt)
     plan = kv4.PrefillPlan(starts, counts)
+    if max(starts) > 1500:
+        assert plan.work(nh // kvh, kvh)[2] > 1
     order = rng.permutation(len(lens)).astype(np.int32)                 # rows through row_index
     shuffled = np.empty_like(tables)
     shuffled[order] = tables
-    out = torch.full((T, nh, d), 5.0, dtype=dt, device="cuda")
-    kv4.prefill_attention(out, dev(q, dt), dev(pool), dev(shuffled), plan, row_index=dev(order))
-    o, mean, flat, big = OK.prefill(q, pool, tables, starts, counts)
+    rows = torch.zeros(T, nh + 1, d, dtype=dt, device="cuda")           # strided q and out
+    rows[:, :nh] = dev(q, dt)
+    big = torch.full((T, nh + 2, d), 5.0, dtype=dt, device="cuda")
+    out = big[:, :nh]
+    kv4.prefill_attention(out, rows[:, :nh], dev(pool), dev(shuffled), plan, row_index=dev(order))
+    check_prefill(out, OK.prefill(q, pool, tables, starts, counts), dt, d)
+    assert (big[:, nh:] == 5).all()
+    again = torch.empty(T, nh, d, dtype=dt, device="cuda")
+    kv4.prefill_attention(again, dev(q, dt), dev(pool), dev(tables), plan)
+    assert torch.equal(again, out)
+
+
+def check_prefill(out, exact, dt, d, rows=slice(None)):
+    o, mean, flat, big = exact
     ds = (d + 8) * 2.0 ** -24 * big[..., None]
-    tol = half_step(o, dt) + mean * (2.0 ** -11 + 2 * ds + 2.0 ** -20) + 2.0 ** -25 * flat
+    tol = half_step(o, dt) + mean * (2.0 ** -11 + 2 * ds + 2.0 ** -20) + 2.0 ** -31 * flat
     err = np.abs(out.double().cpu().numpy() - o)
-    assert (err <= tol).all(), np.max(err / tol)
+    assert (err <= tol)[rows].all(), np.nanmax((err / tol)[rows])
+
+
+def test_prefill_growing_keys_and_query_magnitudes(kv4):
+    """Row maxima that keep rising along the keys (O is rescaled), and rows of very different size."""
+    rng = np.random.default_rng(2)
+    nh, kvh, d, n = 14, 2, 64, 400
+    tables, nb = tables_for(rng, [n])
+    pool = kv4.new_pool(nb, kvh, d)
+    pos = np.arange(n)
+    k = rounded(rng.standard_normal((n, kvh, d)) * (1 + pos[:, None, None] / 8), torch.bfloat16)
+    v = rounded(rng.standard_normal((n, kvh, d)), torch.bfloat16)
+    kv4.append(pool, dev(k, torch.bfloat16), dev(v, torch.bfloat16),
+               dev(tables[0, pos // 16].astype(np.int64) * 16 + pos % 16))
+    q = rng.standard_normal((90, nh, d)) * np.exp2(rng.integers(-40, 4, (90, nh, 1)))
+    q[7, 3] = 0
+    q = rounded(q, torch.bfloat16)
+    out = torch.empty(90, nh, d, dtype=torch.bfloat16, device="cuda")
+    kv4.prefill_attention(out, dev(q, torch.bfloat16), pool, dev(tables), kv4.PrefillPlan([310], [90]))
+    check_prefill(out, OK.prefill(q, pool.cpu().numpy(), tables, [310], [90]), torch.bfloat16, d)
+
+
+def test_prefill_holes_and_nan(kv4):
+    """Blocks that are not there are left out; a NaN reaches the rows that attend to it and no other."""
+    rng = np.random.default_rng(8)
+    nh, kvh, d = 4, 2, 64
+    starts, counts = [100, 30, 0], [60, 50, 40]
+    lens = np.array([160, 80, 40])
+    tables, nb = tables_for(rng, lens)
+    pool = random_pool(rng, nb, kvh, d)
+    tables[0, 2], tables[0, 7], tables[1, 3] = -1, nb + 5, -1
+    q = rounded(rng.standard_normal((150, nh, d)), torch.float16)
+    clean = pool.copy()
+    # values: token 130 of sequence 0, head 1, dims 32-47; keys: token 50 of sequence 1, head 0
+    pool[tables[0, 130 // 16], 1, 16 * d + d + 2 * 16 + 130 % 16] = 0xFF
+    tables[1, 3] = tables[1, 4]
+    tables[1, 4] = -1
+    pool[tables[1, 50 // 16], 0, 16 * d + 0 * 16 + 50 % 16] = 0xFF
+    out = torch.empty(150, nh, d, dtype=torch.float16, device="cuda")
+    kv4.prefill_attention(out, dev(q, torch.float16), dev(pool), dev(tables),
+                          kv4.PrefillPlan(starts, counts))
+    bad = torch.isnan(out).cpu().numpy()
+    want = np.zeros_like(bad)
+    want[30:60, 2:, 32:48] = True                   # positions 130 and on
+    want[60 + 20:110, :2] = True                    # positions 50 and on
+    np.testing.assert_array_equal(bad, want)
+    exact = OK.prefill(q, clean, tables, starts, counts)
+    o, mean, flat, big = exact
+    ds = (d + 8) * 2.0 ** -24 * big[..., None]
+    tol = half_step(o, torch.float16) + mean * (2.0 ** -11 + 2 * ds + 2.0 ** -20) + 2.0 ** -31 * flat
+    err = np.abs(out.double().cpu().numpy() - o)
+    assert (err <= tol)[~want].all()
 
 
 # ---- eviction ---------------------------------------------------------------------------------------

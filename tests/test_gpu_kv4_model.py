@@ -109,7 +109,7 @@ def check_step(kv, tr, slots, starts, counts, weights_before=None):
         err = np.abs(tr.attn[la].reshape(o.shape) - o)
         ds = (D + 8) * 2.0 ** -24 * big[..., None]
         tol = (half_step(o, torch.bfloat16) + mean * (2.0 ** -11 + 2 * ds + 2.0 ** -20) +
-               2.0 ** -25 * flat)
+               2.0 ** -31 * flat)
         assert (err <= tol).all(), (la, np.max(err / tol))
 
 

@@ -65,19 +65,38 @@ def test_survivors_rule():
 def test_prefill_plan_layout():
     from tiny_infra_b200.kv4 import PrefillPlan
     p = PrefillPlan([0, 511, 100, 7], [1, 33, 130, 0], device="cpu")
-    assert (p.num_seqs, p.num_tokens, p.num_tiles) == (4, 164, 1 + 3 + 9)
-    assert p.lens.tolist() == [1, 544, 230, 0]
-    assert p.scratch_blocks == 1 + 34 + 15 and p.max_blocks == 34
-    t = p.tables.numpy()
-    used = t[t >= 0]
-    assert sorted(used.tolist()) == list(range(50))
-    assert (t[0] >= 0).sum() == 1 and (t[1] >= 0).sum() == 34 and (t[3] >= 0).sum() == 0
-    tiles = list(zip(p.tile_seq.tolist(), p.tile_q0.tolist()))
-    assert sorted(tiles) == sorted([(0, 0)] + [(1, 16 * i) for i in range(3)] +
-                                   [(2, 16 * i) for i in range(9)])
-    ends = [[0, 511, 100][s] + min(q + 16, [1, 33, 130][s]) for s, q in tiles]
-    assert ends == sorted(ends, reverse=True)
-    assert PrefillPlan([], [], device="cpu").num_tiles == 0
+    assert (p.num_seqs, p.num_tokens, p.max_blocks) == (4, 164, 34)
+    assert p.start_pos.tolist() == [0, 511, 100, 7]
+    assert p.cu_seqlens.tolist() == [0, 1, 34, 164, 164]
+    assert PrefillPlan([], [], device="cpu").work(7, 2)[2] == 0
+    rng = np.random.default_rng(0)
+    for group in (1, 2, 3, 7, 8, 12, 16):
+        pair = 256 // (1 << (group - 1).bit_length())
+        for _ in range(20):
+            n = int(rng.integers(1, 5))
+            starts, counts = rng.integers(0, 40000, n), rng.integers(0, 900, n)
+            starts[0] *= int(rng.integers(0, 2))
+            items, merges, parts = PrefillPlan(starts, counts, device="cpu").work(group, 2)
+            length = items[:, 3] - items[:, 2]
+            assert (length > 0).all() and (np.diff(length) <= 0).all() and (items[:, 2] % 64 == 0).all()
+            joined = {(s, q): (f, k) for s, q, f, k in merges.tolist()}
+            seen = []
+            for i in range(n):
+                for q0 in range(0, int(counts[i]), pair):
+                    keys = int(starts[i] + min(q0 + pair, counts[i]))
+                    mine = sorted(items[(items[:, 0] == i) & (items[:, 1] == q0)].tolist(),
+                                  key=lambda r: r[2])
+                    ends = [0] + [r[3] for r in mine]                # the ranges cover the keys once
+                    assert [r[2] for r in mine] == ends[:-1] and ends[-1] == keys
+                    got = [r[4] for r in mine]
+                    if len(mine) == 1:
+                        assert got == [-1] and (i, q0) not in joined
+                    else:
+                        f, k = joined[i, q0]
+                        assert got == list(range(f, f + k)) and k == len(mine)
+                        seen += got
+            assert sorted(seen) == list(range(parts))
+            assert len(items) == len(seen) + sum(-(-int(c) // pair) for c in counts) - len(merges)
     for bad in (([0], [1, 2]), ([-1], [3]), ([0], [-3])):
         with pytest.raises(RuntimeError):
             PrefillPlan(*bad, device="cpu")
@@ -152,6 +171,29 @@ def test_c_abi_refusals(native):
     refused(acc(nh=13), 1, b"multiple")
     refused(acc(d=256), 2, b"head_dim")
     refused(acc(q=FAKE + 4), 1, b"aligned")
+
+    assert lib.ti_kv4_prefill_workspace_bytes(3, 2, 64) == 3 * 2 * 2 * 128 * 66 * 4
+    assert lib.ti_kv4_prefill_workspace_bytes(0, 2, 64) == 0
+
+    def pre(out=FAKE, items=FAKE, n=2, merges=None, nm=0, parts=0, nh=14, d=64, bs=16, dt=0, mb=4,
+            ws=None, wb=0, qs=14 * 64):
+        return lib.ti_kv4_prefill_attention(out, 14 * 64, FAKE, qs, FAKE, 8, FAKE, 4, mb, None, FAKE,
+                                            FAKE, items, n, merges, nm, parts, nh, 2, d, bs, dt, ws,
+                                            wb, None)
+    assert pre(n=0) == 0
+    refused(pre(out=None), 1, b"null")
+    refused(pre(items=None), 1, b"null")
+    refused(pre(nm=1), 1, b"null")
+    refused(pre(parts=2), 1, b"null")
+    refused(pre(n=-1), 1, b"negative")
+    refused(pre(mb=0), 1, b"table width")
+    refused(pre(nh=15), 1, b"multiple")
+    refused(pre(nh=34), 2, b"16 query heads")
+    refused(pre(d=96), 2, b"head_dim")
+    refused(pre(bs=8), 2, b"block_size")
+    refused(pre(dt=2), 2, b"dtype")
+    refused(pre(qs=14 * 64 + 4), 1, b"aligned")
+    refused(pre(parts=2, ws=FAKE, wb=100), 4, b"workspace")
 
     def ev(pool=FAKE, layers=1, b=2, keep=4, recent=2, kept=None, ks=0, d=64, bs=16):
         return lib.ti_kv4_evict(pool, FAKE, layers, 8, FAKE, 4, FAKE, 4, None, FAKE, b, 4, 4, keep,

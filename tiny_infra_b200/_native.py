@@ -69,6 +69,9 @@ SIGNATURES: dict[str, tuple] = {
                                       I32, I32, I32, P, SZ, P]),
     "ti_kv4_accumulate_weights": (I32, [P, P, P, I64, P, P, I64, P, I64, P, P, I32, I32, I32, I32,
                                         I32, I32, I32, P]),
+    "ti_kv4_prefill_workspace_bytes": (SZ, [I32, I32, I32]),
+    "ti_kv4_prefill_attention": (I32, [P, I64, P, I64, P, I64, P, I64, I32, P, P, P, P, I32, P, I32,
+                                       I32, I32, I32, I32, I32, I32, P, SZ, P]),
     "ti_kv4_evict": (I32, [P, P, I32, I64, P, I64, P, I64, P, P, I32, I32, I32, I32, I32, P, I64,
                            I32, I32, I32, P]),
 }

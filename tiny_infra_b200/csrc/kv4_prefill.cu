@@ -1,0 +1,525 @@
+// Ragged causal prefill attention over the 4-bit paged KV cache, tcgen05.  Format: kv4.cuh.
+//
+// out = softmax(q K^T / sqrt(D), keys 0 .. own position) V for chunks of query tokens whose K and V are
+// already in the cache.
+//
+// A tile is 128 rows: the query heads of one kv head (a power of two of slots, at most 16) times 128 /
+// slots tokens.  One CTA takes two tiles of neighbouring tokens and a range of keys; both share each
+// 64-key chunk, which four warps read as codes (asynchronous copies, three chunks ahead) and write to
+// shared memory as half precision -- exact, 2.25 times less to read than 16-bit keys and no scratch
+// copy of the cache.  Per chunk and tile:
+//   S = Q K^T   M 128, N 64, into one of two TMEM buffers;
+//   softmax     one row per thread, straight from TMEM: causal mask, a running max that is kept until
+//               a row's grows by more than 2^8 (then O is rescaled in TMEM), P = 2^(s - m) as half
+//               precision back into the S buffer's columns, the A operand of the next product;
+//   O += P V    A from TMEM, V read in place as an MN-major operand; fp32 O in TMEM.
+// The MMA warp issues S of chunk c for both tiles before P V of chunk c-1, so the tensor cores work
+// while the eight softmax warps do.  bf16 queries are scaled by a power of two per row as in the
+// decode kernel; P is held times 2^7 (at most 2^15; steps of 2^-31), its sum taken before rounding.
+// Bound: the exponentials (16 a clock and SM: 512 clocks a tile and chunk, against 365 of MMA).
+//
+// Work: the host cuts every pair of tiles' keys into ranges of about the same size, longest first, so
+// that a few long prefixes fill the GPU; a pair cut into several ranges leaves un-normalised partials
+// that merge_kernel joins in order.
+//
+// A key that is masked in some row of a tile and is NaN costs that row nothing: its score is replaced.
+// A masked value that is NaN would (0 * NaN): NaN groups of V go into the product as zeros, and the
+// first position of one is kept per 16 dims; rows at or behind it get NaN there.
+#include <algorithm>
+#include <atomic>
+
+#include "capi_internal.h"
+#include "common.cuh"
+#include "kv4.cuh"
+#include "tcgen05.cuh"
+
+namespace ti {
+namespace kv4 {
+namespace pre {
+
+constexpr int kChunk = 64;                       // keys per step
+constexpr int kStages = 3;                       // chunks of K and V in half precision
+constexpr int kRaw = 4;                          // chunks of codes
+constexpr int kSoftWarps = 8, kLoadWarps = 4;
+constexpr int kThreads = (kSoftWarps + kLoadWarps + 1) * 32;
+constexpr float kPScale = 7.f;
+constexpr int kItemInts = 6;                     // sequence, first token, key range, part or -1, spare
+constexpr int kMergeInts = 4;                    // sequence, first token, first part, parts
+
+struct Params {
+  void* out;
+  const void* q;
+  const uint8_t* pool;
+  int64_t out_stride, q_stride, num_blocks, bt_stride;
+  const int32_t *tables, *row_index, *start_pos, *cu_seqlens, *items;
+  float* parts;
+  int NH, KVH, group, slots_log2, max_blocks;
+  float scale_log2;
+};
+
+template <int HD>
+struct Smem {
+  static constexpr int kSub = HD / 64;           // 64-dim sub-tiles of a row
+  static constexpr int kQTile = kSub * 16384;
+  static constexpr int kKvTile = kSub * 8192;    // K or V of a chunk
+  static constexpr int kRawChunk = 4 * Tile<HD>::kBytes;
+  static constexpr int kQ = 0, kKv = 2 * kQTile, kRawAt = kKv + kStages * 2 * kKvTile;
+  static constexpr int kInv = kRawAt + kRaw * kRawChunk;         // [2][128] floats
+  static constexpr int kNan = kInv + 1024;                       // [HD/16] ints
+  static constexpr int kOk = kNan + 64;                          // [8] ints
+  static constexpr int kBars = kOk + 64;
+  static constexpr int kTotal = kBars + 192 + 1024;              // and alignment slack
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void st_shared_v4(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_constant__ Params p) {
+  using S = Smem<HD>;
+  using L = Tile<HD>;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~uintptr_t(1023));
+  const uint32_t sb = smem_u32(smem);
+  const uint32_t kv_full = sb + S::kBars, kv_empty = kv_full + 8 * kStages;
+  const uint32_t s_full = kv_empty + 8 * kStages;                // [tile][buffer]
+  const uint32_t p_ready = s_full + 32, pv_done = p_ready + 16;  // [tile]
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(smem + S::kBars + 160);
+  float* s_inv = reinterpret_cast<float*>(smem + S::kInv);
+  int* s_nan = reinterpret_cast<int*>(smem + S::kNan);
+  volatile int* s_ok = reinterpret_cast<int*>(smem + S::kOk);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  constexpr int kMmaWarp = kSoftWarps + kLoadWarps;
+
+  if (warp == kMmaWarp) {
+    if (lane == 0) {
+      for (int i = 0; i < kStages; ++i) {
+        mbar_init(kv_full + 8 * i, kLoadWarps * 32);
+        mbar_init(kv_empty + 8 * i, 1);
+      }
+      for (int i = 0; i < 4; ++i) mbar_init(s_full + 8 * i, 1);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(p_ready + 8 * i, 4);
+        mbar_init(pv_done + 8 * i, 1);
+      }
+      fence_mbar_init();
+    }
+    __syncwarp();
+    tmem_alloc(smem_u32(tslot), 512);
+  }
+  if (tid < HD / 16) s_nan[tid] = 0x7FFFFFFF;
+  pdl_wait();
+
+  const int kvh = blockIdx.x % p.KVH;
+  const int32_t* item = p.items + (int64_t)(blockIdx.x / p.KVH) * kItemInts;
+  const int seq = item[0], q0 = item[1], kb = item[2], ke = item[3], part = item[4];
+  const int tile_tokens = 128 >> p.slots_log2;
+  const int row0 = p.cu_seqlens[seq], count = p.cu_seqlens[seq + 1] - row0;
+  const int start = p.start_pos[seq], cached = start + count;
+  const int ntiles = q0 + tile_tokens < count ? 2 : 1;
+  const int n = (ke - kb + kChunk - 1) / kChunk;
+  const int32_t* table = p.tables + (int64_t)(p.row_index ? p.row_index[seq] : seq) * p.bt_stride;
+
+  // Q: row r of a tile = head slot r % slots of token r / slots (zeros beyond the group or the chunk)
+  for (int i = tid; i < ntiles * 128 * (HD / 8); i += kThreads) {
+    const int c = i % (HD / 8), r = (i / (HD / 8)) & 127, x = i / (128 * (HD / 8));
+    const int h = r & ((1 << p.slots_log2) - 1), t = q0 + x * tile_tokens + (r >> p.slots_log2);
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if (h < p.group && t < count)
+      v = *reinterpret_cast<const uint4*>((const T*)p.q + (int64_t)(row0 + t) * p.q_stride +
+                                          (int64_t)(kvh * p.group + h) * HD + c * 8);
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      // (the HD/8 threads of a row are neighbouring lanes of one warp: kThreads and the loop's bound
+      // are multiples of 32)
+      uint32_t w[4] = {v.x, v.y, v.z, v.w}, top = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) top = max(top, max(w[k] & 0x7FFFu, (w[k] >> 16) & 0x7FFFu));
+#pragma unroll
+      for (int d = HD / 16; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+      const int e = min(max((int)(top >> 7), 15), 254);
+      const float mul = __uint_as_float((uint32_t)(254 + 14 - e) << 23);       // 2^(14 - (e - 127))
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 f = Elem<T>::unpack2(w[k]);
+        w[k] = Elem<__half>::pack2(f.x * mul, f.y * mul);
+      }
+      v = make_uint4(w[0], w[1], w[2], w[3]);
+      if (c == 0) s_inv[x * 128 + r] = __uint_as_float((uint32_t)(e - 14) << 23);
+    } else if (c == 0) {
+      s_inv[x * 128 + r] = 1.f;
+    }
+    *reinterpret_cast<uint4*>(smem + S::kQ + x * S::kQTile + (c >> 3) * 16384 + r * 128 +
+                              (((c & 7) ^ (r & 7)) << 4)) = v;
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tslot;
+  pdl_launch_dependents();
+  // TMEM columns: S buffers of tile x at 128 x and 128 x + 64, O at 256 + 128 x
+  if (warp >= kSoftWarps && warp < kMmaWarp) {
+    // ---- loaders: codes -> half precision
+    const int lt = tid - kSoftWarps * 32;
+    constexpr int kUnits = S::kRawChunk / 16, kTileUnits = L::kBytes / 16;
+    auto block_id = [&](int c, int b) -> int {   // block b of chunk c, -1: none
+      const int blk = kb / kBlock + c * 4 + b;
+      if (c >= n || blk >= p.max_blocks || (int64_t)blk * kBlock >= cached) return -1;
+      const int id = table[blk];
+      return id >= 0 && id < p.num_blocks ? id : -1;
+    };
+    auto issue = [&](int c) {
+      const uint32_t raw = sb + S::kRawAt + (c % kRaw) * S::kRawChunk;
+#pragma unroll
+      for (int i = 0; i < (kUnits + 127) / 128; ++i) {
+        const int u = lt + i * 128;
+        if (u < kUnits) {
+          const int id = block_id(c, u / kTileUnits);
+          if (id >= 0)
+            cp_async16(raw + u * 16, p.pool + ((int64_t)id * p.KVH + kvh) * L::kBytes + (u % kTileUnits) * 16);
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    for (int c = 0; c < kRaw - 1; ++c) issue(c);
+    const int tok = lt >> 1, half = lt & 1;      // this thread's token of a chunk, half of its dims
+    // after a wait that gave up the loop goes on without waiting: all 128 threads keep meeting at the
+    // barrier, and the results are void anyway
+    bool ok = true;
+    for (int c = 0; c < n; ++c) {
+      const int st = c % kStages;
+      asm volatile("cp.async.wait_group %0;" ::"n"(kRaw - 2) : "memory");
+      asm volatile("bar.sync 1, 128;" ::: "memory");   // everyone's copies; chunk c-1 was read
+      issue(c + kRaw - 1);
+      if (warp == kSoftWarps) {
+        const uint32_t have = __ballot_sync(0xffffffffu, lane < 4 && block_id(c, lane & 3) >= 0);
+        if (lane == 0) s_ok[c & 7] = (int)(have & 15u);
+      }
+      const int pos = kb + c * kChunk + tok;
+      const bool live = pos < cached && block_id(c, tok / kBlock) >= 0;
+      const uint8_t* raw = smem + S::kRawAt + (c % kRaw) * S::kRawChunk + (tok / kBlock) * L::kBytes;
+      const int off = tok % kBlock;
+      if (ok && c >= kStages && !mbar_wait(kv_empty + 8 * st, ((c / kStages) - 1) & 1, TI_DEVERR_PREFILL_WAIT)) ok = false;
+      const uint32_t dst = sb + S::kKv + st * 2 * S::kKvTile;
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+#pragma unroll
+        for (int u = 0; u < HD / 64; ++u) {      // 32 dims, two scale groups, at a time
+          const int d0 = half * (HD / 2) + u * 32;
+          uint4 w = make_uint4(0u, 0u, 0u, 0u);
+          uint32_t b0 = 0, b1 = 0;
+          if (live) {
+            w = *reinterpret_cast<const uint4*>(raw + (kv ? L::kV : L::kK) + off * L::kRow + d0 / 2);
+            b0 = raw[(kv ? L::kVs : L::kKs) + (d0 / 16) * kBlock + off];
+            b1 = raw[(kv ? L::kVs : L::kKs) + (d0 / 16 + 1) * kBlock + off];
+            if (kv) {
+              if (b0 >= 0xF8u) { atomicMin(&s_nan[d0 / 16], pos); b0 = 0; }
+              if (b1 >= 0xF8u) { atomicMin(&s_nan[d0 / 16 + 1], pos); b1 = 0; }
+            }
+          }
+          const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+          const uint32_t row = dst + kv * S::kKvTile + (d0 / 64) * 8192 + tok * 128;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint32_t h[4];
+            codes_to_half2(ws[k], h);
+            const uint32_t s2 = (k < 2 ? b0 : b1) * 0x00800080u;
+            const int ch = (d0 % 64) / 8 + k;
+            st_shared_v4(row + ((ch ^ (tok & 7)) << 4), hmul2(h[0], s2), hmul2(h[1], s2),
+                         hmul2(h[2], s2), hmul2(h[3], s2));
+          }
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      mbar_arrive(kv_full + 8 * st);
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+  } else if (warp == kMmaWarp) {
+    if (lane == 0) {
+      constexpr uint32_t id_s = idesc_f16(128, kChunk, false, false, false);
+      constexpr uint32_t id_pv = idesc_f16(128, 64, false, false, true);
+      bool ok = true;
+      for (int c = 0; c <= n && ok; ++c) {
+        if (c < n) {
+          const int st = c % kStages, b = c & 1;
+          ok = mbar_wait(kv_full + 8 * st, (c / kStages) & 1, TI_DEVERR_PREFILL_WAIT);
+          const uint32_t kt = sb + S::kKv + st * 2 * S::kKvTile;
+          for (int x = 0; x < ntiles && ok; ++x) {
+            // (P of chunk c-2 sits in this S buffer)
+            if (c >= 2) ok = mbar_wait(pv_done + 8 * x, c & 1, TI_DEVERR_PREFILL_WAIT);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int k = 0; k < HD / 16; ++k)
+              tc_mma(tmem + 128 * x + 64 * b,
+                     smem_desc_sw128(sb + S::kQ + x * S::kQTile + (k / 4) * 16384 + 32 * (k % 4), false),
+                     smem_desc_sw128(kt + (k / 4) * 8192 + 32 * (k % 4), false), id_s, k > 0 ? 1u : 0u);
+            tc_commit(s_full + 8 * (2 * x + b));
+          }
+        }
+        if (c >= 1 && ok) {
+          const int cp = c - 1, sp = cp % kStages, b = cp & 1;
+          const uint32_t vt = sb + S::kKv + sp * 2 * S::kKvTile + S::kKvTile;
+          for (int x = 0; x < ntiles && ok; ++x) {
+            ok = mbar_wait(p_ready + 8 * x, cp & 1, TI_DEVERR_PREFILL_WAIT);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int u = 0; u < S::kSub; ++u)
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                tc_mma_tmem_a(tmem + 256 + 128 * x + 64 * u, tmem + 128 * x + 64 * b + 8 * k,
+                              smem_desc_sw128(vt + u * 8192 + 2048 * k, true), id_pv,
+                              (cp > 0 || k > 0) ? 1u : 0u);
+            tc_commit(pv_done + 8 * x);
+          }
+          if (ok) tc_commit(kv_empty + 8 * sp);
+        }
+      }
+    }
+  } else if (warp / 4 < ntiles) {
+    // ---- softmax and epilogue of tile x: thread <-> row (TMEM lane) r
+    const int x = warp >> 2, quad = warp & 3, r = quad * 32 + lane;
+    const int h = r & ((1 << p.slots_log2) - 1), t = q0 + x * tile_tokens + (r >> p.slots_log2);
+    const bool mine = h < p.group && t < count;
+    const int qp = start + t;                     // (rows that do not exist: finite nonsense)
+    const int first = start + q0 + x * tile_tokens;
+    const uint32_t trow = tmem + ((uint32_t)(quad * 32) << 16);
+    const uint32_t t_s = trow + 128 * x, t_o = trow + 256 + 128 * x;
+    const float sc = s_inv[x * 128 + r] * p.scale_log2;
+    auto wait_all = [&](uint32_t bar, uint32_t parity) {
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, TI_DEVERR_PREFILL_WAIT));
+    };
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int c = 0; c < n; ++c) {
+      const int b = c & 1, k0 = kb + c * kChunk;
+      // (kv_full of this chunk has completed when its scores have: no wait, but the loaders' flags)
+      if (!wait_all(kv_full + 8 * (c % kStages), (c / kStages) & 1) ||
+          !wait_all(s_full + 8 * (2 * x + b), (c >> 1) & 1)) { ok = false; break; }
+      tc_fence_after();
+      const int have = s_ok[c & 7];
+      float sv[kChunk];
+      tmem_ld32(t_s + 64 * b, sv);
+      tmem_ld32(t_s + 64 * b + 32, sv + 32);
+      if (have != 15 || k0 + kChunk - 1 > first) {
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i)
+          sv[i] = (k0 + i <= qp && ((have >> (i / kBlock)) & 1)) ? sv[i] : -INFINITY;
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < kChunk; ++i) mx = fmaxf(mx, sv[i]);
+      mx *= sc;
+      float alpha = 1.f;
+      if (c == 0) {
+        m = mx;
+      } else if (mx > m + 8.f) {                  // (from no key at all: alpha 0 of zeros)
+        alpha = m == -INFINITY ? 0.f : fast_exp2(m - mx);
+        m = mx;
+      }
+      const float off = kPScale - (m == -INFINITY ? 0.f : m);
+      float sum = 0.f;                            // of the chunk: a long row's total stays exact enough
+      uint32_t pk[kChunk / 2];
+#pragma unroll
+      for (int i = 0; i < kChunk; i += 2) {
+        const float p0 = fast_exp2(fmaf(sv[i], sc, off)), p1 = fast_exp2(fmaf(sv[i + 1], sc, off));
+        sum += p0 + p1;
+        pk[i / 2] = Elem<__half>::pack2(p0, p1);
+      }
+      l = l * alpha + sum;
+      // (each phase is waited for in turn: a parity tells neighbouring phases apart, no more)
+      if (c >= 1 && !wait_all(pv_done + 8 * x, (c - 1) & 1)) { ok = false; break; }
+      if (__any_sync(0xffffffffu, alpha != 1.f)) {
+        tc_fence_after();
+        float ov[32];
+#pragma unroll
+        for (int d = 0; d < HD; d += 32) {
+          tmem_ld32(t_o + d, ov);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) ov[i] *= alpha;
+          tmem_st32(t_o + d, ov);
+        }
+      }
+      tmem_st32_u(t_s + 64 * b, pk);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_ready + 8 * x);
+    }
+    if (ok && wait_all(pv_done + 8 * x, (n - 1) & 1)) {
+      tc_fence_after();
+      const float inv = 1.f / l;
+      T* dst = (T*)p.out + (int64_t)(row0 + t) * p.out_stride + (int64_t)(kvh * p.group + h) * HD;
+      float* po = p.parts + (((int64_t)part * p.KVH + kvh) * 2 + x) * (128 * (HD + 2));
+#pragma unroll
+      for (int d = 0; d < HD; d += 32) {
+        float ov[32];
+        tmem_ld32(t_o + d, ov);
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+          if (qp >= s_nan[d / 16 + g]) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) ov[g * 16 + i] = __int_as_float(0x7FC00000);
+          }
+        if (part >= 0) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<float4*>(po + r * HD + d + i) = make_float4(ov[i], ov[i + 1], ov[i + 2], ov[i + 3]);
+        } else if (mine) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            uint4 u;
+            u.x = Elem<T>::pack2(ov[i] * inv, ov[i + 1] * inv);
+            u.y = Elem<T>::pack2(ov[i + 2] * inv, ov[i + 3] * inv);
+            u.z = Elem<T>::pack2(ov[i + 4] * inv, ov[i + 5] * inv);
+            u.w = Elem<T>::pack2(ov[i + 6] * inv, ov[i + 7] * inv);
+            *reinterpret_cast<uint4*>(dst + d + i) = u;
+          }
+        }
+      }
+      if (part >= 0) {
+        po[128 * HD + r] = m;
+        po[128 * HD + 128 + r] = l;
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Join the key ranges of one (pair of tiles, kv head, tile): 16 rows a CTA, in the ranges' order.
+constexpr int kMergeRows = 16;
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kMergeRows * HD / 4) merge_kernel(const __grid_constant__ Params p,
+                                                                  const int32_t* merges) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int kvh = blockIdx.x % p.KVH, x = blockIdx.y & 1;
+  const int32_t* e = merges + (int64_t)(blockIdx.x / p.KVH) * kMergeInts;
+  const int seq = e[0], q0 = e[1], slot = e[2], n = e[3];
+  const int r = (blockIdx.y >> 1) * kMergeRows + threadIdx.x / (HD / 4), d = threadIdx.x % (HD / 4) * 4;
+  const int row0 = p.cu_seqlens[seq], count = p.cu_seqlens[seq + 1] - row0;
+  const int h = r & ((1 << p.slots_log2) - 1);
+  const int t = q0 + x * (128 >> p.slots_log2) + (r >> p.slots_log2);
+  if (h >= p.group || t >= count) return;         // (rows of an absent second tile end here too)
+  auto part = [&](int i) { return p.parts + (((int64_t)(slot + i) * p.KVH + kvh) * 2 + x) * (128 * (HD + 2)); };
+  float m = -INFINITY, l = 0.f;
+  for (int i = 0; i < n; ++i) m = fmaxf(m, part(i)[128 * HD + r]);
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) {
+    const float* b = part(i);
+    const float mi = b[128 * HD + r];
+    const float c = mi == -INFINITY ? 1.f : fast_exp2(mi - m);   // (no finite score: zeros, or NaN)
+    const float4 v = *reinterpret_cast<const float4*>(b + r * HD + d);
+    l += c * b[128 * HD + 128 + r];
+    o.x += c * v.x;
+    o.y += c * v.y;
+    o.z += c * v.z;
+    o.w += c * v.w;
+  }
+  const float inv = 1.f / l;
+  T* dst = (T*)p.out + (int64_t)(row0 + t) * p.out_stride + (int64_t)(kvh * p.group + h) * HD + d;
+  *reinterpret_cast<uint2*>(dst) = make_uint2(Elem<T>::pack2(o.x * inv, o.y * inv),
+                                              Elem<T>::pack2(o.z * inv, o.w * inv));
+}
+
+template <typename T, int HD>
+static int launch(const Params& p, int num_items, const int32_t* merges, int num_merges, cudaStream_t s) {
+  static std::atomic<uint64_t> ready{0};          // devices whose limit has been raised
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(ready.load(std::memory_order_acquire) & bit)) {
+    cudaError_t e = cudaFuncSetAttribute(prefill_kernel<T, HD>,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<HD>::kTotal);
+    if (e != cudaSuccess) {
+      (void)cudaGetLastError();
+      return set_cuda_error(e, "cudaFuncSetAttribute(kv4 prefill)");
+    }
+    ready.fetch_or(bit, std::memory_order_release);
+  }
+  if (int rc = launch_kernel("kv4 prefill launch", prefill_kernel<T, HD>,
+                             dim3((unsigned)num_items * p.KVH), dim3(kThreads), Smem<HD>::kTotal, s, 1, p))
+    return rc;
+  if (num_merges == 0) return TI_OK;
+  return launch_kernel("kv4 prefill merge launch", merge_kernel<T, HD>,
+                       dim3((unsigned)num_merges * p.KVH, 2 * 128 / kMergeRows),
+                       dim3(kMergeRows * HD / 4), 0, s, 1, p, merges);
+}
+
+}  // namespace pre
+}  // namespace kv4
+}  // namespace ti
+
+using namespace ti;
+
+extern "C" size_t ti_kv4_prefill_workspace_bytes(int num_parts, int num_kv_heads, int head_dim) {
+  if (num_parts <= 0 || num_kv_heads <= 0 || (head_dim != 64 && head_dim != 128)) return 0;
+  return (size_t)num_parts * num_kv_heads * 2 * 128 * (head_dim + 2) * 4;
+}
+
+extern "C" int ti_kv4_prefill_attention(void* out, int64_t out_tok_stride, const void* q,
+                                        int64_t q_tok_stride, const void* pool, int64_t num_blocks,
+                                        const int32_t* block_tables, int64_t bt_stride,
+                                        int max_blocks_per_seq, const int32_t* row_index,
+                                        const int32_t* start_pos, const int32_t* cu_seqlens,
+                                        const int32_t* items, int num_items, const int32_t* merges,
+                                        int num_merges, int num_parts, int num_heads,
+                                        int num_kv_heads, int head_dim, int block_size, int dtype,
+                                        void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  if (num_items == 0) return TI_OK;
+  if (!out || !q || !pool || !block_tables || !start_pos || !cu_seqlens || !items || num_items < 0 ||
+      num_merges < 0 || num_parts < 0 || (num_merges > 0 && !merges) || (num_parts > 0 && !workspace))
+    return set_error(TI_ERR_INVALID_ARGUMENT, "kv4 prefill: null pointer or negative size");
+  if (num_blocks <= 0 || max_blocks_per_seq <= 0 || num_kv_heads <= 0 || num_heads <= 0 ||
+      num_heads % num_kv_heads)
+    return set_error(TI_ERR_INVALID_ARGUMENT,
+                     "kv4 prefill: bad table width, pool size or head counts (num_heads must be a multiple of num_kv_heads)");
+  if (num_heads / num_kv_heads > 16)
+    return set_error(TI_ERR_UNSUPPORTED, "kv4 prefill: at most 16 query heads per kv head");
+  if ((head_dim != 64 && head_dim != 128) || block_size != kv4::kBlock)
+    return set_error(TI_ERR_UNSUPPORTED, "kv4 prefill: head_dim must be 64 or 128, block_size 16");
+  if (dtype != TI_DTYPE_BF16 && dtype != TI_DTYPE_FP16)
+    return set_error(TI_ERR_UNSUPPORTED, "kv4 prefill: dtype must be bf16 or fp16");
+  if (((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(q) |
+        reinterpret_cast<uintptr_t>(pool) | reinterpret_cast<uintptr_t>(workspace)) & 15) ||
+      (out_tok_stride % 8) || (q_tok_stride % 8))
+    return set_error(TI_ERR_INVALID_ARGUMENT, "kv4 prefill: tensors must be 16-byte aligned");
+  if ((int64_t)num_items * num_kv_heads >= (int64_t)1 << 31 ||
+      (int64_t)num_merges * num_kv_heads >= (int64_t)1 << 31)
+    return set_error(TI_ERR_UNSUPPORTED, "kv4 prefill: too many work items");
+  if (workspace_bytes < ti_kv4_prefill_workspace_bytes(num_parts, num_kv_heads, head_dim))
+    return set_error(TI_ERR_WORKSPACE, "kv4 prefill: workspace too small");
+  const int group = num_heads / num_kv_heads;
+  int slots_log2 = 0;
+  while ((1 << slots_log2) < group) ++slots_log2;
+  kv4::pre::Params p{out, q, (const uint8_t*)pool, out_tok_stride, q_tok_stride, num_blocks,
+                     bt_stride, block_tables, row_index, start_pos, cu_seqlens, items,
+                     (float*)workspace, num_heads, num_kv_heads, group, slots_log2,
+                     max_blocks_per_seq, 1.4426950408889634f / sqrtf((float)head_dim)};
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (dtype == TI_DTYPE_BF16)
+    return head_dim == 64 ? kv4::pre::launch<__nv_bfloat16, 64>(p, num_items, merges, num_merges, s)
+                          : kv4::pre::launch<__nv_bfloat16, 128>(p, num_items, merges, num_merges, s);
+  return head_dim == 64 ? kv4::pre::launch<__half, 64>(p, num_items, merges, num_merges, s)
+                        : kv4::pre::launch<__half, 128>(p, num_items, merges, num_merges, s);
+}

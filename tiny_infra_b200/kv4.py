@@ -318,8 +318,7 @@ def accumulate_weights(weights: torch.Tensor, q: torch.Tensor, lse: torch.Tensor
 class PrefillPlan:
     """Layout of a packed prefill: chunk i holds ``counts[i]`` query tokens at positions
     ``starts[i]`` and on, whose K and V are already in the cache.  Built once per batch, used by
-    every layer; it holds the query tiles (16 tokens, longest prefix first) and where the cached
-    tokens are read back to."""
+    every layer; the work items of a head layout are laid out at its first use and kept."""
 
     def __init__(self, starts, counts, device="cuda") -> None:
         starts, counts = np.asarray(starts, np.int64), np.asarray(counts, np.int64)
@@ -328,43 +327,63 @@ class PrefillPlan:
         if not ((starts >= 0).all() and (counts >= 0).all()):
             _fail("starts and counts must be >= 0")
         lens = np.where(counts > 0, starts + counts, 0)
-        blocks = -(-lens // BLOCK)
-        if int(lens.max(initial=0)) >= 2 ** 31 or int(blocks.sum()) >= 2 ** 31:
+        if int(lens.max(initial=0)) >= 2 ** 31 or int(counts.sum()) >= 2 ** 31:
             _fail("prefill too long")
+        self.starts, self.counts, self.device = starts, counts, device
         self.num_seqs, self.num_tokens = len(starts), int(counts.sum())
-        self.max_blocks = int(blocks.max(initial=0))
-        self.scratch_blocks = int(blocks.sum())
-        seq, q0, work = [], [], []
-        for i, (s, n) in enumerate(zip(starts.tolist(), counts.tolist())):
-            for t in range(0, n, 16):
-                seq.append(i)
-                q0.append(t)
-                work.append(s + min(t + 16, n))
-        order = np.argsort(-np.asarray(work, np.int64), kind="stable")
-        self.num_tiles = len(seq)
-        at = np.concatenate([[0], np.cumsum(blocks)[:-1]]) if len(starts) else blocks
-        col = np.arange(max(self.max_blocks, 1))
-        tables = np.where(col < blocks[:, None], at[:, None] + col, -1)
+        self.max_blocks = int((-(-lens // BLOCK)).max(initial=0))
+        self._dev = torch.from_numpy(np.concatenate([starts, [0], np.cumsum(counts)])
+                                     .astype(np.int32)).to(device)
+        self.start_pos, self.cu_seqlens = self._dev[:self.num_seqs], self._dev[self.num_seqs:]
+        self._layouts: dict = {}
 
-        def dev(a):
-            return torch.from_numpy(np.ascontiguousarray(a, np.int32)).to(device)
+    def work(self, group: int, kv_heads: int):
+        """Items and merges (``ti_kv4_prefill_attention``) as host arrays, and the number of parts.
 
-        self.start_pos, self.lens = dev(starts), dev(lens)
-        self.rows = dev(np.arange(self.num_seqs))
-        self.cu_seqlens = dev(np.concatenate([[0], np.cumsum(counts)]))
-        self.tile_seq, self.tile_q0 = dev(np.asarray(seq)[order]), dev(np.asarray(q0)[order])
-        self.tables = dev(tables.reshape(self.num_seqs, max(self.max_blocks, 1)))
+        A pair of tiles is 256 / slots tokens; its keys are cut into ranges of at most a third of
+        what each of 148 SMs would get on average (at least 1024: a range costs a few microseconds
+        of its own), longest items first, so that a few long prefixes still fill the GPU."""
+        slots = 1 << (group - 1).bit_length()
+        pair = 256 // slots
+        seq = np.repeat(np.arange(self.num_seqs), -(-self.counts // pair))
+        per = np.concatenate([np.arange(0, c, pair) for c in self.counts.tolist()] or
+                             [np.zeros(0, np.int64)]).astype(np.int64)
+        keys = self.starts[seq] + np.minimum(per + pair, self.counts[seq])
+        most = max(1024, int(keys.sum()) * kv_heads // (3 * 148))
+        n = -(-keys // most)
+        size = -(-keys // np.maximum(n, 1) // 64) * 64          # a range, whole 64-key steps
+        n = -(-keys // np.maximum(size, 1))
+        first_part = np.cumsum(np.where(n > 1, n, 0)) - np.where(n > 1, n, 0)
+        at = np.repeat(np.arange(len(seq)), n)                  # the pair of each item
+        k = np.arange(len(at)) - np.repeat(np.cumsum(n) - n, n)  # its range within the pair
+        lo = k * size[at]
+        hi = np.minimum(lo + size[at], keys[at])
+        part = np.where(n[at] > 1, first_part[at] + k, -1)
+        items = np.stack([seq[at], per[at], lo, hi, part, np.zeros_like(lo)], 1)
+        items = items[np.argsort(lo - hi, kind="stable")].astype(np.int32)
+        cut = n > 1
+        merges = np.stack([seq[cut], per[cut], first_part[cut], n[cut]], 1).astype(np.int32)
+        return items, merges, int(n[cut].sum())
+
+    def layout(self, group: int, kv_heads: int):
+        """``work`` on the device: pointers and counts, for calls of this head layout."""
+        key = (group, kv_heads)
+        if key not in self._layouts:
+            items, merges, parts = self.work(group, kv_heads)
+            dev = torch.from_numpy(np.concatenate([items.reshape(-1), merges.reshape(-1)])
+                                   ).to(self.device)
+            base = dev.data_ptr()
+            self._layouts[key] = (dev, base, len(items), base + 4 * items.size, len(merges), parts)
+        return self._layouts[key][1:]
 
 
 def prefill_attention(out: torch.Tensor, q: torch.Tensor, pool: torch.Tensor,
                       block_tables: torch.Tensor, plan: PrefillPlan, *,
                       row_index: torch.Tensor | None = None) -> None:
     """Causal attention of the plan's query tokens (q, out [tokens, NH, D]) over their sequences'
-    cached tokens, positions 0 .. their own, scale 1/sqrt(D).
-
-    The cached values are exact in 16 bits, so they are read back once (``dequantize``, 2 *
-    scratch_blocks * KVH * 16 * D values of scratch) and the 16-bit pool's tensor-core prefill
-    kernel runs on them; the read-back is a few per cent of a chunk's attention."""
+    cached tokens, positions 0 .. their own, scale 1/sqrt(D), on the tensor cores straight from the
+    codes.  At most 16 query heads per kv head.  Tokens whose table entry holds no block are left
+    out.  Chunks with long prefixes are cut along the keys and joined by a second launch."""
     dev = _device(pool, out, q, block_tables, plan.start_pos, row_index)
     nb, kvh, d = _pool_shape(pool)
     T, NH, dq, q_stride = _rows("q", q)
@@ -378,28 +397,24 @@ def prefill_attention(out: torch.Tensor, q: torch.Tensor, pool: torch.Tensor,
     if T != plan.num_tokens:
         _fail("q does not have the plan's tokens")
     _index("row_index", row_index, plan.num_seqs)
-    bt_stride, cols = _table("block_tables", block_tables, plan.num_seqs if row_index is None else None)
+    bt_stride, cols = _table("block_tables", block_tables,
+                             plan.num_seqs if row_index is None else None)
     if cols < plan.max_blocks:
         _fail("block_tables is too narrow for the plan")
-    if plan.num_tiles == 0:
+    if T == 0:
         return
-    lib, dt, nblk = N.lib(), N.dtype_code(q.dtype), plan.scratch_blocks
-    half = nblk * kvh * BLOCK * d                       # elements of K, then of V
-    tables, tab_stride = plan.tables.data_ptr(), plan.tables.stride(0)
+    lib = N.lib()
     with _on(dev):
-        stream = _stream(dev)
-        scratch = torch.empty(2 * half, dtype=q.dtype, device=pool.device)
-        k = scratch.data_ptr()
-        v = k + 2 * half
-        N.check(lib.ti_kv4_dequantize(
-            k, v, nblk, pool.data_ptr(), nb, block_tables.data_ptr(), bt_stride, _ptr(row_index),
-            plan.lens.data_ptr(), tables, tab_stride, plan.num_seqs, plan.max_blocks, kvh, d,
-            BLOCK, dt, stream))
-        N.check(lib.ti_paged_prefill_attention(
-            out.data_ptr(), out_stride, q.data_ptr(), q_stride, k, v, nblk, tables, tab_stride,
-            plan.rows.data_ptr(), plan.start_pos.data_ptr(), plan.cu_seqlens.data_ptr(),
-            plan.tile_seq.data_ptr(), plan.tile_q0.data_ptr(), plan.num_tiles, NH, kvh, d, BLOCK,
-            dt, stream))
+        items, num_items, merges, num_merges, parts = plan.layout(NH // kvh, kvh)
+        ws = None
+        if parts:
+            ws = torch.empty(lib.ti_kv4_prefill_workspace_bytes(parts, kvh, d), dtype=torch.uint8,
+                             device=pool.device)
+        N.check(lib.ti_kv4_prefill_attention(
+            out.data_ptr(), out_stride, q.data_ptr(), q_stride, pool.data_ptr(), nb,
+            block_tables.data_ptr(), bt_stride, cols, _ptr(row_index), plan.start_pos.data_ptr(),
+            plan.cu_seqlens.data_ptr(), items, num_items, merges, num_merges, parts, NH, kvh, d,
+            BLOCK, N.dtype_code(q.dtype), _ptr(ws), 0 if ws is None else ws.numel(), _stream(dev)))
 
 
 def evict(pool: torch.Tensor, weights: torch.Tensor, block_tables: torch.Tensor,
