@@ -67,7 +67,8 @@ struct Smem {
   static constexpr int kInv = kRawAt + kRaw * kRawChunk;         // [2][128] floats
   static constexpr int kNan = kInv + 1024;                       // [HD/16] ints
   static constexpr int kOk = kNan + 64;                          // [8] ints
-  static constexpr int kBars = kOk + 64;
+  static constexpr int kIds = kOk + 64;                          // [8][4] ints
+  static constexpr int kBars = kIds + 128;
   static constexpr int kTotal = kBars + 192 + 1024;              // and alignment slack
 };
 
@@ -81,6 +82,33 @@ __device__ __forceinline__ void st_shared_v4(uint32_t a, uint32_t x, uint32_t y,
 __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
   uint32_t d;
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+// Two floats in one 64-bit register, for the packed fp32 instructions.
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
+  return d;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 d;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(v));
+  return d;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
 
@@ -98,8 +126,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
   uint32_t* tslot = reinterpret_cast<uint32_t*>(smem + S::kBars + 160);
   float* s_inv = reinterpret_cast<float*>(smem + S::kInv);
   int* s_nan = reinterpret_cast<int*>(smem + S::kNan);
+  int* s_ids = reinterpret_cast<int*>(smem + S::kIds);
   volatile int* s_ok = reinterpret_cast<int*>(smem + S::kOk);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   constexpr int kMmaWarp = kSoftWarps + kLoadWarps;
 
   if (warp == kMmaWarp) {
@@ -179,13 +208,18 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
       const int id = table[blk];
       return id >= 0 && id < p.num_blocks ? id : -1;
     };
+    // block ids go through a ring of eight chunks, loaded eight chunks ahead (a table read per copy
+    // put its latency into every chunk: 796 us instead of @@ at four chunks of 1024)
+    if (lt < 28) s_ids[lt] = block_id(lt / 4, lt % 4);
+    int next_id = lt < 4 ? block_id(7, lt) : -1;
+    asm volatile("bar.sync 1, 128;" ::: "memory");
     auto issue = [&](int c) {
       const uint32_t raw = sb + S::kRawAt + (c % kRaw) * S::kRawChunk;
 #pragma unroll
       for (int i = 0; i < (kUnits + 127) / 128; ++i) {
         const int u = lt + i * 128;
         if (u < kUnits) {
-          const int id = block_id(c, u / kTileUnits);
+          const int id = s_ids[(c & 7) * 4 + u / kTileUnits];
           if (id >= 0)
             cp_async16(raw + u * 16, p.pool + ((int64_t)id * p.KVH + kvh) * L::kBytes + (u % kTileUnits) * 16);
         }
@@ -203,11 +237,15 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
       asm volatile("bar.sync 1, 128;" ::: "memory");   // everyone's copies; chunk c-1 was read
       issue(c + kRaw - 1);
       if (warp == kSoftWarps) {
-        const uint32_t have = __ballot_sync(0xffffffffu, lane < 4 && block_id(c, lane & 3) >= 0);
+        const uint32_t have = __ballot_sync(0xffffffffu, lane < 4 && s_ids[(c & 7) * 4 + (lane & 3)] >= 0);
         if (lane == 0) s_ok[c & 7] = (int)(have & 15u);
+        if (lane < 4) {                          // (chunk c-1's place: every thread is past it)
+          s_ids[((c + 7) & 7) * 4 + lane] = next_id;
+          next_id = block_id(c + 8, lane);
+        }
       }
       const int pos = kb + c * kChunk + tok;
-      const bool live = pos < cached && block_id(c, tok / kBlock) >= 0;
+      const bool live = pos < cached && s_ids[(c & 7) * 4 + tok / kBlock] >= 0;
       const uint8_t* raw = smem + S::kRawAt + (c % kRaw) * S::kRawChunk + (tok / kBlock) * L::kBytes;
       const int off = tok % kBlock;
       if (ok && c >= kStages && !mbar_wait(kv_empty + 8 * st, ((c / kStages) - 1) & 1, TI_DEVERR_PREFILL_WAIT)) ok = false;
@@ -246,46 +284,61 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
   } else if (warp == kMmaWarp) {
-    if (lane == 0) {
-      constexpr uint32_t id_s = idesc_f16(128, kChunk, false, false, false);
-      constexpr uint32_t id_pv = idesc_f16(128, 64, false, false, true);
-      bool ok = true;
-      for (int c = 0; c <= n && ok; ++c) {
-        if (c < n) {
-          const int st = c % kStages, b = c & 1;
-          ok = mbar_wait(kv_full + 8 * st, (c / kStages) & 1, TI_DEVERR_PREFILL_WAIT);
-          const uint32_t kt = sb + S::kKv + st * 2 * S::kKvTile;
-          for (int x = 0; x < ntiles && ok; ++x) {
-            // (P of chunk c-2 sits in this S buffer)
-            if (c >= 2) ok = mbar_wait(pv_done + 8 * x, c & 1, TI_DEVERR_PREFILL_WAIT);
-            if (!ok) break;
-            tc_fence_after();
+    // ---- MMA issue: the whole warp walks the loop and one elected lane issues, so that descriptors
+    // stay in uniform registers (one lane alone took 100 clocks per MMA: 3000 a chunk)
+    constexpr uint32_t id_s = idesc_f16(128, kChunk, false, false, false);
+    constexpr uint32_t id_pv = idesc_f16(128, 64, false, false, true);
+    const uint64_t qd = smem_desc_sw128(sb + S::kQ, false), kd = smem_desc_sw128(sb + S::kKv, false);
+    const uint64_t vd = smem_desc_sw128(sb + S::kKv + S::kKvTile, true);
+    const bool leader = elect_one();
+    auto wait_all = [&](uint32_t bar, uint32_t parity) {
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, TI_DEVERR_PREFILL_WAIT));
+    };
+    bool ok = true;
+    for (int c = 0, st = 0, sp = 0, ph = 0; c <= n && ok; ++c) {
+      const uint32_t b = c & 1;
+      if (c < n) {
+        ok = wait_all(kv_full + 8 * st, ph);
+        const uint32_t stage = (uint32_t)(st * 2 * S::kKvTile) >> 4;
+        for (int x = 0; x < ntiles && ok; ++x) {
+          // (P of chunk c-2 sits in this S buffer)
+          if (c >= 2) ok = wait_all(pv_done + 8 * x, b);
+          if (!ok) break;
+          tc_fence_after();
+          if (leader) {
 #pragma unroll
             for (int k = 0; k < HD / 16; ++k)
-              tc_mma(tmem + 128 * x + 64 * b,
-                     smem_desc_sw128(sb + S::kQ + x * S::kQTile + (k / 4) * 16384 + 32 * (k % 4), false),
-                     smem_desc_sw128(kt + (k / 4) * 8192 + 32 * (k % 4), false), id_s, k > 0 ? 1u : 0u);
+              tc_mma(tmem + 128 * x + 64 * b, qd + ((x * S::kQTile + (k / 4) * 16384 + 32 * (k % 4)) >> 4),
+                     kd + stage + (((k / 4) * 8192 + 32 * (k % 4)) >> 4), id_s, k > 0 ? 1u : 0u);
             tc_commit(s_full + 8 * (2 * x + b));
           }
+          __syncwarp();
         }
-        if (c >= 1 && ok) {
-          const int cp = c - 1, sp = cp % kStages, b = cp & 1;
-          const uint32_t vt = sb + S::kKv + sp * 2 * S::kKvTile + S::kKvTile;
-          for (int x = 0; x < ntiles && ok; ++x) {
-            ok = mbar_wait(p_ready + 8 * x, cp & 1, TI_DEVERR_PREFILL_WAIT);
-            if (!ok) break;
-            tc_fence_after();
+      }
+      if (c >= 1 && ok) {
+        const uint32_t stage = (uint32_t)(sp * 2 * S::kKvTile) >> 4;
+        for (int x = 0; x < ntiles && ok; ++x) {
+          ok = wait_all(p_ready + 8 * x, b ^ 1u);
+          if (!ok) break;
+          tc_fence_after();
+          if (leader) {
 #pragma unroll
             for (int u = 0; u < S::kSub; ++u)
 #pragma unroll
               for (int k = 0; k < 4; ++k)
-                tc_mma_tmem_a(tmem + 256 + 128 * x + 64 * u, tmem + 128 * x + 64 * b + 8 * k,
-                              smem_desc_sw128(vt + u * 8192 + 2048 * k, true), id_pv,
-                              (cp > 0 || k > 0) ? 1u : 0u);
+                tc_mma_tmem_a(tmem + 256 + 128 * x + 64 * u, tmem + 128 * x + 64 * (b ^ 1u) + 8 * k,
+                              vd + stage + ((u * 8192 + 2048 * k) >> 4), id_pv,
+                              (c > 1 || k > 0) ? 1u : 0u);
             tc_commit(pv_done + 8 * x);
+            if (x == ntiles - 1) tc_commit(kv_empty + 8 * sp);
           }
-          if (ok) tc_commit(kv_empty + 8 * sp);
+          __syncwarp();
         }
+        sp = sp + 1 == kStages ? 0 : sp + 1;
+      }
+      if (++st == kStages) {
+        st = 0;
+        ph ^= 1;
       }
     }
   } else if (warp / 4 < ntiles) {
@@ -318,10 +371,12 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
         for (int i = 0; i < kChunk; ++i)
           sv[i] = (k0 + i <= qp && ((have >> (i / kBlock)) & 1)) ? sv[i] : -INFINITY;
       }
-      float mx = -INFINITY;
+      float mxs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};   // (four short chains)
 #pragma unroll
-      for (int i = 0; i < kChunk; ++i) mx = fmaxf(mx, sv[i]);
-      mx *= sc;
+      for (int i = 0; i < kChunk; i += 8)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mxs[k] = fmaxf(mxs[k], fmaxf(sv[i + 2 * k], sv[i + 2 * k + 1]));
+      const float mx = fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3])) * sc;
       float alpha = 1.f;
       if (c == 0) {
         m = mx;
@@ -330,15 +385,19 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
         m = mx;
       }
       const float off = kPScale - (m == -INFINITY ? 0.f : m);
-      float sum = 0.f;                            // of the chunk: a long row's total stays exact enough
+      // the chunk's sum first, in four chains of pairs: a long row's total stays exact enough
+      const uint64_t sc2 = pair(sc, sc), off2 = pair(off, off);
+      uint64_t sums[4] = {0, 0, 0, 0};
       uint32_t pk[kChunk / 2];
 #pragma unroll
       for (int i = 0; i < kChunk; i += 2) {
-        const float p0 = fast_exp2(fmaf(sv[i], sc, off)), p1 = fast_exp2(fmaf(sv[i + 1], sc, off));
-        sum += p0 + p1;
+        const float2 e = unpair(fma2(pair(sv[i], sv[i + 1]), sc2, off2));
+        const float p0 = fast_exp2(e.x), p1 = fast_exp2(e.y);
+        sums[i / 2 % 4] = add2(sums[i / 2 % 4], pair(p0, p1));
         pk[i / 2] = Elem<__half>::pack2(p0, p1);
       }
-      l = l * alpha + sum;
+      const float2 sum = unpair(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])));
+      l = l * alpha + (sum.x + sum.y);
       // (each phase is waited for in turn: a parity tells neighbouring phases apart, no more)
       if (c >= 1 && !wait_all(pv_done + 8 * x, (c - 1) & 1)) { ok = false; break; }
       if (__any_sync(0xffffffffu, alpha != 1.f)) {
