@@ -11,7 +11,7 @@
 //   S = Q K^T   M 128, N 64, into one of two TMEM buffers;
 //   softmax     one row per thread, straight from TMEM: causal mask, a running max that is kept until
 //               a row's grows by more than 2^8 (then O is rescaled in TMEM), P = 2^(s - m) as half
-//               precision back into the S buffer's columns, the A operand of the next product;
+//               precision back into TMEM, the A operand of the next product;
 //   O += P V    A from TMEM, V read in place as an MN-major operand; fp32 O in TMEM.
 // The MMA warp issues S of chunk c for both tiles before P V of chunk c-1, so the tensor cores work
 // while the eight softmax warps do.  bf16 queries are scaled by a power of two per row as in the
@@ -64,6 +64,12 @@ struct Smem {
   static constexpr int kKvTile = kSub * 8192;    // K or V of a chunk
   static constexpr int kRawChunk = 4 * Tile<HD>::kBytes;
   static constexpr int kQ = 0, kKv = 2 * kQTile, kRawAt = kKv + kStages * 2 * kKvTile;
+  // TMEM columns: S buffers at 128 x + 64 b, then O and P; with D 128, P takes the S buffer's place
+  static constexpr bool kShareP = HD == 128;
+  static __device__ __forceinline__ uint32_t o_col(int x) { return 256 + HD * x; }
+  static __device__ __forceinline__ uint32_t p_col(int x, uint32_t b) {
+    return kShareP ? 128 * x + 64 * b : 384 + 64 * x + 32 * b;
+  }
   static constexpr int kInv = kRawAt + kRaw * kRawChunk;         // [2][128] floats
   static constexpr int kNan = kInv + 1024;                       // [HD/16] ints
   static constexpr int kOk = kNan + 64;                          // [8] ints
@@ -89,6 +95,34 @@ __device__ __forceinline__ bool elect_one() {
   uint32_t p;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
   return p != 0;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// 64 consecutive columns of this thread's TMEM lane: two loads, one wait.
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float (&v)[64]) {
+  uint32_t r[64];
+#define KV4_LD32(o)                                                                                \
+  asm volatile(                                                                                    \
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "                                                    \
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"                                    \
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"                   \
+      : "=r"(r[o]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]), "=r"(r[o + 4]),                \
+        "=r"(r[o + 5]), "=r"(r[o + 6]), "=r"(r[o + 7]), "=r"(r[o + 8]), "=r"(r[o + 9]),            \
+        "=r"(r[o + 10]), "=r"(r[o + 11]), "=r"(r[o + 12]), "=r"(r[o + 13]), "=r"(r[o + 14]),       \
+        "=r"(r[o + 15]), "=r"(r[o + 16]), "=r"(r[o + 17]), "=r"(r[o + 18]), "=r"(r[o + 19]),       \
+        "=r"(r[o + 20]), "=r"(r[o + 21]), "=r"(r[o + 22]), "=r"(r[o + 23]), "=r"(r[o + 24]),       \
+        "=r"(r[o + 25]), "=r"(r[o + 26]), "=r"(r[o + 27]), "=r"(r[o + 28]), "=r"(r[o + 29]),       \
+        "=r"(r[o + 30]), "=r"(r[o + 31])                                                           \
+      : "r"(taddr + o))
+  KV4_LD32(0);
+  KV4_LD32(32);
+#undef KV4_LD32
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
 }
 // Two floats in one 64-bit register, for the packed fp32 instructions.
 __device__ __forceinline__ uint64_t pair(float x, float y) {
@@ -122,7 +156,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
   const uint32_t sb = smem_u32(smem);
   const uint32_t kv_full = sb + S::kBars, kv_empty = kv_full + 8 * kStages;
   const uint32_t s_full = kv_empty + 8 * kStages;                // [tile][buffer]
-  const uint32_t p_ready = s_full + 32, pv_done = p_ready + 16;  // [tile]
+  // p_ready has a barrier per buffer: the softmax of chunk c+1 may end before the MMA warp looks at c
+  const uint32_t p_ready = s_full + 32, pv_done = p_ready + 32;  // [tile][buffer], [tile]
   uint32_t* tslot = reinterpret_cast<uint32_t*>(smem + S::kBars + 160);
   float* s_inv = reinterpret_cast<float*>(smem + S::kInv);
   int* s_nan = reinterpret_cast<int*>(smem + S::kNan);
@@ -137,11 +172,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
         mbar_init(kv_full + 8 * i, kLoadWarps * 32);
         mbar_init(kv_empty + 8 * i, 1);
       }
-      for (int i = 0; i < 4; ++i) mbar_init(s_full + 8 * i, 1);
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < 4; ++i) {
+        mbar_init(s_full + 8 * i, 1);
         mbar_init(p_ready + 8 * i, 4);
-        mbar_init(pv_done + 8 * i, 1);
       }
+      for (int i = 0; i < 2; ++i) mbar_init(pv_done + 8 * i, 1);
       fence_mbar_init();
     }
     __syncwarp();
@@ -197,21 +232,19 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
   tc_fence_after();
   const uint32_t tmem = *tslot;
   pdl_launch_dependents();
-  // TMEM columns: S buffers of tile x at 128 x and 128 x + 64, O at 256 + 128 x
   if (warp >= kSoftWarps && warp < kMmaWarp) {
     // ---- loaders: codes -> half precision
     const int lt = tid - kSoftWarps * 32;
     constexpr int kUnits = S::kRawChunk / 16, kTileUnits = L::kBytes / 16;
-    auto block_id = [&](int c, int b) -> int {   // block b of chunk c, -1: none
+    auto table_entry = [&](int c, int b) -> int {   // of block b of chunk c; -1: none
       const int blk = kb / kBlock + c * 4 + b;
-      if (c >= n || blk >= p.max_blocks || (int64_t)blk * kBlock >= cached) return -1;
-      const int id = table[blk];
-      return id >= 0 && id < p.num_blocks ? id : -1;
+      return c < n && blk < p.max_blocks && (int64_t)blk * kBlock < cached ? table[blk] : -1;
     };
+    auto valid = [&](int id) { return id >= 0 && id < p.num_blocks ? id : -1; };
     // block ids go through a ring of eight chunks, loaded eight chunks ahead (a table read per copy
-    // put its latency into every chunk: 796 us instead of @@ at four chunks of 1024)
-    if (lt < 28) s_ids[lt] = block_id(lt / 4, lt % 4);
-    int next_id = lt < 4 ? block_id(7, lt) : -1;
+    // put its latency into every chunk: 796 us instead of 770 at four chunks of 1024)
+    if (lt < 28) s_ids[lt] = valid(table_entry(lt / 4, lt % 4));
+    int next_id = lt < 4 ? table_entry(7, lt) : -1;
     asm volatile("bar.sync 1, 128;" ::: "memory");
     auto issue = [&](int c) {
       const uint32_t raw = sb + S::kRawAt + (c % kRaw) * S::kRawChunk;
@@ -240,8 +273,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
         const uint32_t have = __ballot_sync(0xffffffffu, lane < 4 && s_ids[(c & 7) * 4 + (lane & 3)] >= 0);
         if (lane == 0) s_ok[c & 7] = (int)(have & 15u);
         if (lane < 4) {                          // (chunk c-1's place: every thread is past it)
-          s_ids[((c + 7) & 7) * 4 + lane] = next_id;
-          next_id = block_id(c + 8, lane);
+          s_ids[((c + 7) & 7) * 4 + lane] = valid(next_id);
+          next_id = table_entry(c + 8, lane);    // (looked at in the next step: nothing waits for it here)
         }
       }
       const int pos = kb + c * kChunk + tok;
@@ -291,55 +324,64 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
     const uint64_t qd = smem_desc_sw128(sb + S::kQ, false), kd = smem_desc_sw128(sb + S::kKv, false);
     const uint64_t vd = smem_desc_sw128(sb + S::kKv + S::kKvTile, true);
     const bool leader = elect_one();
-    auto wait_all = [&](uint32_t bar, uint32_t parity) {
-      return __all_sync(0xffffffffu, mbar_wait(bar, parity, TI_DEVERR_PREFILL_WAIT));
+    auto wait = [&](uint32_t bar, uint32_t parity) { return mbar_wait(bar, parity, TI_DEVERR_PREFILL_WAIT); };
+    // S of chunk c into buffer b of tile x; S of chunk c-2 there has been read (p_ready of c-2)
+    auto scores = [&](int x, uint32_t b, uint32_t stage) {
+      tc_fence_after();
+      if (leader) {
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k)
+          tc_mma(tmem + 128 * x + 64 * b, qd + ((x * S::kQTile + (k / 4) * 16384 + 32 * (k % 4)) >> 4),
+                 kd + stage + (((k / 4) * 8192 + 32 * (k % 4)) >> 4), id_s, k > 0 ? 1u : 0u);
+        tc_commit(s_full + 8 * (2 * x + b));
+      }
+      __syncwarp();
+    };
+    // O += P V for the chunk whose weights are in buffer b
+    auto values = [&](int x, uint32_t b, uint32_t stage, bool begin, uint32_t empty) {
+      tc_fence_after();
+      if (leader) {
+#pragma unroll
+        for (int u = 0; u < S::kSub; ++u)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            tc_mma_tmem_a(tmem + S::o_col(x) + 64 * u, tmem + S::p_col(x, b) + 8 * k,
+                          vd + stage + ((u * 8192 + 2048 * k) >> 4), id_pv, (!begin || k > 0) ? 1u : 0u);
+        tc_commit(pv_done + 8 * x);
+        if (empty) tc_commit(empty);
+      }
+      __syncwarp();
     };
     bool ok = true;
-    for (int c = 0, st = 0, sp = 0, ph = 0; c <= n && ok; ++c) {
+    for (int c = 0, st = 0, sp = 0, ph = 0; c <= n; ++c) {
       const uint32_t b = c & 1;
       if (c < n) {
-        ok = wait_all(kv_full + 8 * st, ph);
+        ok &= wait(kv_full + 8 * st, ph);
         const uint32_t stage = (uint32_t)(st * 2 * S::kKvTile) >> 4;
-        for (int x = 0; x < ntiles && ok; ++x) {
-          // (P of chunk c-2 sits in this S buffer)
-          if (c >= 2) ok = wait_all(pv_done + 8 * x, b);
-          if (!ok) break;
-          tc_fence_after();
-          if (leader) {
-#pragma unroll
-            for (int k = 0; k < HD / 16; ++k)
-              tc_mma(tmem + 128 * x + 64 * b, qd + ((x * S::kQTile + (k / 4) * 16384 + 32 * (k % 4)) >> 4),
-                     kd + stage + (((k / 4) * 8192 + 32 * (k % 4)) >> 4), id_s, k > 0 ? 1u : 0u);
-            tc_commit(s_full + 8 * (2 * x + b));
-          }
-          __syncwarp();
+        // (D 128: P of chunk c-2 sits in the S buffer.  D 64 has columns of its own for P.)
+        if (S::kShareP && c >= 2) ok &= wait(pv_done, b);
+        scores(0, b, stage);
+        if (ntiles == 2) {
+          if (S::kShareP && c >= 2) ok &= wait(pv_done + 8, b);
+          scores(1, b, stage);
+        }
+        if (++st == kStages) {
+          st = 0;
+          ph ^= 1;
         }
       }
-      if (c >= 1 && ok) {
-        const uint32_t stage = (uint32_t)(sp * 2 * S::kKvTile) >> 4;
-        for (int x = 0; x < ntiles && ok; ++x) {
-          ok = wait_all(p_ready + 8 * x, b ^ 1u);
-          if (!ok) break;
-          tc_fence_after();
-          if (leader) {
-#pragma unroll
-            for (int u = 0; u < S::kSub; ++u)
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                tc_mma_tmem_a(tmem + 256 + 128 * x + 64 * u, tmem + 128 * x + 64 * (b ^ 1u) + 8 * k,
-                              vd + stage + ((u * 8192 + 2048 * k) >> 4), id_pv,
-                              (c > 1 || k > 0) ? 1u : 0u);
-            tc_commit(pv_done + 8 * x);
-            if (x == ntiles - 1) tc_commit(kv_empty + 8 * sp);
-          }
-          __syncwarp();
+      if (c >= 1) {
+        const uint32_t stage = (uint32_t)(sp * 2 * S::kKvTile) >> 4, empty = kv_empty + 8 * sp;
+        const uint32_t phase = ((c - 1) >> 1) & 1;
+        ok &= wait(p_ready + 8 * (b ^ 1u), phase);
+        values(0, b ^ 1u, stage, c == 1, ntiles == 1 ? empty : 0u);
+        if (ntiles == 2) {
+          ok &= wait(p_ready + 16 + 8 * (b ^ 1u), phase);
+          values(1, b ^ 1u, stage, c == 1, empty);
         }
-        sp = sp + 1 == kStages ? 0 : sp + 1;
+        if (++sp == kStages) sp = 0;
       }
-      if (++st == kStages) {
-        st = 0;
-        ph ^= 1;
-      }
+      if (!__all_sync(0xffffffffu, ok)) break;     // a wait gave up: the error bit is set
     }
   } else if (warp / 4 < ntiles) {
     // ---- softmax and epilogue of tile x: thread <-> row (TMEM lane) r
@@ -349,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
     const int qp = start + t;                     // (rows that do not exist: finite nonsense)
     const int first = start + q0 + x * tile_tokens;
     const uint32_t trow = tmem + ((uint32_t)(quad * 32) << 16);
-    const uint32_t t_s = trow + 128 * x, t_o = trow + 256 + 128 * x;
+    const uint32_t t_s = trow + 128 * x, t_o = trow + S::o_col(x);
     const float sc = s_inv[x * 128 + r] * p.scale_log2;
     auto wait_all = [&](uint32_t bar, uint32_t parity) {
       return __all_sync(0xffffffffu, mbar_wait(bar, parity, TI_DEVERR_PREFILL_WAIT));
@@ -359,48 +401,53 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
     for (int c = 0; c < n; ++c) {
       const int b = c & 1, k0 = kb + c * kChunk;
       // (kv_full of this chunk has completed when its scores have: no wait, but the loaders' flags)
-      if (!wait_all(kv_full + 8 * (c % kStages), (c / kStages) & 1) ||
-          !wait_all(s_full + 8 * (2 * x + b), (c >> 1) & 1)) { ok = false; break; }
+      const bool got = mbar_wait(s_full + 8 * (2 * x + b), (c >> 1) & 1, TI_DEVERR_PREFILL_WAIT) &&
+                       mbar_wait(kv_full + 8 * (c % kStages), (c / kStages) & 1, TI_DEVERR_PREFILL_WAIT);
+      if (!__all_sync(0xffffffffu, got)) { ok = false; break; }
       tc_fence_after();
       const int have = s_ok[c & 7];
       float sv[kChunk];
-      tmem_ld32(t_s + 64 * b, sv);
-      tmem_ld32(t_s + 64 * b + 32, sv + 32);
+      tmem_ld64(t_s + 64 * b, sv);
       if (have != 15 || k0 + kChunk - 1 > first) {
 #pragma unroll
         for (int i = 0; i < kChunk; ++i)
           sv[i] = (k0 + i <= qp && ((have >> (i / kBlock)) & 1)) ? sv[i] : -INFINITY;
       }
-      float mxs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};   // (four short chains)
-#pragma unroll
-      for (int i = 0; i < kChunk; i += 8)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) mxs[k] = fmaxf(mxs[k], fmaxf(sv[i + 2 * k], sv[i + 2 * k + 1]));
-      const float mx = fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3])) * sc;
-      float alpha = 1.f;
-      if (c == 0) {
-        m = mx;
-      } else if (mx > m + 8.f) {                  // (from no key at all: alpha 0 of zeros)
-        alpha = m == -INFINITY ? 0.f : fast_exp2(m - mx);
-        m = mx;
-      }
-      const float off = kPScale - (m == -INFINITY ? 0.f : m);
-      // the chunk's sum first, in four chains of pairs: a long row's total stays exact enough
-      const uint64_t sc2 = pair(sc, sc), off2 = pair(off, off);
-      uint64_t sums[4] = {0, 0, 0, 0};
+      // Weights against the running max as it stands, beside the chunk's own max; only when some row
+      // of the warp outgrew it by 2^8 (or had none) are they taken again.
+      float mxs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      float alpha = 1.f, sum = 0.f;
       uint32_t pk[kChunk / 2];
+      auto weights = [&](bool with_max) {
+        const float off = kPScale - (m == -INFINITY ? 0.f : m);
+        const uint64_t sc2 = pair(sc, sc), off2 = pair(off, off);
+        // the chunk's sum first, in four chains of pairs: a long row's total stays exact enough
+        uint64_t sums[4] = {0, 0, 0, 0};
 #pragma unroll
-      for (int i = 0; i < kChunk; i += 2) {
-        const float2 e = unpair(fma2(pair(sv[i], sv[i + 1]), sc2, off2));
-        const float p0 = fast_exp2(e.x), p1 = fast_exp2(e.y);
-        sums[i / 2 % 4] = add2(sums[i / 2 % 4], pair(p0, p1));
-        pk[i / 2] = Elem<__half>::pack2(p0, p1);
+        for (int i = 0; i < kChunk; i += 2) {
+          const float2 e = unpair(fma2(pair(sv[i], sv[i + 1]), sc2, off2));
+          const float p0 = fast_exp2(e.x), p1 = fast_exp2(e.y);
+          if (with_max) mxs[i / 2 % 4] = max3(mxs[i / 2 % 4], sv[i], sv[i + 1]);
+          sums[i / 2 % 4] = add2(sums[i / 2 % 4], pair(p0, p1));
+          pk[i / 2] = Elem<__half>::pack2(p0, p1);
+        }
+        const float2 t2 = unpair(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])));
+        sum = t2.x + t2.y;
+      };
+      weights(true);
+      const float mx = max3(fmaxf(mxs[0], mxs[1]), mxs[2], mxs[3]) * sc;
+      if (__any_sync(0xffffffffu, mx > m + 8.f)) {
+        if (mx > m + 8.f) {                       // (from no key at all: alpha 0 of zeros)
+          alpha = m == -INFINITY ? 0.f : fast_exp2(m - mx);
+          m = mx;
+        }
+        weights(false);
       }
-      const float2 sum = unpair(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])));
-      l = l * alpha + (sum.x + sum.y);
-      // (each phase is waited for in turn: a parity tells neighbouring phases apart, no more)
-      if (c >= 1 && !wait_all(pv_done + 8 * x, (c - 1) & 1)) { ok = false; break; }
-      if (__any_sync(0xffffffffu, alpha != 1.f)) {
+      l = l * alpha + sum;
+      // O is touched only to rescale, after P V of chunk c-1.  (A parity tells neighbouring phases apart,
+      // no more: the scores of chunk c come after P V of chunk c-2, so the wait is for the right one.)
+      if (c >= 1 && __any_sync(0xffffffffu, alpha != 1.f)) {
+        if (!wait_all(pv_done + 8 * x, (c - 1) & 1)) { ok = false; break; }
         tc_fence_after();
         float ov[32];
 #pragma unroll
@@ -411,11 +458,15 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
           tmem_st32(t_o + d, ov);
         }
       }
-      tmem_st32_u(t_s + 64 * b, pk);
+      // (P of chunk c-2 has been used: a commit, here s_full's, covers all MMAs issued before it)
+      tmem_st32_u(trow + S::p_col(x, b), pk);
       tmem_st_wait();
+      // the last chunk: P V of the one before must be seen before P V of this one can be done, or the
+      // wait below could not tell their parities apart
+      if (c == n - 1 && c >= 1 && !wait_all(pv_done + 8 * x, (c - 1) & 1)) { ok = false; break; }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(p_ready + 8 * x);
+      if (lane == 0) mbar_arrive(p_ready + 8 * (2 * x + b));
     }
     if (ok && wait_all(pv_done + 8 * x, (n - 1) & 1)) {
       tc_fence_after();
