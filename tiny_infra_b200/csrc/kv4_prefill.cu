@@ -81,6 +81,9 @@ struct Smem {
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void st_shared_v4(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w)
                : "memory");
@@ -102,8 +105,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 // 64 consecutive columns of this thread's TMEM lane: two loads, one wait.
-__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float (&v)[64]) {
-  uint32_t r[64];
+__device__ __forceinline__ void tmem_ld64_start(uint32_t taddr, uint32_t (&r)[64]) {
 #define KV4_LD32(o)                                                                                \
   asm volatile(                                                                                    \
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 "                                                    \
@@ -120,7 +122,12 @@ __device__ __forceinline__ void tmem_ld64(uint32_t taddr, float (&v)[64]) {
   KV4_LD32(0);
   KV4_LD32(32);
 #undef KV4_LD32
+}
+__device__ __forceinline__ void tmem_ld64_end(uint32_t (&r)[64], float (&v)[64]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+  // (the registers are written before this point: nothing that reads them may move up)
+#pragma unroll
+  for (int i = 0; i < 64; ++i) asm volatile("" : "+r"(r[i]));
 #pragma unroll
   for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
 }
@@ -236,30 +243,42 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
     // ---- loaders: codes -> half precision
     const int lt = tid - kSoftWarps * 32;
     constexpr int kUnits = S::kRawChunk / 16, kTileUnits = L::kBytes / 16;
-    auto table_entry = [&](int c, int b) -> int {   // of block b of chunk c; -1: none
-      const int blk = kb / kBlock + c * 4 + b;
-      return c < n && blk < p.max_blocks && (int64_t)blk * kBlock < cached ? table[blk] : -1;
+    // Block ids come through a ring of eight chunks in shared memory, copied there seven chunks ahead
+    // and looked at where they are used.  (A table read per copy put its latency into every chunk: 796
+    // us instead of 770 at four chunks of 1024; ids that pass through a register are waited for
+    // where they are loaded, which kept the softmax waiting for the loaders: 536 instead of 502.)
+    auto want_id = [&](int c, int b) {              // of block b of chunk c
+      const int blk = kb / kBlock + c * 4 + b, at = (c & 7) * 4 + b;
+      if (c < n && blk < p.max_blocks && (int64_t)blk * kBlock < cached)
+        cp_async4(sb + S::kIds + at * 4, table + blk);
+      else
+        s_ids[at] = -1;
     };
-    auto valid = [&](int id) { return id >= 0 && id < p.num_blocks ? id : -1; };
-    // block ids go through a ring of eight chunks, loaded eight chunks ahead (a table read per copy
-    // put its latency into every chunk: 796 us instead of 770 at four chunks of 1024)
-    if (lt < 28) s_ids[lt] = valid(table_entry(lt / 4, lt % 4));
-    int next_id = lt < 4 ? table_entry(7, lt) : -1;
+    const uint32_t num_blocks = (uint32_t)min(p.num_blocks, (int64_t)0x7FFFFFFF);
+    auto valid = [&](int id) { return (uint32_t)id < num_blocks; };
+    if (lt < 28) want_id(lt / 4, lt % 4);
+    asm volatile("cp.async.wait_all;" ::: "memory");
     asm volatile("bar.sync 1, 128;" ::: "memory");
     auto issue = [&](int c) {
       const uint32_t raw = sb + S::kRawAt + (c % kRaw) * S::kRawChunk;
+      constexpr int kEach = (kUnits + 127) / 128;
+      int id[kEach];
 #pragma unroll
-      for (int i = 0; i < (kUnits + 127) / 128; ++i) {
+      for (int i = 0; i < kEach; ++i) {
         const int u = lt + i * 128;
-        if (u < kUnits) {
-          const int id = s_ids[(c & 7) * 4 + u / kTileUnits];
-          if (id >= 0)
-            cp_async16(raw + u * 16, p.pool + ((int64_t)id * p.KVH + kvh) * L::kBytes + (u % kTileUnits) * 16);
-        }
+        id[i] = u < kUnits ? s_ids[(c & 7) * 4 + u / kTileUnits] : -1;
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const int u = lt + i * 128;
+        if (valid(id[i]))
+          cp_async16(raw + u * 16, p.pool + ((int64_t)id[i] * p.KVH + kvh) * L::kBytes + (u % kTileUnits) * 16);
+      }
     };
-    for (int c = 0; c < kRaw - 1; ++c) issue(c);
+    for (int c = 0; c < kRaw - 1; ++c) {
+      issue(c);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
     const int tok = lt >> 1, half = lt & 1;      // this thread's token of a chunk, half of its dims
     // after a wait that gave up the loop goes on without waiting: all 128 threads keep meeting at the
     // barrier, and the results are void anyway
@@ -269,43 +288,52 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
       asm volatile("cp.async.wait_group %0;" ::"n"(kRaw - 2) : "memory");
       asm volatile("bar.sync 1, 128;" ::: "memory");   // everyone's copies; chunk c-1 was read
       issue(c + kRaw - 1);
-      if (warp == kSoftWarps) {
-        const uint32_t have = __ballot_sync(0xffffffffu, lane < 4 && s_ids[(c & 7) * 4 + (lane & 3)] >= 0);
+      if (warp == kMmaWarp - 1) {                // (the warp with the fewest copies)
+        if (lane < 4) want_id(c + 7, lane);      // in chunk c-1's place: every thread is past it
+        const uint32_t have = __ballot_sync(0xffffffffu, lane < 4 && valid(s_ids[(c & 7) * 4 + (lane & 3)]));
         if (lane == 0) s_ok[c & 7] = (int)(have & 15u);
-        if (lane < 4) {                          // (chunk c-1's place: every thread is past it)
-          s_ids[((c + 7) & 7) * 4 + lane] = valid(next_id);
-          next_id = table_entry(c + 8, lane);    // (looked at in the next step: nothing waits for it here)
-        }
       }
+      asm volatile("cp.async.commit_group;" ::: "memory");
       const int pos = kb + c * kChunk + tok;
-      const bool live = pos < cached && s_ids[(c & 7) * 4 + tok / kBlock] >= 0;
+      const bool live = pos < cached && valid(s_ids[(c & 7) * 4 + tok / kBlock]);
       const uint8_t* raw = smem + S::kRawAt + (c % kRaw) * S::kRawChunk + (tok / kBlock) * L::kBytes;
       const int off = tok % kBlock;
+      // (all reads before the first write: the compiler keeps their order)
+      uint4 w[2][S::kSub];
+      uint32_t by[2][S::kSub][2];
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+        for (int u = 0; u < S::kSub; ++u) {      // 32 dims, two scale groups, at a time
+          const int d0 = half * (HD / 2) + u * 32;
+          w[kv][u] = make_uint4(0u, 0u, 0u, 0u);
+          by[kv][u][0] = by[kv][u][1] = 0;
+          if (live) {
+            w[kv][u] = *reinterpret_cast<const uint4*>(raw + (kv ? L::kV : L::kK) + off * L::kRow + d0 / 2);
+#pragma unroll
+            for (int g = 0; g < 2; ++g) by[kv][u][g] = raw[(kv ? L::kVs : L::kKs) + (d0 / 16 + g) * kBlock + off];
+          }
+        }
       if (ok && c >= kStages && !mbar_wait(kv_empty + 8 * st, ((c / kStages) - 1) & 1, TI_DEVERR_PREFILL_WAIT)) ok = false;
       const uint32_t dst = sb + S::kKv + st * 2 * S::kKvTile;
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv) {
 #pragma unroll
-        for (int u = 0; u < HD / 64; ++u) {      // 32 dims, two scale groups, at a time
+        for (int u = 0; u < S::kSub; ++u) {
           const int d0 = half * (HD / 2) + u * 32;
-          uint4 w = make_uint4(0u, 0u, 0u, 0u);
-          uint32_t b0 = 0, b1 = 0;
-          if (live) {
-            w = *reinterpret_cast<const uint4*>(raw + (kv ? L::kV : L::kK) + off * L::kRow + d0 / 2);
-            b0 = raw[(kv ? L::kVs : L::kKs) + (d0 / 16) * kBlock + off];
-            b1 = raw[(kv ? L::kVs : L::kKs) + (d0 / 16 + 1) * kBlock + off];
-            if (kv) {
-              if (b0 >= 0xF8u) { atomicMin(&s_nan[d0 / 16], pos); b0 = 0; }
-              if (b1 >= 0xF8u) { atomicMin(&s_nan[d0 / 16 + 1], pos); b1 = 0; }
-            }
+          uint32_t(&b2)[2] = by[kv][u];
+          if (kv) {
+#pragma unroll
+            for (int g = 0; g < 2; ++g)
+              if (b2[g] >= 0xF8u) { atomicMin(&s_nan[d0 / 16 + g], pos); b2[g] = 0; }
           }
-          const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+          const uint32_t ws[4] = {w[kv][u].x, w[kv][u].y, w[kv][u].z, w[kv][u].w};
           const uint32_t row = dst + kv * S::kKvTile + (d0 / 64) * 8192 + tok * 128;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             uint32_t h[4];
             codes_to_half2(ws[k], h);
-            const uint32_t s2 = (k < 2 ? b0 : b1) * 0x00800080u;
+            const uint32_t s2 = b2[k / 2] * 0x00800080u;
             const int ch = (d0 % 64) / 8 + k;
             st_shared_v4(row + ((ch ^ (tok & 7)) << 4), hmul2(h[0], s2), hmul2(h[1], s2),
                          hmul2(h[2], s2), hmul2(h[3], s2));
@@ -325,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
     const uint64_t vd = smem_desc_sw128(sb + S::kKv + S::kKvTile, true);
     const bool leader = elect_one();
     auto wait = [&](uint32_t bar, uint32_t parity) { return mbar_wait(bar, parity, TI_DEVERR_PREFILL_WAIT); };
-    // S of chunk c into buffer b of tile x; S of chunk c-2 there has been read (p_ready of c-2)
+    // S of a chunk into buffer b of tile x
     auto scores = [&](int x, uint32_t b, uint32_t stage) {
       tc_fence_after();
       if (leader) {
@@ -352,36 +380,26 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
       }
       __syncwarp();
     };
+    auto full = [&](int c) { return wait(kv_full + 8 * (c % kStages), (c / kStages) & 1); };
+    auto stage = [&](int c) { return (uint32_t)((c % kStages) * 2 * S::kKvTile) >> 4; };
     bool ok = true;
-    for (int c = 0, st = 0, sp = 0, ph = 0; c <= n; ++c) {
+    for (int c = 0; c < 2 && c < n; ++c) {
+      ok &= full(c);
+      for (int x = 0; x < ntiles; ++x) scores(x, c, stage(c));
+    }
+    // A tile's weights of chunk c are answered with its P V of chunk c and its S of chunk c+2, whose
+    // buffer they came from.
+    for (int c = 0; c < n && __all_sync(0xffffffffu, ok); ++c) {   // (a wait that gave up: the error bit is set)
       const uint32_t b = c & 1;
-      if (c < n) {
-        ok &= wait(kv_full + 8 * st, ph);
-        const uint32_t stage = (uint32_t)(st * 2 * S::kKvTile) >> 4;
-        // (D 128: P of chunk c-2 sits in the S buffer.  D 64 has columns of its own for P.)
-        if (S::kShareP && c >= 2) ok &= wait(pv_done, b);
-        scores(0, b, stage);
-        if (ntiles == 2) {
-          if (S::kShareP && c >= 2) ok &= wait(pv_done + 8, b);
-          scores(1, b, stage);
-        }
-        if (++st == kStages) {
-          st = 0;
-          ph ^= 1;
+      for (int x = 0; x < ntiles; ++x) {
+        ok &= wait(p_ready + 8 * (2 * x + b), (c >> 1) & 1);
+        values(x, b, stage(c), c == 0, x == ntiles - 1 ? kv_empty + 8 * (c % kStages) : 0u);
+        if (c + 2 < n) {
+          if (x == 0) ok &= full(c + 2);
+          if (S::kShareP) ok &= wait(pv_done + 8 * x, b);          // (P is where S goes)
+          scores(x, b, stage(c + 2));
         }
       }
-      if (c >= 1) {
-        const uint32_t stage = (uint32_t)(sp * 2 * S::kKvTile) >> 4, empty = kv_empty + 8 * sp;
-        const uint32_t phase = ((c - 1) >> 1) & 1;
-        ok &= wait(p_ready + 8 * (b ^ 1u), phase);
-        values(0, b ^ 1u, stage, c == 1, ntiles == 1 ? empty : 0u);
-        if (ntiles == 2) {
-          ok &= wait(p_ready + 16 + 8 * (b ^ 1u), phase);
-          values(1, b ^ 1u, stage, c == 1, empty);
-        }
-        if (++sp == kStages) sp = 0;
-      }
-      if (!__all_sync(0xffffffffu, ok)) break;     // a wait gave up: the error bit is set
     }
   } else if (warp / 4 < ntiles) {
     // ---- softmax and epilogue of tile x: thread <-> row (TMEM lane) r
@@ -398,16 +416,27 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
     };
     float m = -INFINITY, l = 0.f;
     bool ok = true;
-    for (int c = 0; c < n; ++c) {
+    for (int c = 0, st = 0, ph = 0; c < n; ++c) {
       const int b = c & 1, k0 = kb + c * kChunk;
-      // (kv_full of this chunk has completed when its scores have: no wait, but the loaders' flags)
-      const bool got = mbar_wait(s_full + 8 * (2 * x + b), (c >> 1) & 1, TI_DEVERR_PREFILL_WAIT) &&
-                       mbar_wait(kv_full + 8 * (c % kStages), (c / kStages) & 1, TI_DEVERR_PREFILL_WAIT);
-      if (!__all_sync(0xffffffffu, got)) { ok = false; break; }
+      // (kv_full of this chunk has completed when its scores have: no wait, but the loaders' flags;
+      // both are asked at once, they are mostly there)
+      const uint32_t sbar = s_full + 8 * (2 * x + b), kbar = kv_full + 8 * st;
+      const bool there = mbar_try_wait(sbar, (c >> 1) & 1) & mbar_try_wait(kbar, ph);
+      if (!__all_sync(0xffffffffu, there)) {
+        const bool got = mbar_wait(sbar, (c >> 1) & 1, TI_DEVERR_PREFILL_WAIT) &&
+                         mbar_wait(kbar, ph, TI_DEVERR_PREFILL_WAIT);
+        if (!__all_sync(0xffffffffu, got)) { ok = false; break; }
+      }
+      if (++st == kStages) {
+        st = 0;
+        ph ^= 1;
+      }
       tc_fence_after();
-      const int have = s_ok[c & 7];
       float sv[kChunk];
-      tmem_ld64(t_s + 64 * b, sv);
+      uint32_t sr[kChunk];
+      tmem_ld64_start(t_s + 64 * b, sr);
+      const int have = s_ok[c & 7];
+      tmem_ld64_end(sr, sv);
       if (have != 15 || k0 + kChunk - 1 > first) {
 #pragma unroll
         for (int i = 0; i < kChunk; ++i)
@@ -436,7 +465,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
       };
       weights(true);
       const float mx = max3(fmaxf(mxs[0], mxs[1]), mxs[2], mxs[3]) * sc;
-      if (__any_sync(0xffffffffu, mx > m + 8.f)) {
+      const bool outgrown = __any_sync(0xffffffffu, mx > m + 8.f);
+      if (outgrown) {
         if (mx > m + 8.f) {                       // (from no key at all: alpha 0 of zeros)
           alpha = m == -INFINITY ? 0.f : fast_exp2(m - mx);
           m = mx;
@@ -446,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
       l = l * alpha + sum;
       // O is touched only to rescale, after P V of chunk c-1.  (A parity tells neighbouring phases apart,
       // no more: the scores of chunk c come after P V of chunk c-2, so the wait is for the right one.)
-      if (c >= 1 && __any_sync(0xffffffffu, alpha != 1.f)) {
+      if (outgrown && c >= 1) {
         if (!wait_all(pv_done + 8 * x, (c - 1) & 1)) { ok = false; break; }
         tc_fence_after();
         float ov[32];

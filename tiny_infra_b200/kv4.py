@@ -340,24 +340,33 @@ class PrefillPlan:
     def work(self, group: int, kv_heads: int):
         """Items and merges (``ti_kv4_prefill_attention``) as host arrays, and the number of parts.
 
-        A pair of tiles is 256 / slots tokens; its keys are cut into ranges of at most a third of
-        what each of 148 SMs would get on average (at least 1024: a range costs a few microseconds
-        of its own), longest items first, so that a few long prefixes still fill the GPU."""
+        A pair of tiles is 256 / slots tokens.  Pairs with more keys than a third of what each
+        of 148 SMs would get on average (at least 1024: a range costs a few microseconds of its
+        own) are cut: their keys, one pair behind the other, at every multiple of that size, so
+        that all items but the ends of pairs are of one size and a few long prefixes still fill
+        the GPU.  Longest items first."""
         slots = 1 << (group - 1).bit_length()
         pair = 256 // slots
         seq = np.repeat(np.arange(self.num_seqs), -(-self.counts // pair))
         per = np.concatenate([np.arange(0, c, pair) for c in self.counts.tolist()] or
                              [np.zeros(0, np.int64)]).astype(np.int64)
         keys = self.starts[seq] + np.minimum(per + pair, self.counts[seq])
-        most = max(1024, int(keys.sum()) * kv_heads // (3 * 148))
-        n = -(-keys // most)
-        size = -(-keys // np.maximum(n, 1) // 64) * 64          # a range, whole 64-key steps
-        n = -(-keys // np.maximum(size, 1))
+        steps = -(-keys // 64)                                  # a range is whole 64-key steps
+        unit = max(16, -(-int(steps.sum()) * kv_heads // (3 * 148)))
+        cut = steps > unit
+        begin = np.cumsum(np.where(cut, steps, 0)) - steps      # of a cut pair among them
+        end = begin + steps
+        # cuts first .. last, in units; none within an eighth of a unit of either end
+        first, last = begin // unit + 1, (end - 1) // unit
+        first = first + (first * unit - begin < unit // 8)
+        last = last - (end - last * unit < unit // 8)
+        n = np.where(cut, last - first + 2, 1)
         first_part = np.cumsum(np.where(n > 1, n, 0)) - np.where(n > 1, n, 0)
         at = np.repeat(np.arange(len(seq)), n)                  # the pair of each item
         k = np.arange(len(at)) - np.repeat(np.cumsum(n) - n, n)  # its range within the pair
-        lo = k * size[at]
-        hi = np.minimum(lo + size[at], keys[at])
+        at_cut = (first[at] + k) * unit - begin[at]             # where range k of a cut pair ends
+        lo = np.where(k > 0, at_cut - unit, 0) * 64
+        hi = np.where(k < n[at] - 1, at_cut * 64, keys[at])
         part = np.where(n[at] > 1, first_part[at] + k, -1)
         items = np.stack([seq[at], per[at], lo, hi, part, np.zeros_like(lo)], 1)
         items = items[np.argsort(lo - hi, kind="stable")].astype(np.int32)
