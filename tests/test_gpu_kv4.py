@@ -614,6 +614,71 @@ def test_run_together_and_in_graphs(kv4):
         torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_prefill_captured_and_side_by_side(kv4, d):
+    """Long prefixes cut into ranges (two launches): captured and replayed, and two calls at once
+    on streams of their own, give the eager result bit for bit."""
+    nh, kvh, starts, counts = 14, 2, [5000, 0, 9000], [40, 3, 130]
+    blocks = [-(-(s + c) // 16) for s, c in zip(starts, counts)]
+    rng = np.random.default_rng(8)
+    pool = kv4.new_pool(sum(blocks), kvh, d)
+    pool.copy_(torch.from_numpy(rng.integers(0, 80, tuple(pool.shape), dtype=np.uint8)))
+    tab = torch.full((3, max(blocks)), -1, dtype=torch.int32)
+    for i, n in enumerate(blocks):
+        tab[i, :n] = torch.arange(n) + sum(blocks[:i])
+    tab = tab.cuda()
+    plan, late = kv4.PrefillPlan(starts, counts), kv4.PrefillPlan(starts, counts)
+    assert plan.work(nh // kvh, kvh)[2] > 1
+    qs = [torch.from_numpy(rng.standard_normal((sum(counts), nh, d))).to("cuda", torch.bfloat16)
+          for _ in range(2)]
+    want, outs, graphs = [], [torch.zeros_like(q) for q in qs], []
+    for q in qs:
+        o = torch.zeros_like(q)
+        kv4.prefill_attention(o, q, pool, tab, plan)
+        want.append(o)
+    torch.cuda.synchronize()
+    assert not want[0].isnan().any()
+    for q, o in zip(qs, outs):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            with pytest.raises(RuntimeError, match="before the capture"):
+                kv4.prefill_attention(o, q, pool, tab, late)
+            kv4.prefill_attention(o, q, pool, tab, plan)
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for captured in (True, False):
+        for _ in range(5):
+            for s, g, q, o in zip(streams, graphs, qs, outs):
+                with torch.cuda.stream(s):
+                    if captured:
+                        g.replay()
+                    else:
+                        kv4.prefill_attention(o, q, pool, tab, plan)
+            torch.cuda.synchronize()
+            for o, w in zip(outs, want):
+                assert torch.equal(o, w)
+                o.zero_()
+            torch.cuda.synchronize()
+
+
+def test_rows_that_overlap_are_refused(kv4):
+    z = lambda *s: torch.zeros(*s, dtype=torch.bfloat16, device="cuda")             # noqa: E731
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")             # noqa: E731
+    pool, same = kv4.new_pool(4, 2, 64), z(1, 4, 64).expand(3, 4, 64)
+    slots = torch.arange(3, device="cuda")
+    tables = torch.zeros(8, 32, dtype=torch.float32, device="cuda")
+    for f in (lambda: kv4.decode_attention(same, z(3, 4, 64), pool, i32(3, 3), i32(3)),
+              lambda: kv4.prefill_attention(same, z(3, 4, 64), pool, i32(1, 3), kv4.PrefillPlan([0], [3])),
+              lambda: kv4.rope_append(pool, z(1, 8 * 64).expand(3, 8 * 64), 4, slots, tables, tables, i32(3))):
+        with pytest.raises(RuntimeError, match="overlap"):
+            f()
+    # a query that all rows share is read, not written
+    out = z(3, 4, 64)
+    kv4.decode_attention(out, same, pool, i32(3, 3), i32(3) + 5)
+    torch.cuda.synchronize()
+    assert torch.equal(out, z(3, 4, 64))
+
+
 def test_refusals(kv4):
     z = lambda *s, dt=torch.bfloat16: torch.zeros(*s, dtype=dt, device="cuda")      # noqa: E731
     i32 = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")             # noqa: E731

@@ -649,7 +649,8 @@ extern "C" int ti_kv4_append(void* pool, float* weights, const void* k, int64_t 
                       num_kv_heads};
   if (num_kv_heads > 32767)
     return set_error(TI_ERR_UNSUPPORTED, "kv4_append: at most 32767 kv heads");
-  // few tokens in small blocks, so that they spread over the SMs
+  // Few tokens in small blocks, so that they spread over the SMs: 256 tokens of 2 kv heads, 64 dims, 1.51
+  // us against 1.68 with 256 threads; 16384 tokens 4.72 with 64 threads against 3.37.
   const int threads = num_tokens <= 1024 ? 64 : 256;
   const dim3 grid(kv4::grid_for((int64_t)num_tokens * (head_dim / 16), threads), 2 * num_kv_heads);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);

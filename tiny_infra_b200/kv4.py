@@ -20,6 +20,7 @@ is launched.
 from __future__ import annotations
 
 import contextlib
+import functools
 
 import numpy as np
 import torch
@@ -108,6 +109,16 @@ def _rows(name: str, t: torch.Tensor):
     if t.numel() and (inner != 1 or (head != d and heads > 1)):
         _fail(f"{name} must have contiguous [heads, head_dim] rows")
     return T, heads, d, tok
+
+
+def _out_rows(out: torch.Tensor, q: torch.Tensor) -> int:
+    """Token stride of an output of q's shape whose rows do not overlap."""
+    T, heads, d, tok = _rows("out", out)
+    if out.shape != q.shape or out.dtype != q.dtype:
+        _fail("out must have q's shape and dtype")
+    if T > 1 and tok < heads * d:
+        _fail("out's rows overlap")
+    return tok
 
 
 def _attention(q, pool, block_tables, context_lens, row_index):
@@ -199,6 +210,8 @@ def rope_append(pool: torch.Tensor, qkv: torch.Tensor, num_heads: int,
             qkv.shape[1] != (num_heads + 2 * kvh) * d or (qkv.numel() and qkv.stride(1) != 1):
         _fail("qkv must be 16-bit [tokens, (num_heads + 2 * kv heads) * head_dim] rows")
     T = qkv.shape[0]
+    if T > 1 and qkv.stride(0) < qkv.shape[1]:
+        _fail("qkv's rows overlap")
     if slot_mapping.dtype != torch.int64 or not slot_mapping.is_contiguous() or \
             slot_mapping.numel() != T:
         _fail("slot_mapping must be contiguous int64 [tokens]")
@@ -252,7 +265,16 @@ def _workspace(dev: int, nbytes: int, stream: int) -> torch.Tensor:
     (so graphs that replay at the same time do not share it), zeroed by the graph itself."""
     if torch.cuda.is_current_stream_capturing():
         return torch.zeros(nbytes, dtype=torch.uint8, device=torch.device("cuda", dev))
-    return _ws.get(torch.device("cuda", dev), nbytes, stream)
+    return _ws.get(_cuda(dev), nbytes, stream)
+
+
+_cuda = functools.lru_cache(maxsize=None)(functools.partial(torch.device, "cuda"))
+
+
+@functools.lru_cache(maxsize=4096)
+def _decode_bytes(dev: int, *sizes: int) -> int:
+    """Workspace of a decode call on ``dev`` (the current device), asked once per sizes."""
+    return int(N.lib().ti_kv4_attention_workspace_bytes(*sizes))
 
 
 def decode_attention(out: torch.Tensor, q: torch.Tensor, pool: torch.Tensor,
@@ -270,9 +292,7 @@ def decode_attention(out: torch.Tensor, q: torch.Tensor, pool: torch.Tensor,
     dev = _device(pool, out, q, block_tables, context_lens, row_index, lse)
     B, NH, nb, kvh, d, q_stride, bt_stride, cols = _attention(q, pool, block_tables, context_lens,
                                                               row_index)
-    _, _, _, out_stride = _rows("out", out)
-    if out.shape != q.shape or out.dtype != q.dtype:
-        _fail("out must have q's shape and dtype")
+    out_stride = _out_rows(out, q)
     if lse is not None:
         _head_sums("lse", lse, B, NH)
     if B == 0:
@@ -280,8 +300,7 @@ def decode_attention(out: torch.Tensor, q: torch.Tensor, pool: torch.Tensor,
     lib = N.lib()
     with _on(dev):
         stream = _stream(dev)
-        need = lib.ti_kv4_attention_workspace_bytes(B, NH, kvh, d, cols)
-        ws = _workspace(dev, need, stream)
+        ws = _workspace(dev, _decode_bytes(dev, B, NH, kvh, d, cols), stream)
         N.check(lib.ti_kv4_attention_decode(
             out.data_ptr(), out_stride, _ptr(lse), q.data_ptr(), q_stride, pool.data_ptr(), nb,
             block_tables.data_ptr(), bt_stride, _ptr(row_index), context_lens.data_ptr(), B, NH,
@@ -318,7 +337,9 @@ def accumulate_weights(weights: torch.Tensor, q: torch.Tensor, lse: torch.Tensor
 class PrefillPlan:
     """Layout of a packed prefill: chunk i holds ``counts[i]`` query tokens at positions
     ``starts[i]`` and on, whose K and V are already in the cache.  Built once per batch, used by
-    every layer; the work items of a head layout are laid out at its first use and kept."""
+    every layer; the work items of a head layout are laid out at its first use and kept.  A graph
+    that captured a call reads the plan's memory: lay the plan out before the capture and keep it as
+    long as the graph."""
 
     def __init__(self, starts, counts, device="cuda") -> None:
         starts, counts = np.asarray(starts, np.int64), np.asarray(counts, np.int64)
@@ -378,6 +399,9 @@ class PrefillPlan:
         """``work`` on the device: pointers and counts, for calls of this head layout."""
         key = (group, kv_heads)
         if key not in self._layouts:
+            if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+                _fail("this head layout of the plan is new: run it once, or call layout(), "
+                      "before the capture")
             items, merges, parts = self.work(group, kv_heads)
             dev = torch.from_numpy(np.concatenate([items.reshape(-1), merges.reshape(-1)])
                                    ).to(self.device)
@@ -396,11 +420,9 @@ def prefill_attention(out: torch.Tensor, q: torch.Tensor, pool: torch.Tensor,
     dev = _device(pool, out, q, block_tables, plan.start_pos, row_index)
     nb, kvh, d = _pool_shape(pool)
     T, NH, dq, q_stride = _rows("q", q)
-    _, _, _, out_stride = _rows("out", out)
+    out_stride = _out_rows(out, q)
     if dq != d:
         _fail("head_dim does not match the pool's tiles")
-    if out.shape != q.shape or out.dtype != q.dtype:
-        _fail("out must have q's shape and dtype")
     if NH <= 0 or NH % kvh or NH > 16 * kvh:
         _fail("query heads must be a multiple of the kv heads, at most 16 per kv head")
     if T != plan.num_tokens:
