@@ -421,11 +421,12 @@ int ti_kv4_attention_decode(void* out, int64_t out_seq_stride, float* lse, const
  * start_pos[i] + j, whose K and V are in the pool; each attends to positions 0 .. its own of table
  * row row_index[i] (NULL: i).  At most 16 query heads per kv head.  The caller lays out the work: a
  * tile is 128 / slots tokens, slots = the query heads per kv head rounded up to a power of two; an
- * item (6 int32: sequence, first token of two neighbouring tiles within the chunk, first key, end of
- * the keys, part or -1, 0) is two tiles over keys [first, end), first a multiple of 64.  Items of one
- * pair that cover its keys 0 .. last query position in several ranges name consecutive parts
- * (0 .. num_parts-1, their partial results in the workspace), and a merge (4 int32: sequence, first
- * token, first part, parts) joins them; a single item has part -1.  Every pair of tiles is covered.
+ * item (6 int32: sequence, first token within the chunk, first key, end of the keys, part or -1,
+ * tiles) is up to 3 (head_dim 128: 2) neighbouring tiles over keys [first, end), first a multiple of
+ * 64.  Items of the same tiles that cover their keys 0 .. last query position in several ranges name
+ * consecutive parts (0 .. num_parts-1, their partial results in the workspace), and a merge (5 int32:
+ * sequence, first token, first part, parts, tiles) joins them; a single item has part -1.  Every tile
+ * is covered once.
  * tiny_infra_b200.kv4.PrefillPlan builds both lists. */
 size_t ti_kv4_prefill_workspace_bytes(int num_parts, int num_kv_heads, int head_dim);
 int ti_kv4_prefill_attention(void* out, int64_t out_tok_stride, const void* q,
@@ -440,7 +441,7 @@ int ti_kv4_prefill_attention(void* out, int64_t out_tok_stride, const void* q,
 
 /* weights_out = weights + sum over the kv head's query heads of exp(q.k / sqrt(head_dim) - lse), for
  * each cached token of the batch (float32 [num_blocks, num_kv_heads, 16]; weights_out may be
- * weights; other tokens are neither read nor written).  lse as ti_kv4_attention_decode gives it for
+ * weights; other tokens' totals are not written).  lse as ti_kv4_attention_decode gives it for
  * the same arguments.  The sequences of a call share no block. */
 int ti_kv4_accumulate_weights(float* weights_out, const float* weights, const void* q,
                               int64_t q_seq_stride, const float* lse, const void* pool,

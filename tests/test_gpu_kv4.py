@@ -426,6 +426,17 @@ def test_prefill(kv4, nh, kvh, d, dtn, starts, counts):
     assert torch.equal(again, out)
 
 
+@pytest.mark.parametrize("nh,kvh,d,dtn,starts,counts,tiles", [
+    (64, 4, 64, "bf16", [0, 100] * 19 + [2100, 1600], [24, 23] * 18 + [7, 1, 24, 20], 3),
+    (36, 4, 64, "fp16", [0] * 19 + [1700], [24] * 20, 2),
+    (36, 4, 128, "fp16", [50] * 19 + [1700, 0], [16] * 20 + [290], 2),
+    (3, 1, 128, "bf16", [0, 1700], [70, 31], 1),
+])
+def test_prefill_tiles_of_an_item(kv4, nh, kvh, d, dtn, starts, counts, tiles):
+    assert (kv4.PrefillPlan(starts, counts).work(nh // kvh, kvh, d)[0][:, 5] == tiles).all()
+    test_prefill(kv4, nh, kvh, d, dtn, starts, counts)
+
+
 def check_prefill(out, exact, dt, d, rows=slice(None)):
     o, mean, flat, big = exact
     ds = (d + 8) * 2.0 ** -24 * big[..., None]

@@ -71,15 +71,20 @@ def test_prefill_plan_layout():
     assert PrefillPlan([], [], device="cpu").work(7, 2)[2] == 0
     rng = np.random.default_rng(0)
     for group in (1, 2, 3, 7, 8, 12, 16):
-        pair = 256 // (1 << (group - 1).bit_length())
-        for _ in range(20):
+        for d, most in ((64, 3), (128, 2)) * 10:
             n = int(rng.integers(1, 5))
             starts, counts = rng.integers(0, 40000, n), rng.integers(0, 900, n)
             starts[0] *= int(rng.integers(0, 2))
-            items, merges, parts = PrefillPlan(starts, counts, device="cpu").work(group, 2)
+            items, merges, parts = PrefillPlan(starts, counts, device="cpu").work(group, 2, d)
+            if not len(items):
+                assert counts.sum() == 0
+                continue
+            tiles = int(items[0, 5])
+            assert 1 <= tiles <= most and (items[:, 5] == tiles).all() and (merges[:, 4] == tiles).all()
+            pair = tiles * (128 >> (group - 1).bit_length())
             length = items[:, 3] - items[:, 2]
             assert (length > 0).all() and (np.diff(length) <= 0).all() and (items[:, 2] % 64 == 0).all()
-            joined = {(s, q): (f, k) for s, q, f, k in merges.tolist()}
+            joined = {(s, q): (f, k) for s, q, f, k, _ in merges.tolist()}
             seen = []
             for i in range(n):
                 for q0 in range(0, int(counts[i]), pair):
@@ -172,7 +177,8 @@ def test_c_abi_refusals(native):
     refused(acc(d=256), 2, b"head_dim")
     refused(acc(q=FAKE + 4), 1, b"aligned")
 
-    assert lib.ti_kv4_prefill_workspace_bytes(3, 2, 64) == 3 * 2 * 2 * 128 * 66 * 4
+    assert lib.ti_kv4_prefill_workspace_bytes(3, 2, 64) == 3 * 2 * 3 * 128 * 66 * 4
+    assert lib.ti_kv4_prefill_workspace_bytes(3, 2, 128) == 3 * 2 * 2 * 128 * 130 * 4
     assert lib.ti_kv4_prefill_workspace_bytes(0, 2, 64) == 0
 
     def pre(out=FAKE, items=FAKE, n=2, merges=None, nm=0, parts=0, nh=14, d=64, bs=16, dt=0, mb=4,

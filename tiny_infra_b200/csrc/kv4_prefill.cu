@@ -4,23 +4,30 @@
 // already in the cache.
 //
 // A tile is 128 rows: the query heads of one kv head (a power of two of slots, at most 16) times 128 /
-// slots tokens.  One CTA takes two tiles of neighbouring tokens and a range of keys; both share each
-// 64-key chunk, which four warps read as codes (asynchronous copies, three chunks ahead) and write to
-// shared memory as half precision -- exact, 2.25 times less to read than 16-bit keys and no scratch
-// copy of the cache.  Per chunk and tile:
-//   S = Q K^T   M 128, N 64, into one of two TMEM buffers;
-//   softmax     one row per thread, straight from TMEM: causal mask, a running max that is kept until
-//               a row's grows by more than 2^8 (then O is rescaled in TMEM), P = 2^(s - m) as half
-//               precision back into TMEM, the A operand of the next product;
+// slots tokens.  One CTA takes up to three tiles of neighbouring tokens (two for D = 128: what tensor
+// memory holds) and a range of keys; they share each 64-key chunk, which four warps read as codes
+// (asynchronous copies, three chunks ahead) and write to shared memory as half precision -- exact, 2.25
+// times less to read than 16-bit keys and no scratch copy of the cache.  Per chunk and tile:
+//   S = Q K^T   M 128, N 64, into TMEM; the softmax warps free it once it is in registers, and S of the
+//               next chunk is computed under their arithmetic;
+//   softmax     one row per thread: causal mask, a running max that is kept until a row's grows by more
+//               than 2^8 (then O is rescaled in TMEM), P = 2^(s - m) as half precision back into TMEM,
+//               the A operand of the next product;
 //   O += P V    A from TMEM, V read in place as an MN-major operand; fp32 O in TMEM.
-// The MMA warp issues S of chunk c for both tiles before P V of chunk c-1, so the tensor cores work
-// while the eight softmax warps do.  bf16 queries are scaled by a power of two per row as in the
-// decode kernel; P is held times 2^7 (at most 2^15; steps of 2^-31), its sum taken before rounding.
-// Bound: the exponentials (16 a clock and SM: 512 clocks a tile and chunk, against 365 of MMA).
+// bf16 queries are scaled by a power of two per row as in the decode kernel; P is held times 2^7 (at
+// most 2^15; steps of 2^-31), its sum taken before rounding.
 //
-// Work: the host cuts every pair of tiles' keys into ranges of about the same size, longest first, so
-// that a few long prefixes fill the GPU; a pair cut into several ranges leaves un-normalised partials
-// that merge_kernel joins in order.
+// Bound: four chunks of 1024 tokens behind prefixes up to 32767 (14 heads over 2, D = 64) take 436 us.
+// The exponentials alone would take 230 (one warp instruction in 8 clocks of a scheduler: 512 clocks a
+// tile and chunk), the MMAs 146 at their full rate.  The three warps of a scheduler that have them to
+// do mostly run in step, so half of a chunk's 2600 clocks the exponential unit is busy, and half it
+// waits for their other work: waits, tensor memory, the max.  Two tiles a CTA with double-buffered
+// scores: 473 us; two threads a row: 534.  A warp order by flags in shared memory cost registers and
+// more time than it gave (524 to 765).
+//
+// Work: the host cuts the keys of long sequences into ranges of the same size, longest first, so that a
+// few long prefixes fill the GPU; tiles cut into several ranges leave un-normalised partials that
+// merge_kernel joins in order.
 //
 // A key that is masked in some row of a tile and is NaN costs that row nothing: its score is replaced.
 // A masked value that is NaN would (0 * NaN): NaN groups of V go into the product as zeros, and the
@@ -40,11 +47,11 @@ namespace pre {
 constexpr int kChunk = 64;                       // keys per step
 constexpr int kStages = 3;                       // chunks of K and V in half precision
 constexpr int kRaw = 4;                          // chunks of codes
-constexpr int kSoftWarps = 8, kLoadWarps = 4;
-constexpr int kThreads = (kSoftWarps + kLoadWarps + 1) * 32;
+constexpr int kLoadWarps = 4;
 constexpr float kPScale = 7.f;
-constexpr int kItemInts = 6;                     // sequence, first token, key range, part or -1, spare
-constexpr int kMergeInts = 4;                    // sequence, first token, first part, parts
+constexpr int kStagger = 500, kStaggerFrom = 16; // clocks, chunks
+constexpr int kItemInts = 6;                     // sequence, first token, key range, part or -1, tiles
+constexpr int kMergeInts = 5;                    // sequence, first token, first part, parts, tiles
 
 struct Params {
   void* out;
@@ -63,15 +70,17 @@ struct Smem {
   static constexpr int kQTile = kSub * 16384;
   static constexpr int kKvTile = kSub * 8192;    // K or V of a chunk
   static constexpr int kRawChunk = 4 * Tile<HD>::kBytes;
-  static constexpr int kQ = 0, kKv = 2 * kQTile, kRawAt = kKv + kStages * 2 * kKvTile;
-  // TMEM columns: S buffers at 128 x + 64 b, then O and P; with D 128, P takes the S buffer's place
-  static constexpr bool kShareP = HD == 128;
-  static __device__ __forceinline__ uint32_t o_col(int x) { return 256 + HD * x; }
-  static __device__ __forceinline__ uint32_t p_col(int x, uint32_t b) {
-    return kShareP ? 128 * x + 64 * b : 384 + 64 * x + 32 * b;
-  }
-  static constexpr int kInv = kRawAt + kRaw * kRawChunk;         // [2][128] floats
-  static constexpr int kNan = kInv + 1024;                       // [HD/16] ints
+  static constexpr int kTiles = HD == 64 ? 3 : 2;                // query tiles of a CTA
+  static constexpr int kSoftWarps = 4 * kTiles;
+  static constexpr int kThreads = (kSoftWarps + kLoadWarps + 1) * 32;
+  static constexpr int kQ = 0, kKv = kTiles * kQTile, kRawAt = kKv + kStages * 2 * kKvTile;
+  // TMEM columns: scores, weights (half precision, two a column) and O of every tile
+  static __device__ __forceinline__ uint32_t s_col(int x) { return 64 * x; }
+  static __device__ __forceinline__ uint32_t p_col(int x) { return 64 * kTiles + 32 * x; }
+  static __device__ __forceinline__ uint32_t o_col(int x) { return 96 * kTiles + HD * x; }
+  static_assert((96 + HD) * kTiles <= 512, "tensor memory");
+  static constexpr int kInv = kRawAt + kRaw * kRawChunk;         // [kTiles][128] floats
+  static constexpr int kNan = kInv + kTiles * 512;                       // [HD/16] ints
   static constexpr int kOk = kNan + 64;                          // [8] ints
   static constexpr int kIds = kOk + 64;                          // [8][4] ints
   static constexpr int kBars = kIds + 128;
@@ -154,17 +163,18 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 }
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(Smem<HD>::kThreads, 1) prefill_kernel(const __grid_constant__ Params p) {
   using S = Smem<HD>;
+  constexpr int kThreads = S::kThreads, kSoftWarps = S::kSoftWarps;
   using L = Tile<HD>;
   extern __shared__ __align__(16) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
   const uint32_t sb = smem_u32(smem);
   const uint32_t kv_full = sb + S::kBars, kv_empty = kv_full + 8 * kStages;
-  const uint32_t s_full = kv_empty + 8 * kStages;                // [tile][buffer]
-  // p_ready has a barrier per buffer: the softmax of chunk c+1 may end before the MMA warp looks at c
-  const uint32_t p_ready = s_full + 32, pv_done = p_ready + 32;  // [tile][buffer], [tile]
+  // per tile, a phase per chunk: scores written, scores read, weights written, P V done
+  const uint32_t s_full = kv_empty + 8 * kStages, s_read = s_full + 8 * S::kTiles;
+  const uint32_t p_ready = s_read + 8 * S::kTiles, pv_done = p_ready + 8 * S::kTiles;
   uint32_t* tslot = reinterpret_cast<uint32_t*>(smem + S::kBars + 160);
   float* s_inv = reinterpret_cast<float*>(smem + S::kInv);
   int* s_nan = reinterpret_cast<int*>(smem + S::kNan);
@@ -179,11 +189,12 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
         mbar_init(kv_full + 8 * i, kLoadWarps * 32);
         mbar_init(kv_empty + 8 * i, 1);
       }
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < S::kTiles; ++i) {
         mbar_init(s_full + 8 * i, 1);
+        mbar_init(s_read + 8 * i, 4);
         mbar_init(p_ready + 8 * i, 4);
+        mbar_init(pv_done + 8 * i, 1);
       }
-      for (int i = 0; i < 2; ++i) mbar_init(pv_done + 8 * i, 1);
       fence_mbar_init();
     }
     __syncwarp();
@@ -198,7 +209,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
   const int tile_tokens = 128 >> p.slots_log2;
   const int row0 = p.cu_seqlens[seq], count = p.cu_seqlens[seq + 1] - row0;
   const int start = p.start_pos[seq], cached = start + count;
-  const int ntiles = q0 + tile_tokens < count ? 2 : 1;
+  const int ntiles = min(min(item[5], S::kTiles), (count - q0 + tile_tokens - 1) / tile_tokens);
   const int n = (ke - kb + kChunk - 1) / kChunk;
   const int32_t* table = p.tables + (int64_t)(p.row_index ? p.row_index[seq] : seq) * p.bt_stride;
 
@@ -353,27 +364,25 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
     const uint64_t vd = smem_desc_sw128(sb + S::kKv + S::kKvTile, true);
     const bool leader = elect_one();
     auto wait = [&](uint32_t bar, uint32_t parity) { return mbar_wait(bar, parity, TI_DEVERR_PREFILL_WAIT); };
-    // S of a chunk into buffer b of tile x
-    auto scores = [&](int x, uint32_t b, uint32_t stage) {
+    auto scores = [&](int x, uint32_t stage) {
       tc_fence_after();
       if (leader) {
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k)
-          tc_mma(tmem + 128 * x + 64 * b, qd + ((x * S::kQTile + (k / 4) * 16384 + 32 * (k % 4)) >> 4),
+          tc_mma(tmem + S::s_col(x), qd + ((x * S::kQTile + (k / 4) * 16384 + 32 * (k % 4)) >> 4),
                  kd + stage + (((k / 4) * 8192 + 32 * (k % 4)) >> 4), id_s, k > 0 ? 1u : 0u);
-        tc_commit(s_full + 8 * (2 * x + b));
+        tc_commit(s_full + 8 * x);
       }
       __syncwarp();
     };
-    // O += P V for the chunk whose weights are in buffer b
-    auto values = [&](int x, uint32_t b, uint32_t stage, bool begin, uint32_t empty) {
+    auto values = [&](int x, uint32_t stage, bool begin, uint32_t empty) {   // O += P V
       tc_fence_after();
       if (leader) {
 #pragma unroll
         for (int u = 0; u < S::kSub; ++u)
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            tc_mma_tmem_a(tmem + S::o_col(x) + 64 * u, tmem + S::p_col(x, b) + 8 * k,
+            tc_mma_tmem_a(tmem + S::o_col(x) + 64 * u, tmem + S::p_col(x) + 8 * k,
                           vd + stage + ((u * 8192 + 2048 * k) >> 4), id_pv, (!begin || k > 0) ? 1u : 0u);
         tc_commit(pv_done + 8 * x);
         if (empty) tc_commit(empty);
@@ -382,22 +391,20 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
     };
     auto full = [&](int c) { return wait(kv_full + 8 * (c % kStages), (c / kStages) & 1); };
     auto stage = [&](int c) { return (uint32_t)((c % kStages) * 2 * S::kKvTile) >> 4; };
-    bool ok = true;
-    for (int c = 0; c < 2 && c < n; ++c) {
-      ok &= full(c);
-      for (int x = 0; x < ntiles; ++x) scores(x, c, stage(c));
-    }
-    // A tile's weights of chunk c are answered with its P V of chunk c and its S of chunk c+2, whose
-    // buffer they came from.
-    for (int c = 0; c < n && __all_sync(0xffffffffu, ok); ++c) {   // (a wait that gave up: the error bit is set)
-      const uint32_t b = c & 1;
+    bool ok = full(0);
+    for (int x = 0; x < ntiles; ++x) scores(x, stage(0));
+    // P V of chunk c-1 and S of chunk c+1, tile by tile: a tile's weights of c-1 and its having read
+    // the scores of c come one soon after the other.
+    for (int c = 0; c <= n && __all_sync(0xffffffffu, ok); ++c) {   // (a wait that gave up: the error bit is set)
       for (int x = 0; x < ntiles; ++x) {
-        ok &= wait(p_ready + 8 * (2 * x + b), (c >> 1) & 1);
-        values(x, b, stage(c), c == 0, x == ntiles - 1 ? kv_empty + 8 * (c % kStages) : 0u);
-        if (c + 2 < n) {
-          if (x == 0) ok &= full(c + 2);
-          if (S::kShareP) ok &= wait(pv_done + 8 * x, b);          // (P is where S goes)
-          scores(x, b, stage(c + 2));
+        if (c >= 1) {
+          ok &= wait(p_ready + 8 * x, (c - 1) & 1);
+          values(x, stage(c - 1), c == 1, x == ntiles - 1 ? kv_empty + 8 * ((c - 1) % kStages) : 0u);
+        }
+        if (c + 1 < n) {
+          if (x == 0) ok &= full(c + 1);
+          ok &= wait(s_read + 8 * x, c & 1);
+          scores(x, stage(c + 1));
         }
       }
     }
@@ -409,7 +416,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
     const int qp = start + t;                     // (rows that do not exist: finite nonsense)
     const int first = start + q0 + x * tile_tokens;
     const uint32_t trow = tmem + ((uint32_t)(quad * 32) << 16);
-    const uint32_t t_s = trow + 128 * x, t_o = trow + S::o_col(x);
+    const uint32_t t_s = trow + S::s_col(x), t_o = trow + S::o_col(x);
     const float sc = s_inv[x * 128 + r] * p.scale_log2;
     auto wait_all = [&](uint32_t bar, uint32_t parity) {
       return __all_sync(0xffffffffu, mbar_wait(bar, parity, TI_DEVERR_PREFILL_WAIT));
@@ -417,13 +424,13 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int c = 0, st = 0, ph = 0; c < n; ++c) {
-      const int b = c & 1, k0 = kb + c * kChunk;
+      const int k0 = kb + c * kChunk;
       // (kv_full of this chunk has completed when its scores have: no wait, but the loaders' flags;
       // both are asked at once, they are mostly there)
-      const uint32_t sbar = s_full + 8 * (2 * x + b), kbar = kv_full + 8 * st;
-      const bool there = mbar_try_wait(sbar, (c >> 1) & 1) & mbar_try_wait(kbar, ph);
+      const uint32_t sbar = s_full + 8 * x, kbar = kv_full + 8 * st;
+      const bool there = mbar_try_wait(sbar, c & 1) & mbar_try_wait(kbar, ph);
       if (!__all_sync(0xffffffffu, there)) {
-        const bool got = mbar_wait(sbar, (c >> 1) & 1, TI_DEVERR_PREFILL_WAIT) &&
+        const bool got = mbar_wait(sbar, c & 1, TI_DEVERR_PREFILL_WAIT) &&
                          mbar_wait(kbar, ph, TI_DEVERR_PREFILL_WAIT);
         if (!__all_sync(0xffffffffu, got)) { ok = false; break; }
       }
@@ -431,53 +438,53 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
         st = 0;
         ph ^= 1;
       }
+      // The tiles of long items start some clocks apart: 436 us instead of 448 at four chunks of 1024
+      // (900 clocks: 443; they drift back into step).  Short ones would end later by as much.
+      if (c == 0 && x > 0 && n >= kStaggerFrom) {
+        const long long t0 = clock64();
+        while (clock64() - t0 < kStagger * x) {}
+      }
       tc_fence_after();
       float sv[kChunk];
       uint32_t sr[kChunk];
-      tmem_ld64_start(t_s + 64 * b, sr);
+      tmem_ld64_start(t_s, sr);
       const int have = s_ok[c & 7];
       tmem_ld64_end(sr, sv);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(s_read + 8 * x);
       if (have != 15 || k0 + kChunk - 1 > first) {
 #pragma unroll
         for (int i = 0; i < kChunk; ++i)
           sv[i] = (k0 + i <= qp && ((have >> (i / kBlock)) & 1)) ? sv[i] : -INFINITY;
       }
-      // Weights against the running max as it stands, beside the chunk's own max; only when some row
-      // of the warp outgrew it by 2^8 (or had none) are they taken again.
       float mxs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      float alpha = 1.f, sum = 0.f;
-      uint32_t pk[kChunk / 2];
-      auto weights = [&](bool with_max) {
-        const float off = kPScale - (m == -INFINITY ? 0.f : m);
-        const uint64_t sc2 = pair(sc, sc), off2 = pair(off, off);
-        // the chunk's sum first, in four chains of pairs: a long row's total stays exact enough
-        uint64_t sums[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < kChunk; i += 2) {
-          const float2 e = unpair(fma2(pair(sv[i], sv[i + 1]), sc2, off2));
-          const float p0 = fast_exp2(e.x), p1 = fast_exp2(e.y);
-          if (with_max) mxs[i / 2 % 4] = max3(mxs[i / 2 % 4], sv[i], sv[i + 1]);
-          sums[i / 2 % 4] = add2(sums[i / 2 % 4], pair(p0, p1));
-          pk[i / 2] = Elem<__half>::pack2(p0, p1);
-        }
-        const float2 t2 = unpair(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])));
-        sum = t2.x + t2.y;
-      };
-      weights(true);
+      for (int i = 0; i < kChunk; i += 2) mxs[i / 2 % 4] = max3(mxs[i / 2 % 4], sv[i], sv[i + 1]);
       const float mx = max3(fmaxf(mxs[0], mxs[1]), mxs[2], mxs[3]) * sc;
       const bool outgrown = __any_sync(0xffffffffu, mx > m + 8.f);
-      if (outgrown) {
-        if (mx > m + 8.f) {                       // (from no key at all: alpha 0 of zeros)
-          alpha = m == -INFINITY ? 0.f : fast_exp2(m - mx);
-          m = mx;
-        }
-        weights(false);
+      float alpha = 1.f;
+      if (outgrown && mx > m + 8.f) {             // (from no key at all: alpha 0 of zeros)
+        alpha = m == -INFINITY ? 0.f : fast_exp2(m - mx);
+        m = mx;
       }
-      l = l * alpha + sum;
-      // O is touched only to rescale, after P V of chunk c-1.  (A parity tells neighbouring phases apart,
-      // no more: the scores of chunk c come after P V of chunk c-2, so the wait is for the right one.)
+      const float off = kPScale - (m == -INFINITY ? 0.f : m);
+      const uint64_t sc2 = pair(sc, sc), off2 = pair(off, off);
+      // the chunk's sum first, in four chains of pairs: a long row's total stays exact enough
+      uint64_t sums[4] = {0, 0, 0, 0};
+      uint32_t pk[kChunk / 2];
+#pragma unroll
+      for (int i = 0; i < kChunk; i += 2) {
+        const float2 e = unpair(fma2(pair(sv[i], sv[i + 1]), sc2, off2));
+        const float p0 = fast_exp2(e.x), p1 = fast_exp2(e.y);
+        sums[i / 2 % 4] = add2(sums[i / 2 % 4], pair(p0, p1));
+        pk[i / 2] = Elem<__half>::pack2(p0, p1);
+      }
+      const float2 t2 = unpair(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])));
+      l = l * alpha + (t2.x + t2.y);
+      // P V of chunk c-1 has long been done: P's place is free, and O is at rest for a rescale
+      if (c >= 1 && !wait_all(pv_done + 8 * x, (c - 1) & 1)) { ok = false; break; }
       if (outgrown && c >= 1) {
-        if (!wait_all(pv_done + 8 * x, (c - 1) & 1)) { ok = false; break; }
         tc_fence_after();
         float ov[32];
 #pragma unroll
@@ -488,21 +495,17 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
           tmem_st32(t_o + d, ov);
         }
       }
-      // (P of chunk c-2 has been used: a commit, here s_full's, covers all MMAs issued before it)
-      tmem_st32_u(trow + S::p_col(x, b), pk);
+      tmem_st32_u(trow + S::p_col(x), pk);
       tmem_st_wait();
-      // the last chunk: P V of the one before must be seen before P V of this one can be done, or the
-      // wait below could not tell their parities apart
-      if (c == n - 1 && c >= 1 && !wait_all(pv_done + 8 * x, (c - 1) & 1)) { ok = false; break; }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(p_ready + 8 * (2 * x + b));
+      if (lane == 0) mbar_arrive(p_ready + 8 * x);
     }
     if (ok && wait_all(pv_done + 8 * x, (n - 1) & 1)) {
       tc_fence_after();
       const float inv = 1.f / l;
       T* dst = (T*)p.out + (int64_t)(row0 + t) * p.out_stride + (int64_t)(kvh * p.group + h) * HD;
-      float* po = p.parts + (((int64_t)part * p.KVH + kvh) * 2 + x) * (128 * (HD + 2));
+      float* po = p.parts + (((int64_t)part * p.KVH + kvh) * S::kTiles + x) * (128 * (HD + 2));
 #pragma unroll
       for (int d = 0; d < HD; d += 32) {
         float ov[32];
@@ -551,15 +554,17 @@ __global__ void __launch_bounds__(kMergeRows * HD / 4) merge_kernel(const __grid
                                                                   const int32_t* merges) {
   pdl_wait();
   pdl_launch_dependents();
-  const int kvh = blockIdx.x % p.KVH, x = blockIdx.y & 1;
+  constexpr int kTiles = Smem<HD>::kTiles;
+  const int kvh = blockIdx.x % p.KVH, x = blockIdx.y % kTiles;
   const int32_t* e = merges + (int64_t)(blockIdx.x / p.KVH) * kMergeInts;
   const int seq = e[0], q0 = e[1], slot = e[2], n = e[3];
-  const int r = (blockIdx.y >> 1) * kMergeRows + threadIdx.x / (HD / 4), d = threadIdx.x % (HD / 4) * 4;
+  if (x >= e[4]) return;
+  const int r = (blockIdx.y / kTiles) * kMergeRows + threadIdx.x / (HD / 4), d = threadIdx.x % (HD / 4) * 4;
   const int row0 = p.cu_seqlens[seq], count = p.cu_seqlens[seq + 1] - row0;
   const int h = r & ((1 << p.slots_log2) - 1);
   const int t = q0 + x * (128 >> p.slots_log2) + (r >> p.slots_log2);
   if (h >= p.group || t >= count) return;         // (rows of an absent second tile end here too)
-  auto part = [&](int i) { return p.parts + (((int64_t)(slot + i) * p.KVH + kvh) * 2 + x) * (128 * (HD + 2)); };
+  auto part = [&](int i) { return p.parts + (((int64_t)(slot + i) * p.KVH + kvh) * kTiles + x) * (128 * (HD + 2)); };
   float m = -INFINITY, l = 0.f;
   for (int i = 0; i < n; ++i) m = fmaxf(m, part(i)[128 * HD + r]);
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -597,11 +602,11 @@ static int launch(const Params& p, int num_items, const int32_t* merges, int num
     ready.fetch_or(bit, std::memory_order_release);
   }
   if (int rc = launch_kernel("kv4 prefill launch", prefill_kernel<T, HD>,
-                             dim3((unsigned)num_items * p.KVH), dim3(kThreads), Smem<HD>::kTotal, s, 1, p))
+                             dim3((unsigned)num_items * p.KVH), dim3(Smem<HD>::kThreads), Smem<HD>::kTotal, s, 1, p))
     return rc;
   if (num_merges == 0) return TI_OK;
   return launch_kernel("kv4 prefill merge launch", merge_kernel<T, HD>,
-                       dim3((unsigned)num_merges * p.KVH, 2 * 128 / kMergeRows),
+                       dim3((unsigned)num_merges * p.KVH, Smem<HD>::kTiles * 128 / kMergeRows),
                        dim3(kMergeRows * HD / 4), 0, s, 1, p, merges);
 }
 
@@ -613,7 +618,7 @@ using namespace ti;
 
 extern "C" size_t ti_kv4_prefill_workspace_bytes(int num_parts, int num_kv_heads, int head_dim) {
   if (num_parts <= 0 || num_kv_heads <= 0 || (head_dim != 64 && head_dim != 128)) return 0;
-  return (size_t)num_parts * num_kv_heads * 2 * 128 * (head_dim + 2) * 4;
+  return (size_t)num_parts * num_kv_heads * (head_dim == 64 ? 3 : 2) * 128 * (head_dim + 2) * 4;
 }
 
 extern "C" int ti_kv4_prefill_attention(void* out, int64_t out_tok_stride, const void* q,

@@ -358,24 +358,28 @@ class PrefillPlan:
         self.start_pos, self.cu_seqlens = self._dev[:self.num_seqs], self._dev[self.num_seqs:]
         self._layouts: dict = {}
 
-    def work(self, group: int, kv_heads: int):
+    def work(self, group: int, kv_heads: int, head_dim: int = 64):
         """Items and merges (``ti_kv4_prefill_attention``) as host arrays, and the number of parts.
 
-        A pair of tiles is 256 / slots tokens.  Pairs with more keys than a third of what each
-        of 148 SMs would get on average (at least 1024: a range costs a few microseconds of its
-        own) are cut: their keys, one pair behind the other, at every multiple of that size, so
-        that all items but the ends of pairs are of one size and a few long prefixes still fill
-        the GPU.  Longest items first."""
+        An item is up to three tiles (head_dim 128: two) of 128 / slots tokens, which share their
+        keys' way through the chip: as many as leave an item for each of 148 SMs, ranges of 1024
+        keys counted as items.  Items with more keys than a third of what each SM would get on
+        average (at least 1024: a range costs a few microseconds of its own) are cut: their keys,
+        one item behind the other, at every multiple of that size, so that all pieces but the
+        ends are of one size and a few long prefixes still fill the GPU.  Longest first."""
         slots = 1 << (group - 1).bit_length()
-        pair = 256 // slots
-        seq = np.repeat(np.arange(self.num_seqs), -(-self.counts // pair))
-        per = np.concatenate([np.arange(0, c, pair) for c in self.counts.tolist()] or
-                             [np.zeros(0, np.int64)]).astype(np.int64)
-        keys = self.starts[seq] + np.minimum(per + pair, self.counts[seq])
+        for tiles in (3, 2, 1) if head_dim == 64 else (2, 1):
+            step = tiles * (128 // slots)
+            seq = np.repeat(np.arange(self.num_seqs), -(-self.counts // step))
+            per = np.concatenate([np.arange(0, c, step) for c in self.counts.tolist()] or
+                                 [np.zeros(0, np.int64)]).astype(np.int64)
+            keys = self.starts[seq] + np.minimum(per + step, self.counts[seq])
+            if int((-(-keys // 1024)).sum()) * kv_heads >= 148:
+                break
         steps = -(-keys // 64)                                  # a range is whole 64-key steps
         unit = max(16, -(-int(steps.sum()) * kv_heads // (3 * 148)))
         cut = steps > unit
-        begin = np.cumsum(np.where(cut, steps, 0)) - steps      # of a cut pair among them
+        begin = np.cumsum(np.where(cut, steps, 0)) - steps      # of a cut item among them
         end = begin + steps
         # cuts first .. last, in units; none within an eighth of a unit of either end
         first, last = begin // unit + 1, (end - 1) // unit
@@ -383,26 +387,27 @@ class PrefillPlan:
         last = last - (end - last * unit < unit // 8)
         n = np.where(cut, last - first + 2, 1)
         first_part = np.cumsum(np.where(n > 1, n, 0)) - np.where(n > 1, n, 0)
-        at = np.repeat(np.arange(len(seq)), n)                  # the pair of each item
-        k = np.arange(len(at)) - np.repeat(np.cumsum(n) - n, n)  # its range within the pair
-        at_cut = (first[at] + k) * unit - begin[at]             # where range k of a cut pair ends
+        at = np.repeat(np.arange(len(seq)), n)                  # the item of each piece
+        k = np.arange(len(at)) - np.repeat(np.cumsum(n) - n, n)  # its place within the item
+        at_cut = (first[at] + k) * unit - begin[at]             # where piece k of a cut item ends
         lo = np.where(k > 0, at_cut - unit, 0) * 64
         hi = np.where(k < n[at] - 1, at_cut * 64, keys[at])
         part = np.where(n[at] > 1, first_part[at] + k, -1)
-        items = np.stack([seq[at], per[at], lo, hi, part, np.zeros_like(lo)], 1)
+        items = np.stack([seq[at], per[at], lo, hi, part, np.full_like(lo, tiles)], 1)
         items = items[np.argsort(lo - hi, kind="stable")].astype(np.int32)
         cut = n > 1
-        merges = np.stack([seq[cut], per[cut], first_part[cut], n[cut]], 1).astype(np.int32)
+        merges = np.stack([seq[cut], per[cut], first_part[cut], n[cut],
+                           np.full_like(n[cut], tiles)], 1).astype(np.int32)
         return items, merges, int(n[cut].sum())
 
-    def layout(self, group: int, kv_heads: int):
+    def layout(self, group: int, kv_heads: int, head_dim: int):
         """``work`` on the device: pointers and counts, for calls of this head layout."""
-        key = (group, kv_heads)
+        key = (group, kv_heads, head_dim)
         if key not in self._layouts:
             if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
                 _fail("this head layout of the plan is new: run it once, or call layout(), "
                       "before the capture")
-            items, merges, parts = self.work(group, kv_heads)
+            items, merges, parts = self.work(group, kv_heads, head_dim)
             dev = torch.from_numpy(np.concatenate([items.reshape(-1), merges.reshape(-1)])
                                    ).to(self.device)
             base = dev.data_ptr()
@@ -436,7 +441,7 @@ def prefill_attention(out: torch.Tensor, q: torch.Tensor, pool: torch.Tensor,
         return
     lib = N.lib()
     with _on(dev):
-        items, num_items, merges, num_merges, parts = plan.layout(NH // kvh, kvh)
+        items, num_items, merges, num_merges, parts = plan.layout(NH // kvh, kvh, d)
         ws = None
         if parts:
             ws = torch.empty(lib.ti_kv4_prefill_workspace_bytes(parts, kvh, d), dtype=torch.uint8,
