@@ -37,7 +37,9 @@ __device__ __forceinline__ void store_group(uint8_t* tile, bool is_v, int off, i
 // ---- append -------------------------------------------------------------------------------------
 // One thread per (token, group of 16 dims), grid.y over K and V of the heads: 32 bytes in, 9 bytes
 // out.  The groups of a token run over neighbouring lanes and then the tokens, so a warp reads whole
-// lines and writes whole 32-byte rows of codes and runs of scale bytes.
+// lines and writes whole 32-byte rows of codes and runs of scale bytes.  Bound: HBM, then the
+// conversions' instructions: 16384 tokens of 8 kv heads of 128 dims, 86 MB, 20 us from cold caches (4.3
+// TB/s, 77 % of the issue slots); 256 tokens of 2 heads of 64, 1.5 us, one chain of latencies.
 struct AppendParams {
   uint8_t* pool;
   float* weights;                    // attention-weight totals to clear for the new tokens, or null
@@ -166,6 +168,8 @@ struct DequantParams {
   int rows, max_blocks, KVH;
 };
 
+// (Append and read-back of 16384 tokens of 8 kv heads of 128 dims, one behind the other, the codes
+// then in L2: 37 us for 172 MB, 4.6 TB/s, 0.70 of measured copy.)
 constexpr int kDequantThreads = 256;
 constexpr int kDequantUnroll = 2;                // tiles per thread
 
@@ -234,11 +238,13 @@ __global__ void __launch_bounds__(kDequantThreads) dequantize_kernel(DequantPara
 // evict_kernel: the weights become order-preserving 32-bit keys in shared memory, read once.  The
 // lightest kept key is found two bits at a time from the top (how many keys are at least each of the
 // three trial values?), leaving out the bits that all keys share and stopping as soon as a count is
-// exact, which for distinct weights is after about log2(n) bits below the exponent.  Ranks come from one scan of (heavier, equal) counts;
-// the survivors' slots replace the keys in shared memory (a rank is never behind its token), then a
-// warp per block of 16 survivors moves their codes, scales and weights.  A survivor's place is never
-// behind its old one and a round reads all of its tokens before it writes any, so the move may be in
-// place.  Bound: HBM for a large batch, the chain of barriers for one sequence.
+// exact, which for distinct weights is after about log2(n) bits below the exponent.  Ranks come from
+// one scan of (heavier, equal) counts; the survivors' slots replace the keys in shared memory (a rank
+// is never behind its token), then a warp per block of 16 survivors moves their codes, scales and
+// weights.  A survivor's place is never behind its old one and a round reads all of its tokens before
+// it writes any, so the move may be in place.  Bound: HBM for a large batch (24 layers x 32 sequences of
+// U[600, 4096] to 1000: 100 us, 353 MB, 3.5 TB/s; the survivors' codes are gathered 32 bytes at a time),
+// the chain of barriers for one sequence (24 layers x 2048 to 1024: 9 us).
 //
 // evict_long_kernel: the same for sequences whose keys exceed shared memory, the weights read again
 // in each pass.

@@ -316,7 +316,7 @@ def accumulate_weights(weights: torch.Tensor, q: torch.Tensor, lse: torch.Tensor
 
     ``lse`` float32 [B, NH] as ``decode_attention`` gives it for the same arguments; weights and
     out (default: weights itself) float32 [num_blocks, KVH, 16], of which only the sequences' own
-    tokens are read and written.  The sequences of a call share no block."""
+    tokens are written.  The sequences of a call share no block."""
     out = weights if out is None else out
     dev = _device(pool, weights, q, lse, block_tables, context_lens, row_index, out)
     B, NH, nb, kvh, d, q_stride, bt_stride, cols = _attention(q, pool, block_tables, context_lens,

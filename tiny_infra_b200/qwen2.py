@@ -13,8 +13,8 @@ Per layer the decode forward is 8 kernel launches:
 (no merge when every sequence fits 32 blocks: the attention then finishes each sequence in one
 CTA; prefill: one ragged prefill-attention launch instead of the attention and its merge)
 A cache with ``kv_bits=4`` (``KVCacheManager``) runs the same layers on the 4-bit pool: QKV GEMM
-(+bias) -> RoPE and quantised append -> 4-bit paged attention (prefill: read back, then the ragged
-prefill attention); when the cache tracks attention weights, each decode token, and the last
+(+bias) -> RoPE and quantised append -> 4-bit paged attention (prefill: the ragged prefill
+attention on the codes); when the cache tracks attention weights, each decode token, and the last
 ``OBSERVE`` tokens of a prefill chunk, add theirs to the cached tokens' totals.
 
 with the residual stream kept in float32 (the reference keeps it in the model dtype; float32
