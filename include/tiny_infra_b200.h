@@ -383,11 +383,13 @@ int ti_kv4_append(void* pool, float* weights, const void* k, int64_t k_tok_strid
 
 /* ti_rope_kv_append for the 4-bit pool: rows [q | k | v] of T new tokens (ti_rope_kv_append's
  * layout); q and k are rotated in place, then k and v quantised into slot_mapping[t] as
- * ti_kv4_append would from the rotated rows. */
+ * ti_kv4_append would from the rotated rows.  cos and sin have num_positions rows; a token whose
+ * position is not one of them is left alone and raises TI_DEVERR_BAD_INPUT. */
 int ti_rope_kv4_append(void* qkv, int64_t qkv_stride, void* pool, float* weights,
                        const int64_t* slot_mapping, const float* cos, const float* sin,
-                       const int32_t* pos, int num_tokens, int64_t num_blocks, int num_heads,
-                       int num_kv_heads, int head_dim, int block_size, int dtype, void* stream);
+                       int num_positions, const int32_t* pos, int num_tokens, int64_t num_blocks,
+                       int num_heads, int num_kv_heads, int head_dim, int block_size, int dtype,
+                       void* stream);
 
 /* Read the first lens[r] tokens of table row row_index[r] (NULL: r) back as 16-bit values: block j
  * goes to block out_tables[r][j] of k_out / v_out [out_blocks, num_kv_heads, 16, head_dim] (< 0:

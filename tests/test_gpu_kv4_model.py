@@ -13,6 +13,7 @@ import pytest
 import torch
 
 from oracle import kv4 as OK
+from tiny_infra_b200 import _native as N
 from tests.test_gpu_kv4 import dev, half_step, rounded
 
 pytestmark = pytest.mark.gpu
@@ -73,6 +74,30 @@ def test_rope_append_is_rope_then_append(cuda_device, dtn, nh, kvh, d, tokens):
     assert torch.equal(w.transpose(1, 2).reshape(nb * 16, kvh) == 0, zero[:, None].expand(-1, kvh))
     with pytest.raises(RuntimeError):
         kv4.rope_append(pool, qkv[:, :-d], nh, slots, cos, sin, pos)
+
+
+def test_rope_append_checks_positions(cuda_device):
+    """Tokens whose position has no row in both tables are left alone and flagged; the others go on."""
+    from tiny_infra_b200 import kv4
+    N.device_status()
+    g = torch.Generator(device="cuda").manual_seed(3)
+    nh, kvh, d = 4, 2, 64
+    qkv = torch.randn(5, (nh + 2 * kvh) * d, generator=g, device="cuda").to(torch.bfloat16)
+    f = torch.randn(40, d // 2, generator=g, device="cuda")
+    cos, sin = f.cos(), f.sin()[:30].contiguous()
+    slots = torch.arange(5, device="cuda") * 16
+    for at in ([0, 29, 30, 39, 7], [-1, 3, 2 ** 31 - 1, -2 ** 31, 40]):
+        pos = torch.tensor(at, dtype=torch.int32, device="cuda")
+        good = (pos >= 0) & (pos < 30)
+        want, ref = qkv.clone(), kv4.new_pool(5, kvh, d)
+        rows = want[good].contiguous()
+        kv4.rope_append(ref, rows, nh, slots[good], cos, sin, pos[good])
+        want[good] = rows
+        assert N.device_status() == 0
+        got, pool = qkv.clone(), kv4.new_pool(5, kvh, d)
+        kv4.rope_append(pool, got, nh, slots, cos, sin, pos)
+        assert N.device_status() == N.TI_DEVERR_BAD_INPUT
+        assert torch.equal(got, want) and torch.equal(pool, ref)
     with pytest.raises(RuntimeError):
         kv4.rope_append(pool, qkv, nh, slots, cos[:, :-1].contiguous(), sin, pos)
     with pytest.raises(RuntimeError):

@@ -215,12 +215,13 @@ def test_c_abi_refusals(native):
     refused(ev(pool=FAKE + 8), 1, b"aligned")
     refused(ev(layers=70000), 2, b"65535")
 
-    def rope(qkv=FAKE, stride=18 * 64, n=4, nb=8, d=64, bs=16, dt=0, nh=14):
-        return lib.ti_rope_kv4_append(qkv, stride, FAKE, None, FAKE, FAKE, FAKE, FAKE, n, nb, nh, 2,
-                                      d, bs, dt, None)
+    def rope(qkv=FAKE, stride=18 * 64, n=4, nb=8, d=64, bs=16, dt=0, nh=14, rows=32):
+        return lib.ti_rope_kv4_append(qkv, stride, FAKE, None, FAKE, FAKE, FAKE, rows, FAKE, n, nb,
+                                      nh, 2, d, bs, dt, None)
     assert rope(n=0) == 0
     refused(rope(qkv=None), 1, b"null")
     refused(rope(nh=0), 1, b"negative size")
+    refused(rope(rows=-1), 1, b"negative size")
     refused(rope(d=32), 2, b"head_dim")
     refused(rope(dt=2), 2, b"dtype")
     refused(rope(stride=18 * 64 + 4), 1, b"aligned")

@@ -61,7 +61,7 @@ SIGNATURES: dict[str, tuple] = {
                                                    P]),
     "ti_kv4_tile_bytes": (SZ, [I32]),
     "ti_kv4_append": (I32, [P, P, P, I64, I64, P, I64, I64, P, I32, I64, I32, I32, I32, I32, P]),
-    "ti_rope_kv4_append": (I32, [P, I64, P, P, P, P, P, P, I32, I64, I32, I32, I32, I32, I32, P]),
+    "ti_rope_kv4_append": (I32, [P, I64, P, P, P, P, P, I32, P, I32, I64, I32, I32, I32, I32, I32, P]),
     "ti_kv4_dequantize": (I32, [P, P, I64, P, I64, P, I64, P, P, P, I64, I32, I32, I32, I32, I32,
                                 I32, P]),
     "ti_kv4_attention_workspace_bytes": (SZ, [I32, I32, I32, I32, I32]),

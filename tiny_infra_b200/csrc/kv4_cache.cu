@@ -91,7 +91,7 @@ struct RopeAppendParams {
   int64_t pool_slots;
   const float *cos, *sin;
   const int32_t* pos;
-  int tokens, NH, KVH;
+  int positions, tokens, NH, KVH;
 };
 
 template <typename T, int HD>
@@ -107,14 +107,16 @@ __global__ void __launch_bounds__(128) rope_append_kernel(RopeAppendParams p) {
     const int t = (int)(i / per_tok), r = (int)(i - (int64_t)t * per_tok);
     T* row = (T*)p.qkv + t * p.stride;
     const int64_t slot = p.slots[t];
-    const bool write = slot >= 0 && slot < p.pool_slots;
-    if (slot >= p.pool_slots && r == 0) raise_device_error(TI_DEVERR_BAD_INPUT);
+    const int pos = p.pos[t];
+    const bool write = slot >= 0 && slot < p.pool_slots, turn = (uint32_t)pos < (uint32_t)p.positions;
+    if ((slot >= p.pool_slots || !turn) && r == 0) raise_device_error(TI_DEVERR_BAD_INPUT);
+    if (!turn) continue;
     const int off = (int)slot & (kBlock - 1);
     uint8_t* tiles = p.pool + (int64_t)((uint64_t)(write ? slot : 0) / kBlock) * p.KVH * L::kBytes;
     if (r < turns) {
       const int h = r / kPieces, piece = r % kPieces, d0 = piece * kGroup;
       T* base = row + (int64_t)h * HD;             // q heads, then k heads
-      const int64_t tab = (int64_t)p.pos[t] * kHalf + d0;
+      const int64_t tab = (int64_t)pos * kHalf + d0;
       uint4 x[2][2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -669,13 +671,13 @@ extern "C" int ti_kv4_append(void* pool, float* weights, const void* k, int64_t 
 
 extern "C" int ti_rope_kv4_append(void* qkv, int64_t qkv_stride, void* pool, float* weights,
                                   const int64_t* slot_mapping, const float* cos, const float* sin,
-                                  const int32_t* pos, int num_tokens, int64_t num_blocks,
-                                  int num_heads, int num_kv_heads, int head_dim, int block_size,
-                                  int dtype, void* stream) {
+                                  int num_positions, const int32_t* pos, int num_tokens,
+                                  int64_t num_blocks, int num_heads, int num_kv_heads,
+                                  int head_dim, int block_size, int dtype, void* stream) {
   clear_error();
   if (num_tokens == 0) return TI_OK;
   if (!qkv || !pool || !slot_mapping || !cos || !sin || !pos || num_tokens < 0 ||
-      num_blocks <= 0 || num_heads <= 0 || num_kv_heads <= 0)
+      num_positions < 0 || num_blocks <= 0 || num_heads <= 0 || num_kv_heads <= 0)
     return set_error(TI_ERR_INVALID_ARGUMENT, "rope_kv4_append: null pointer, negative size or empty pool");
   if ((head_dim != 64 && head_dim != 128) || block_size != kv4::kBlock)
     return set_error(TI_ERR_UNSUPPORTED, "rope_kv4_append: head_dim must be 64 or 128, block_size 16");
@@ -686,7 +688,7 @@ extern "C" int ti_rope_kv4_append(void* qkv, int64_t qkv_stride, void* pool, flo
         reinterpret_cast<uintptr_t>(cos) | reinterpret_cast<uintptr_t>(sin)) & 15))
     return set_error(TI_ERR_INVALID_ARGUMENT, "rope_kv4_append: tensors must be 16-byte aligned");
   kv4::RopeAppendParams p{qkv, qkv_stride, (uint8_t*)pool, weights, slot_mapping,
-                          num_blocks * kv4::kBlock, cos, sin, pos, num_tokens, num_heads,
+                          num_blocks * kv4::kBlock, cos, sin, pos, num_positions, num_tokens, num_heads,
                           num_kv_heads};
   const int64_t work = (int64_t)num_tokens * ((num_heads + num_kv_heads) * (head_dim / 32) +
                                               num_kv_heads * (head_dim / 16));

@@ -13,7 +13,8 @@ its 16 dims (an unsigned 8-bit float), exact in bf16 and fp16.  ``head_dim`` is 
 * ``accumulate_weights``  add each cached token's attention weight to its running total
 * ``evict``               keep the recent tokens and the heaviest older ones, moved to the front
 
-A block-table entry that is negative or outside the pool holds no tokens.  Every call runs on the
+A block-table entry that is negative or outside the pool holds no tokens; entries of ``row_index``
+are rows of the block table.  Every call runs on the
 current CUDA stream of its tensors' device; argument errors raise ``RuntimeError`` before anything
 is launched.
 """
@@ -203,7 +204,8 @@ def rope_append(pool: torch.Tensor, qkv: torch.Tensor, num_heads: int,
                 positions: torch.Tensor, *, weights: torch.Tensor | None = None) -> None:
     """Rows [q | k | v] of the fused projection, ``qkv`` [T, (num_heads + 2 KVH) * D]: rotate q and k
     in place (rotate-half, tables ``cos`` / ``sin`` float32 [*, D/2], ``positions`` int32 [T]) and
-    ``append`` the rotated k and v."""
+    ``append`` the rotated k and v.  A token whose position is not in the tables is left alone and
+    raises TI_DEVERR_BAD_INPUT."""
     dev = _device(pool, qkv, slot_mapping, cos, sin, positions, weights)
     nb, kvh, d = _pool_shape(pool)
     if qkv.dim() != 2 or qkv.dtype not in _HALF or num_heads <= 0 or \
@@ -226,8 +228,8 @@ def rope_append(pool: torch.Tensor, qkv: torch.Tensor, num_heads: int,
     with _on(dev):
         N.check(N.lib().ti_rope_kv4_append(
             qkv.data_ptr(), qkv.stride(0), pool.data_ptr(), _ptr(weights), slot_mapping.data_ptr(),
-            cos.data_ptr(), sin.data_ptr(), positions.data_ptr(), T, nb, num_heads, kvh, d, BLOCK,
-            N.dtype_code(qkv.dtype), _stream(dev)))
+            cos.data_ptr(), sin.data_ptr(), min(len(cos), len(sin)), positions.data_ptr(), T, nb,
+            num_heads, kvh, d, BLOCK, N.dtype_code(qkv.dtype), _stream(dev)))
 
 
 def dequantize(pool: torch.Tensor, block_tables: torch.Tensor, lens: torch.Tensor,

@@ -422,8 +422,8 @@ class Qwen2ForCausalLM:
                             64 if T <= 512 else 128, 8 if T <= 512 else 1, stream))
         N.check(lib.ti_rope_kv4_append(
             qkv.data_ptr(), QKV, pool.data_ptr(), _ptr(weights), pb.slot_mapping.data_ptr(),
-            cos.data_ptr(), sin.data_ptr(), pb.positions.data_ptr(), T, nb, NH, KVH, D, bs, dt,
-            stream))
+            cos.data_ptr(), sin.data_ptr(), min(len(cos), len(sin)), pb.positions.data_ptr(), T, nb,
+            NH, KVH, D, bs, dt, stream))
         mark(li, "qkv")
         if pb.decode:
             N.check(lib.ti_kv4_attention_decode(
