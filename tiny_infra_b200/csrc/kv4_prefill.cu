@@ -5,7 +5,7 @@
 //
 // A tile is 128 rows: the query heads of one kv head (a power of two of slots, at most 16) times 128 /
 // slots tokens.  One CTA takes up to three tiles of neighbouring tokens (two for D = 128: what tensor
-// memory holds) and a range of keys; they share each 64-key chunk, which four warps read as codes
+// memory holds) and a range of keys; they share each 64-key chunk, which three warps read as codes
 // (asynchronous copies, three chunks ahead) and write to shared memory as half precision -- exact, 2.25
 // times less to read than 16-bit keys and no scratch copy of the cache.  Per chunk and tile:
 //   S = Q K^T   M 128, N 64, into TMEM; the softmax warps free it once it is in registers, and S of the
@@ -17,13 +17,15 @@
 // bf16 queries are scaled by a power of two per row as in the decode kernel; P is held times 2^7 (at
 // most 2^15; steps of 2^-31), its sum taken before rounding.
 //
-// Bound: four chunks of 1024 tokens behind prefixes up to 32767 (14 heads over 2, D = 64) take 436 us.
+// Bound: four chunks of 1024 tokens behind prefixes up to 32767 (14 heads over 2, D = 64) take 414 us.
 // The exponentials alone would take 230 (one warp instruction in 8 clocks of a scheduler: 512 clocks a
 // tile and chunk), the MMAs 146 at their full rate.  The three warps of a scheduler that have them to
-// do mostly run in step, so half of a chunk's 2600 clocks the exponential unit is busy, and half it
-// waits for their other work: waits, tensor memory, the max.  Two tiles a CTA with double-buffered
-// scores: 473 us; two threads a row: 534.  A warp order by flags in shared memory cost registers and
-// more time than it gave (524 to 765).
+// do mostly run in step, so for half of a chunk's clocks the exponential unit is busy, and half it
+// waits for their other work: waits, tensor memory, the max.  What was measured on the way: two tiles a
+// CTA with double-buffered scores 473 us; two threads a row 534; three tiles with a fourth loader warp,
+// 17 warps of 96 registers instead of 16 of 128, 436; the max taken beside the exponentials, which then
+// may have to be taken again, 444.  An order of the warps by flags in shared memory cost registers and
+// more time than it gave (524 to 765 against 436).
 //
 // Work: the host cuts the keys of long sequences into ranges of the same size, longest first, so that a
 // few long prefixes fill the GPU; tiles cut into several ranges leave un-normalised partials that
@@ -47,7 +49,8 @@ namespace pre {
 constexpr int kChunk = 64;                       // keys per step
 constexpr int kStages = 3;                       // chunks of K and V in half precision
 constexpr int kRaw = 4;                          // chunks of codes
-constexpr int kLoadWarps = 4;
+constexpr int kLoadWarps = 3;
+constexpr int kLoaders = kLoadWarps * 32;
 constexpr float kPScale = 7.f;
 constexpr int kStagger = 500, kStaggerFrom = 16; // clocks, chunks
 constexpr int kItemInts = 6;                     // sequence, first token, key range, part or -1, tiles
@@ -186,7 +189,7 @@ __global__ void __launch_bounds__(Smem<HD>::kThreads, 1) prefill_kernel(const __
   if (warp == kMmaWarp) {
     if (lane == 0) {
       for (int i = 0; i < kStages; ++i) {
-        mbar_init(kv_full + 8 * i, kLoadWarps * 32);
+        mbar_init(kv_full + 8 * i, kLoaders);
         mbar_init(kv_empty + 8 * i, 1);
       }
       for (int i = 0; i < S::kTiles; ++i) {
@@ -269,19 +272,19 @@ __global__ void __launch_bounds__(Smem<HD>::kThreads, 1) prefill_kernel(const __
     auto valid = [&](int id) { return (uint32_t)id < num_blocks; };
     if (lt < 28) want_id(lt / 4, lt % 4);
     asm volatile("cp.async.wait_all;" ::: "memory");
-    asm volatile("bar.sync 1, 128;" ::: "memory");
+    asm volatile("bar.sync 1, 96;" ::: "memory");
     auto issue = [&](int c) {
       const uint32_t raw = sb + S::kRawAt + (c % kRaw) * S::kRawChunk;
-      constexpr int kEach = (kUnits + 127) / 128;
+      constexpr int kEach = kUnits / kLoaders;
+      static_assert(kUnits % kLoaders == 0, "whole rounds of copies");
       int id[kEach];
 #pragma unroll
       for (int i = 0; i < kEach; ++i) {
-        const int u = lt + i * 128;
-        id[i] = u < kUnits ? s_ids[(c & 7) * 4 + u / kTileUnits] : -1;
+        id[i] = s_ids[(c & 7) * 4 + (lt + i * kLoaders) / kTileUnits];
       }
 #pragma unroll
       for (int i = 0; i < kEach; ++i) {
-        const int u = lt + i * 128;
+        const int u = lt + i * kLoaders;
         if (valid(id[i]))
           cp_async16(raw + u * 16, p.pool + ((int64_t)id[i] * p.KVH + kvh) * L::kBytes + (u % kTileUnits) * 16);
       }
@@ -290,65 +293,62 @@ __global__ void __launch_bounds__(Smem<HD>::kThreads, 1) prefill_kernel(const __
       issue(c);
       asm volatile("cp.async.commit_group;" ::: "memory");
     }
-    const int tok = lt >> 1, half = lt & 1;      // this thread's token of a chunk, half of its dims
-    // after a wait that gave up the loop goes on without waiting: all 128 threads keep meeting at the
+    // a piece is 32 dims, two scale groups, of a token's K or V; whole warps take whole runs of them
+    constexpr int kPieces = kChunk * 2 * (HD / 32), kRounds = (kPieces + kLoaders - 1) / kLoaders;
+    // after a wait that gave up the loop goes on without waiting: all the threads keep meeting at the
     // barrier, and the results are void anyway
     bool ok = true;
     for (int c = 0; c < n; ++c) {
       const int st = c % kStages;
       asm volatile("cp.async.wait_group %0;" ::"n"(kRaw - 2) : "memory");
-      asm volatile("bar.sync 1, 128;" ::: "memory");   // everyone's copies; chunk c-1 was read
+      asm volatile("bar.sync 1, 96;" ::: "memory");   // everyone's copies; chunk c-1 was read
       issue(c + kRaw - 1);
-      if (warp == kMmaWarp - 1) {                // (the warp with the fewest copies)
+      if (warp == kMmaWarp - 1) {                // (the warp with the fewest pieces)
         if (lane < 4) want_id(c + 7, lane);      // in chunk c-1's place: every thread is past it
         const uint32_t have = __ballot_sync(0xffffffffu, lane < 4 && valid(s_ids[(c & 7) * 4 + (lane & 3)]));
         if (lane == 0) s_ok[c & 7] = (int)(have & 15u);
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
-      const int pos = kb + c * kChunk + tok;
-      const bool live = pos < cached && valid(s_ids[(c & 7) * 4 + tok / kBlock]);
-      const uint8_t* raw = smem + S::kRawAt + (c % kRaw) * S::kRawChunk + (tok / kBlock) * L::kBytes;
-      const int off = tok % kBlock;
-      // (all reads before the first write: the compiler keeps their order)
-      uint4 w[2][S::kSub];
-      uint32_t by[2][S::kSub][2];
-#pragma unroll
-      for (int kv = 0; kv < 2; ++kv)
-#pragma unroll
-        for (int u = 0; u < S::kSub; ++u) {      // 32 dims, two scale groups, at a time
-          const int d0 = half * (HD / 2) + u * 32;
-          w[kv][u] = make_uint4(0u, 0u, 0u, 0u);
-          by[kv][u][0] = by[kv][u][1] = 0;
-          if (live) {
-            w[kv][u] = *reinterpret_cast<const uint4*>(raw + (kv ? L::kV : L::kK) + off * L::kRow + d0 / 2);
-#pragma unroll
-            for (int g = 0; g < 2; ++g) by[kv][u][g] = raw[(kv ? L::kVs : L::kKs) + (d0 / 16 + g) * kBlock + off];
-          }
-        }
-      if (ok && c >= kStages && !mbar_wait(kv_empty + 8 * st, ((c / kStages) - 1) & 1, TI_DEVERR_PREFILL_WAIT)) ok = false;
+      const uint8_t* raw = smem + S::kRawAt + (c % kRaw) * S::kRawChunk;
       const uint32_t dst = sb + S::kKv + st * 2 * S::kKvTile;
+      // (all reads before the first write: the compiler keeps their order)
+      uint4 w[kRounds];
+      uint32_t by[kRounds][2];
 #pragma unroll
-      for (int kv = 0; kv < 2; ++kv) {
+      for (int i = 0; i < kRounds; ++i) {
+        const int e = lt + i * kLoaders, tok = e / (HD / 32) % kChunk, d0 = e % (HD / 32) * 32;
+        const bool v = e / (HD / 32) >= kChunk;
+        const uint8_t* tile = raw + (tok / kBlock) * L::kBytes;
+        w[i] = make_uint4(0u, 0u, 0u, 0u);
+        by[i][0] = by[i][1] = 0;
+        if (e < kPieces && kb + c * kChunk + tok < cached && valid(s_ids[(c & 7) * 4 + tok / kBlock])) {
+          w[i] = *reinterpret_cast<const uint4*>(tile + (v ? L::kV : L::kK) + tok % kBlock * L::kRow + d0 / 2);
 #pragma unroll
-        for (int u = 0; u < S::kSub; ++u) {
-          const int d0 = half * (HD / 2) + u * 32;
-          uint32_t(&b2)[2] = by[kv][u];
-          if (kv) {
+          for (int g = 0; g < 2; ++g)
+            by[i][g] = tile[(v ? L::kVs : L::kKs) + (d0 / 16 + g) * kBlock + tok % kBlock];
+        }
+      }
+      if (ok && c >= kStages && !mbar_wait(kv_empty + 8 * st, ((c / kStages) - 1) & 1, TI_DEVERR_PREFILL_WAIT)) ok = false;
 #pragma unroll
-            for (int g = 0; g < 2; ++g)
-              if (b2[g] >= 0xF8u) { atomicMin(&s_nan[d0 / 16 + g], pos); b2[g] = 0; }
-          }
-          const uint32_t ws[4] = {w[kv][u].x, w[kv][u].y, w[kv][u].z, w[kv][u].w};
-          const uint32_t row = dst + kv * S::kKvTile + (d0 / 64) * 8192 + tok * 128;
+      for (int i = 0; i < kRounds; ++i) {
+        const int e = lt + i * kLoaders, tok = e / (HD / 32) % kChunk, d0 = e % (HD / 32) * 32;
+        const bool v = e / (HD / 32) >= kChunk;
+        if (e >= kPieces) break;
+        if (v) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            uint32_t h[4];
-            codes_to_half2(ws[k], h);
-            const uint32_t s2 = b2[k / 2] * 0x00800080u;
-            const int ch = (d0 % 64) / 8 + k;
-            st_shared_v4(row + ((ch ^ (tok & 7)) << 4), hmul2(h[0], s2), hmul2(h[1], s2),
-                         hmul2(h[2], s2), hmul2(h[3], s2));
-          }
+          for (int g = 0; g < 2; ++g)
+            if (by[i][g] >= 0xF8u) { atomicMin(&s_nan[d0 / 16 + g], kb + c * kChunk + tok); by[i][g] = 0; }
+        }
+        const uint32_t ws[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+        const uint32_t row = dst + (v ? S::kKvTile : 0) + (d0 / 64) * 8192 + tok * 128;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          uint32_t h[4];
+          codes_to_half2(ws[k], h);
+          const uint32_t s2 = by[i][k / 2] * 0x00800080u;
+          const int ch = (d0 % 64) / 8 + k;
+          st_shared_v4(row + ((ch ^ (tok & 7)) << 4), hmul2(h[0], s2), hmul2(h[1], s2),
+                       hmul2(h[2], s2), hmul2(h[3], s2));
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -438,8 +438,8 @@ __global__ void __launch_bounds__(Smem<HD>::kThreads, 1) prefill_kernel(const __
         st = 0;
         ph ^= 1;
       }
-      // The tiles of long items start some clocks apart: 436 us instead of 448 at four chunks of 1024
-      // (900 clocks: 443; they drift back into step).  Short ones would end later by as much.
+      // The tiles of long items start some clocks apart: 414 us instead of 424 at four chunks of 1024
+      // (1000 clocks: 424; they drift back into step).  Short ones would end later by as much.
       if (c == 0 && x > 0 && n >= kStaggerFrom) {
         const long long t0 = clock64();
         while (clock64() - t0 < kStagger * x) {}
