@@ -683,6 +683,8 @@ def test_rows_that_overlap_are_refused(kv4):
               lambda: kv4.rope_append(pool, z(1, 8 * 64).expand(3, 8 * 64), 4, slots, tables, tables, i32(3))):
         with pytest.raises(RuntimeError, match="overlap"):
             f()
+    with pytest.raises(RuntimeError, match="shape"):
+        kv4.decode_attention(z(3, 256), z(3, 4, 64), pool, i32(3, 3), i32(3))
     # a query that all rows share is read, not written
     out = z(3, 4, 64)
     kv4.decode_attention(out, same, pool, i32(3, 3), i32(3) + 5)

@@ -154,6 +154,9 @@ class Workspace:
     def get(self, device: torch.device, nbytes: int, stream: int | None = None) -> torch.Tensor:
         idx = device.index if device.index is not None else torch.cuda.current_device()
         key = (idx, stream)
+        buf = self._buf.get(key)
+        if buf is not None and buf.numel() >= nbytes:
+            return buf                   # (entries are only ever replaced, by larger ones)
         with self._lock:
             buf = self._buf.get(key)
             if buf is None or buf.numel() < nbytes:

@@ -30,6 +30,7 @@ from . import _native as N
 
 BLOCK = 16
 _HALF = (torch.bfloat16, torch.float16)
+_CODE = {t: N.dtype_code(t) for t in _HALF}
 _ws = N.Workspace()
 
 
@@ -52,23 +53,20 @@ def _device(*tensors) -> int:
 
 def _on(dev: int):
     """Launches go to the current device: make it the tensors' one."""
-    return _HERE if dev == torch.cuda.current_device() else torch.cuda.device(dev)
+    return _HERE if dev == torch._C._cuda_getDevice() else torch.cuda.device(dev)
 
 
 _HERE = contextlib.nullcontext()
-
-
-def _stream(dev: int) -> int:
-    return torch._C._cuda_getCurrentRawStream(dev)
+_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _pool_shape(pool: torch.Tensor, layered: bool = False):
-    dims = pool.dim()
+    shape = pool.shape
     if pool.dtype != torch.uint8 or not pool.is_contiguous() or \
-            not (dims == 3 or layered and dims == 4):
+            not (len(shape) == 3 or layered and len(shape) == 4):
         _fail("pool must be a contiguous uint8 [num_blocks, num_kv_heads, 18 * head_dim] tensor"
               + (" or [layers, ...]" if layered else ""))
-    nb, kvh, tile = pool.shape[-3:]
+    nb, kvh, tile = shape if len(shape) == 3 else shape[1:]
     if tile != 1152 and tile != 2304:
         _fail("pool tiles must be 18 * head_dim bytes, head_dim 64 or 128")
     if nb <= 0 or kvh <= 0:
@@ -87,9 +85,10 @@ def _index(name: str, t: torch.Tensor | None, numel: int | None = None) -> None:
 
 def _table(name: str, t: torch.Tensor, rows: int | None):
     """(row stride, columns) of a block table."""
-    if t.dtype != torch.int32 or t.dim() != 2:
+    shape = t.shape
+    if t.dtype != torch.int32 or len(shape) != 2:
         _fail(f"{name} must be int32 [rows, max_blocks]")
-    n, cols = t.shape
+    n, cols = shape
     if cols <= 0:
         _fail(f"{name} has no columns")
     stride, inner = t.stride()
@@ -103,20 +102,24 @@ def _table(name: str, t: torch.Tensor, rows: int | None):
 def _rows(name: str, t: torch.Tensor):
     """Shape and token stride of a [T, heads, D] tensor of a 16-bit type whose tokens' heads are
     contiguous."""
-    if t.dim() != 3 or t.dtype not in _HALF:
+    shape = t.shape
+    if len(shape) != 3 or t.dtype not in _HALF:
         _fail(f"{name} must be bf16 or fp16 [tokens, heads, head_dim]")
-    T, heads, d = t.shape
+    T, heads, d = shape
     tok, head, inner = t.stride()
-    if t.numel() and (inner != 1 or (head != d and heads > 1)):
+    if (inner != 1 or (head != d and heads > 1)) and T * heads * d:
         _fail(f"{name} must have contiguous [heads, head_dim] rows")
     return T, heads, d, tok
 
 
 def _out_rows(out: torch.Tensor, q: torch.Tensor) -> int:
     """Token stride of an output of q's shape whose rows do not overlap."""
-    T, heads, d, tok = _rows("out", out)
     if out.shape != q.shape or out.dtype != q.dtype:
         _fail("out must have q's shape and dtype")
+    T, heads, d = q.shape
+    tok, head, inner = out.stride()
+    if (inner != 1 or (head != d and heads > 1)) and T * heads * d:
+        _fail("out must have contiguous [heads, head_dim] rows")
     if T > 1 and tok < heads * d:
         _fail("out's rows overlap")
     return tok
@@ -195,7 +198,7 @@ def append(pool: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slot_mapping: t
     with _on(dev):
         N.check(N.lib().ti_kv4_append(
             pool.data_ptr(), _ptr(weights), k.data_ptr(), k_tok, k_head, v.data_ptr(), v_tok,
-            v_head, slot_mapping.data_ptr(), T, nb, kvh, d, BLOCK, N.dtype_code(k.dtype),
+            v_head, slot_mapping.data_ptr(), T, nb, kvh, d, BLOCK, _CODE[k.dtype],
             _stream(dev)))
 
 
@@ -229,7 +232,7 @@ def rope_append(pool: torch.Tensor, qkv: torch.Tensor, num_heads: int,
         N.check(N.lib().ti_rope_kv4_append(
             qkv.data_ptr(), qkv.stride(0), pool.data_ptr(), _ptr(weights), slot_mapping.data_ptr(),
             cos.data_ptr(), sin.data_ptr(), min(len(cos), len(sin)), positions.data_ptr(), T, nb,
-            num_heads, kvh, d, BLOCK, N.dtype_code(qkv.dtype), _stream(dev)))
+            num_heads, kvh, d, BLOCK, _CODE[qkv.dtype], _stream(dev)))
 
 
 def dequantize(pool: torch.Tensor, block_tables: torch.Tensor, lens: torch.Tensor,
@@ -259,14 +262,14 @@ def dequantize(pool: torch.Tensor, block_tables: torch.Tensor, lens: torch.Tenso
             k_out.data_ptr(), v_out.data_ptr(), k_out.shape[0], pool.data_ptr(), nb,
             block_tables.data_ptr(), bt_stride, _ptr(row_index), lens.data_ptr(),
             out_tables.data_ptr(), ot_stride, rows, cols, kvh, d, BLOCK,
-            N.dtype_code(k_out.dtype), _stream(dev)))
+            _CODE[k_out.dtype], _stream(dev)))
 
 
 def _workspace(dev: int, nbytes: int, stream: int) -> torch.Tensor:
     """Zeroed scratch, one per (device, stream); inside a stream capture one of the graph's own
     (so graphs that replay at the same time do not share it), zeroed by the graph itself."""
-    if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(nbytes, dtype=torch.uint8, device=torch.device("cuda", dev))
+    if torch._C._cuda_isCurrentStreamCapturing():
+        return torch.zeros(nbytes, dtype=torch.uint8, device=_cuda(dev))
     return _ws.get(_cuda(dev), nbytes, stream)
 
 
@@ -306,7 +309,7 @@ def decode_attention(out: torch.Tensor, q: torch.Tensor, pool: torch.Tensor,
         N.check(lib.ti_kv4_attention_decode(
             out.data_ptr(), out_stride, _ptr(lse), q.data_ptr(), q_stride, pool.data_ptr(), nb,
             block_tables.data_ptr(), bt_stride, _ptr(row_index), context_lens.data_ptr(), B, NH,
-            kvh, d, BLOCK, cols, N.dtype_code(q.dtype), ws.data_ptr(), ws.numel(), stream))
+            kvh, d, BLOCK, cols, _CODE[q.dtype], ws.data_ptr(), ws.numel(), stream))
 
 
 def accumulate_weights(weights: torch.Tensor, q: torch.Tensor, lse: torch.Tensor,
@@ -332,7 +335,7 @@ def accumulate_weights(weights: torch.Tensor, q: torch.Tensor, lse: torch.Tensor
         N.check(N.lib().ti_kv4_accumulate_weights(
             out.data_ptr(), weights.data_ptr(), q.data_ptr(), q_stride, lse.data_ptr(),
             pool.data_ptr(), nb, block_tables.data_ptr(), bt_stride, _ptr(row_index),
-            context_lens.data_ptr(), B, NH, kvh, d, BLOCK, cols, N.dtype_code(q.dtype),
+            context_lens.data_ptr(), B, NH, kvh, d, BLOCK, cols, _CODE[q.dtype],
             _stream(dev)))
 
 
@@ -452,7 +455,7 @@ def prefill_attention(out: torch.Tensor, q: torch.Tensor, pool: torch.Tensor,
             out.data_ptr(), out_stride, q.data_ptr(), q_stride, pool.data_ptr(), nb,
             block_tables.data_ptr(), bt_stride, cols, _ptr(row_index), plan.start_pos.data_ptr(),
             plan.cu_seqlens.data_ptr(), items, num_items, merges, num_merges, parts, NH, kvh, d,
-            BLOCK, N.dtype_code(q.dtype), _ptr(ws), 0 if ws is None else ws.numel(), _stream(dev)))
+            BLOCK, _CODE[q.dtype], _ptr(ws), 0 if ws is None else ws.numel(), _stream(dev)))
 
 
 def evict(pool: torch.Tensor, weights: torch.Tensor, block_tables: torch.Tensor,
