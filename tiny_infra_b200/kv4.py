@@ -241,9 +241,14 @@ def dequantize(pool: torch.Tensor, block_tables: torch.Tensor, lens: torch.Tenso
     """Read the first ``lens[r]`` tokens of each table row back into 16-bit pools ``k_out`` /
     ``v_out`` [out_blocks, KVH, 16, D]: block j of row r goes to block ``out_tables[r, j]`` (a
     negative entry skips it), zeros behind the row's length and where the source entry holds no
-    block.  ``row_index`` selects the rows of ``block_tables``.  The target blocks are distinct."""
+    block.  ``row_index`` selects the rows of ``block_tables``.  The target blocks are distinct.
+
+    A pool of all layers [layers, num_blocks, KVH, 18 D], as ``evict`` takes it, is read as one of
+    layers * num_blocks blocks: block b of layer l is entry l * num_blocks + b."""
     dev = _device(pool, block_tables, lens, out_tables, k_out, v_out, row_index)
-    nb, kvh, d = _pool_shape(pool)
+    nb, kvh, d = _pool_shape(pool, layered=True)
+    if pool.dim() == 4:
+        nb *= pool.shape[0]
     if k_out.dim() != 4 or k_out.shape != v_out.shape or k_out.dtype != v_out.dtype or \
             k_out.dtype not in _HALF or not k_out.is_contiguous() or \
             not v_out.is_contiguous() or k_out.shape[1:] != (kvh, BLOCK, d):
