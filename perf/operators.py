@@ -433,8 +433,8 @@ def run(st):
         return st["new"]
     kv4.evict(st["pool"], st["weights"], st["tables"], st["lens"], st["case"]["keep"],
               st["case"]["recent"], out_block_tables=st["dst"], kept=st["kept"])
-    kv4.dequantize(st["pool"].flatten(0, 1), st["read"], st["read_lens"], st["read_to"],
-                   st["k_out"], st["v_out"])
+    kv4.dequantize(st["pool"], st["read"], st["read_lens"], st["read_to"], st["k_out"],
+                   st["v_out"])
     return st["kept"], st["weights"][:, :st["front"]], st["k_out"], st["v_out"]
 
 
