@@ -50,3 +50,23 @@ def test_dequantize_takes_the_pool_of_all_layers(recorded):
         kv4.dequantize(torch.zeros(1, 3, 5, 2, 18 * 64, dtype=torch.uint8), _i32(2, 3), _i32(2),
                        _i32(2, 3), out, out.clone())
     assert not rec.calls
+
+
+def _host_cache(**kw):
+    """The scheduler's view of a cache (tests/test_scheduler_trace.py), with attributes of its own."""
+    from tests.test_scheduler_trace import _HostKV
+    kv = _HostKV(dict(max_batch_size=3, max_seq_len=32, block_size=16, head_dim=64))
+    for name, value in kw.items():
+        setattr(kv, name, value)
+    return kv
+
+
+def test_batcher_refuses_eviction_without_totals():
+    """A cache that keeps no attention-weight totals (16-bit, or without track_weights) cannot evict:
+    said when the batcher is made, not in the middle of its requests."""
+    from tiny_infra_b200.scheduler import ContinuousBatcher
+    with pytest.raises(ValueError, match="track_weights"):
+        ContinuousBatcher(None, _host_cache(attn_weights=None), backend=object(), evict_above=20)
+    for kv, kw in ((_host_cache(attn_weights=object()), dict(evict_above=20)),
+                   (_host_cache(attn_weights=None), {})):
+        ContinuousBatcher(None, kv, backend=object(), **kw)

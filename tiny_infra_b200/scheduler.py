@@ -109,6 +109,9 @@ class ContinuousBatcher:
                                  "0 <= evict_recent <= evict_keep")
             if evict_above > kv_cache.max_seq_len:
                 raise ValueError("evict_above is beyond the cache's max_seq_len")
+            if hasattr(kv_cache, "attn_weights") and kv_cache.attn_weights is None:
+                raise ValueError("evict_above needs a cache that keeps attention weights "
+                                 "(kv_bits=4 and track_weights)")
         elif evict_keep is not None or evict_recent is not None:
             raise ValueError("evict_keep and evict_recent need evict_above")
         self.evict_above, self.evict_keep, self.evict_recent = evict_above, evict_keep, evict_recent
