@@ -55,3 +55,48 @@ def test_evict_all_layers_and_read_them_back(kv4, dtn, d, kvh, layers):
                     x[:, max(0, int(n) - 16 * j):] = 0
                     want[dst[la, i, j]] = x
         np.testing.assert_array_equal(g.double().cpu().numpy(), rounded(want, dt))
+
+
+@pytest.fixture(scope="module")
+def model(cuda_device):
+    from tiny_infra_b200.config import QwenConfig
+    from tiny_infra_b200.qwen2 import Qwen2ForCausalLM
+    cfg = QwenConfig(num_layers=2, vocab_size=4096)
+    m = Qwen2ForCausalLM(cfg).load_reference_state_dict(
+        Qwen2ForCausalLM.random_state_dict(cfg, seed=2, std=0.05))
+    m.deterministic = True
+    return m
+
+
+def manager(batch=4, max_seq=256, **kw):
+    from tiny_infra_b200.cache_manager import KVCacheManager
+    return KVCacheManager(batch, max_seq, 2, 2, 64, **{"kv_bits": 4, **kw})
+
+
+def test_batcher_ends_one_sequence_at_its_last_position(kv4, model):
+    """Two requests on a cache of 80 positions: the one that reaches them ends with its error after
+    its tokens, the other completes."""
+    import asyncio
+
+    from tiny_infra_b200.scheduler import ContinuousBatcher
+    kv = manager(2, 64, track_weights=True, max_positions=80)
+    sched = ContinuousBatcher(model, kv, evict_above=48, evict_keep=24, evict_recent=8)
+
+    async def main():
+        loop = asyncio.create_task(sched.run_loop())
+
+        async def one(prompt, n):
+            got, error = [], None
+            try:
+                async for t in sched.generate_stream(prompt, n, temperature=0.0):
+                    got.append(t)
+            except ValueError as e:
+                error = e
+            return got, error
+        outs = await asyncio.gather(one(list(range(40)), 100), one([5, 6, 7], 60))
+        loop.cancel()
+        return outs
+    (long, error), (short, none) = asyncio.run(main())
+    assert len(long) == 1 + 40 and "Position" in str(error)
+    assert len(short) == 60 and none is None
+    assert len(kv.free_blocks) == kv.total_physical_blocks

@@ -70,3 +70,58 @@ def test_batcher_refuses_eviction_without_totals():
     for kv, kw in ((_host_cache(attn_weights=object()), dict(evict_above=20)),
                    (_host_cache(attn_weights=None), {})):
         ContinuousBatcher(None, kv, backend=object(), **kw)
+
+
+def _manager(**kw):
+    """A KVCacheManager's host logic without its device pool."""
+    from tiny_infra_b200.cache_manager import BlockAllocator, KVCacheManager
+    kv = KVCacheManager.__new__(KVCacheManager)
+    kv.max_batch_size, kv.max_seq_len, kv.max_positions = 3, 32, 32
+    kv.block_size, kv.head_dim, kv.device = 16, 64, torch.device("cpu")
+    kv.alloc = BlockAllocator(3, 32, 16)
+    kv.total_physical_blocks, kv.max_blocks_per_seq = 6, 2
+    kv._seq_host, kv._bt_host, kv._evicted = kv.alloc.seq_len, kv.alloc.block_tables, False
+    kv.block_tables = torch.full((3, 2), -1, dtype=torch.int32)
+    kv.seq_len, kv.pos_offset = _i32(3), _i32(3)
+    kv.kv4_pool = kv.attn_weights = object()
+    for name, value in kw.items():
+        setattr(kv, name, value)
+    return kv
+
+
+def test_one_sequence_at_its_last_position_ends_alone():
+    """A sequence that has used up the cache's positions ends with its own error; the others go on."""
+    import asyncio
+
+    from tests.test_scheduler_trace import _StandInBackend
+    from tiny_infra_b200.scheduler import ContinuousBatcher, GenerationRequest
+    kv = _manager(max_positions=40)
+
+    def evict(slots, keep, recent):              # the device part is the GPU tests'
+        for s in slots:
+            kv.alloc.truncate(s, keep)
+        kv._evicted = True
+    kv.evict = evict
+    kv.free_batch_slot = kv.alloc.free_slot
+
+    class Backend(_StandInBackend):
+        def decode(self, slots, reqs):
+            kv._check_positions(slots, 1)        # as KVCacheManager.plan_decode does
+            return super().decode(slots, reqs)
+    sched = ContinuousBatcher(None, kv, backend=Backend(kv, 1000), evict_above=20, evict_keep=12)
+
+    async def run():
+        for n, m in ((18, 60), (5, 9), (3, 30)):
+            sched.requests_queue.put_nowait(GenerationRequest(list(range(n)), m, 0.0))
+        sched._fill_active_slots()
+        reqs = list(sched.active_slots)
+        while sched._has_active_requests():
+            sched._step_generation()
+        return reqs
+    reqs = asyncio.run(run())
+    # positions 18 .. 39 are decoded: the token of the prefill and 22 more
+    assert [len(r.generated_tokens) for r in reqs] == [23, 9, 30]
+    assert isinstance(reqs[0].error, ValueError) and "Position" in str(reqs[0].error)
+    assert reqs[1].error is None and reqs[2].error is None
+    assert sched.stats()["requests_failed"] == 1 and sched.stats()["requests_finished"] == 2
+    assert sorted(kv.alloc.free_blocks) == list(range(6))

@@ -249,6 +249,17 @@ class KVCacheManager:
         """Position of the slot's next token: its cached length plus the tokens evicted."""
         return int(self._seq_host[slot] + self.alloc.pos_offset[slot])
 
+    def at_last_position(self, slots) -> list[int]:
+        """Those of the slots that lost tokens to eviction and have no position for a next one."""
+        if not self._evicted:
+            return []                    # the allocator's max_seq_len is the tighter bound
+        return [s for s in slots if self.alloc.pos_offset[s] > 0 and
+                self.position_host(s) >= self.max_positions]
+
+    def position_error(self, slot: int) -> ValueError:
+        return ValueError(f"Position exceeds the maximum of {self.max_positions} for batch index "
+                          f"{slot}.")
+
     def _check_positions(self, slots, counts) -> None:
         """No position beyond the model's (cached lengths are checked by the allocator)."""
         if not self._evicted:
@@ -257,8 +268,7 @@ class KVCacheManager:
         off = self.alloc.pos_offset[sl]
         over = off + self._seq_host[sl] + np.asarray(counts) > self.max_positions
         if over.any():
-            raise ValueError(f"Position exceeds the maximum of {self.max_positions} for batch index "
-                             f"{int(sl[np.argmax(over)])}.")
+            raise self.position_error(int(sl[np.argmax(over)]))
 
     def plan_tokens(self, slots, counts, *, strict_len: bool = True):
         """``BlockAllocator.plan_tokens`` on the host mirror; the new block-table entries are

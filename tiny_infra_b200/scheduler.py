@@ -99,7 +99,8 @@ class ContinuousBatcher:
         track_weights=True)``): before a decode step, sequences that hold that many tokens or more
         are brought down to ``evict_keep`` (default: half), of which ``evict_recent`` (default: a
         quarter of that) are the latest ones, so generation may run past the cached length, up to
-        the cache's ``max_positions``.
+        the cache's ``max_positions`` (which is ``max_seq_len`` unless the cache was given more).  A
+        sequence that reaches it ends with an error of its own.
         """
         if evict_above is not None:
             evict_keep = evict_above // 2 if evict_keep is None else int(evict_keep)
@@ -295,6 +296,14 @@ class ContinuousBatcher:
             if full:
                 self.kv_cache.evict(full, self.evict_keep, self.evict_recent)
                 self._stats.evictions += len(full)
+            # a sequence that has used up the cache's positions ends alone, the others step on
+            ended = getattr(self.kv_cache, "at_last_position", lambda slots: [])(decode_indices)
+            for s in ended:
+                self._finish_request(s, reason="Error during decode",
+                                     error=self.kv_cache.position_error(s))
+            decode_indices = [s for s in decode_indices if s not in ended]
+            if not decode_indices:
+                return
         reqs = [self.active_slots[s] for s in decode_indices]
         tokens = self.backend.decode(decode_indices, reqs)
         self._stats.decode_steps += 1
