@@ -125,3 +125,25 @@ def test_one_sequence_at_its_last_position_ends_alone():
     assert reqs[1].error is None and reqs[2].error is None
     assert sched.stats()["requests_failed"] == 1 and sched.stats()["requests_finished"] == 2
     assert sorted(kv.alloc.free_blocks) == list(range(6))
+
+
+@pytest.mark.parametrize("lens,cols", [((32, 0, 20), 2), ((9, 16, 5), 1)])
+def test_manager_evicts_through_the_columns_in_use(monkeypatch, lens, cols):
+    """The table that the kernel gets is as wide as the longest sequence that shrinks, whatever the
+    cache's max_seq_len: its shared memory and its choice of a kernel go by that width."""
+    from tiny_infra_b200 import kv4
+    kv = _manager()
+    kv.alloc.plan_tokens([0, 1, 2], lens)
+    kv.alloc.advance([0, 1, 2], lens)
+    kv.block_tables.copy_(torch.from_numpy(kv._bt_host))
+    kv.seq_len.copy_(torch.from_numpy(kv._seq_host))
+    seen = []
+    monkeypatch.setattr(kv4, "evict", lambda pool, weights, tables, ctx, keep, recent, row_index: seen.append(
+        (tables.clone(), tables.data_ptr(), ctx.tolist(), keep, recent, row_index.tolist())))
+    before = kv.block_tables.clone()
+    assert kv.evict([0, 1, 2], 8, 3) == [s for s in range(3) if lens[s] > 8]
+    (tables, ptr, ctx, keep, recent, rows), = seen
+    assert ptr == kv.block_tables.data_ptr() and torch.equal(tables, before[:, :cols])
+    assert ctx == [lens[s] for s in rows] and (keep, recent) == (8, 3)
+    assert kv._seq_host.tolist() == [min(n, 8) for n in lens] == kv.seq_len.tolist()
+    assert torch.equal(kv.block_tables, torch.from_numpy(kv._bt_host))

@@ -394,7 +394,9 @@ class KVCacheManager:
         host = torch.tensor([shrink, [self.seq_len_host(s) for s in shrink]], dtype=torch.int32)
         dev = host.to(self.device)
         rows, lens = dev[0].contiguous(), dev[1].contiguous()
-        kv4.evict(self.kv4_pool, self.attn_weights, self.block_tables, lens, keep, recent,
+        # the columns in use: the kernel's shared memory goes by the table's width
+        used = -(-max(self.seq_len_host(s) for s in shrink) // self.block_size)
+        kv4.evict(self.kv4_pool, self.attn_weights, self.block_tables[:, :used], lens, keep, recent,
                   row_index=rows)
         idx = rows.long()
         self.block_tables[idx, -(-keep // self.block_size):] = -1
