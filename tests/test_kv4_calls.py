@@ -147,3 +147,22 @@ def test_manager_evicts_through_the_columns_in_use(monkeypatch, lens, cols):
     assert ctx == [lens[s] for s in rows] and (keep, recent) == (8, 3)
     assert kv._seq_host.tolist() == [min(n, 8) for n in lens] == kv.seq_len.tolist()
     assert torch.equal(kv.block_tables, torch.from_numpy(kv._bt_host))
+
+
+def test_evict_sizes_beyond_32_bits(recorded):
+    """keep and recent reach C as 32-bit numbers: larger ones mean that nothing is evicted, as any
+    keep beyond the lengths does, not a small one."""
+    kv4, rec = recorded
+    pool, w = torch.zeros(5, 2, 18 * 64, dtype=torch.uint8), torch.zeros(5, 2, 16)
+    for keep, recent, want in ((7, 3, [7, 3]), (2 ** 31 - 1, 0, [2 ** 31 - 1, 0]),
+                               (2 ** 31, 2 ** 31, [2 ** 31 - 1] * 2),
+                               (2 ** 32 + 5, 2, [2 ** 31 - 1, 2]),
+                               (2 ** 40, 2 ** 33 + 1, [2 ** 31 - 1] * 2)):
+        kv4.evict(pool, w, _i32(2, 3), _i32(2), keep, recent)
+        name, args = rec.calls.pop()
+        assert name == "ti_kv4_evict" and args[13:15] == want
+    for keep, recent in ((0, 0), (2 ** 32, 2 ** 32 + 1), (4, -1)):
+        with pytest.raises(RuntimeError, match="keep"):
+            kv4.evict(pool, w, _i32(2, 3), _i32(2), keep, recent)
+    with pytest.raises(RuntimeError, match="kept"):
+        kv4.evict(pool, w, _i32(2, 3), _i32(2), 2 ** 32 + 5, 2, kept=_i32(1, 2, 2, 5))

@@ -29,6 +29,7 @@ import torch
 from . import _native as N
 
 BLOCK = 16
+_MOST = 2 ** 31 - 1
 _HALF = (torch.bfloat16, torch.float16)
 _CODE = {t: N.dtype_code(t) for t in _HALF}
 _ws = N.Workspace()
@@ -502,6 +503,8 @@ def evict(pool: torch.Tensor, weights: torch.Tensor, block_tables: torch.Tensor,
         _fail("kept must be contiguous int32 [layers, batch, num_kv_heads, >= keep]")
     if B == 0 or layers == 0:
         return
+    # (lengths are 32-bit: beyond them any keep evicts nothing)
+    keep, recent = min(keep, _MOST), min(recent, _MOST)
     with _on(dev):
         N.check(N.lib().ti_kv4_evict(
             pool.data_ptr(), weights.data_ptr(), layers, nb, block_tables.data_ptr(), bt_stride,
