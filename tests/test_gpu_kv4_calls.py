@@ -100,3 +100,54 @@ def test_batcher_ends_one_sequence_at_its_last_position(kv4, model):
     assert len(long) == 1 + 40 and "Position" in str(error)
     assert len(short) == 60 and none is None
     assert len(kv.free_blocks) == kv.total_physical_blocks
+
+
+def test_model_decode_captured_first_and_twice(kv4, model):
+    """A decode forward on a 4-bit cache, captured as the first call of its stream: what runs on the
+    stream afterwards is right before the graph has replayed once, and two graphs captured on one
+    stream replay at the same time."""
+    rng = np.random.default_rng(4)
+    lens = [600, 40, 333]                       # units that are cut: their joins count arrivals
+    kvs = [manager(3, 2048) for _ in range(2)]
+    cos, sin = model.rope_tables(2048)
+    ids = rng.integers(0, 4096, sum(lens))
+    pbs, want, hidden = [], [], []
+    for kv in kvs:
+        pb = model.plan(kv, [0, 1, 2], lens, ids)
+        model.forward_packed(pb, kv, cos, sin, rows="last")
+        kv.advance_device([0, 1, 2], lens)
+        pbs.append(model.plan(kv, [0, 1, 2], [1, 1, 1], [7, 8, 9]))
+        hidden.append(torch.randn(3, model.config.hidden_size, device="cuda",
+                                  generator=torch.Generator(device="cuda").manual_seed(1)))
+        # (a forward of the same token writes the same bytes into the cache again)
+        want.append(model.forward_packed(pbs[-1], kv, cos, sin, hidden_in=hidden[-1], return_hidden=True))
+    assert torch.equal(*want) and not torch.isnan(want[0]).any()
+    torch.cuda.synchronize()
+    side, replay = torch.cuda.Stream(), [torch.cuda.Stream() for _ in range(2)]
+    graphs, outs = [], []
+    for kv, pb, h in zip(kvs, pbs, hidden):
+        bufs = model.scratch(3, {})             # of the graph's own
+        out = torch.empty_like(h)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            out.copy_(h)
+            model._layers(pb, kv, cos, sin, out, side.cuda_stream, bufs=bufs)
+        graphs.append((g, bufs))
+        outs.append(out)
+    torch.cuda.synchronize()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            got = model.forward_packed(pbs[0], kvs[0], cos, sin, hidden_in=hidden[0], return_hidden=True)
+            assert torch.equal(got, want[0])
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for s, (g, _) in zip(replay, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            assert torch.equal(o, w)

@@ -319,8 +319,12 @@ class Qwen2ForCausalLM:
         four = kv_cache.kv_bits == 4
         if pb.decode and ws is None:
             need = self.attention_workspace_bytes(kv_cache, pb.num_seqs)
-            # (the 4-bit attention's counters have to be zero: its own buffer per stream)
-            ws = self._ws.get(self.device, need, stream if four else None)
+            if four:             # its counters have to be zero: per stream, and per captured graph
+                dev = hidden.get_device()
+                with kv4._on(dev):
+                    ws = kv4._workspace(dev, need, stream)
+            else:
+                ws = self._ws.get(self.device, need)
         if pb.decode and not four:
             # the batch's attention work split, resolved once for all layers
             if plan is None:
