@@ -151,3 +151,25 @@ def test_model_decode_captured_first_and_twice(kv4, model):
         torch.cuda.synchronize()
         for o, w in zip(outs, want):
             assert torch.equal(o, w)
+
+
+@pytest.mark.parametrize("default", [torch.bfloat16, torch.float64])
+def test_model_under_another_default_dtype(kv4, model, default):
+    """Prefill with totals, decode and eviction do not depend on torch's default dtype."""
+    ids, runs = np.random.default_rng(6).integers(0, 4096, 45), []
+    for dt in (torch.float32, default):
+        torch.set_default_dtype(dt)
+        try:
+            kv = manager(2, 64, track_weights=True)
+            cos, sin = model.rope_tables(64)
+            logits = []
+            for slots, counts in (([0, 1], [40, 5]), ([0, 1], [1, 1])):
+                pb = model.plan(kv, slots, counts, ids[:sum(counts)])
+                logits.append(model.forward_packed(pb, kv, cos, sin, rows="last"))
+                kv.advance_device(slots, counts)
+            assert kv.evict([0], 20, 4) == [0]
+        finally:
+            torch.set_default_dtype(torch.float32)
+        runs.append((*logits, kv.attn_weights, kv.kv4_pool))
+    for a, b in zip(*runs):
+        assert a.dtype == b.dtype and torch.equal(a, b)

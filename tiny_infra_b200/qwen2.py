@@ -448,7 +448,8 @@ class Qwen2ForCausalLM:
             # one token per sequence at a time (a call's sequences share no block)
             rows, table, lens = pb.observe
             obs = q.index_select(0, rows)
-            out, sums = torch.empty_like(obs), torch.empty(len(rows), NH, device=self.device)
+            out = torch.empty_like(obs)
+            sums = torch.empty(len(rows), NH, dtype=torch.float32, device=self.device)
             for r in range(0, len(rows), 4096):
                 e = slice(r, r + 4096)
                 kv4.decode_attention(out[e], obs[e], pool, bt, lens[e], row_index=table[e],
