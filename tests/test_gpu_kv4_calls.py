@@ -173,3 +173,37 @@ def test_model_under_another_default_dtype(kv4, model, default):
         runs.append((*logits, kv.attn_weights, kv.kv4_pool))
     for a, b in zip(*runs):
         assert a.dtype == b.dtype and torch.equal(a, b)
+
+
+def test_plan_dropped_behind_a_call_on_another_stream(kv4):
+    """The plan's memory stays its own until the side stream's call, queued behind 20 ms of waiting,
+    is done: allocations of the plan's stream do not get it."""
+    from tiny_infra_b200 import _native as N
+    nh, kvh, d, starts, counts = 14, 2, 64, [5000, 0, 9000], [40, 3, 130]
+    rng = np.random.default_rng(2)
+    tables, nb = tables_for(rng, [s + c for s, c in zip(starts, counts)])
+    pool, tab = dev(random_pool(rng, nb, kvh, d)), dev(tables)
+    q = dev(rng.standard_normal((sum(counts), nh, d)), torch.bfloat16)
+    want, out = torch.empty_like(q), torch.zeros_like(q)
+    side, other = torch.cuda.Stream(), kv4.PrefillPlan(starts, counts)
+    for stream in (torch.cuda.current_stream(), side):     # (what a stream's first call allocates)
+        with torch.cuda.stream(stream):
+            kv4.prefill_attention(want, q, pool, tab, other)
+        torch.cuda.synchronize()
+    plan = kv4.PrefillPlan(starts, counts)
+    plan.layout(nh // kvh, kvh, d)
+    torch.cuda.synchronize()
+    sizes = [(t.data_ptr(), t.numel()) for t, _ in plan._tensors]
+    assert len(sizes) == 2
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(40_000_000)
+        kv4.prefill_attention(out, q, pool, tab, plan)
+    done = torch.cuda.Event()
+    done.record(side)
+    del plan
+    fresh = [torch.empty(n, dtype=torch.int32, device="cuda") for _, n in sizes for _ in range(4)]
+    early = not done.query()
+    torch.cuda.synchronize()
+    assert early                                # the call was still waiting
+    assert not {p for p, _ in sizes} & {t.data_ptr() for t in fresh}
+    assert torch.equal(out, want) and N.device_status() == 0

@@ -166,3 +166,39 @@ def test_evict_sizes_beyond_32_bits(recorded):
             kv4.evict(pool, w, _i32(2, 3), _i32(2), keep, recent)
     with pytest.raises(RuntimeError, match="kept"):
         kv4.evict(pool, w, _i32(2, 3), _i32(2), 2 ** 32 + 5, 2, kept=_i32(1, 2, 2, 5))
+
+
+def test_plan_is_held_for_the_streams_that_use_it(recorded, monkeypatch):
+    """A plan's device tensors are its own: a call on another stream than theirs tells the allocator,
+    once, so that a plan dropped behind the call does not give their memory away under it."""
+    kv4, rec = recorded
+    held, here = [], [0]
+    monkeypatch.setattr(kv4, "_stream", lambda dev: here[0])
+    monkeypatch.setattr(kv4.PrefillPlan, "_home", lambda plan: here[0], raising=False)
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, s: held.append((t.data_ptr(), s)))
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda dev=None: f"stream {here[0]}")
+    monkeypatch.setattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: capturing[0])
+    capturing = [False]
+    plan = kv4.PrefillPlan([0, 5000], [3, 2], device="cpu")
+    q = {kvh: torch.zeros(5, 4, 64, dtype=torch.bfloat16) for kvh in (1, 2)}
+    pools = {kvh: torch.zeros(3, kvh, 18 * 64, dtype=torch.uint8) for kvh in (1, 2)}
+
+    def call(kvh, stream):
+        here[0] = stream
+        kv4.prefill_attention(torch.empty_like(q[kvh]), q[kvh], pools[kvh], _i32(2, 400), plan)
+        out, held[:] = sorted(held), []
+        return out
+    base = plan.start_pos.data_ptr()
+    assert call(2, 0) == []                      # the stream that made it
+    first = plan._layouts[2, 2, 64][0].data_ptr()
+    assert call(2, 7) == sorted([(base, "stream 7"), (first, "stream 7")])
+    assert call(2, 7) == []
+    assert call(1, 9) == sorted([(base, "stream 9"), (first, "stream 9")])     # a layout of 9's own
+    second = plan._layouts[4, 1, 64][0].data_ptr()
+    assert call(1, 7) == [(second, "stream 7")]
+    assert call(1, 0) == [(second, "stream 0")]
+    capturing[0] = True                          # a graph keeps the plan itself
+    assert call(2, 11) == []
+    capturing[0] = False
+    assert len(call(2, 11)) == 3
+    assert all(name.startswith("ti_kv4_prefill") for name, _ in rec.calls)

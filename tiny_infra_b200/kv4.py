@@ -348,9 +348,9 @@ def accumulate_weights(weights: torch.Tensor, q: torch.Tensor, lse: torch.Tensor
 class PrefillPlan:
     """Layout of a packed prefill: chunk i holds ``counts[i]`` query tokens at positions
     ``starts[i]`` and on, whose K and V are already in the cache.  Built once per batch, used by
-    every layer; the work items of a head layout are laid out at its first use and kept.  A graph
-    that captured a call reads the plan's memory: lay the plan out before the capture and keep it as
-    long as the graph."""
+    every layer, on any stream; the work items of a head layout are laid out at its first use and
+    kept.  A graph that captured a call reads the plan's memory: lay the plan out before the capture
+    and keep it as long as the graph."""
 
     def __init__(self, starts, counts, device="cuda") -> None:
         starts, counts = np.asarray(starts, np.int64), np.asarray(counts, np.int64)
@@ -368,6 +368,24 @@ class PrefillPlan:
                                      .astype(np.int32)).to(device)
         self.start_pos, self.cu_seqlens = self._dev[:self.num_seqs], self._dev[self.num_seqs:]
         self._layouts: dict = {}
+        self._tensors, self._held = [(self._dev, self._home())], {}
+
+    def _home(self) -> int | None:
+        """The stream that a device tensor made now belongs to."""
+        dev = self._dev.get_device()
+        return _stream(dev) if dev >= 0 else None
+
+    def hold(self, dev: int, stream: int) -> None:
+        """Calls on ``stream``, the current one of ``dev``, read the plan's tensors: the memory of
+        those that belong to another stream is not handed out again before these calls are done.
+        (Inside a capture nothing is noted: its graph needs the plan itself.)"""
+        if self._held.get(stream, 0) == len(self._tensors) or \
+                torch._C._cuda_isCurrentStreamCapturing():
+            return
+        for t, home in self._tensors[self._held.get(stream, 0):]:
+            if home != stream:
+                t.record_stream(torch.cuda.current_stream(dev))
+        self._held[stream] = len(self._tensors)
 
     def work(self, group: int, kv_heads: int, head_dim: int = 64):
         """Items and merges (``ti_kv4_prefill_attention``) as host arrays, and the number of parts.
@@ -422,6 +440,7 @@ class PrefillPlan:
             dev = torch.from_numpy(np.concatenate([items.reshape(-1), merges.reshape(-1)])
                                    ).to(self.device)
             base = dev.data_ptr()
+            self._tensors.append((dev, self._home()))
             self._layouts[key] = (dev, base, len(items), base + 4 * items.size, len(merges), parts)
         return self._layouts[key][1:]
 
@@ -453,6 +472,8 @@ def prefill_attention(out: torch.Tensor, q: torch.Tensor, pool: torch.Tensor,
     lib = N.lib()
     with _on(dev):
         items, num_items, merges, num_merges, parts = plan.layout(NH // kvh, kvh, d)
+        stream = _stream(dev)
+        plan.hold(dev, stream)
         ws = None
         if parts:
             ws = torch.empty(lib.ti_kv4_prefill_workspace_bytes(parts, kvh, d), dtype=torch.uint8,
@@ -461,7 +482,7 @@ def prefill_attention(out: torch.Tensor, q: torch.Tensor, pool: torch.Tensor,
             out.data_ptr(), out_stride, q.data_ptr(), q_stride, pool.data_ptr(), nb,
             block_tables.data_ptr(), bt_stride, cols, _ptr(row_index), plan.start_pos.data_ptr(),
             plan.cu_seqlens.data_ptr(), items, num_items, merges, num_merges, parts, NH, kvh, d,
-            BLOCK, _CODE[q.dtype], _ptr(ws), 0 if ws is None else ws.numel(), _stream(dev)))
+            BLOCK, _CODE[q.dtype], _ptr(ws), 0 if ws is None else ws.numel(), stream))
 
 
 def evict(pool: torch.Tensor, weights: torch.Tensor, block_tables: torch.Tensor,
