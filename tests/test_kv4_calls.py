@@ -202,3 +202,34 @@ def test_plan_is_held_for_the_streams_that_use_it(recorded, monkeypatch):
     capturing[0] = False
     assert len(call(2, 11)) == 3
     assert all(name.startswith("ti_kv4_prefill") for name, _ in rec.calls)
+
+
+class _Untouched:
+    """In a tensor's place: any use of it is an error."""
+
+    def __getattr__(self, name):
+        raise AssertionError(f"used: {name}")
+
+    def __setitem__(self, key, value):
+        raise AssertionError("written")
+
+
+def test_caches_that_cannot_evict_pay_nothing_for_it():
+    """Without totals nothing is ever evicted: reading the device's lengths back and freeing a slot
+    do not touch the positions' offsets (a copy to the host, a fill)."""
+    for totals in (None, object()):
+        kv = _manager(attn_weights=totals)
+        if totals is None:
+            kv.pos_offset = _Untouched()
+        kv.alloc.plan_tokens([1], [20])
+        kv.seq_len[1] = 20
+        kv.block_tables.copy_(torch.from_numpy(kv._bt_host))
+        kv.sync_from_device()
+        assert (kv.seq_len_host(1), kv.position_host(1)) == (20, 20)
+        kv.free_batch_slot(1)
+        assert kv.seq_len_host(1) == 0 and len(kv.free_blocks) == 6
+    kv.pos_offset[2] = 5                         # set on the device, as the lengths may be
+    kv.sync_from_device()
+    assert kv.position_host(2) == 5 and kv._evicted
+    kv.free_batch_slot(2)
+    assert kv.pos_offset[2] == 0 and kv.position_host(2) == 0

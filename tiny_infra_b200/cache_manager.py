@@ -239,8 +239,9 @@ class KVCacheManager:
         scheduler does with ``kv_cache.seq_len[idx] += n``."""
         self._seq_host[:] = self.seq_len.cpu().numpy()
         self._bt_host[:] = self.block_tables.cpu().numpy()
-        self.alloc.pos_offset[:] = self.pos_offset.cpu().numpy()
-        self._evicted = bool(self.alloc.pos_offset.any())
+        if self.attn_weights is not None:     # (else nothing is ever evicted)
+            self.alloc.pos_offset[:] = self.pos_offset.cpu().numpy()
+            self._evicted = bool(self.alloc.pos_offset.any())
 
     def seq_len_host(self, slot: int) -> int:
         return int(self._seq_host[slot])
@@ -371,7 +372,8 @@ class KVCacheManager:
         self.alloc.free_slot(batch_idx)
         self.block_tables[batch_idx].fill_(-1)
         self.seq_len[batch_idx] = 0
-        self.pos_offset[batch_idx] = 0
+        if self.attn_weights is not None:
+            self.pos_offset[batch_idx] = 0
 
     # ---- eviction ---------------------------------------------------------------------------
     def evict(self, slots, keep: int, recent: int) -> list[int]:

@@ -223,7 +223,7 @@ class Qwen2ForCausalLM:
         cu[1:] = np.cumsum(counts)
         T = int(cu[-1])
         # positions go on behind evicted tokens; everything else follows the cached lengths
-        first = np.array([kv_cache.position_host(s) for s in slots], np.int32)
+        first = start + kv_cache.alloc.pos_offset[np.asarray(slots, np.int64)]
         pos = np.concatenate([first[i] + np.arange(counts[i], dtype=np.int32)
                               for i in range(nseq)]) if T else np.zeros(0, np.int32)
         decode = bool((counts == 1).all())
