@@ -393,8 +393,9 @@ int ti_rope_kv4_append(void* qkv, int64_t qkv_stride, void* pool, float* weights
 
 /* Read the first lens[r] tokens of table row row_index[r] (NULL: r) back as 16-bit values: block j
  * goes to block out_tables[r][j] of k_out / v_out [out_blocks, num_kv_heads, 16, head_dim] (< 0:
- * skipped; >= out_blocks: not written, TI_DEVERR_BAD_INPUT), zeros behind the length and where the
- * source entry holds no block.  block_tables and out_tables have at least max_blocks columns. */
+ * skipped; >= out_blocks: not written, TI_DEVERR_BAD_INPUT), with zeros behind the length in its last
+ * block and where the source entry holds no block.  Blocks wholly behind the length are not written,
+ * and their entries not looked at.  block_tables and out_tables have at least max_blocks columns. */
 int ti_kv4_dequantize(void* k_out, void* v_out, int64_t out_blocks, const void* pool,
                       int64_t num_blocks, const int32_t* block_tables, int64_t bt_stride,
                       const int32_t* row_index, const int32_t* lens, const int32_t* out_tables,

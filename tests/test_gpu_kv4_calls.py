@@ -207,3 +207,22 @@ def test_plan_dropped_behind_a_call_on_another_stream(kv4):
     assert early                                # the call was still waiting
     assert not {p for p, _ in sizes} & {t.data_ptr() for t in fresh}
     assert torch.equal(out, want) and N.device_status() == 0
+
+
+def test_dequantize_leaves_blocks_behind_the_length(kv4):
+    """Zeros fill the last block behind a row's length; a target block that lies wholly behind it is
+    neither written nor looked at, whatever its entry."""
+    from tiny_infra_b200 import _native as N
+    rng = np.random.default_rng(3)
+    pool = random_pool(rng, 4, 2, 64)
+    lens, src = np.array([17, 0, 16], np.int32), np.array([[0, 1, 2], [0, 1, 2], [3, 0, 1]], np.int32)
+    dst = np.array([[4, 0, 1], [2, 3, 99], [5, 6, 2 ** 31 - 1]], np.int32)
+    ko = torch.full((7, 2, 16, 64), 9.0, dtype=torch.bfloat16, device="cuda")
+    vo = ko.clone()
+    kv4.dequantize(dev(pool), dev(src), dev(lens), dev(dst), ko, vo)
+    assert N.device_status() == 0
+    for g, vals in zip((ko, vo), OK.untile(pool)):
+        want = np.full(g.shape, 9.0)
+        want[4], want[0], want[5] = vals[0], vals[1], vals[3]
+        want[0][:, 1:] = 0
+        np.testing.assert_array_equal(g.double().cpu().numpy(), rounded(want, torch.bfloat16))

@@ -154,7 +154,8 @@ __global__ void __launch_bounds__(128) rope_append_kernel(RopeAppendParams p) {
 // ---- read back ------------------------------------------------------------------------------------
 // One thread per (table entry, head, token, 8 dims), K and V both: 8 bytes of codes and 2 scales in,
 // 32 bytes out, the lanes of a warp on neighbouring 16 bytes (with 16 dims per thread the 16-byte
-// stores took half a sector each: 122 us instead of 105 for 393 MB); zeros behind the row's length.
+// stores took half a sector each: 122 us instead of 105 for 393 MB); zeros behind the row's length in
+// its last block, and nothing for the blocks behind that.
 // grid = (runs of a row's blocks, head, row).
 struct DequantParams {
   void *k_out, *v_out;

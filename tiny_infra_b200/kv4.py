@@ -241,8 +241,10 @@ def dequantize(pool: torch.Tensor, block_tables: torch.Tensor, lens: torch.Tenso
                row_index: torch.Tensor | None = None) -> None:
     """Read the first ``lens[r]`` tokens of each table row back into 16-bit pools ``k_out`` /
     ``v_out`` [out_blocks, KVH, 16, D]: block j of row r goes to block ``out_tables[r, j]`` (a
-    negative entry skips it), zeros behind the row's length and where the source entry holds no
-    block.  ``row_index`` selects the rows of ``block_tables``.  The target blocks are distinct.
+    negative entry skips it), with zeros behind the row's length in its last block and where the
+    source entry holds no block.  Blocks that lie wholly behind the length are not written, and their
+    entries not looked at.  ``row_index`` selects the rows of ``block_tables``.  The target blocks
+    are distinct.
 
     A pool of all layers [layers, num_blocks, KVH, 18 D], as ``evict`` takes it, is read as one of
     layers * num_blocks blocks: block b of layer l is entry l * num_blocks + b."""
