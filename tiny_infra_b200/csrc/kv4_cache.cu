@@ -39,7 +39,7 @@ __device__ __forceinline__ void store_group(uint8_t* tile, bool is_v, int off, i
 // out.  The groups of a token run over neighbouring lanes and then the tokens, so a warp reads whole
 // lines and writes whole 32-byte rows of codes and runs of scale bytes.  Bound: HBM, then the
 // conversions' instructions: 16384 tokens of 8 kv heads of 128 dims, 86 MB, 20 us from cold caches (4.3
-// TB/s, 77 % of the issue slots); 256 tokens of 2 heads of 64, 1.5 us, one chain of latencies.
+// TB/s, 77 % of the issue slots); 256 tokens of 2 heads of 64, 1.6 us, one chain of latencies.
 struct AppendParams {
   uint8_t* pool;
   float* weights;                    // attention-weight totals to clear for the new tokens, or null
@@ -668,9 +668,9 @@ extern "C" int ti_kv4_append(void* pool, float* weights, const void* k, int64_t 
                       num_kv_heads};
   if (num_kv_heads > 32767)
     return set_error(TI_ERR_UNSUPPORTED, "kv4_append: at most 32767 kv heads");
-  // Few tokens in small blocks, so that they spread over the SMs: 256 tokens of 2 kv heads, 64 dims, 1.51
-  // us against 1.68 with 256 threads; 16384 tokens 4.72 with 64 threads against 3.37.
-  const int threads = num_tokens <= 1024 ? 64 : 256;
+  // (64 threads for few tokens: 1.59 us against 1.67 at 1024 tokens of 2 kv heads of 64 dims, 1.64 against
+  // 1.54 at 64; of 8 heads of 128 2.57 against 2.37 at 1024, 1.74 against 1.65 at 256)
+  constexpr int threads = 256;
   const dim3 grid(kv4::grid_for((int64_t)num_tokens * (head_dim / 16), threads), 2 * num_kv_heads);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   auto go = [&](auto kern) { return launch_kernel("kv4_append launch", kern, grid, dim3(threads), 0, s, 1, p); };
