@@ -226,3 +226,37 @@ def test_dequantize_leaves_blocks_behind_the_length(kv4):
         want[4], want[0], want[5] = vals[0], vals[1], vals[3]
         want[0][:, 1:] = 0
         np.testing.assert_array_equal(g.double().cpu().numpy(), rounded(want, torch.bfloat16))
+
+
+@pytest.mark.parametrize("batch", [1, 8])
+def test_evict_through_tables_of_any_width(kv4, batch):
+    """The same eviction, bit for bit, whatever the table's width: keys in shared memory, few CTAs to
+    an SM and more units than those, and beyond shared memory."""
+    rng = np.random.default_rng(batch)
+    layers, kvh, d, keep, recent = 24, 2, 64, 40, 9
+    lens = rng.integers(1, 200, batch).astype(np.int32)
+    lens[0] = 199
+    runs = []
+    tables, nb = tables_for(rng, lens)
+    pool = np.stack([random_pool(rng, nb, kvh, d) for _ in range(layers)])
+    w = rng.integers(0, 50, (layers, nb, kvh, 16)).astype(np.float32)
+    for width in (tables.shape[1], 1200, 1600, 2048, 3000, 3100):
+        t = np.full((batch, width), -1, np.int32)
+        t[:, :tables.shape[1]] = tables
+        dp, dw = dev(pool), dev(w)
+        kept = torch.full((layers, batch, kvh, keep), -7, dtype=torch.int32, device="cuda")
+        kv4.evict(dp, dw, dev(t), dev(lens), keep, recent, kept=kept)
+        # (places behind the survivors hold anything)
+        ko = torch.zeros(layers * batch * 3, kvh, 16, d, dtype=torch.float16, device="cuda")
+        vo = torch.zeros_like(ko)
+        off = np.arange(layers)[:, None, None] * nb
+        src = np.where(tables[:, :3] >= 0, tables[:, :3] + off, -1).astype(np.int32).reshape(-1, 3)
+        new = dev(np.tile(np.minimum(lens, keep), layers).astype(np.int32))
+        kv4.dequantize(dp, dev(src), new, dev(np.arange(len(src) * 3, dtype=np.int32).reshape(-1, 3)), ko, vo)
+        runs.append((kept, ko, vo))
+    want = OK.evict(pool, w, tables, lens, keep, recent)
+    for (la, b, h), idx in want.items():
+        np.testing.assert_array_equal(runs[0][0][la, b, h, :len(idx)].cpu().numpy(), idx)
+    for other in runs[1:]:
+        for a, b in zip(runs[0], other):
+            assert torch.equal(a, b)

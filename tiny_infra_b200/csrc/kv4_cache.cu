@@ -82,6 +82,8 @@ __global__ void append_kernel(AppendParams p) {
 // The decode and prefill layers' form, on rows [q | k | v] of the fused projection: q and k are rotated
 // in place and rounded to the type, as ti_rope_inplace does, then k and v are quantised from those
 // values.  One thread per 16 dims and their 16 partners of a q or k head, or per 16 dims of v.
+// Measured, 14 query heads over 2 of 64 dims: 256 tokens 2.9 us, 16384 tokens 20.3 us (76 MB at 3.7
+// TB/s); 32 over 8 of 128, 16384 tokens: 94 us (407 MB at 4.3 TB/s, 0.66 of measured copy).
 struct RopeAppendParams {
   void* qkv;
   int64_t stride;
@@ -257,10 +259,12 @@ __global__ void __launch_bounds__(kDequantThreads) dequantize_kernel(DequantPara
 // weights.  A survivor's place is never behind its old one and a round reads all of its tokens before
 // it writes any, so the move may be in place.  Bound: HBM for a large batch (24 layers x 32 sequences of
 // U[600, 4096] to 1000: 100 us, 353 MB, 3.5 TB/s; the survivors' codes are gathered 32 bytes at a time),
-// the chain of barriers for one sequence (24 layers x 2048 to 1024: 9 us).
+// the chain of barriers for one sequence (24 layers x 2048 to 1024: 9 us).  The keys' place goes by the
+// table's width, so a caller passes the columns in use, as the cache manager does: 24 layers x 2048 to
+// 1024 take 16 us (events around a call) through 128 columns and 37 through 8192.
 //
-// evict_long_kernel: the same for sequences whose keys exceed shared memory, the weights read again
-// in each pass.
+// evict_long_kernel: the same for sequences whose keys exceed shared memory, or fill so much of it that
+// few CTAs fit (see the launch), the weights read again in each pass.
 struct EvictParams {
   uint8_t* pool;
   float* weights;
@@ -778,16 +782,24 @@ extern "C" int ti_kv4_evict(void* pool, float* weights, int num_layers, int64_t 
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   // the widest table bounds the sequences' lengths; slots are 32 bits in shared memory
   const int64_t tokens = (int64_t)max_blocks_per_seq * kv4::kBlock;
-  if (tokens > kv4::kEvictMaxTokens || num_blocks > (int64_t)1 << 28)
+  // With fewer than three CTAs to an SM (tables above some 18000 tokens) a second wave of them costs more
+  // than reading the weights again: 24 layers, half of the tokens kept, us here / in the long kernel:
+  // 96 units (2 heads, 2 sequences) of 32768 tokens 197 / 321; 192 units of 24576 186 / 285, of 32768
+  // 385 / 373; 384 units of 16384 204 / 236, of 24576 482 / 346, of 32768 863 / 453; 768 units of 16384
+  // 390 / 458, of 24576 743 / 679.
+  const int64_t units = (int64_t)num_kv_heads * batch * num_layers;
+  const int64_t per_sm = 227 * 1024 / (tokens * 4 + 2048);
+  const bool waves = per_sm < 3 && units > per_sm * kv4::sm_count();
+  if (tokens > kv4::kEvictMaxTokens || num_blocks > (int64_t)1 << 28 || waves)
     return launch_kernel("kv4_evict launch", head_dim == 64 ? kv4::evict_long_kernel<64> : kv4::evict_long_kernel<128>,
                          grid, dim3(kv4::kEvictLongThreads), 0, s, 1, p);
-  // Many (layer, sequence, head) units: small CTAs, several per SM; few: wide ones, the chain of one
-  // unit counts.  24 layers x 2 heads, one sequence of 2048: 17 us with 512 threads, 23 with 256; 32
-  // sequences of up to 4096: 111 and 99 (cold caches).
+  // Many (layer, sequence, head) units: small CTAs, several per SM (while the table is narrow: see
+  // above); few: wide ones, the chain of one unit counts.  24 layers x 2 heads, one sequence of 2048:
+  // 17 us with 512 threads, 23 with 256; 32 sequences of up to 4096: 111 and 99 (cold caches).
   auto go = [&](auto hd) {
     constexpr int HD = decltype(hd)::value;
     static std::atomic<uint64_t> ready[2];
-    const bool small = (int64_t)num_kv_heads * batch * num_layers > 2 * kv4::sm_count();
+    const bool small = units > 2 * kv4::sm_count();
     auto kern = small ? kv4::evict_kernel<HD, 256> : kv4::evict_kernel<HD, 512>;
     int dev = 0;
     cudaGetDevice(&dev);
