@@ -403,7 +403,8 @@ int ti_kv4_dequantize(void* k_out, void* v_out, int64_t out_blocks, const void* 
                       int block_size, int dtype, void* stream);
 
 /* Decode attention over the 4-bit pool: out / q [batch, num_heads, head_dim] (row strides in
- * elements, multiples of 8, 16-byte aligned), at most 16 query heads per kv head, batch <= 4096.
+ * elements, multiples of 8, 16-byte aligned), at most 16 query heads per kv head, batch <= 4096,
+ * batch * max_blocks_per_seq * num_kv_heads (twice beyond 8 query heads per kv head) < 2^29.
  * lse (float32 [batch, num_heads] or NULL) = ln of the row's sum of exp(q.k / sqrt(head_dim)).
  * context_lens 0 leaves the rows of out and lse untouched; a sequence without a block gets NaN and
  * lse -inf.  The workspace (ti_kv4_attention_workspace_bytes, 16-byte aligned) must be zero before

@@ -38,11 +38,12 @@ namespace kv4 {
 // the scores' factor takes it back.  Weights are held as 2^14 p in half precision: 2^-11 relative
 // (the 16-bit outputs round by as much) down to p = 2^-28; their sum is taken before that rounding.
 //
-// Measured, 14 query heads over 2 of 64 dims: 256 x U[8192, 32768] tokens 135 us back to back (0.76 GB at
-// 5.6 TB/s, 0.85 of measured copy, 70 % of the issue slots); 256 x U[128, 2048] 18.6 us, where a warp has
-// four steps and the length scan, three dependent loads before the first step and the joins are as long
-// as the stream; 8 x U[1, 512] 7.7 us, latency.  32 heads over 8 of 128, 32 x U[1024, 8192]: 45 us, 3.8
-// TB/s (a scale serves twice the dims a lane, but a step is 32 tokens: its fixed work weighs double).
+// Measured, 14 query heads over 2 of 64 dims: 256 x U[8192, 32768] tokens 152 us over 24 pools in turn, as
+// a model's layers are (0.76 GB at 5.1 TB/s, 0.77 of measured copy), 135 us with one pool read again and
+// again (5.6 TB/s, 0.85; 70 % of the issue slots); 256 x U[128, 2048] 18.6 us, where a warp has four
+// steps and the length scan, three dependent loads before the first step and the joins are as long as
+// the stream; 8 x U[1, 512] 7.7 us, latency.  32 heads over 8 of 128, 32 x U[1024, 8192]: 45 us, 3.8 TB/s
+// (a scale serves twice the dims a lane, but a step is 32 tokens: its fixed work weighs double).
 struct DecodeParams {
   void* out;
   float* lse;                        // [batch, NH] or null
@@ -989,7 +990,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) weights_kernel(const __grid_co
 
 constexpr int kMaxCtas = 256;
 constexpr size_t kCounterBytes = kMaxCtas * 4;
-// Widest table that runs one CTA per unit.  8 sequences, 14 heads of 64 dims over 2: 512 tokens 7.7 us
+// Widest table that runs one CTA per unit (the lengths are on the device: a short context behind a wider
+// table takes the even cut).  8 sequences, 14 heads of 64 dims over 2: 512 tokens 7.7 us
 // against 8.6 for the even cut, 1536 tokens 9.9 against 10.8, 2048 tokens 10.7 against 11.0, 4096 tokens
 // 14.9 against 11.2; 32 heads of 128 over 8: 1536 tokens 13.2 against 14.2, 2048 tokens 14.9 against 14.4.
 constexpr int kUnitBlocks = 96;

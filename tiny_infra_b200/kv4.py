@@ -297,7 +297,8 @@ def decode_attention(out: torch.Tensor, q: torch.Tensor, pool: torch.Tensor,
     """Single-query attention, scale 1/sqrt(head_dim): out[b] = softmax(q[b] K^T) V over the first
     ``context_lens[b]`` cached tokens of row ``row_index[b]`` (default b) of ``block_tables``.
 
-    q, out: [B, NH, D] bf16 or fp16, at most 16 query heads per kv head, B at most 4096.  ``lse``
+    q, out: [B, NH, D] bf16 or fp16, at most 16 query heads per kv head, B at most 4096, B * table
+    columns * kv heads (twice beyond 8 query heads per kv head) below 2^29.  ``lse``
     (float32 [B, NH]) receives the natural log of each row's sum of exp(scores).  A sequence of
     length 0 leaves its rows of ``out`` and ``lse`` as they were; one whose table holds no block
     gets NaN, and -inf in ``lse``.  One launch; results do not depend on the batch's other rows'
@@ -329,7 +330,7 @@ def accumulate_weights(weights: torch.Tensor, q: torch.Tensor, lse: torch.Tensor
 
     ``lse`` float32 [B, NH] as ``decode_attention`` gives it for the same arguments; weights and
     out (default: weights itself) float32 [num_blocks, KVH, 16], of which only the sequences' own
-    tokens are written.  The sequences of a call share no block."""
+    tokens are written.  The sequences of a call share no block.  Sizes as ``decode_attention``'s."""
     out = weights if out is None else out
     dev = _device(pool, weights, q, lse, block_tables, context_lens, row_index, out)
     B, NH, nb, kvh, d, q_stride, bt_stride, cols = _attention(q, pool, block_tables, context_lens,
@@ -500,7 +501,9 @@ def evict(pool: torch.Tensor, weights: torch.Tensor, block_tables: torch.Tensor,
     place of 18 D, float32.  The survivors go to the blocks of ``out_block_tables`` (rows as
     ``block_tables``'; default: the same blocks, in place; otherwise blocks that hold none of the
     call's tokens).  ``kept`` (int32 [layers, B, KVH, >= keep]) receives their old positions.  The
-    caller shortens the lengths to min(context_lens, keep) and frees the blocks behind.  A sequence
+    caller shortens the lengths to min(context_lens, keep) and frees the blocks behind.  Pass the
+    columns of ``block_tables`` that are in use: what a call costs goes by the table's width, not by
+    the lengths, which are on the device.  A sequence
     with a needed table entry outside the pool is left as it is and raises TI_DEVERR_BAD_INPUT.
     The sequences of a call share no block."""
     dev = _device(pool, weights, block_tables, context_lens, row_index, out_block_tables, kept)
