@@ -233,3 +233,34 @@ def test_caches_that_cannot_evict_pay_nothing_for_it():
     assert kv.position_host(2) == 5 and kv._evicted
     kv.free_batch_slot(2)
     assert kv.pos_offset[2] == 0 and kv.position_host(2) == 0
+
+
+def test_last_position_after_an_eviction_by_hand():
+    """The same where the program evicts between ticks, and the batcher does not."""
+    import asyncio
+
+    from tests.test_scheduler_trace import _StandInBackend
+    from tiny_infra_b200.scheduler import ContinuousBatcher, GenerationRequest
+    kv = _manager(max_positions=34)
+    kv.free_batch_slot = kv.alloc.free_slot
+
+    class Backend(_StandInBackend):
+        def decode(self, slots, reqs):
+            kv._check_positions(slots, 1)
+            return super().decode(slots, reqs)
+    sched = ContinuousBatcher(None, kv, backend=Backend(kv, 1000))
+
+    async def run():
+        for n, m in ((30, 20), (5, 12)):
+            sched.requests_queue.put_nowait(GenerationRequest(list(range(n)), m, 0.0))
+        sched._fill_active_slots()
+        reqs = list(sched.active_slots)
+        sched._step_generation()                 # the prefills
+        kv.alloc.truncate(0, 10)
+        kv._evicted = True
+        while sched._has_active_requests():
+            sched._step_generation()
+        return reqs
+    reqs = asyncio.run(run())
+    assert [None if r is None else len(r.generated_tokens) for r in reqs] == [5, 12, None]
+    assert "Position" in str(reqs[0].error) and reqs[1].error is None

@@ -296,8 +296,9 @@ class ContinuousBatcher:
             if full:
                 self.kv_cache.evict(full, self.evict_keep, self.evict_recent)
                 self._stats.evictions += len(full)
-            # a sequence that has used up the cache's positions ends alone, the others step on
-            ended = getattr(self.kv_cache, "at_last_position", lambda slots: [])(decode_indices)
+        # a sequence that has used up the cache's positions ends alone, the others step on
+        ended = getattr(self.kv_cache, "at_last_position", lambda slots: [])(decode_indices)
+        if ended:
             for s in ended:
                 self._finish_request(s, reason="Error during decode",
                                      error=self.kv_cache.position_error(s))
