@@ -176,7 +176,7 @@ def test_model_under_another_default_dtype(kv4, model, default):
 
 
 def test_plan_dropped_behind_a_call_on_another_stream(kv4):
-    """The plan's memory stays its own until the side stream's call, queued behind 20 ms of waiting,
+    """The plan's memory stays its own until the side stream's call, queued behind 100 ms of waiting,
     is done: allocations of the plan's stream do not get it."""
     from tiny_infra_b200 import _native as N
     nh, kvh, d, starts, counts = 14, 2, 64, [5000, 0, 9000], [40, 3, 130]
@@ -196,7 +196,7 @@ def test_plan_dropped_behind_a_call_on_another_stream(kv4):
     sizes = [(t.data_ptr(), t.numel()) for t, _ in plan._tensors]
     assert len(sizes) == 2
     with torch.cuda.stream(side):
-        torch.cuda._sleep(40_000_000)
+        torch.cuda._sleep(200_000_000)
         kv4.prefill_attention(out, q, pool, tab, plan)
     done = torch.cuda.Event()
     done.record(side)
