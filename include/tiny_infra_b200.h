@@ -469,6 +469,91 @@ int ti_kv4_evict(void* pool, float* weights, int num_layers, int64_t num_blocks,
                  int32_t* kept, int64_t kept_stride, int num_kv_heads, int head_dim,
                  int block_size, void* stream);
 
+/* ---- block tables and slots on the device ----------------------------------------------------
+ * No counterpart in the reference.  The free list is a ring of int32: ring[0] the place of its first
+ * entry, ring[1] the number of its entries, ring[2 .. 2 + ring_size) block ids.
+ *
+ * ti_reserve_slots: sequence i (table row row_index[i], NULL: i; negative: padding) gets counts[i] new
+ * tokens behind the lens[row] cached ones.  Negative entries of the row that they fall in take blocks
+ * from the front of the ring, sequence by sequence in ascending order; the first sequence that needs
+ * more than what is left gets none, nor does any later one that needs a block.  granted[i] = counts[i]
+ * or 0; cu_seqlens[num_seqs + 1] = running sum of the counts.  The packed tokens' slots (block *
+ * block_size + offset, -1 without room) and positions (lens[row] + pos_offset[row] (NULL: 0) + index)
+ * go to slot_mapping and positions [capacity]; places behind them get -1 and 0.  parents [capacity] (NULL:
+ * none): index of each token's parent within its sequence, earlier than itself, negative for a root;
+ * positions then follow the depth, and masks [capacity, mask_words] receive bits of the ancestors and
+ * the token itself.  A row beyond num_rows or named before, a length out of the row, a count below 0, a
+ * parent that is no earlier node, a node without a bit, more tokens than capacity or a ring out of its
+ * bounds raise TI_DEVERR_BAD_INPUT (no blocks, no bits, no places for these).  At most 4096 sequences;
+ * with row_index at most 32768 rows.
+ *
+ * ti_release_blocks: entries of the row behind ceil(keep_lens[i] / block_size) become -1, their blocks
+ * go to the ring's end, row by row in ascending order.  If the ring has no room for all of them nothing
+ * changes (TI_DEVERR_BAD_INPUT). */
+int ti_reserve_slots(int32_t* block_tables, int64_t bt_stride, int num_rows, int max_blocks_per_seq,
+                     int block_size, const int32_t* row_index, const int32_t* lens,
+                     const int32_t* pos_offset, const int32_t* counts, int num_seqs, int32_t* ring,
+                     int64_t ring_size, int64_t* slot_mapping, int32_t* positions, int64_t capacity,
+                     int32_t* cu_seqlens, int32_t* granted, const int32_t* parents, int32_t* masks,
+                     int mask_words, void* stream);
+int ti_release_blocks(int32_t* block_tables, int64_t bt_stride, int num_rows, int max_blocks_per_seq,
+                      int block_size, const int32_t* row_index, const int32_t* keep_lens, int num_seqs,
+                      int32_t* ring, int64_t ring_size, void* stream);
+
+/* ---- drafted trees -----------------------------------------------------------------------------
+ * No counterpart in the reference.  Sequence i's nodes are rows cu_seqlens[i] .. cu_seqlens[i+1]-1; their
+ * K and V are in the pool at positions context_lens[i] + node of table row row_index[i] (NULL: i).
+ *
+ * ti_tree_attention: out / q [num_tokens, num_heads, head_dim] (token strides in elements, multiples of
+ * 8, 16-byte aligned); node t attends to the context_lens[i] cached tokens and to the nodes whose bits
+ * row t of masks [num_tokens, mask_words] has (bit b of word w: node 32 w + b; mask_words 0: the nodes
+ * up to itself).  lse (float32 [num_tokens, num_heads] or NULL) = ln of the row's sum of exp(q.k /
+ * sqrt(head_dim)).  A node that sees nothing gets zeros and -inf; table entries that are negative or >=
+ * num_blocks hold no tokens; keys that a node does not see do not reach it whatever they hold; rows
+ * behind cu_seqlens[num_seqs] are left as they were.  At most 16 query heads per kv head, head_dim 64
+ * or 128, block_size 16, at most 4096 sequences.  The workspace (ti_tree_attention_workspace_bytes,
+ * 16-byte aligned) must be zero before its first call, and every call leaves its counters zero; calls
+ * that share it must not overlap on the GPU.
+ *
+ * ti_tree_accept: the path from node 0 to the first later node c with parents[c] = the current one and
+ * tokens[c] = targets[current], and on, for at most max_path (<= 1024) nodes.  num [num_seqs] = its
+ * length; path, out_tokens [num_seqs, max_path] = its nodes and the targets at them (-1 behind).  In every
+ * layer of key_cache / value_cache [num_layers, num_blocks, num_kv_heads, block_size, head_dim] (elements
+ * of elem_bytes, rows of a multiple of 16 bytes) the j-th node's values move from slot_mapping[its row]
+ * to out_slots[cu_seqlens[i] + j] (the same array: in place; otherwise slots that hold none of the
+ * nodes; negative: skipped; outside the pool: skipped, TI_DEVERR_BAD_INPUT).  seq_lens (or NULL):
+ * seq_lens[row_index[i]] (NULL: i; of num_rows) += num[i]. */
+size_t ti_tree_attention_workspace_bytes(int num_heads, int num_kv_heads, int head_dim);
+int ti_tree_attention(void* out, int64_t out_tok_stride, float* lse, const void* q, int64_t q_tok_stride,
+                      const void* k_cache, const void* v_cache, int64_t num_blocks,
+                      const int32_t* block_tables, int64_t bt_stride, int num_rows,
+                      int max_blocks_per_seq, const int32_t* row_index, const int32_t* context_lens,
+                      const int32_t* cu_seqlens, int num_seqs, int num_tokens, const int32_t* masks,
+                      int mask_words, int num_heads, int num_kv_heads, int head_dim, int block_size,
+                      int dtype, void* workspace, size_t workspace_bytes, void* stream);
+int ti_tree_accept(void* key_cache, void* value_cache, int num_layers, int64_t num_blocks,
+                   int num_kv_heads, int head_dim, int block_size, int elem_bytes,
+                   const int32_t* tokens, const int32_t* parents, const int32_t* targets,
+                   const int32_t* cu_seqlens, int num_seqs, int num_tokens,
+                   const int64_t* slot_mapping, const int64_t* out_slots, int32_t* num, int32_t* path,
+                   int32_t* out_tokens, int max_path, int32_t* seq_lens, const int32_t* row_index,
+                   int num_rows, void* stream);
+
+/* ---- sampler: temperature / top-k / top-p / min-p / draw, in 64 bits ---------------------------
+ * No counterpart in the reference (ti_sample is its sampler).  Row r of logits [rows, vocab] (leading
+ * dimension ld, bf16 / fp16 / fp32): z = x / temperatures[r]; in the order of descending z (equal: the
+ * lower index) the kept tokens are a prefix: down to the top_ks[r]-th and all equal to it (<= 0 or >=
+ * vocab: all), of these the shortest whose probability exceeds top_ps[r] (>= 1: all), of these those
+ * with exp(z - max z) >= min(min_ps[r], 1).  out_tokens[r] = the first whose cumulative probability
+ * among the kept exceeds uniforms[r]; logprobs[r] = ln of its probability among them.  Temperature <= 0
+ * or NaN: the first of the largest, 0.  NaN counts as -inf, which is never drawn; without any other value
+ * -1 and -inf.  +inf: equally likely, all others impossible.  top_ks, top_ps, min_ps, logprobs may be
+ * NULL.  At most 2^24 tokens. */
+int ti_sample_ex(const void* logits, int64_t ld, int dtype, int rows, int vocab,
+                 const float* temperatures, const int32_t* top_ks, const float* top_ps,
+                 const float* min_ps, const float* uniforms, int32_t* out_tokens, float* logprobs,
+                 void* stream);
+
 #ifdef __cplusplus
 }
 #endif

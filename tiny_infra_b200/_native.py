@@ -74,6 +74,15 @@ SIGNATURES: dict[str, tuple] = {
                                        I32, I32, I32, I32, I32, I32, P, SZ, P]),
     "ti_kv4_evict": (I32, [P, P, I32, I64, P, I64, P, I64, P, P, I32, I32, I32, I32, I32, P, I64,
                            I32, I32, I32, P]),
+    "ti_reserve_slots": (I32, [P, I64, I32, I32, I32, P, P, P, P, I32, P, I64, P, P, I64, P, P, P, P,
+                               I32, P]),
+    "ti_release_blocks": (I32, [P, I64, I32, I32, I32, P, P, I32, P, I64, P]),
+    "ti_tree_attention_workspace_bytes": (SZ, [I32, I32, I32]),
+    "ti_tree_attention": (I32, [P, I64, P, P, I64, P, P, I64, P, I64, I32, I32, P, P, P, I32, I32, P,
+                                I32, I32, I32, I32, I32, I32, P, SZ, P]),
+    "ti_tree_accept": (I32, [P, P, I32, I64, I32, I32, I32, I32, P, P, P, P, I32, I32, P, P, P, P, P,
+                             I32, P, P, I32, P]),
+    "ti_sample_ex": (I32, [P, I64, I32, I32, I32, P, P, P, P, P, P, P, P]),
 }
 
 TI_EPI_STORE, TI_EPI_SWIGLU, TI_EPI_RESIDUAL, TI_EPI_ARGMAX = 0, 1, 2, 3

@@ -21,6 +21,7 @@ import numpy as np
 import torch
 
 from . import _native as N
+from . import kv4
 
 
 def effective_top_k(top_k: int, vocab: int) -> int:
@@ -80,6 +81,61 @@ def launch_sample(logits: torch.Tensor, params_dev: torch.Tensor, out_tokens: to
         pd[0].data_ptr(), pd[1].data_ptr(), pd[2].data_ptr(), pd[3].data_ptr(),
         out_tokens.data_ptr(), slots.data_ptr() if slots is not None else None,
         seq_len.data_ptr() if seq_len is not None else None, seq_inc, stream))
+
+
+def _row_values(name: str, t: torch.Tensor | None, dtype, rows: int) -> None:
+    if t is not None and (t.dtype != dtype or not t.is_contiguous() or t.numel() != rows):
+        raise RuntimeError(f"{name} must be contiguous {str(dtype)[6:]} [rows]")
+
+
+def sample(logits: torch.Tensor, temperatures: torch.Tensor, uniforms: torch.Tensor, *,
+           top_ks: torch.Tensor | None = None, top_ps: torch.Tensor | None = None,
+           min_ps: torch.Tensor | None = None, out: torch.Tensor | None = None,
+           logprobs: torch.Tensor | None = None) -> torch.Tensor:
+    """A token per row of ``logits`` [rows, V] (bf16, fp16 or float32, any row stride), every row by its
+    own parameters and in 64 bits; returns ``out`` (int32 [rows], made if not given).
+
+    z = x / temperature, and in the order of descending z (equal ones: the lower index first) a row
+    keeps the tokens down to the ``top_ks``-th and all that equal it (int32; <= 0 or >= V: all), of these
+    the shortest prefix whose probability exceeds ``top_ps`` (>= 1: all), of these the ones at least
+    ``min_ps`` times as probable as the likeliest (<= 0: all; 1 and more: those that equal it).  The token
+    is the first whose cumulative probability among the kept ones exceeds ``uniforms`` (in [0, 1)).
+    ``logprobs`` (float32 [rows]) receives the log of its probability among them.  A temperature of 0 (or
+    below, or NaN) takes the first of the largest values, log probability 0.
+
+    NaN counts as -inf, which is never drawn; a row of nothing else gives -1 (log probability -inf).
+    With +inf among the values, those are equally likely and all others impossible.
+
+    ``launch_sample`` above resolves the reference's batch rules and weighs in 32 bits; here a draw next
+    to the border of two tokens falls as in exact arithmetic."""
+    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.numel() and logits.stride(1) != 1):
+        raise RuntimeError("logits must be [rows, vocab] with contiguous rows")
+    rows, vocab = logits.shape
+    dev = logits.get_device()
+    if dev < 0:
+        raise RuntimeError("logits must be a CUDA tensor")
+    code = N.dtype_code(logits.dtype)
+    if out is None:
+        out = torch.empty(rows, dtype=torch.int32, device=logits.device)
+    for name, t, dtype in (("temperatures", temperatures, torch.float32),
+                           ("uniforms", uniforms, torch.float32), ("top_ks", top_ks, torch.int32),
+                           ("top_ps", top_ps, torch.float32), ("min_ps", min_ps, torch.float32),
+                           ("out", out, torch.int32), ("logprobs", logprobs, torch.float32)):
+        if t is not None:
+            if t.get_device() != dev:
+                raise RuntimeError(f"{name} must be on the logits' device")
+            _row_values(name, t, dtype, rows)
+    if rows == 0:
+        return out
+    if vocab == 0:
+        raise RuntimeError("logits have no columns")
+    ptr = kv4._ptr
+    with kv4._on(dev):
+        N.check(N.lib().ti_sample_ex(
+            logits.data_ptr(), logits.stride(0), code, rows, vocab, temperatures.data_ptr(),
+            ptr(top_ks), ptr(top_ps), ptr(min_ps), uniforms.data_ptr(), out.data_ptr(),
+            ptr(logprobs), kv4._stream(dev)))
+    return out
 
 
 def request_uniforms(requests) -> list[float]:
