@@ -20,10 +20,22 @@ import functools
 import torch
 
 from . import _native as N
-from .kv4 import (_CODE, _HALF, _device, _fail, _head_sums, _index, _on, _out_rows, _ptr, _rows, _stream,
-                  _table, _workspace)
+from .kv4 import (_CODE, _HALF, _cuda, _device, _fail, _head_sums, _index, _on, _out_rows, _ptr, _rows, _stream,
+                  _table)
 
 BLOCK = 16
+_COUNTERS = 4096                        # bytes at a workspace's front that have to be zero before its first call
+_ws = N.Workspace()
+
+
+def _workspace(dev: int, nbytes: int, stream: int) -> torch.Tensor:
+    """Scratch with zeroed counters, one per (device, stream); inside a stream capture one of the graph's own,
+    whose counters the graph zeroes itself, so graphs that replay at the same time do not share it."""
+    if torch._C._cuda_isCurrentStreamCapturing():
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=_cuda(dev))
+        ws[:_COUNTERS].zero_()
+        return ws
+    return _ws.get(_cuda(dev), nbytes, stream)
 
 
 @functools.lru_cache(maxsize=256)
