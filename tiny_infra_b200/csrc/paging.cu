@@ -26,6 +26,8 @@ constexpr int kMaxSeqs = 4096;
 constexpr int kMaxRows = 32768;          // with row_index: a word of shared memory each
 constexpr int64_t kFusedTokens = 65536;
 constexpr int kExpand = 256;             // threads of the second launch
+constexpr int kAhead = 8;                // table columns (times 32) that a warp has in flight
+constexpr int kTokens = 4;               // neighbouring tokens of a thread, in the second launch
 
 struct Params {
   int32_t *tables, *ring;
@@ -34,12 +36,17 @@ struct Params {
   int64_t* slots;
   int32_t *positions, *cu, *granted, *masks;
   int64_t capacity, ring_size;
-  int seqs, rows, cols, block, mask_words, fused;
+  int seqs, rows, cols, block, shift, mask_words, fused;   // shift: log2 of the block size, or -1
 };
 
-// Dynamic shared memory: needs [seqs], token offsets [seqs + 1], owners [rows] (with row_index).
+__device__ __forceinline__ int64_t block_of(const Params& p, int64_t pos) {
+  return p.shift >= 0 ? pos >> p.shift : pos / p.block;
+}
+
+// Dynamic shared memory: needs [seqs], their sums [seqs], token offsets [seqs + 1], owners [rows] (with
+// row_index).
 static size_t smem_bytes(int seqs, int rows, bool indexed) {
-  return ((size_t)2 * seqs + 1 + (indexed ? rows : 0)) * 4;
+  return ((size_t)3 * seqs + 1 + (indexed ? rows : 0)) * 4;
 }
 
 __device__ __forceinline__ void st_peer_i32(uint32_t addr, int v) {
@@ -102,9 +109,9 @@ __device__ __forceinline__ void expand(const Params& p, const int* s_cu, int64_t
       const int len = p.lens[row];
       pos = (int64_t)len + (p.pos_offset ? p.pos_offset[row] : 0) + j;
       if (__ldcg(p.granted + lo) > 0) {
-        const int at = len + j;                   // (granted: within the row)
-        const int b = __ldcg(p.tables + (int64_t)row * p.bt_stride + at / p.block);
-        if (b >= 0) slot = (int64_t)b * p.block + at % p.block;
+        const int at = len + j, col = (int)block_of(p, at);      // (granted: within the row)
+        const int b = __ldcg(p.tables + (int64_t)row * p.bt_stride + col);
+        if (b >= 0) slot = (int64_t)b * p.block + (at - col * p.block);
       }
     }
   }
@@ -140,7 +147,8 @@ __global__ void __launch_bounds__(kThreads, 1) reserve_kernel(const __grid_const
   extern __shared__ int s_dyn[];
   __shared__ long long warp_sums[32];
   __shared__ int s_stop;
-  int* s_need = s_dyn;                            // blocks each sequence needs, then the sums before it
+  int* s_raw = s_dyn;                             // blocks each sequence needs (negative: not to be served)
+  int* s_need = s_raw + p.seqs;                   // the sums before it
   int* s_cu = s_need + p.seqs;
   int* s_owner = s_cu + p.seqs + 1;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -182,17 +190,20 @@ __global__ void __launch_bounds__(kThreads, 1) reserve_kernel(const __grid_const
     const bool ok = whole_row(i, row, n, len);
     if (ok && n > 0) {
       const int32_t* t = p.tables + (int64_t)row * p.bt_stride;
-      const int last = (len + n - 1) / p.block;
-      for (int c0 = len / p.block; c0 <= last; c0 += 32) {
-        const int c = c0 + lane;
-        need += __popc(__ballot_sync(0xffffffffu, c <= last && __ldcg(t + min(c, last)) < 0));
+      const int last = (int)block_of(p, len + n - 1);
+      for (int c0 = (int)block_of(p, len); c0 <= last; c0 += 32 * kAhead) {
+        int id[kAhead];                            // (kAhead loads in flight)
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) id[a] = c0 + 32 * a + lane <= last ? __ldcg(t + c0 + 32 * a + lane) : 0;
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) need += __popc(__ballot_sync(0xffffffffu, id[a] < 0));
       }
     }
     bad |= !ok && row >= 0 && n > 0;              // (a negative row is padding)
     // (the top bit: not to be served; it stays out of the sums)
     const int word = ok ? need : (int)0x80000000;
     for (uint32_t c = lane; c < ctas; c += 32)
-      st_peer_i32(map_peer(smem_u32(s_need + i), c), word);
+      st_peer_i32(map_peer(smem_u32(s_raw + i), c), word);
   }
   if (bad && lane == 0) raise_device_error(TI_DEVERR_BAD_INPUT);
   int head = p.ring[0], have = p.ring[1];
@@ -203,56 +214,47 @@ __global__ void __launch_bounds__(kThreads, 1) reserve_kernel(const __grid_const
   }
   if (ctas > 1) cluster_sync(); else __syncthreads();
 
-  // ---- sums, by every CTA for itself; needs and counts go to registers first, the sums replace them
-  constexpr int kEach = (kMaxSeqs + kThreads - 1) / kThreads;
-  int need_of[kEach], n_of[kEach];
-#pragma unroll
-  for (int k = 0; k < kEach; ++k) {
-    const int i = tid + k * kThreads;
-    need_of[k] = i < p.seqs ? s_need[i] : 0;
-    n_of[k] = i < p.seqs ? s_cu[i] : 0;
-    if (i < p.seqs) s_need[i] = max(need_of[k], 0);
-  }
+  // ---- sums, by every CTA for itself
+  for (int i = tid; i < p.seqs; i += kThreads) s_need[i] = max(s_raw[i], 0);
   __syncthreads();
   const int total = exclusive_sums(s_need, p.seqs, warp_sums);
   const int tokens = exclusive_sums(s_cu, p.seqs, warp_sums);
   if (tid == 0) s_cu[p.seqs] = tokens;
-#pragma unroll
-  for (int k = 0; k < kEach; ++k) {
-    const int i = tid + k * kThreads;
-    if (i < p.seqs && need_of[k] > 0 && s_need[i] + need_of[k] > have) atomicMin(&s_stop, i);
-  }
+  for (int i = tid; i < p.seqs; i += kThreads)
+    if (s_raw[i] > 0 && (long long)s_need[i] + s_raw[i] > have) atomicMin(&s_stop, i);
   __syncthreads();
   const int stop = s_stop;                        // the first sequence that does not fit
-#pragma unroll
-  for (int k = 0; k < kEach; ++k) {
-    const int i = tid + k * kThreads;
-    if (i < p.seqs) {
-      const bool served = need_of[k] == 0 || (need_of[k] > 0 && i < stop);
-      if (rank == 0) {
-        p.granted[i] = served ? n_of[k] : 0;
-        p.cu[i] = s_cu[i];
-      }
+  if (rank == 0)
+    for (int i = tid; i < p.seqs; i += kThreads) {
+      const bool served = s_raw[i] == 0 || (s_raw[i] > 0 && i < stop);
+      p.granted[i] = served ? s_cu[i + 1] - s_cu[i] : 0;
+      p.cu[i] = s_cu[i];
     }
-  }
   // ---- the rows that are served
   for (int i = warp * (int)ctas + (int)rank; i < stop; i += kWarps * (int)ctas) {
-    const int base = s_need[i], next = i + 1 < p.seqs ? s_need[i + 1] : total;
-    if (next == base) continue;
+    if (s_raw[i] <= 0) continue;
+    const int base = s_need[i], next = base + s_raw[i];
     const int row = p.row_index ? p.row_index[i] : i, len = p.lens[row];
-    const int n = s_cu[i + 1] - s_cu[i], last = (len + n - 1) / p.block;
+    const int n = s_cu[i + 1] - s_cu[i], last = (int)block_of(p, len + n - 1);
     int32_t* t = p.tables + (int64_t)row * p.bt_stride;
     int taken = base;
-    for (int c0 = len / p.block; c0 <= last && taken < next; c0 += 32) {
-      const int c = c0 + lane;
-      const bool want = c <= last && __ldcg(t + min(c, last)) < 0;
-      const uint32_t all = __ballot_sync(0xffffffffu, want);
-      if (want) {
+    for (int c0 = (int)block_of(p, len); c0 <= last && taken < next; c0 += 32 * kAhead) {
+      int id[kAhead], from[kAhead];
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) id[a] = c0 + 32 * a + lane <= last ? __ldcg(t + c0 + 32 * a + lane) : 0;
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) {
+        const uint32_t all = __ballot_sync(0xffffffffu, id[a] < 0);
         int64_t at = (int64_t)head + taken + __popc(all & ((1u << lane) - 1));
         if (at >= p.ring_size) at -= p.ring_size;
-        __stcg(t + c, p.ring[2 + at]);
+        from[a] = id[a] < 0 ? (int)at : -1;
+        taken += __popc(all);
       }
-      taken += __popc(all);
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) id[a] = from[a] >= 0 ? p.ring[2 + from[a]] : 0;
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a)
+        if (from[a] >= 0) __stcg(t + c0 + 32 * a + lane, id[a]);
     }
   }
   if (rank == 0 && tid == 0) {
@@ -273,15 +275,44 @@ __global__ void __launch_bounds__(kThreads, 1) reserve_kernel(const __grid_const
     expand(p, s_cu, t);
 }
 
+// Four neighbouring tokens of one sequence, whose entry is looked up where the block changes; anything else
+// (the end of a sequence among them, trees) token by token.
+__device__ __forceinline__ void expand_run(const Params& p, const int* s_cu, int64_t t) {
+  int lo = 0, hi = p.seqs - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (s_cu[mid] <= t) lo = mid; else hi = mid - 1;
+  }
+  const int row = p.seqs == 0 ? -1 : p.row_index ? p.row_index[lo] : lo;
+  if (p.parents || t + kTokens > p.capacity || row < 0 || row >= p.rows || t + kTokens > s_cu[lo + 1] ||
+      __ldcg(p.granted + lo) == 0) {
+    for (int64_t i = t; i < min(t + kTokens, p.capacity); ++i) expand(p, s_cu, i);
+    return;
+  }
+  const int at = p.lens[row] + (int)(t - s_cu[lo]), pos = at + (p.pos_offset ? p.pos_offset[row] : 0);
+  const int32_t* table = p.tables + (int64_t)row * p.bt_stride;
+  int col = (int)block_of(p, at), off = at - col * p.block, b = __ldcg(table + col);
+#pragma unroll
+  for (int i = 0; i < kTokens; ++i) {
+    if (off == p.block) {
+      off = 0;
+      b = __ldcg(table + ++col);
+    }
+    p.slots[t + i] = b >= 0 ? (int64_t)b * p.block + off : -1;
+    p.positions[t + i] = pos + i;
+    ++off;
+  }
+}
+
 __global__ void __launch_bounds__(kExpand) expand_kernel(const __grid_constant__ Params p) {
   extern __shared__ int s_cu_dyn[];
   pdl_wait();
   pdl_launch_dependents();
   for (int i = threadIdx.x; i <= p.seqs; i += kExpand) s_cu_dyn[i] = p.cu[i];
   __syncthreads();
-  for (int64_t t = (int64_t)blockIdx.x * kExpand + threadIdx.x; t < p.capacity;
-       t += (int64_t)gridDim.x * kExpand)
-    expand(p, s_cu_dyn, t);
+  for (int64_t t = ((int64_t)blockIdx.x * kExpand + threadIdx.x) * kTokens; t < p.capacity;
+       t += (int64_t)gridDim.x * kExpand * kTokens)
+    expand_run(p, s_cu_dyn, t);
 }
 
 // p.counts: the tokens that each row keeps.
@@ -312,9 +343,12 @@ __global__ void __launch_bounds__(kThreads, 1) release_kernel(const __grid_const
     int n = 0;
     if (ok) {
       const int32_t* t = p.tables + (int64_t)row * p.bt_stride;
-      for (int64_t c0 = ((int64_t)p.counts[i] + p.block - 1) / p.block; c0 < p.cols; c0 += 32) {
-        const int64_t c = c0 + lane;
-        n += __popc(__ballot_sync(0xffffffffu, c < p.cols && __ldcg(t + min(c, (int64_t)p.cols - 1)) >= 0));
+      for (int64_t c0 = block_of(p, (int64_t)p.counts[i] + p.block - 1); c0 < p.cols; c0 += 32 * kAhead) {
+        int id[kAhead];
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) id[a] = c0 + 32 * a + lane < p.cols ? __ldcg(t + c0 + 32 * a + lane) : -1;
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) n += __popc(__ballot_sync(0xffffffffu, id[a] >= 0));
       }
     }
     bad |= !ok && row >= 0;
@@ -334,17 +368,21 @@ __global__ void __launch_bounds__(kThreads, 1) release_kernel(const __grid_const
     const int row = p.row_index ? p.row_index[i] : i;
     int32_t* t = p.tables + (int64_t)row * p.bt_stride;
     int done = base;
-    for (int64_t c0 = ((int64_t)p.counts[i] + p.block - 1) / p.block; c0 < p.cols && done < next; c0 += 32) {
-      const int64_t c = c0 + lane;
-      const int id = c < p.cols ? __ldcg(t + c) : -1;
-      const uint32_t all = __ballot_sync(0xffffffffu, id >= 0);
-      if (id >= 0) {
-        int64_t at = (int64_t)head + have + done + __popc(all & ((1u << lane) - 1));
-        while (at >= p.ring_size) at -= p.ring_size;
-        p.ring[2 + at] = id;
-        __stcg(t + c, -1);
+    for (int64_t c0 = block_of(p, (int64_t)p.counts[i] + p.block - 1); c0 < p.cols && done < next; c0 += 32 * kAhead) {
+      int id[kAhead];
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) id[a] = c0 + 32 * a + lane < p.cols ? __ldcg(t + c0 + 32 * a + lane) : -1;
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) {
+        const uint32_t all = __ballot_sync(0xffffffffu, id[a] >= 0);
+        if (id[a] >= 0) {
+          int64_t at = (int64_t)head + have + done + __popc(all & ((1u << lane) - 1));
+          while (at >= p.ring_size) at -= p.ring_size;
+          p.ring[2 + at] = id[a];
+          __stcg(t + c0 + 32 * a + lane, -1);
+        }
+        done += __popc(all);
       }
-      done += __popc(all);
     }
   }
   if (ctas > 1) cluster_sync(); else __syncthreads();    // every CTA has read the ring's state
@@ -366,6 +404,13 @@ static int raise_limit(K kern, std::atomic<uint64_t>& ready) {
   }
   ready.fetch_or(bit, std::memory_order_release);
   return TI_OK;
+}
+
+static int shift_of(int block) {
+  if (block <= 0 || (block & (block - 1))) return -1;
+  int s = 0;
+  while ((1 << s) < block) ++s;
+  return s;
 }
 
 static int check_sizes(const Params& p) {
@@ -402,7 +447,7 @@ extern "C" int ti_reserve_slots(int32_t* block_tables, int64_t bt_stride, int nu
     return set_error(TI_ERR_INVALID_ARGUMENT, "reserve slots: null pointer or bad size");
   paging::Params p{block_tables, ring, bt_stride, row_index, lens, counts, pos_offset, parents,
                    slot_mapping, positions, cu_seqlens, granted, masks, capacity, ring_size,
-                   num_seqs, num_rows, max_blocks_per_seq, block_size, mask_words,
+                   num_seqs, num_rows, max_blocks_per_seq, block_size, paging::shift_of(block_size), mask_words,
                    capacity <= paging::kFusedTokens};
   if (int rc = paging::check_sizes(p)) return rc;
   static std::atomic<uint64_t> ready{0};
@@ -413,7 +458,7 @@ extern "C" int ti_reserve_slots(int32_t* block_tables, int64_t bt_stride, int nu
                                 paging::smem_bytes(num_seqs, num_rows, row_index), s, dim3(ctas), p))
     return rc;
   if (p.fused) return TI_OK;
-  const unsigned grid = (unsigned)std::min<int64_t>((capacity + paging::kExpand - 1) / paging::kExpand, 148 * 8);
+  const unsigned grid = (unsigned)std::min<int64_t>((capacity + paging::kExpand * paging::kTokens - 1) / (paging::kExpand * paging::kTokens), 148 * 8);
   return launch_kernel("reserve tokens launch", paging::expand_kernel, dim3(grid), dim3(paging::kExpand),
                        (size_t)(num_seqs + 1) * 4, s, 1, p);
 }
@@ -437,6 +482,7 @@ extern "C" int ti_release_blocks(int32_t* block_tables, int64_t bt_stride, int n
   p.rows = num_rows;
   p.cols = max_blocks_per_seq;
   p.block = block_size;
+  p.shift = paging::shift_of(block_size);
   if (int rc = paging::check_sizes(p)) return rc;
   static std::atomic<uint64_t> ready{0};
   if (int rc = paging::raise_limit(paging::release_kernel, ready)) return rc;
