@@ -167,7 +167,7 @@ extern "C" int ti_tree_accept(void* key_cache, void* value_cache, int num_layers
   p.total = num_tokens;
   const int64_t items = (int64_t)num_layers * 2 * p.per_layer;
   // a CTA walks its tree again: as few as still fill the GPU
-  const int64_t want = std::max<int64_t>(1, (148 * 6 + num_seqs - 1) / num_seqs);
+  const int64_t want = std::max<int64_t>(1, (148 * 12 + num_seqs - 1) / num_seqs);
   const unsigned y = (unsigned)std::min<int64_t>(std::min<int64_t>((items + accept::kThreads - 1) / accept::kThreads, want), 65535);
   return launch_kernel_cl("tree accept launch", accept::accept_kernel, dim3((unsigned)num_seqs, y),
                           dim3(accept::kThreads), (size_t)max_path * 20, reinterpret_cast<cudaStream_t>(stream),

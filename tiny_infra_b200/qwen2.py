@@ -16,6 +16,8 @@ A cache with ``kv_bits=4`` (``KVCacheManager``) runs the same layers on the 4-bi
 (+bias) -> RoPE and quantised append -> 4-bit paged attention (prefill: the ragged prefill
 attention on the codes); when the cache tracks attention weights, each decode token, and the last
 ``OBSERVE`` tokens of a prefill chunk, add theirs to the cached tokens' totals.
+A batch with ``tree_masks`` (``speculative.TreeDecoder`` makes them; 16-bit cache) holds drafted trees:
+the layers attend with ``tree.attention``.
 
 with the residual stream kept in float32 (the reference keeps it in the model dtype; float32
 is closer to the float32 oracle).  The lm_head runs only on the rows whose logits are needed
@@ -29,7 +31,7 @@ import numpy as np
 import torch
 
 from . import _native as N
-from . import kv4
+from . import kv4, tree
 from .config import QwenConfig
 
 GATE_UP_GROUP = 8           # gate/up weight rows interleaved 8 gate, 8 up (TI_EPI_SWIGLU16)
@@ -62,6 +64,7 @@ class PackedBatch:
     last_rows: torch.Tensor        # int64 [nseq] row of each sequence's last token
     kv4_plan: kv4.PrefillPlan | None = None   # prefill layout on a 4-bit cache
     observe: tuple | None = None   # rows, slots, lengths of the chunks' last OBSERVE tokens
+    tree_masks: torch.Tensor | None = None    # int32 [T, words]: the tokens are drafted trees (``tree``)
 
 
 class Qwen2ForCausalLM:
@@ -374,6 +377,10 @@ class Qwen2ForCausalLM:
                         bt.data_ptr(), bt.stride(0), pb.seq_slots.data_ptr(), pb.ctx_lens.data_ptr(),
                         pb.num_seqs, NH, KVH, D, kv_cache.block_size, maxb, dt, ws.data_ptr(),
                         ws.numel(), plan.data_ptr(), N.TI_ATTN_EARLY_KV if early else 0, stream))
+                elif pb.tree_masks is not None:
+                    tree.attention(attn[:T].view(T, NH, D), qkv[:T, :NH * D].view(T, NH, D), kc, vc, bt,
+                                   pb.start_pos, pb.cu_seqlens, masks=pb.tree_masks,
+                                   row_index=pb.seq_slots)
                 else:
                     N.check(lib.ti_paged_prefill_attention(
                         attn.data_ptr(), NH * D, qkv.data_ptr(), QKV, kc.data_ptr(), vc.data_ptr(), nb,
