@@ -22,14 +22,15 @@
 //                keys, on fixed-point weights, by rank 0 alone.
 // All sums have a fixed order: the same token on every run.
 //
-// Bound, 151936 tokens: 256 rows of everything the whole vocabulary can ask (fp32, 156 MB) take 218 us: one
+// Bound, 151936 tokens: 256 rows of everything the whole vocabulary can ask (fp32, 156 MB) take 231 us: one
 // pass from HBM (26 us), the histogram's shared-memory atomics (42 us; 4.6 clocks a warp instruction), the
 // polynomials (72 us; 14 double-precision operations an element at 64 a clock and SM, 8 clocks a warp), and
-// 20 us for the places.  256 rows of temperature 0.7, top-k 20, top-p 0.9 (bf16, 78 MB) take 48: a pass
-// from HBM, one from L2, 7 us to the token.  One such row takes 15: a chain of passes, cluster barriers
-// and code that is run for the first time.  Measured on the way, one row: exponentials and scans inlined for
-// each use 26 us, every CTA collecting into rank 0's list 22 us; 256 rows: radix selects 5200 us,
-// branches for the sums above the intervals 880 us (fp32) instead of masks 221.
+// 15 us for the places.  256 rows of temperature 0.7, top-k 20, top-p 0.9 (bf16, 78 MB) take 62 (48 with one
+// CTA a row): a pass from HBM, one from L2, 7 us to the token.  One such row takes 14: a chain of passes,
+// cluster barriers and code that is run for the first time.  Measured on the way, one row: exponentials and
+// scans inlined for each use 26 us, every CTA collecting into rank 0's list 22 us; 256 rows: radix selects
+// 5200 us, branches for the sums above the intervals 880 us (fp32) instead of masks 221; collecting by the
+// first eighth's bound in the first pass 86 us instead of 62 (top-k 20).
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -188,7 +189,7 @@ struct Shared {
   u64 part64[kWarps];
   unsigned part_n[kWarps];
   float fpart[kWarps], fpart2[kWarps], kth, kth2;
-  int ipart[kWarps], k_bin;
+  int ipart[kWarps], k_bin, edge[4];
   uint32_t key;
   int found, index;
   u64 acc, upto;
@@ -742,43 +743,45 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       // less one.  So each bin's true sum is between (1 - d) and (1 + 2 d) times what is held, and so are
       // sums over bins; the last bin has the tokens below the range too, its sum may be next to nothing.
       const double d = 1.0 / ((double)p.quanta * 0.98 - 1.0);
+      double sum[E];                               // down to each of this thread's bins
       {
-        double v[E], own = 0, most = exp2(-(double)(tid * E) * width) / (double)p.quanta;
+        double own = 0, most = exp2(-(double)(tid * E) * width) / (double)p.quanta;
         const double ratio = exp2(-width);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-          v[e] = (double)sh.hist[tid * E + e] * most;
-          own += v[e];
+          sum[e] = own += (double)sh.hist[tid * E + e] * most;
           most *= ratio;
         }
-        double run = block_scan(own, sh.scan_d) - own;
+        const double before = block_scan(own, sh.scan_d) - own;
 #pragma unroll
-        for (int e = 0; e < E; ++e) sh.prefix[tid * E + e] = run += v[e];
+        for (int e = 0; e < E; ++e) sh.prefix[tid * E + e] = sum[e] += before;
+        if (tid < 4) sh.edge[tid] = kBins - 1;
       }
       __syncthreads();
       auto upto = [&](int b) { return b < 0 ? 0.0 : sh.prefix[b]; };
       // Bins in which the sum can first exceed q of the kept one, when what is kept ends in bins keep_a + 1 ..
       // keep_b: s(b) > q s(end) is (1 - q) s(b) > q (s(end) - s(b)), the difference a sum of bins too, so
-      // that a place near the end is known as well as one near the beginning.  Binary searches, by every
-      // thread alike.
+      // that a place near the end is known as well as one near the beginning.
       int keep_a = kBins - 1, keep_b = kBins - 1;
       const double last = sh.prefix[kBins - 1] - sh.prefix[kBins - 2];
-      auto search = [&](double q, double low_scale, double high_scale, double end) {
-        int lo = 0, hi = kBins - 1;
-#pragma unroll 1
-        while (lo < hi) {
-          const int mid = (lo + hi) >> 1;
-          const double s = sh.prefix[mid];
-          if ((1.0 - q) * s * low_scale > q * (end - s) * high_scale) hi = mid; else lo = mid + 1;
-        }
-        return lo;
-      };
-      auto bracket = [&](double q) {
+      auto bracket = [&](double q, int slot) {
         // (the last bin may hold nothing: it does not count towards a sum that is to be small)
-        const double end_a = upto(keep_a) - (keep_a == kBins - 1 ? last : 0.0);
+        const double end_a = upto(keep_a) - (keep_a == kBins - 1 ? last : 0.0), end_b = upto(keep_b);
+        const double up = 1.0 + 2.0 * d, down = 1.0 - d;
+        unsigned f = kBins - 1, l = kBins - 1;
+#pragma unroll
+        for (int e = E - 1; e >= 0; --e) {
+          if ((1.0 - q) * sum[e] * up > q * (end_a - sum[e]) * down) f = tid * E + e;
+          if ((1.0 - q) * sum[e] * down > q * (end_b - sum[e]) * up) l = tid * E + e;
+        }
+        f = __reduce_min_sync(0xffffffffu, f);
+        l = __reduce_min_sync(0xffffffffu, l);
+        if (lane == 0 && f < kBins - 1) atomicMin(&sh.edge[slot], (int)f);
+        if (lane == 0 && l < kBins - 1) atomicMin(&sh.edge[slot + 1], (int)l);
+        __syncthreads();
         Interval iv;
-        iv.first = search(q, 1.0 + 2.0 * d, 1.0 - d, end_a);
-        iv.last = max(search(q, 1.0 - d, 1.0 + 2.0 * d, upto(keep_b)), iv.first);
+        iv.first = sh.edge[slot];
+        iv.last = max(sh.edge[slot + 1], iv.first);
         return iv;
       };
       Interval ik, ip;
@@ -789,7 +792,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         keep_b = ik.first;
       }
       if (top_p < 1.f) {
-        ip = bracket(fmax(0.0, (double)top_p));
+        ip = bracket(fmax(0.0, (double)top_p), 0);
         keep_a = min(keep_a, ip.first - 1);
         keep_b = min(keep_b, ip.last);
       }
@@ -799,7 +802,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         keep_a = min(keep_a, max(b - 3, -1));
         keep_b = min(keep_b, min(b + 2, kBins - 1));
       }
-      const Interval iu = bracket(u);
+      const Interval iu = bracket(u, 2);
       __syncthreads();
       if (tid == 0) {
         // the union of the intervals, in order
@@ -826,27 +829,32 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         for (int a = 0; a <= out; ++a) { sh.iv[a].first = first[a]; sh.iv[a].last = end[a]; }
       }
       __syncthreads();
-      // an interval's values (lane 2 a: the largest, lane 2 a + 1: the smallest of its bins; lane 6: the
-      // largest of top-k's bin), and whether the tokens fit the list
-      if (warp == 0) {
-        const int m = sh.intervals;
-        if (lane < 2 * m || (lane == 6 && k > 0)) {
-          // keys lo < hi of neighbouring values whose bins are on either side of the edge before bin e
-          const int e = lane == 6 ? ik.first : lane & 1 ? sh.iv[lane >> 1].last + 1 : sh.iv[lane >> 1].first;
-          // (they are near best - e / per: two bins on either side, if that is right)
-          uint32_t lo = key_of(best - (float)(e + 2) / per), hi = key_of(fminf(best, best - (float)(e - 2) / per));
-          if (!(bin(value_of(lo)) >= e)) lo = key_of(-INFINITY);
-          if (bin(value_of(hi)) >= e) hi = key_of(best);
+      // an interval's values (warp 2 a: the largest, warp 2 a + 1: the smallest of its bins; warp 6: the
+      // largest of top-k's bin), and whether the tokens fit the list (warp 7)
+      const int m = sh.intervals;
+      if (warp < 2 * m || (warp == 6 && k > 0)) {
+        // keys lo < hi of neighbouring values whose bins are on either side of the edge before bin e, found in
+        // steps of 32 places at once; they are near best - e / per: two bins on either side, if that is right
+        const int e = warp == 6 ? ik.first : warp & 1 ? sh.iv[warp >> 1].last + 1 : sh.iv[warp >> 1].first;
+        uint32_t lo = key_of(best - (float)(e + 2) / per), hi = key_of(fminf(best, best - (float)(e - 2) / per));
+        if (!(bin(value_of(lo)) >= e)) lo = key_of(-INFINITY);
+        if (bin(value_of(hi)) >= e) hi = key_of(best);
 #pragma unroll 1
-          while (hi - lo > 1) {
-            const uint32_t mid = lo + (hi - lo) / 2;
-            if (bin(value_of(mid)) >= e) lo = mid; else hi = mid;
-          }
-          const float above = e == 0 ? best : value_of(lo), below = e == kBins ? -3.402823466e38f : value_of(hi);
-          if (lane == 6) sh.k_high = above;
-          else if (lane & 1) sh.iv[lane >> 1].low = below;
-          else sh.iv[lane >> 1].high = above;
+        while (hi - lo > 1) {
+          const uint32_t step = (hi - lo + 32) / 33, mid = min(lo + step * (uint32_t)(lane + 1), hi);
+          const uint32_t in = __ballot_sync(0xffffffffu, mid < hi && bin(value_of(mid)) >= e);
+          const int n = __popc(in);                // (they are the first n places)
+          const uint32_t next = lo + step * (uint32_t)(n + 1);
+          lo += step * (uint32_t)n;
+          hi = min(hi, next);
         }
+        if (lane == 0) {
+          const float above = e == 0 ? best : value_of(lo), below = e == kBins ? -3.402823466e38f : value_of(hi);
+          if (warp == 6) sh.k_high = above;
+          else if (warp & 1) sh.iv[warp >> 1].low = below;
+          else sh.iv[warp >> 1].high = above;
+        }
+      } else if (warp == 7) {
         float n = 0;
         for (int a = 0; a < m; ++a)
           for (int b = sh.iv[a].first + lane; b <= sh.iv[a].last; b += 32)
