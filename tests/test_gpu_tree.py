@@ -155,6 +155,9 @@ def test_reserve_parent_behind_its_child():
     from tiny_infra_b200 import _native as N
     rng = np.random.default_rng(8)
     tables, ring = _layout(rng, [4], 4, 3)
+    assert _reserve(tables, [4], [4], ring, 4, parents=[-1, 3, 1, 2])["pos"].tolist() == [4, 4, 5, 6]
+    assert _status() == N.TI_DEVERR_BAD_INPUT
+    tables, ring = _layout(rng, [4], 4, 3)
     got = _reserve(tables, [4], [4], ring, 4, parents=[-1, 3, 1, 2], words=1)
     assert got["masks"].ravel().tolist() == [1, 2, 6, 14]      # node 1 is taken for a root
     assert got["pos"].tolist() == [4, 4, 5, 6] and _status() == N.TI_DEVERR_BAD_INPUT
@@ -401,6 +404,20 @@ def test_attention_unseen_values_stay_out(nh, kvh, d, dtype, bad):
     assert _status() == 0
 
 
+def test_attention_one_token():
+    """Sizes of one, and a token stride that means nothing then."""
+    rng = np.random.default_rng(9)
+    for ctx in (0, 16, 200):
+        s = _scene(rng, 1, 1, 64, torch.bfloat16, [ctx], [1])
+        _check_attention(s, behind=0, strides=False)
+    from tiny_infra_b200 import tree
+    q = torch.zeros(3, 1, 67, dtype=torch.bfloat16, device="cuda")[:1, :, :64].expand(1, 1, 64)
+    q = q.as_strided((1, 1, 64), (67, 64, 1))
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    tree.attention(out, q, s["k"].cuda(), s["v"].cuda(), _dev(s["tables"]), _dev(s["ctx"]), _dev(s["cu"]))
+    assert torch.isfinite(out).all() and _status() == 0
+
+
 def test_attention_large_scores():
     """Scores of hundreds, growing along the keys, so that the running maximum moves all the time."""
     rng = np.random.default_rng(8)
@@ -481,6 +498,54 @@ def test_sample_nan_and_infinities():
         for k, p in ((None, None), (np.full(8, 20), np.full(8, 0.9)), (None, np.full(8, 0.9))):
             _check_draw(x, np.full(8, t), u, k, p, np.full(8, 0.0), torch.float32)
             _check_draw(x, np.full(8, t), u, k, p, np.full(8, 0.1), torch.bfloat16)
+
+
+def test_sample_parameters_out_of_range():
+    """NaN and values beyond a parameter's range keep everything, or the first of the largest (temperature)."""
+    rng = np.random.default_rng(3)
+    x = torch.from_numpy(rng.standard_normal((5, 5003)) * 2)
+    nan, u = float("nan"), rng.random(5)
+    full = _draw(x, np.ones(5), u, None, None, None, torch.float32)
+    for k, p, m in ((np.full(5, -3), np.full(5, nan), np.full(5, nan)), (np.full(5, 9000), np.full(5, 7.0), np.full(5, -1.0))):
+        got = _draw(x, np.ones(5), u, k, p, m, torch.float32)
+        assert (got[0] == full[0]).all() and (got[1] == full[1]).all()
+    top = x.float().argmax(1).numpy()
+    for t in (nan, -1.0):
+        assert (_draw(x, np.full(5, t), u, None, None, None, torch.float32)[0] == top).all()
+    got = _draw(x, np.ones(5), np.array([-1.0, nan, 2.0, 1.0, 0.0]), None, None, None, torch.float32)[0]
+    want = _draw(x, np.ones(5), np.array([0.0, 0.0, 1 - 2.0 ** -24, 1 - 2.0 ** -24, 0.0]), None, None, None, torch.float32)[0]
+    assert (got == want).all() and _status() == 0
+
+
+def test_sample_equal_and_flat_rows():
+    """Rows of one value (thousands of ties), rows that hardly differ, and a few large vocabularies."""
+    rng = np.random.default_rng(4)
+    for vocab in (9001, 151936):
+        x = torch.zeros(6, vocab, dtype=torch.float64)
+        x[1] = 3.5
+        x[2] = torch.from_numpy(rng.standard_normal(vocab) * 1e-3)
+        x[3, vocab // 2:] = -1.0
+        x[4] = torch.from_numpy(np.round(rng.standard_normal(vocab)))
+        x[5] = torch.linspace(-30, 30, vocab)
+        u = rng.random(6)
+        for k, p, m in ((None, None, None), (None, np.full(6, 0.7), None), (np.full(6, 5000), np.full(6, 0.9), None),
+                        (np.full(6, 40), np.full(6, 0.9), None), (None, None, np.full(6, 0.3)),
+                        (None, np.full(6, 0.999), np.full(6, 0.01))):
+            _check_draw(x, np.full(6, 0.8), u, k, p, m, torch.float32)
+    x = torch.from_numpy(rng.standard_normal((2, 1 << 18)) * 2)
+    _check_draw(x, np.ones(2), rng.random(2), None, None, None, torch.bfloat16)
+    x = torch.from_numpy(rng.standard_normal((2, (1 << 20) + 3)) * 2)
+    _check_draw(x, np.ones(2), rng.random(2), np.array([0, 30]), np.full(2, 0.95), None, torch.float32)
+
+
+def test_sample_far_from_the_top():
+    """Draws in the thin tail, where a place is known by what is behind it; extreme temperatures."""
+    rng = np.random.default_rng(5)
+    x = torch.from_numpy(rng.standard_normal((24, 151936)) * rng.choice([0.5, 1.5, 2.5], (24, 1)))
+    u = 1 - 10.0 ** -rng.uniform(2, 6.5, 24)
+    _check_draw(x, np.full(24, 1.1), u, None, None, None, torch.float32)
+    _check_draw(x, np.full(24, 1.1), u, None, np.full(24, 0.9995), None, torch.float32)
+    _check_draw(x[:6, :20000], np.array([1e-4, 1e-30, 1e3, 1e30, 30.0, 1e-2]), u[:6], None, None, None, torch.float32)
 
 
 def test_sample_frequencies():

@@ -127,7 +127,7 @@ __device__ __forceinline__ void expand(const Params& p, const int* s_cu, int64_t
         const int w = (a >> 5) - w0;
 #pragma unroll
         for (int k = 0; k < 4; ++k) m[k] |= w == k ? 1u << (a & 31) : 0u;
-        bad |= a >= 32 * p.mask_words;
+        bad |= p.mask_words > 0 && a >= 32 * p.mask_words;
         const int up = p.parents[first + a];
         bad |= up >= a;
         a = up >= a ? -1 : up;
@@ -137,7 +137,7 @@ __device__ __forceinline__ void expand(const Params& p, const int* s_cu, int64_t
         if (w0 + k < p.mask_words) p.masks[t * p.mask_words + w0 + k] = (int32_t)m[k];
     }
     if (j >= 0) pos += depth - 1 - j;
-    if (bad && p.mask_words) raise_device_error(TI_DEVERR_BAD_INPUT);
+    if (bad) raise_device_error(TI_DEVERR_BAD_INPUT);
   }
   p.slots[t] = slot;
   p.positions[t] = (int32_t)pos;

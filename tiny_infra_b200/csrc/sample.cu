@@ -458,7 +458,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   int k = p.top_ks ? p.top_ks[r] : 0;
   if (k <= 0 || k >= V) k = 0;
   const float top_p = p.top_ps ? p.top_ps[r] : 1.f;
-  const double least = p.min_ps ? fmin((double)p.min_ps[r], 1.0) : 0.0;
+  const float min_p = p.min_ps ? p.min_ps[r] : 0.f;
+  const double least = min_p > 0.f ? fmin((double)min_p, 1.0) : 0.0;
   const double u = fmin(fmax((double)p.uniforms[r], 0.0), 1.0 - 1.0 / 16777216.0);
   const int share = (int)((((int64_t)(V + 7) / 8 + ctas - 1) / ctas) * 8);
   const int j0 = (int)min((int64_t)V, (int64_t)rank * share), j1 = min(V, j0 + share);

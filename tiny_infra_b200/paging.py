@@ -98,7 +98,8 @@ def reserve(block_tables: torch.Tensor, seq_lens: torch.Tensor, counts: torch.Te
     and itself, as ``tree.attention`` takes them.  A tree with more nodes than bits raises
     TI_DEVERR_BAD_INPUT and loses the bits.
 
-    ``seq_lens`` is not advanced; blocks reserved once stay in the row.  At most 4096 sequences."""
+    ``seq_lens`` is not advanced; blocks reserved once stay in the row.  At most 4096 sequences, 32768 table
+    rows with ``row_index``.  Calls that share a ring or a table follow one another."""
     dev = _device(block_tables, seq_lens, counts, ring, slot_mapping, positions, cu_seqlens, row_index,
                   granted, pos_offset, parents, masks)
     B = counts.numel()

@@ -97,8 +97,8 @@ def sample(logits: torch.Tensor, temperatures: torch.Tensor, uniforms: torch.Ten
 
     z = x / temperature, and in the order of descending z (equal ones: the lower index first) a row
     keeps the tokens down to the ``top_ks``-th and all that equal it (int32; <= 0 or >= V: all), of these
-    the shortest prefix whose probability exceeds ``top_ps`` (>= 1: all), of these the ones at least
-    ``min_ps`` times as probable as the likeliest (<= 0: all; 1 and more: those that equal it).  The token
+    the shortest prefix whose probability exceeds ``top_ps`` (>= 1 or NaN: all), of these the ones at least
+    ``min_ps`` times as probable as the likeliest (<= 0 or NaN: all; 1 and more: those that equal it).  The token
     is the first whose cumulative probability among the kept ones exceeds ``uniforms`` (in [0, 1)).
     ``logprobs`` (float32 [rows]) receives the log of its probability among them.  A temperature of 0 (or
     below, or NaN) takes the first of the largest values, log probability 0.

@@ -64,6 +64,8 @@ def attention(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor, v_cache
     dev = _device(out, q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, masks, row_index, lse)
     T, NH, d, q_stride = _rows("q", q)
     out_stride = _out_rows(out, q)
+    if T == 1:
+        q_stride = out_stride = NH * d              # (a single token's stride means nothing)
     shape = k_cache.shape
     if len(shape) != 4 or v_cache.shape != shape or shape[2] != BLOCK or shape[3] != d or \
             not k_cache.is_contiguous() or not v_cache.is_contiguous():
@@ -117,7 +119,7 @@ def accept(key_cache: torch.Tensor, value_cache: torch.Tensor, tokens: torch.Ten
 
     K and V of the path's j-th node move from its slot to that of place j, ``out_slots[cu_seqlens[i] + j]``
     (default: ``slot_mapping`` itself, so that the kept nodes follow the sequence's cached tokens;
-    otherwise slots that hold none of the call's nodes), in every layer of ``key_cache`` / ``value_cache``
+    otherwise slots that hold none of the call's nodes; distinct either way), in every layer of ``key_cache`` / ``value_cache``
     [layers, num_blocks, KVH, block_size, D] (or of one layer).  Negative slots are skipped; slots
     outside the pool too, raising TI_DEVERR_BAD_INPUT.  ``seq_lens[row_index[i]]`` (default row i)
     advances by the path's length.  At most 1024 places."""
