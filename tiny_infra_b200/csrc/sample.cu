@@ -14,7 +14,7 @@
 //                largest value, and m times the largest weight is one for min-p: one more pass collects
 //                what reaches the bound; rank 0 sorts that, and reads everything off its prefix sums;
 //   all tokens   a histogram of weights (4096 bins of equal width in x, a bin's sum in units of 2^-14 of its
-//                largest weight; counts too, if top-k has to be placed) bounds the sum down to any bin
+//                middle weight; counts too, if top-k has to be placed) bounds the sum down to any bin
 //                from both sides, to a few parts in 2^14; so it names the few bins in which top-k's,
 //                top-p's and the draw's place can lie.  The next pass adds up the weights above each of
 //                these intervals, in 64 bits, and collects what is in them;
@@ -87,37 +87,35 @@ __device__ __forceinline__ void scan8(const T* row, int j0, int j1, F&& f) {
   const bool aligned = (reinterpret_cast<uintptr_t>(row) & 15) == 0;
   const int full = aligned ? (j1 - j0) / 8 : 0, steps = (j1 - j0 + 7) / 8;
   const uint4* pv = reinterpret_cast<const uint4*>(row + j0);
+  uint4 raw[U][kRaw];
+  auto fetch = [&](uint4 (&to)[kRaw], int v) {
+    if (v < full)
+#pragma unroll
+      for (int i = 0; i < kRaw; ++i) to[i] = __ldg(pv + v * kRaw + i);
+  };
+#pragma unroll
+  for (int u = 0; u < U; ++u) fetch(raw[u], (int)threadIdx.x + u * kThreads);
 #pragma unroll 1
-  for (int v = threadIdx.x; v < steps; v += U * kThreads) {
-    uint4 raw[U][kRaw];
+  for (int v = threadIdx.x; v < steps; v += kThreads) {
+    uint4 cur[kRaw];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (v + u * kThreads < full)
+    for (int i = 0; i < kRaw; ++i) {
+      cur[i] = raw[0][i];
 #pragma unroll
-        for (int i = 0; i < kRaw; ++i) raw[u][i] = __ldg(pv + (v + u * kThreads) * kRaw + i);
-#pragma unroll 1
-    for (int u = 0; u < U; ++u) {
-      const int step = v + u * kThreads, j = j0 + step * 8;
-      if (step >= steps) break;
-      uint4 cur[kRaw];
-#pragma unroll
-      for (int i = 0; i < kRaw; ++i) {
-        cur[i] = raw[0][i];
-#pragma unroll
-        for (int q = 1; q < U; ++q)
-          if (u == q) cur[i] = raw[q][i];
-      }
-      float x[8];
-      if (step < full) {
-        const T* e = reinterpret_cast<const T*>(cur);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = load(e, i);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = j + i < j1 ? load(row, j + i) : -INFINITY;
-      }
-      f(x, j);
+      for (int u = 0; u + 1 < U; ++u) raw[u][i] = raw[u + 1][i];
     }
+    fetch(raw[U - 1], v + U * kThreads);
+    const int j = j0 + v * 8;
+    float x[8];
+    if (v < full) {
+      const T* e = reinterpret_cast<const T*>(cur);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = load(e, i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = j + i < j1 ? load(row, j + i) : -INFINITY;
+    }
+    f(x, j);
   }
 }
 
@@ -134,14 +132,16 @@ __device__ __noinline__ double exp_once(double x) { return exp(x); }
 struct Weights {
   float top;
   double inv, inv2;                      // 1 / t, log2(e) / t
+  unsigned low_word;                     // high word of -1000 / inv2
   // exp((x - top) / t) to the last bits; x finite or -inf, or top itself
   __device__ __forceinline__ double exact(float x) const { return x == top ? 1.0 : exp_once(((double)x - (double)top) * inv); }
   // the same for sums (see above); next to nothing for -inf and NaN
   __device__ __forceinline__ double fast(float x) const {
-    double y = ((double)x - (double)top) * inv2;
-    y = y > -1000.0 ? y : -1000.0;
-    const double t = y + 6755399441055744.0;             // 1.5 * 2^52: the nearest integer in the low word
-    const double r = y - (t - 6755399441055744.0);
+    const double d = (double)x - (double)top;
+    // (no double-precision instruction: d is not positive, and its high word grows with its size)
+    const double c = __hiloint2double((int)min((unsigned)__double2hiint(d) | 0x80000000u, low_word), __double2loint(d));
+    const double t = fma(c, inv2, 6755399441055744.0);   // 1.5 * 2^52: the nearest integer in the low word
+    const double r = fma(c, inv2, -(t - 6755399441055744.0));
     double q = 1.3255224878668817e-06;
     q = fma(q, r, 1.5310079402249296e-05);
     q = fma(q, r, 0.00015403455852453838);
@@ -467,7 +467,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   // ---- the largest value and its first place, the smallest finite one, thread maxima
   float best = -INFINITY, smallest = INFINITY;
   int at = 0x7fffffff;
-  scan8<4>(row, j0, j1, [&](const float (&x)[8], int j) {
+  scan8<2>(row, j0, j1, [&](const float (&x)[8], int j) {
     // (a thread sees its places in ascending order)
     const float a = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
     if (a > best) {
@@ -476,8 +476,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       for (int i = 7; i >= 0; --i)
         if (x[i] == a) at = j + i;
     }
+    // (infinities and NaN among the eight are rare)
+    const float b = fminf(fminf(fminf(x[0], x[1]), fminf(x[2], x[3])), fminf(fminf(x[4], x[5]), fminf(x[6], x[7])));
+    if (b > -INFINITY) {
+      smallest = fminf(smallest, b);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) smallest = fminf(smallest, x[i] > -INFINITY ? x[i] : INFINITY);
+      for (int i = 0; i < 8; ++i) smallest = fminf(smallest, x[i] > -INFINITY ? x[i] : INFINITY);
+    }
   });
   const bool by_rank = !greedy && k > 0 && k <= kThreads;
   // (and each of q CTAs' ceil(k / q)-th largest: the least of them has k values above it too)
@@ -557,7 +563,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     }
     return;
   }
-  const Weights w{best, 1.0 / (double)temp, 1.4426950408889634 / (double)temp};
+  const Weights w{best, 1.0 / (double)temp, 1.4426950408889634 / (double)temp,
+                  (unsigned)__double2hiint(-1000.0 / 1.4426950408889634 * (double)temp)};
   auto collect = [&](float x, int j) {
     const int slot = atomicAdd(&sh.count, 1);
     if (slot < kList) sh.list[slot] = ((u64)key_of(x) << 32) | (uint32_t)~(uint32_t)j;
@@ -623,13 +630,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       }
     };
     if (sum_all && best < INFINITY)
-      scan8<4>(row, j0, j1, [&](const float (&x)[8], int j) {
+      scan8<2>(row, j0, j1, [&](const float (&x)[8], int j) {
         reach(x, j);
 #pragma unroll
         for (int i = 0; i < 8; ++i) s[3] += w.fast(x[i]);
       });
     else
-      scan8<4>(row, j0, j1, reach);
+      scan8<2>(row, j0, j1, reach);
     hand_over();
     send_sums(s);
     meet();
@@ -673,24 +680,30 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   // bins of equal width from the maximum down to the smallest value, or 40 octaves
   const double octaves = fmin(((double)best - (double)smallest) * w.inv2, kOctaves);
   if (!done && best < INFINITY && octaves > 0.0) {
-    const float per = (float)((double)kBins * w.inv2 / octaves);     // bins a unit of x
-    const double width = w.inv2 / (double)per;                       // octaves of a bin (at most 40 / 4096)
-    auto bin = [&](float x) { return x == best ? 0 : min(kBins - 1, __float2int_rz((best - x) * per)); };
+    // (bin b: the values whose distance from the maximum rounds to b; halves to even, monotonic all the same)
+    const float per = (float)fmin((double)(kBins - 1) * w.inv2 / octaves, 1e38);   // bins a unit of x
+    const double width = w.inv2 / (double)per;                       // octaves of a bin (at most 40 / 4095)
+    constexpr float kRound = 12582912.f;                             // 1.5 * 2^23: the nearest integer in the low bits
+    auto rounded = [&](float x) { return fminf(fmaf(best - x, per, kRound), kRound + (float)(kBins - 1)); };
+    auto bin = [&](float x) { return __float_as_int(rounded(x)) - __float_as_int(kRound); };
     for (int b = tid; b < kBins; b += kThreads) {
       sh.hist[b] = 0;
       if (k > 0) sh.hist_n[b] = 0;
     }
     if (tid == 0) sh.count = sh.total = 0;
     __syncthreads();
-    const float drop = (float)(-0.6931471805599453 * width);         // 2^(-width f) = 1 + drop f + (drop f)^2 / 2 ..
+    // a weight in units of its bin's middle: 2^(-width f), f from -1/2 to 1/2, as a polynomial; the sum with 2^23
+    // leaves its nearest integer in the low bits
+    const float drop = (float)(-0.6931471805599453 * width);
+    const float c2 = p.quanta * 0.5f * drop * drop, c1 = p.quanta * drop, c0 = p.quanta + 8388608.f;
     auto weigh = [&](float x) {
-      const float at_bin = x == best ? 0.f : (best - x) * per;
-      const int b = min(kBins - 1, __float2int_rz(at_bin));
-      const float f = fminf(at_bin - (float)b, 1.f) * drop;          // (the last bin: not below its own end)
-      atomicAdd(&sh.hist[b], (unsigned)__float2int_rz(p.quanta * fmaf(f, fmaf(f, 0.5f, 1.f), 1.f)));
+      const float t = rounded(x);
+      const int b = __float_as_int(t) - __float_as_int(kRound);
+      const float f = fminf(fmaf(best - x, per, kRound - t), 0.5f);  // (the last bin: not below its own end)
+      atomicAdd(&sh.hist[b], __float_as_uint(fmaf(f, fmaf(f, c2, c1), c0)) & 0x7fffffu);
       return b;
     };
-    scan8<4>(row, j0, j1, [&](const float (&x)[8], int) {
+    scan8<2>(row, j0, j1, [&](const float (&x)[8], int) {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         if (x[i] > -INFINITY) {
@@ -739,11 +752,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         }
         __syncthreads();
       }
-      // sums down to each bin.  A weight was cut to a unit and is off by 32-bit rounding: the true one is less
-      // than 2 units above and 1 below; a token has at least 0.98 of the units of its bin's largest weight,
-      // less one.  So each bin's true sum is between (1 - d) and (1 + 2 d) times what is held, and so are
-      // sums over bins; the last bin has the tokens below the range too, its sum may be next to nothing.
-      const double d = 1.0 / ((double)p.quanta * 0.98 - 1.0);
+      // sums down to each bin.  A weight was rounded to a unit, and the distance from the maximum to 24 bits,
+      // which moves it by 0.03 units at most; a token has at least 0.99 of the units of its bin's middle, less
+      // one.  So each bin's true sum is between (1 - d) and (1 + d) times what is held, and so are sums over
+      // bins; the last bin has the tokens below the range too, its sum may be next to nothing.
+      const double d = 0.6 / ((double)p.quanta * 0.99 - 1.0);
       double sum[E];                               // down to each of this thread's bins
       {
         double own = 0, most = exp2(-(double)(tid * E) * width) / (double)p.quanta;
@@ -768,7 +781,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       auto bracket = [&](double q, int slot) {
         // (the last bin may hold nothing: it does not count towards a sum that is to be small)
         const double end_a = upto(keep_a) - (keep_a == kBins - 1 ? last : 0.0), end_b = upto(keep_b);
-        const double up = 1.0 + 2.0 * d, down = 1.0 - d;
+        const double up = 1.0 + d, down = 1.0 - d;
         unsigned f = kBins - 1, l = kBins - 1;
 #pragma unroll
         for (int e = E - 1; e >= 0; --e) {
@@ -801,7 +814,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         // (the bins around the value of weight m)
         const int b = (int)fmin(fmax(-log2(least) / width, 0.0), (double)(kBins - 1));
         keep_a = min(keep_a, max(b - 3, -1));
-        keep_b = min(keep_b, min(b + 2, kBins - 1));
+        keep_b = min(keep_b, min(b + 3, kBins - 1));
       }
       const Interval iu = bracket(u, 2);
       __syncthreads();
@@ -883,11 +896,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         low[a] = a < m ? sh.iv[a].low : INFINITY;
       }
       double s[5] = {0, 0, 0, 0, 0};
-      auto masked = [](bool yes, double e) {
-        const int k = yes ? -1 : 0;
-        return __hiloint2double(__double2hiint(e) & k, __double2loint(e) & k);
-      };
-      scan8<2>(row, j0, j1, [&](const float (&x)[8], int j) {
+      // e or next to nothing: without its high word it is below 2^-1000
+      auto masked = [](bool yes, double e) { return __hiloint2double(yes ? __double2hiint(e) : 0, __double2loint(e)); };
+      scan8<1>(row, j0, j1, [&](const float (&x)[8], int j) {
         unsigned in = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -905,10 +916,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
           }
           if (least > 0.0) s[4] += masked(e >= least, e);
         }
-        if (in) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (in >> i & 1) collect(x[i], j + i);
+#pragma unroll 1
+        for (; in; in &= in - 1) {                 // (one or two of a warp's 256: read again rather than selected)
+          const int i = j + __ffs(in) - 1;
+          collect(load(row, i), i);
         }
       });
       hand_over();
