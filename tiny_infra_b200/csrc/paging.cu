@@ -10,7 +10,12 @@
 // One cluster does either: a warp counts a sequence's entries, the counts go to every CTA's shared
 // memory, each CTA sums them up itself, and the warp that counted a row writes it, so rows wait for one
 // barrier only.  Tokens follow in the same launch, or, above kFusedTokens, in a second one over the
-// whole GPU (one cluster alone writes too slowly).  Bound: latency, dependent trips to memory.
+// whole GPU (one cluster alone writes too slowly: 64 prompts of up to 16384 tokens took 44 us).
+//
+// Bound: latency, dependent trips to memory.  One token for each of 256 sequences takes 7.3 us on the device,
+// trees of up to 64 nodes for 64 sequences 10.0; as calls 17 and 18, of which the host is 10.  The 64 prompts
+// (655000 tokens, 8 MB of slots and positions) take 24.5 us as a call: two launches, the second
+// bound by its writes and by one division or shift and one table load a token.
 #include <algorithm>
 #include <atomic>
 

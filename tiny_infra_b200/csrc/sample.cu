@@ -22,15 +22,17 @@
 //                keys, on fixed-point weights, by rank 0 alone.
 // All sums have a fixed order: the same token on every run.
 //
-// Bound, 151936 tokens: 256 rows of everything the whole vocabulary can ask (fp32, 156 MB) take 231 us: one
-// pass from HBM (26 us), the histogram's shared-memory atomics (42 us; 4.6 clocks a warp instruction), the
-// polynomials (72 us; 14 double-precision operations an element at 64 a clock and SM, 8 clocks a warp), and
-// 15 us for the places.  256 rows of temperature 0.7, top-k 20, top-p 0.9 (bf16, 78 MB) take 62 (48 with one
-// CTA a row): a pass from HBM, one from L2, 7 us to the token.  One such row takes 14: a chain of passes,
-// cluster barriers and code that is run for the first time.  Measured on the way, one row: exponentials and
-// scans inlined for each use 26 us, every CTA collecting into rank 0's list 22 us; 256 rows: radix selects
-// 5200 us, branches for the sums above the intervals 880 us (fp32) instead of masks 221; collecting by the
-// first eighth's bound in the first pass 86 us instead of 62 (top-k 20).
+// Bound, 151936 tokens: 256 rows of everything the whole vocabulary can ask (fp32, 156 MB) take 206 us.  Of
+// the same on bf16 logits with top-p alone (192 us) the maximum's pass is 17 us, the histogram's 53 (shared-memory
+// atomics, 4.6 clocks a warp instruction), the weights' 70 to 87 (17 double-precision operations an element
+// at 16 a clock and scheduler are 37 of them: each adds 2.2; the rest is issue slots), and barriers, places and
+// the draw 25 a CTA, of which an SM has three or four, two at a time.  256 rows of temperature 0.7, top-k 20,
+// top-p 0.9 (bf16, 78 MB) take 53 (39 with one CTA a row): a pass from HBM, one from L2, 7 us to the token.
+// One such row takes 13.5 as a call: a chain of passes, cluster barriers and code that is run for the first
+// time.  Measured on the way, one row: exponentials and scans inlined for each use 26 us, every CTA
+// collecting into rank 0's list 22 us; 256 rows: radix selects 5200 us, branches for the sums above the
+// intervals 880 us (fp32) instead of masks; loads four steps at a time instead of always two in flight 225
+// instead of 206; collecting by the first eighth's bound in the first pass 86 us instead of 62 (top-k 20).
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -961,8 +963,10 @@ static int launch(const Params& p, int rows, cudaStream_t s) {
   }
   // CTAs of a row: while all of them fit the GPU (two an SM) and each has a share worth a barrier, or up to
   // twice as many while the shares are long, since one row that asks for the whole vocabulary is then the
-  // end of the launch (256 rows of 151936, two CTAs each instead of one: mixed 140 us instead of 199, all
-  // open 217 instead of 207, all top-k 20 63 instead of 48; 256 rows of 32000: 59, 80, 35 against 58, 60, 20)
+  // end of the launch (256 rows of 151936, two CTAs each instead of one: mixed 126 us instead of 172, all
+  // open 206 instead of 214, all top-k 20 53 instead of 39; with four, mixed 140, open 252; 256 rows of 32000
+  // gain nothing).  Pairs of which one CTA leaves where a row does not need it are no way out: the GPU keeps
+  // its place until the pair ends (open 347, all top-k 20 71)
   unsigned ctas = 1;
   while (ctas < (unsigned)kCluster) {
     const int64_t next = (int64_t)rows * ctas * 2;
