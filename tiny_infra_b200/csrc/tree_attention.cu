@@ -21,11 +21,12 @@
 // pairs by whichever CTA of a pair comes second: no CTA waits for another, the joins of a long sequence
 // go on side by side, and their order does not depend on who comes when.
 //
-// Bound: 32 trees of 64 nodes behind 2048 to 8192 tokens (14 heads over 2, D = 64) take 102 us.  Their
-// exponentials alone would take 37 (8 clocks a warp instruction), the MMAs 28; a chunk of two tiles takes
-// 1900 clocks, of which the exponential unit is busy for 1024: two softmax warps a scheduler do not hide
-// each other's trips to tensor memory and barriers (three tiles: 2450 clocks).  8 trees of up to 16 nodes
-// behind 16384 to 32768 tokens (32 heads over 8, D = 128): 136 to 171 us, 0.9 to 0.72 of measured copy.
+// Bound: 32 trees of 64 nodes behind 2048 to 8192 tokens (14 heads over 2, D = 64) take 94 us.  Their
+// exponentials alone would take 37 (8 clocks a warp instruction), the MMAs 28; a chunk of three tiles takes
+// 2450 clocks, of which the exponential unit is busy for 1536 (two tiles: 1900 and 1024; four tiles as two
+// and two instead of three and one take 104 us): the softmax warps of a scheduler do not hide each other's
+// trips to tensor memory and barriers.  8 trees of up to 16 nodes behind 16384 to 32768 tokens (32 heads over
+// 8, D = 128): 136 to 171 us, 0.9 to 0.72 of measured copy.
 // Measured on the way: one warp for all MMAs, which then wait for each other's operands, 313 us instead of
 // 194 in the latter case; one warp for all TMA boxes 155 instead of 136.  Small batches are a chain of
 // dependent trips: 7.8 us on the device for 4 trees of up to 8 nodes.
@@ -102,12 +103,11 @@ struct Item {
 };
 static_assert(sizeof(Item) <= 64, "ring entries");
 
-// A sequence as the load warp sees it; start and len: the place of its first unit on the line of work, and
-// a unit's length there; k: a unit's pieces.
+// A sequence as the load warp sees it; start: the place of its first unit on the line of work.
 struct Seq {
   SeqWork w;
-  int ctx, row0, nodes, row, k;
-  unsigned start, len;
+  int ctx, row0, nodes, row;
+  unsigned start;
 };
 
 template <int TILES>
@@ -129,18 +129,22 @@ struct Walk {
   Plan plan;
   unsigned begin, end;
   Seq mine, cur;
-  int seq, unit;
+  int seq;
+  Units at;                              // of the current sequence: its full ones, or what is left
+  int unit, k;                           // the next one, and its pieces
+  unsigned start, len;                   // where they begin on the line of work, and a unit's length there
+  bool rest;
   unsigned* starts;
 
   __device__ __forceinline__ Walk(const Params& p, unsigned* starts_) : starts(starts_) {
     const int lane = threadIdx.x & 31, each = (p.seqs + 31) / 32;
     const int i0 = min(p.seqs, lane * each), i1 = min(p.seqs, i0 + each);
     unsigned jobs = 0, units = 0;
-    mine.w = SeqWork{0, 0, 0, 0, 0, 0, 0};
+    mine.w = SeqWork{0, 0, 0, {0, 0, 0, 0}, {0, 0, 0, 0}};
     for (int i = i0; i < i1; ++i) {
       mine = sequence<TILES>(p, i);
-      jobs += (unsigned)mine.w.units * (unsigned)mine.w.jobs;
-      units += (unsigned)mine.w.units;
+      jobs += seq_jobs(mine.w);
+      units += (unsigned)(mine.w.full.count + mine.w.rest.count);
     }
     plan = Plan{dense_share(__reduce_add_sync(0xffffffffu, jobs), kCtas), 0u};
     if (__reduce_add_sync(0xffffffffu, units) <= (unsigned)kCtas) {
@@ -148,7 +152,7 @@ struct Walk {
         unsigned n = 0;
         for (int i = i0; i < i1; ++i) {
           if (each > 1) mine = sequence<TILES>(p, i);
-          n += mine.w.units ? (unsigned)(mine.w.units * pieces(mine.w, per)) : 0u;
+          n += seq_pieces(mine.w, per);
         }
         return __reduce_add_sync(0xffffffffu, n) <= (unsigned)kCtas;
       };
@@ -164,10 +168,8 @@ struct Walk {
     unsigned own = 0;
     for (int i = i0; i < i1; ++i) {
       if (each > 1) mine = sequence<TILES>(p, i);
-      mine.k = mine.w.units ? pieces(mine.w, plan.per) : 0;
-      mine.len = length(mine.w, plan, mine.k);
       if (each > 1) starts[i] = own;
-      own += (unsigned)mine.w.units * mine.len;
+      own += seq_length(mine.w, plan);
     }
     unsigned v = own;
 #pragma unroll
@@ -180,7 +182,7 @@ struct Walk {
     end = min(total, begin + plan.per);
     if (each <= 1) {
       mine.start = v - own;
-      if (i0 >= i1) mine.w.units = 0;
+      if (i0 >= i1) mine.w.full.count = mine.w.rest.count = 0;
       const unsigned here = __ballot_sync(0xffffffffu, begin >= mine.start && begin < v);
       seq = here ? __ffs(here) - 1 : 0;
     } else {
@@ -194,48 +196,69 @@ struct Walk {
       seq = lo;
     }
     load(p);
-    unit = begin > cur.start && cur.w.units > 1 ? (int)((begin - cur.start) / cur.len) : 0;
+    if (begin > cur.start && begin < end) {
+      unit = (int)((begin - cur.start) / len);
+      if (unit >= cur.w.full.count && cur.w.rest.count) {
+        second();
+        unit = (int)((begin - start) / len);
+      }
+    }
+  }
+  // from the sequence's full units to those of what is left
+  __device__ __forceinline__ void second() {
+    start += (unsigned)at.count * len;
+    at = cur.w.rest;
+    k = pieces(at, plan);
+    len = length(at, plan, k);
+    unit = 0;
+    rest = true;
   }
   __device__ __forceinline__ void load(const Params& p) {
     if (p.seqs > 32) {
       cur = sequence<TILES>(p, seq);
-      cur.k = cur.w.units ? pieces(cur.w, plan.per) : 0;
-      cur.len = length(cur.w, plan, cur.k);
       cur.start = starts[seq];
-      return;
-    }
-    int* to = reinterpret_cast<int*>(&cur);
-    const int* from = reinterpret_cast<const int*>(&mine);
+    } else {
+      int* to = reinterpret_cast<int*>(&cur);
+      const int* from = reinterpret_cast<const int*>(&mine);
 #pragma unroll
-    for (int i = 0; i < (int)(sizeof(Seq) / 4); ++i) to[i] = __shfl_sync(0xffffffffu, from[i], seq);
+      for (int i = 0; i < (int)(sizeof(Seq) / 4); ++i) to[i] = __shfl_sync(0xffffffffu, from[i], seq);
+    }
+    at = cur.w.full;
+    k = pieces(at, plan);
+    len = length(at, plan, k);
+    start = cur.start;
+    unit = 0;
+    rest = false;
   }
   __device__ __forceinline__ bool next(const Params& p, Item& it) {
     while (begin < end) {
-      while (unit >= cur.w.units) {
-        if (++seq >= p.seqs) return false;
-        unit = 0;
-        load(p);
+      while (unit >= at.count) {
+        if (!rest && cur.w.rest.count) {
+          second();
+        } else {
+          if (++seq >= p.seqs) return false;
+          load(p);
+        }
       }
-      const unsigned at = cur.start + (unsigned)unit * cur.len;
-      if (at >= end) return false;
+      const unsigned place = start + (unsigned)unit * len;
+      if (place >= end) return false;
       const int u = unit++;
-      it.c0 = chunk_at(begin, at, cur.w, plan, cur.k);
-      it.c1 = chunk_at(end, at, cur.w, plan, cur.k);
+      it.c0 = chunk_at(begin, place, at, plan, k);
+      it.c1 = chunk_at(end, place, at, plan, k);
       if (it.c0 >= it.c1) continue;
-      it.kvh = cur.w.groups == 1 ? u : u / cur.w.groups;
-      const int g = u - it.kvh * cur.w.groups;
+      it.kvh = rest || cur.w.groups == 1 ? u : u / cur.w.groups;
       it.nodes = cur.nodes;
       it.ctx = cur.ctx;
       it.row0 = cur.row0;
       it.keys = cur.w.keys;
       it.table = cur.row >= 0 ? p.tables + (int64_t)cur.row * p.bt_stride : nullptr;
-      it.tile0 = g * cur.w.width;
-      it.tiles = min(cur.w.width, cur.w.tiles - it.tile0);
+      it.tile0 = (rest ? cur.w.groups : u - it.kvh * cur.w.groups) * cur.w.full.width;
+      it.tiles = at.width;
       it.first = blockIdx.x;
       it.parts = 1;
-      if (it.c0 > 0 || it.c1 < cur.w.chunks) {
-        it.first = first_cta(at, cur.w, plan, cur.k);
-        it.parts = last_cta(at, cur.w, plan, cur.k) - it.first + 1;
+      if (it.c0 > 0 || it.c1 < at.chunks) {
+        it.first = first_cta(place, at, plan, k);
+        it.parts = last_cta(place, at, plan, k) - it.first + 1;
       }
       return true;
     }
