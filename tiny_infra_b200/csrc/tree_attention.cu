@@ -540,29 +540,29 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
         const int R = (it.tile0 + (turns ? 0 : x)) * 128 + r, node = R / p.group;
         return Row{(int64_t)it.row0 + node, node, R - node * p.group, node < it.nodes && (turns || x < it.tiles)};
       };
-      // (the first mask words wait in shared memory for the chunks that need them)
-      if (ok && p.masks) {
+      // Q: this thread's row of the tile (zeros where there is none), swizzled, K-major; the first mask words
+      // wait in shared memory for the chunks that need them.  One trip to memory for both
+      if (ok) {
         const Row w = row();
+        const bool fill = turns ? x == 0 : x < it.tiles;
         uint2 first = make_uint2(0u, 0u);
-        if (w.mine) {
+        uint4 v[HD / 8];
+        if (w.mine && p.masks) {
           const uint32_t* src = reinterpret_cast<const uint32_t*>(p.masks) + w.t * p.mask_words;
           first.x = src[0];
           if (p.mask_words > 1) first.y = src[1];
         }
-        s_mask[x * 128 + r] = first;               // (read by this thread only)
-      }
-      // Q: this thread's row of the tile (zeros where there is none), swizzled, K-major
-      if (ok && (turns ? x == 0 : x < it.tiles)) {
-        const Row w = row();
         const uint4* src = reinterpret_cast<const uint4*>((const T*)p.q + w.t * p.q_stride +
                                                           (int64_t)(it.kvh * p.group + w.h) * HD);
-        uint4 v[HD / 8];
 #pragma unroll
-        for (int c = 0; c < HD / 8; ++c) v[c] = w.mine ? src[c] : make_uint4(0u, 0u, 0u, 0u);
+        for (int c = 0; c < HD / 8; ++c) v[c] = w.mine && fill ? src[c] : make_uint4(0u, 0u, 0u, 0u);
+        s_mask[x * 128 + r] = first;               // (read by this thread only)
+        if (fill) {
 #pragma unroll
-        for (int c = 0; c < HD / 8; ++c)
-          *reinterpret_cast<uint4*>(smem + (turns ? 0 : x) * C::kQTile + (c >> 3) * 16384 + r * 128 +
-                                    (((c & 7) ^ (r & 7)) << 4)) = v[c];
+          for (int c = 0; c < HD / 8; ++c)
+            *reinterpret_cast<uint4*>(smem + (turns ? 0 : x) * C::kQTile + (c >> 3) * 16384 + r * 128 +
+                                      (((c & 7) ^ (r & 7)) << 4)) = v[c];
+        }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
       __syncwarp();
