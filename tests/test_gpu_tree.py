@@ -333,6 +333,19 @@ def test_attention_many_sequences():
     _check_attention(_scene(rng, 2, 1, 64, torch.bfloat16, ctx, counts))
 
 
+@pytest.mark.parametrize("nh,kvh,d,dtype", [HEADS[0], HEADS[2], HEADS[3]])
+def test_attention_full_units_and_what_is_left(nh, kvh, d, dtype):
+    """Trees of one to eleven tiles: alone, in few sequences behind long contexts, and in many."""
+    rng = np.random.default_rng(nh)
+    group = nh // kvh
+    nodes = lambda tiles: max(1, tiles * 128 // group - int(rng.integers(0, 5)))         # noqa: E731
+    for tiles in (3, 4, 5, 7):
+        _check_attention(_scene(rng, nh, kvh, d, dtype, [700], [nodes(tiles)]))
+    _check_attention(_scene(rng, nh, kvh, d, dtype, [2500, 0, 1300, 40], [nodes(4), 0, nodes(11), nodes(1)]))
+    many = [nodes(int(n)) if n else 0 for n in rng.integers(0, 6, 37)]
+    _check_attention(_scene(rng, nh, kvh, d, dtype, rng.integers(0, 300, 37).tolist(), many))
+
+
 def test_attention_large_trees():
     rng = np.random.default_rng(4)
     _check_attention(_scene(rng, 7, 1, 64, torch.bfloat16, [100, 3], [300, 129]))
@@ -515,6 +528,39 @@ def test_sample_parameters_out_of_range():
     got = _draw(x, np.ones(5), np.array([-1.0, nan, 2.0, 1.0, 0.0]), None, None, None, torch.float32)[0]
     want = _draw(x, np.ones(5), np.array([0.0, 0.0, 1 - 2.0 ** -24, 1 - 2.0 ** -24, 0.0]), None, None, None, torch.float32)[0]
     assert (got == want).all() and _status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [8, 4088, 4096, 4104, 12304, 20488, 150008])
+def test_sample_aligned_rows(vocab, dtype):
+    """Rows that wide loads can read, lengths around whole rounds of them; what lies behind a row is the next."""
+    from tiny_infra_b200 import sampler
+    rng = np.random.default_rng(vocab)
+    rows = 9
+    x = torch.from_numpy(rng.standard_normal((rows, vocab)) * 2).to(dtype)
+    x[::2] += 9                                              # (the next row must not be seen)
+    u, f = rng.random(rows), lambda v: torch.full((rows,), v, device="cuda")             # noqa: E731
+    d, du = x.cuda(), _dev(u.astype(np.float32))
+    for k, p, m in ((0, 1.0, 0.0), (0, 0.9, 0.0), (20, 0.9, 0.0), (3000, 0.8, 0.0), (0, 1.0, 0.05)):
+        tok = sampler.sample(d, f(0.8), du, top_ks=torch.full((rows,), k, dtype=torch.int32, device="cuda"),
+                             top_ps=f(p), min_ps=f(m)).cpu().numpy()
+        for i in range(rows):
+            t32 = [float(np.float32(v)) for v in (0.8, u[i], p, m)]
+            assert tok[i] == oracle.sample(x[i].double().numpy(), t32[0], t32[1], k, t32[2], t32[3])[0], (k, p, m, i)
+    assert _status() == 0
+
+
+def test_sample_temperatures_from_tiny_to_huge():
+    """Where one value is all, where all are equally likely, and logits as small as the temperature."""
+    rng = np.random.default_rng(11)
+    t = np.array([1e-44, 1e-40, 3e-37, 2e-36, 1e-30, 1e-6, 1e4, 1e30, 3e38], np.float32)
+    u, n = rng.random(len(t)), len(t)
+    plain = rng.standard_normal((n, 6007))
+    near = np.clip(t.astype(np.float64)[:, None] * rng.standard_normal((n, 6007)) * 2, -3e38, 3e38)
+    for x in (plain, near):
+        x[:, ::5] = -float("inf")
+        for p in (None, np.full(n, 0.9)):
+            _check_draw(torch.from_numpy(x.astype(np.float32)), t, u, None, p, None, torch.float32)
 
 
 def test_sample_equal_and_flat_rows():

@@ -681,9 +681,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   // ---- all tokens
   // bins of equal width from the maximum down to the smallest value, or 40 octaves
   const double octaves = fmin(((double)best - (double)smallest) * w.inv2, kOctaves);
-  if (!done && best < INFINITY && octaves > 0.0) {
+  const double bins = (double)(kBins - 1) * w.inv2 / octaves;        // a unit of x
+  if (!done && best < INFINITY && octaves > 0.0 && bins < 1e38) {    // (temperatures from 1e-36 on)
     // (bin b: the values whose distance from the maximum rounds to b; halves to even, monotonic all the same)
-    const float per = (float)fmin((double)(kBins - 1) * w.inv2 / octaves, 1e38);   // bins a unit of x
+    const float per = (float)bins;
     const double width = w.inv2 / (double)per;                       // octaves of a bin (at most 40 / 4095)
     constexpr float kRound = 12582912.f;                             // 1.5 * 2^23: the nearest integer in the low bits
     auto rounded = [&](float x) { return fminf(fmaf(best - x, per, kRound), kRound + (float)(kBins - 1)); };
