@@ -6,13 +6,15 @@
 //
 // One launch: each CTA of a sequence walks its tree (a warp looks at 32 nodes at once; a few hundred
 // nanoseconds in shared memory) and moves its share of layers and heads.  A thread moves 16 bytes of
-// one (layer, K or V, head) for all places of the path, in ascending order, eight loads ahead of their
+// one (layer, K or V, head) for all places of the path, in ascending order, four loads ahead of their
 // stores.  In place this is safe: path[j] >= j, so the slot of place j, which is node j's, is read for no
 // place behind j.
 //
 // Bound: HBM, each kept byte read and written once.  256 trees of up to 64 nodes (24 layers, 8 heads of 128, 4.0
-// nodes kept on average: 202 MB) take 46 to 50 us, 4.2 TB/s or 0.65 of measured copy: the rows are 256 bytes
-// long and lie 4 KB apart.  8 trees of 8 nodes take 4.1 us on the device and 16 as a call: the host.
+// nodes kept on average: 202 MB) take 41 us, 4.9 TB/s or 0.75 of measured copy: the rows are 256 bytes long and
+// lie 4 KB apart.  Four loads ahead in 32 registers, so that 8 CTAs fit an SM, and three rounds of them:
+// 47 us with eight loads, 5 CTAs an SM and one and a half rounds.  8 trees of 8 nodes take 4.3 us in a graph and 16 as
+// a call: the host.
 #include <algorithm>
 
 #include "capi_internal.h"
@@ -23,7 +25,7 @@ namespace accept {
 
 constexpr int kThreads = 256;
 constexpr int kStage = 512;              // nodes of a tree held in shared memory; more are read in place
-constexpr int kAhead = 8;
+constexpr int kAhead = 4;
 
 struct Params {
   uint4 *kc, *vc;
@@ -36,7 +38,7 @@ struct Params {
   int deep, rows, block, kvh, units, layers, total;
 };
 
-__global__ void __launch_bounds__(kThreads) accept_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kThreads, 8) accept_kernel(const __grid_constant__ Params p) {
   extern __shared__ int64_t s_move[];            // source and target unit of each place
   __shared__ int s_parent[kStage], s_token[kStage], s_target[kStage];
   __shared__ int s_num;
@@ -176,7 +178,7 @@ extern "C" int ti_tree_accept(void* key_cache, void* value_cache, int num_layers
   p.layers = num_layers;
   p.total = num_tokens;
   // a CTA walks its tree again: as few as still fill the GPU
-  const int64_t want = std::max<int64_t>(1, (148 * 12 + num_seqs - 1) / num_seqs);
+  const int64_t want = std::max<int64_t>(1, (148 * 24 + num_seqs - 1) / num_seqs);
   const unsigned y = (unsigned)std::min<int64_t>(std::min<int64_t>((items + accept::kThreads - 1) / accept::kThreads, want), 65535);
   return launch_kernel_cl("tree accept launch", accept::accept_kernel, dim3((unsigned)num_seqs, y),
                           dim3(accept::kThreads), (size_t)max_path * 20, reinterpret_cast<cudaStream_t>(stream),
