@@ -519,7 +519,8 @@ int ti_release_blocks(int32_t* block_tables, int64_t bt_stride, int num_rows, in
  * tokens[c] = targets[current], and on, for at most max_path (<= 1024) nodes.  num [num_seqs] = its
  * length; path, out_tokens [num_seqs, max_path] = its nodes and the targets at them (-1 behind).  In every
  * layer of key_cache / value_cache [num_layers, num_blocks, num_kv_heads, block_size, head_dim] (elements
- * of elem_bytes, rows of a multiple of 16 bytes) the j-th node's values move from slot_mapping[its row]
+ * of elem_bytes, rows of a multiple of 16 bytes, a token's rows of all layers below 2^30 times that) the
+ * j-th node's values move from slot_mapping[its row]
  * to out_slots[cu_seqlens[i] + j] (the same array: in place; otherwise slots that hold none of the
  * nodes; negative: skipped; outside the pool: skipped, TI_DEVERR_BAD_INPUT).  seq_lens (or NULL):
  * seq_lens[row_index[i]] (NULL: i; of num_rows) += num[i]. */

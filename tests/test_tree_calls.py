@@ -240,6 +240,15 @@ def test_c_entry_points_refuse():
     assert draw(rows=0) == 0
 
 
+def test_accept_refuses_tokens_beyond_32_bits():
+    """A token's K and V in 16-byte units, and a block's row of them, are counted in 32 bits."""
+    from tiny_infra_b200 import _native as N
+    lib, a = N.lib(), 1 << 20
+    for layers, kvh, d, bs in ((1 << 20, 1 << 10, 64, 16), (1 << 30, 1 << 30, 1 << 30, 16), (1, 1, 1 << 12, 1 << 28)):
+        rc = lib.ti_tree_accept(a, a, layers, 6, kvh, d, bs, 2, a, a, a, a, 3, 9, a, a, a, a, a, 8, None, None, 0, None)
+        assert rc != 0 and "2^30" in lib.ti_last_error().decode()
+
+
 def test_step_by_step_forms_follow_the_host_allocator():
     from tiny_infra_b200.cache_manager import BlockAllocator
     rng = np.random.default_rng(0)
