@@ -162,10 +162,11 @@ extern "C" int ti_tree_accept(void* key_cache, void* value_cache, int num_layers
   p.out_tokens = out_tokens;
   p.seq_lens = seq_lens;
   p.row_index = row_index;
-  p.units = head_dim * elem_bytes / 16;
+  p.units = (int)((int64_t)head_dim * elem_bytes / 16);
   p.num_slots = num_blocks * block_size;
   // (32 bits: 64-bit divisions, two an item, took 48.6 us where these take 47.3)
-  if (2.0 * num_layers * num_kv_heads * p.units > 0x3fffffff || (double)block_size * p.units > 0x3fffffff)
+  const double row = (double)head_dim * elem_bytes / 16;
+  if (2.0 * num_layers * num_kv_heads * row > 0x3fffffff || block_size * row > 0x3fffffff)
     return set_error(TI_ERR_UNSUPPORTED, "tree accept: a token's K and V have more than 2^30 16-byte units");
   p.per_layer = (unsigned)num_kv_heads * (unsigned)p.units;
   const int64_t items = (int64_t)num_layers * 2 * p.per_layer;
