@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from oracle import tree as oracle
+from tests.test_gpu_tree import _attend as _attend_host
 from tests.test_gpu_tree import _check_attention, _dev, _limits, _random_parents, _scene, _status
 
 pytestmark = pytest.mark.gpu
@@ -32,6 +33,20 @@ def test_attention_same_bits_every_run():
         d["out"].zero_()
         _attend(d)
         assert torch.equal(d["out"], first[0]) and torch.equal(d["lse"], first[1])
+
+
+@pytest.mark.parametrize("masks", ["tree", None])
+@pytest.mark.parametrize("nh,kvh,d,dtype", [(2, 1, 64, torch.bfloat16), (2, 1, 128, torch.float16), (14, 2, 64, torch.float16)])
+def test_attention_many_short_sequences_of_one_to_three_chunks(nh, kvh, d, dtype, masks):
+    """More units than CTAs, so that a CTA has several one behind the other, and few chunks a unit, so that the
+    next one may use fewer of the CTA's slots: each gets its own sums, on every run."""
+    rng = np.random.default_rng(11)
+    n = 500
+    s = _scene(rng, nh, kvh, d, dtype, rng.choice([20, 100, 170], n).tolist(), rng.integers(1, 5, n).tolist(), masks=masks)
+    first = _check_attention(s)
+    for _ in range(4):
+        again = _attend_host(s)
+        assert torch.equal(again[0], first[0]) and torch.equal(again[1], first[1])
 
 
 def test_attention_on_two_streams_and_in_two_graphs():

@@ -684,7 +684,9 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
       }
       if (ok && jobs > 0 && !wait_all(pv_done + 8 * x, (done + jobs - 1) & 1)) ok = false;
       tc_fence_before();
-      if (turns) s_ml[x * 128 + r] = make_float2(m, l);
+      // (slots with a job only, which are those that slot 0 reads: a slot without one waits for nothing that
+      // this item's slot 0 does last, and may be here while it still reads the last item's entries)
+      if (turns && jobs > 0) s_ml[x * 128 + r] = make_float2(m, l);
       if (bar_or(1, C::kSoftWarps * 32, !ok)) break;       // (a wait gave up: everyone leaves)
       dirty = bar_or(1, C::kSoftWarps * 32, dirty);
       tc_fence_after();
@@ -872,7 +874,7 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
       }
       g += n;
       // (the next item's products wait for q_full, to which every softmax warp arrives: O of the other
-      // slots, their sums and Q's tiles are free by then)
+      // slots, Q's tiles and the sums of slots that have a product to wait for are free by then)
     }
   }
   tc_fence_before();
