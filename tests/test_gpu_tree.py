@@ -326,6 +326,30 @@ def test_attention_long_contexts(nh, kvh, d, dtype):
         _check_attention(_scene(rng, nh, kvh, d, dtype, ctx, counts))
 
 
+@pytest.mark.parametrize("masks", ["tree", "random", None])
+@pytest.mark.parametrize("nh,kvh,d,dtype", HEADS)
+def test_attention_weights_in_two_parts(nh, kvh, d, dtype, masks):
+    """Weights as the sum of two values of the cache's type, as in the decode and prefill attention over the same
+    cache.  The first is off by half a step at most, the second is the rest and off by half a step of that:
+    half^2 of the weight, and for fp16, whose weights are held times 2^7 and whose steps end at 2^-24,
+    2^-25 / 2^7 of the largest (kept below 2^8 times a row's own, so 2^-32 of it).  One, two and three tiles a
+    unit, one chunk and many."""
+    rng = np.random.default_rng(nh + d)
+    wide = 128 // (nh // kvh)
+    for ctx, counts in (([0, 1, 30, 70], [3, 9, 1, 5]), ([500, 90], [2 * wide + 1, wide + 3]), ([1500], [8])):
+        s = _scene(rng, nh, kvh, d, dtype, ctx, counts, masks=masks)
+        out, _ = _attend(s)
+        as64 = lambda t: t.double().numpy()                                              # noqa: E731
+        ref, _, size, big = oracle.attention(as64(s["q"]), as64(s["k"]), as64(s["v"]), s["tables"], s["ctx"], s["cu"],
+                                             s["masks"])
+        half, score = torch.finfo(dtype).eps / 2, 2.0 ** -20 + 2.0 ** -20 * big
+        low = 2.0 ** -32 * float(s["v"].abs().max()) * (sum(ctx) + sum(counts)) + 2.0 ** -25 if dtype == torch.float16 else 0.0
+        lim = half * np.abs(ref) + (1 + half) * (half * half + 2 * score[..., None]) * size + low
+        off = np.abs(out.double().numpy() - ref)
+        assert (off <= lim).all(), (off / np.maximum(lim, 1e-30)).max()
+    assert _status() == 0
+
+
 def test_attention_many_sequences():
     rng = np.random.default_rng(3)
     n = 700

@@ -10,9 +10,13 @@
 // pool.  Per chunk and tile:
 //   S = Q K^T   M 128, N 64, into TMEM; freed as soon as the softmax warps have it in registers;
 //   softmax     one row per thread, a running max that is kept until a row's grows by more than 2^8
-//               (then O is rescaled in TMEM), P = 2^(s - m) in the pool's type back into TMEM, the A
-//               operand of the next product; the sum is taken before that rounding;
-//   O += P V    A from TMEM, V in place as an MN-major operand; fp32 O in TMEM.
+//               (then O is rescaled in TMEM), P = 2^(s - m) back into TMEM as the sum of two values of the
+//               pool's type, P and what its rounding left (17 bits in all for bf16, 22 for fp16, as in the
+//               decode and prefill attention over the same pool); the sum is taken before that rounding;
+//   O += P V    twice, A from TMEM, V in place as an MN-major operand; fp32 O in TMEM.
+// O and both parts of P fill 384 of the 512 columns for three tiles of 64 dims (and for two of 128); the
+// scores have two buffers of 64, which the CTA's jobs (a tile's chunk each) take in turn: a buffer is free
+// once its scores are in registers.
 // Trees of one tile (up to 18 nodes of 7 heads) would leave two thirds of the softmax warps without work:
 // there the slots take the chunks in turn, each with an O of its own, joined at the end in TMEM.
 //
@@ -27,6 +31,9 @@
 // and two instead of three and one take 104 us): the softmax warps of a scheduler do not hide each other's
 // trips to tensor memory and barriers.  8 trees of up to 16 nodes behind 16384 to 32768 tokens (32 heads over
 // 8, D = 128): 136 to 171 us, 0.9 to 0.72 of measured copy.
+// Weights in two parts instead of one: 111 us instead of 100 for the former, 156 instead of 139 for the
+// latter (calls in a row on three pools in turn), for an error against 64 bits that is the output's own
+// rounding alone.
 // Measured on the way: one warp for all MMAs, which then wait for each other's operands, 313 us instead of
 // 194 in the latter case; one warp for all TMA boxes 155 instead of 136.  Small batches are a chain of
 // dependent trips: 11.7 us in a graph for 4 trees of up to 8 nodes, with the memset of the counters.
@@ -88,11 +95,12 @@ struct Cfg {
   static constexpr int kMask = kItems + kRing * 64;       // [kTiles][128] first two mask words
   static constexpr int kSched = kMask + kTiles * 1024;    // [seqs + 1] ints
   static int smem(int seqs) { return kSched + (seqs + 1) * 4 + 1024; }
-  // TMEM columns: scores, weights (two 16-bit values a column) and O of every slot
-  static __device__ __forceinline__ uint32_t s_col(int x) { return 64 * x; }
-  static __device__ __forceinline__ uint32_t p_col(int x) { return 64 * kTiles + 32 * x; }
-  static __device__ __forceinline__ uint32_t o_col(int x) { return 96 * kTiles + HD * x; }
-  static_assert((96 + HD) * kTiles <= 512, "tensor memory");
+  // TMEM columns: two buffers of scores; weights (two 16-bit values a column, 32 columns of first parts and
+  // 32 of second ones) and O of every slot
+  static __device__ __forceinline__ uint32_t s_col(uint32_t buffer) { return 64 * buffer; }
+  static __device__ __forceinline__ uint32_t p_col(int x) { return 128 + 64 * x; }
+  static __device__ __forceinline__ uint32_t o_col(int x) { return 128 + 64 * kTiles + HD * x; }
+  static_assert(128 + (64 + HD) * kTiles <= 512, "tensor memory");
   static constexpr int64_t kPart = 128 * (HD + 2);        // floats of a part of one tile: O, then (m, l)
 };
 
@@ -322,10 +330,10 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
   extern __shared__ __align__(16) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sb = smem_u32(smem);
-  // per stage: chunk there, chunk done with; per slot, a phase per job: scores written, scores read,
-  // weights written, P V done; per item: Q there, the item itself there
+  // per stage: chunk there, chunk done with; per slot, a phase per job: scores written, weights written, P V
+  // done; per buffer of scores, a phase for every second job: read; per item: Q there, the item itself there
   const uint32_t kv_full = sb + C::kBars, kv_empty = kv_full + 8 * kStages, s_full = kv_empty + 8 * kStages;
-  const uint32_t s_read = s_full + 8 * kTiles, p_ready = s_read + 8 * kTiles, pv_done = p_ready + 8 * kTiles;
+  const uint32_t s_read = s_full + 8 * kTiles, p_ready = s_read + 16, pv_done = p_ready + 8 * kTiles;
   const uint32_t q_full = pv_done + 8 * kTiles, item_full = q_full + 8;   // (item_full: one per ring entry)
   uint32_t* tslot = reinterpret_cast<uint32_t*>(smem + C::kBars + 496);
   volatile int* s_ok = reinterpret_cast<volatile int*>(smem + C::kOk);
@@ -344,10 +352,10 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
       }
       for (int i = 0; i < kTiles; ++i) {
         mbar_init(s_full + 8 * i, 1);
-        mbar_init(s_read + 8 * i, 4);
         mbar_init(p_ready + 8 * i, 4);
         mbar_init(pv_done + 8 * i, 1);
       }
+      for (int i = 0; i < 2; ++i) mbar_init(s_read + 8 * i, 4);
       mbar_init(q_full, C::kSoftWarps);
       for (int i = 0; i < kRing; ++i) mbar_init(item_full + 8 * i, 1);
       fence_mbar_init();
@@ -448,6 +456,7 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
     const bool leader = elect_one();
     int g = 0, items = 0;
     uint32_t done[kTiles] = {};                    // jobs of each slot so far
+    uint32_t job = 0;                              // jobs whose scores have been issued
     bool ok = true;
     auto wait = [&](uint32_t bar, uint32_t parity) {
       ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, TI_DEVERR_PREFILL_WAIT));
@@ -472,13 +481,15 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
             if (turns ? q * kTiles + x >= n : x >= tiles) continue;
             const int c = g + (turns ? q * kTiles + x : q), st = c % kStages;
             if ((x == 0 || turns) && !wait(kv_full + 8 * st, (c / kStages) & 1)) break;
-            if (q > 0 && !wait(s_read + 8 * x, (done[x] + q - 1) & 1)) break;
+            const uint32_t buffer = job & 1;
+            if (job >= 2 && !wait(s_read + 8 * buffer, ((job >> 1) - 1) & 1)) break;
+            ++job;
             tc_fence_after();
             if (leader) {
               const uint32_t at = (uint32_t)st * (C::kStage >> 4), qt = turns ? 0u : (uint32_t)x * (C::kQTile >> 4);
 #pragma unroll
               for (int k = 0; k < HD / 16; ++k)
-                tc_mma(tmem + C::s_col(x), qd + qt + (((k / 4) * 16384 + 32 * (k % 4)) >> 4),
+                tc_mma(tmem + C::s_col(buffer), qd + qt + (((k / 4) * 16384 + 32 * (k % 4)) >> 4),
                        kd + at + (((k / 4) * 8192 + 32 * (k % 4)) >> 4), id_s, k > 0 ? 1u : 0u);
               tc_commit(s_full + 8 * x);
             }
@@ -499,9 +510,9 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
 #pragma unroll
               for (int u = 0; u < C::kSub; ++u)
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
+                for (int k = 0; k < 8; ++k)         // (keys 16 k .. of the first parts, then of the second)
                   tc_mma_tmem_a(tmem + C::o_col(x) + 64 * u, tmem + C::p_col(x) + 8 * k,
-                                vd + at + ((u * 8192 + 2048 * k) >> 4), id_pv, (q > 0 || k > 0) ? 1u : 0u);
+                                vd + at + ((u * 8192 + 2048 * (k & 3)) >> 4), id_pv, (q > 0 || k > 0) ? 1u : 0u);
               tc_commit(pv_done + 8 * x);
               if (turns || x == tiles - 1) tc_commit(kv_empty + 8 * st);
             }
@@ -519,10 +530,10 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
     // ---- softmax and epilogue: thread <-> row (TMEM lane) r of slot x
     const int x = warp >> 2, quad = warp & 3, r = quad * 32 + lane;
     const uint32_t trow = tmem + ((uint32_t)(quad * 32) << 16);
-    const uint32_t t_s = trow + C::s_col(x), t_o = trow + C::o_col(x);
+    const uint32_t t_o = trow + C::o_col(x);
     const float sc = p.scale_log2;
     int g = 0, items = 0;
-    uint32_t done = 0;                             // jobs of this slot so far
+    uint32_t done = 0, before = 0;                 // jobs of this slot so far; of all slots
     bool ok = true;
     auto wait_all = [&](uint32_t bar, uint32_t parity) {
       return __all_sync(0xffffffffu, mbar_wait(bar, parity, TI_DEVERR_PREFILL_WAIT));
@@ -602,6 +613,7 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
       for (int k = 0, c = turns ? x : 0; k < jobs && ok; ++k, c += step) {
         const int st = (g + c) % kStages;
         const uint32_t par = (done + k) & 1;
+        const uint32_t buffer = (before + (uint32_t)(turns ? c : c * it.tiles + x)) & 1;
         // (the chunk has been there since before its scores: no wait, but the loader's word)
         const bool there = mbar_try_wait(s_full + 8 * x, par) & mbar_try_wait(kv_full + 8 * st, ((g + c) / kStages) & 1);
         if (!__all_sync(0xffffffffu, there) &&
@@ -614,7 +626,7 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
           const int flags = s_ok[st];
           if ((flags & 16) && (x == 0 || turns)) dirty |= mend_values(st, (it.c0 + c) * kChunk, flags);
           __syncwarp();
-          if (lane == 0) mbar_arrive(s_read + 8 * x);
+          if (lane == 0) mbar_arrive(s_read + 8 * buffer);
           // (behind the last job's product: this job's phase of p_ready must not begin earlier)
           if (k >= 1 && !wait_all(pv_done + 8 * x, (done + k - 1) & 1)) { ok = false; break; }
           if (lane == 0) mbar_arrive(p_ready + 8 * x);
@@ -622,12 +634,12 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
         }
         float sv[kChunk];
         uint32_t sr[kChunk];
-        tmem_ld64_start(t_s, sr);
+        tmem_ld64_start(trow + C::s_col(buffer), sr);
         const int flags = s_ok[st];
         tmem_ld64_end(sr, sv);
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(s_read + 8 * x);
+        if (lane == 0) mbar_arrive(s_read + 8 * buffer);
         if (flags & 16) {
           const Row w = row();
           if (x == 0 || turns) dirty |= mend_values(st, (it.c0 + c) * kChunk, flags);
@@ -649,26 +661,11 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
           alpha = m == -INFINITY ? 0.f : fast_exp2(m - mx);
           m = mx;
         }
-        const float off = kPScale - (m == -INFINITY ? 0.f : m);
-        const uint64_t sc2 = pair(sc, sc), off2 = pair(off, off);
-        // the chunk's sum first, in four chains of pairs: a long row's total stays exact enough
-        uint64_t sums[4] = {0, 0, 0, 0};
-        uint32_t pk[kChunk / 2];
-#pragma unroll
-        for (int i = 0; i < kChunk; i += 2) {
-          const float2 e = unpair(fma2(pair(sv[i], sv[i + 1]), sc2, off2));
-          const float p0 = fast_exp2(e.x), p1 = fast_exp2(e.y);
-          sums[i / 2 % 4] = add2(sums[i / 2 % 4], pair(p0, p1));
-          pk[i / 2] = Elem<T>::pack2(p0, p1);
-        }
-        const float2 t2 = unpair(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])));
-        l = l * alpha + (t2.x + t2.y);
-        // P V of the slot's last job has long been done: P's place is free, and O at rest for a rescale
-        if (k >= 1 && !wait_all(pv_done + 8 * x, (done + k - 1) & 1)) { ok = false; break; }
-        if (outgrown && k >= 1) {
+        if (outgrown && k >= 1) {                  // O at rest, for a rescale (here, while the weights need no registers)
+          if (!wait_all(pv_done + 8 * x, (done + k - 1) & 1)) { ok = false; break; }
           tc_fence_after();
           float ov[32];
-#pragma unroll
+#pragma unroll 1
           for (int d = 0; d < HD; d += 32) {
             tmem_ld32(t_o + d, ov);
 #pragma unroll
@@ -676,7 +673,27 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
             tmem_st32(t_o + d, ov);
           }
         }
+        const float off = kPScale - (m == -INFINITY ? 0.f : m);
+        const uint64_t sc2 = pair(sc, sc), off2 = pair(off, off);
+        // the chunk's sum first, in four chains of pairs: a long row's total stays exact enough
+        uint64_t sums[4] = {0, 0, 0, 0};
+        uint32_t pk[kChunk];                       // first parts, then what their rounding left
+#pragma unroll
+        for (int i = 0; i < kChunk; i += 2) {
+          const float2 e = unpair(fma2(pair(sv[i], sv[i + 1]), sc2, off2));
+          const float p0 = fast_exp2(e.x), p1 = fast_exp2(e.y);
+          sums[i / 2 % 4] = add2(sums[i / 2 % 4], pair(p0, p1));
+          pk[i / 2] = Elem<T>::pack2(p0, p1);
+          const float2 h = Elem<T>::unpack2(pk[i / 2]);
+          const float2 rest = unpair(fma2(pair(h.x, h.y), pair(-1.f, -1.f), pair(p0, p1)));
+          pk[kChunk / 2 + i / 2] = Elem<T>::pack2(rest.x, rest.y);
+        }
+        const float2 t2 = unpair(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])));
+        l = l * alpha + (t2.x + t2.y);
+        // P V of the slot's last job has long been done: P's place is free
+        if (k >= 1 && !wait_all(pv_done + 8 * x, (done + k - 1) & 1)) { ok = false; break; }
         tmem_st32_u(trow + C::p_col(x), pk);
+        tmem_st32_u(trow + C::p_col(x) + 32, pk + 32);
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
@@ -691,6 +708,7 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
       dirty = bar_or(1, C::kSoftWarps * 32, dirty);
       tc_fence_after();
       done += (uint32_t)jobs;
+      before += (uint32_t)(turns ? n : n * it.tiles);
       ++items;
       // ---- a tile's result: (m, l) here, O in tensor memory
       if (turns ? x == 0 : x < it.tiles) {
