@@ -280,3 +280,15 @@ def test_ancestor_bits_and_sampling_forms():
     assert [draw(u) for u in (0.0, 0.39, 0.41, 0.71, 0.95)] == [0, 0, 2, 3, 1]
     assert draw(0.99, k=2) == 2 and draw(0.99, p=0.5) == 2 and draw(0.99, p=0.3) == 0 and draw(0.99, m=0.6) == 2
     assert oracle.sample(x, 0.0, 0.9) == (0, 0.0)
+
+
+def test_tree_decoder_refuses_slots_that_are_none():
+    """Before a block is assigned or anything is sent to the device."""
+    from types import SimpleNamespace
+
+    from tiny_infra_b200.speculative import TreeDecoder
+    model = SimpleNamespace(device=torch.device("cpu"), rope_tables=lambda n: (None, None))
+    dec = TreeDecoder(model, SimpleNamespace(kv_bits=16, max_positions=64, max_batch_size=4))
+    for slots in ([-1], [4], [0, -4], [3, 1 << 40]):
+        with pytest.raises(ValueError, match="from 0 to 3"):
+            dec.step(slots, [([5], [-1])] * len(slots))

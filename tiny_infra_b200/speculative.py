@@ -30,11 +30,13 @@ class TreeDecoder:
         # the host hands out the blocks; the device's calls find every entry assigned
         self.no_blocks = paging.free_list([], capacity=1, device=model.device)
 
-    @staticmethod
-    def _check(slots, trees) -> tuple[list[int], np.ndarray, np.ndarray]:
+    def _check(self, slots, trees) -> tuple[list[int], np.ndarray, np.ndarray]:
         """Node counts, packed tokens and parents of ``trees``."""
         if len(slots) != len(trees) or len(set(int(s) for s in slots)) != len(slots):
             raise ValueError("step needs one tree per slot, and distinct slots")
+        if any(not 0 <= int(s) < self.kv.max_batch_size for s in slots):
+            # (a negative one would count from the end on the host, and index the lengths on the device)
+            raise ValueError(f"step needs slots from 0 to {self.kv.max_batch_size - 1}")
         counts, tokens, parents = [], [], []
         for toks, par in trees:
             n = len(toks)
