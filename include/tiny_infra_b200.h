@@ -523,7 +523,8 @@ int ti_release_blocks(int32_t* block_tables, int64_t bt_stride, int num_rows, in
  * j-th node's values move from slot_mapping[its row]
  * to out_slots[cu_seqlens[i] + j] (the same array: in place; otherwise slots that hold none of the
  * nodes; negative: skipped; outside the pool: skipped, TI_DEVERR_BAD_INPUT).  seq_lens (or NULL):
- * seq_lens[row_index[i]] (NULL: i; of num_rows) += num[i]. */
+ * seq_lens[row_index[i]] (NULL: i; of num_rows) += num[i]; with it, a tree whose node 0 or place 0 has a
+ * negative slot was not run: num[i] = 0, nothing moves. */
 size_t ti_tree_attention_workspace_bytes(int num_heads, int num_kv_heads, int head_dim);
 int ti_tree_attention(void* out, int64_t out_tok_stride, float* lse, const void* q, int64_t q_tok_stride,
                       const void* k_cache, const void* v_cache, int64_t num_blocks,

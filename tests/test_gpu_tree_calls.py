@@ -262,6 +262,56 @@ def test_a_step_of_everything_together():
     assert int(lens.sum()) > 6 * S and _status() == 0
 
 
+@pytest.mark.parametrize("scratch", [False, True])
+def test_a_pool_too_short_for_some(scratch):
+    """reserve -> accept with a pool that does not reach: a sequence that was not served emits nothing, keeps its
+    length and its cache, and goes on when there are blocks; the others do not notice.  scratch: the nodes
+    are in blocks of their own, and the slots that the path moves to are the reserved ones."""
+    from tiny_infra_b200 import paging, tree
+    rng = np.random.default_rng(12)
+    counts, lens0 = [20, 7, 40, 3], [30, 17, 16, 0]
+    T, P, NB, L, KVH, D = sum(counts), 6, 40, 2, 2, 64
+    kc, vc = (torch.from_numpy(rng.standard_normal((L, NB, KVH, 16, D))).bfloat16().cuda() for _ in range(2))
+    tables = torch.full((4, 6), -1, dtype=torch.int32, device="cuda")
+    tables[0, :2], tables[1, :2], tables[2, :1] = (_dev(np.arange(a, b, dtype=np.int32)) for a, b in ((0, 2), (2, 4), (4, 5)))
+    # blocks needed: 2, 0, 3, 1; two are there, and the last sequence comes behind the one that ends the list
+    ring, lens = paging.free_list([5, 6], capacity=20), _dev(np.array(lens0, np.int32))
+    parents = np.concatenate([np.arange(-1, n - 1) for n in counts]).astype(np.int32)
+    tokens = np.arange(T, dtype=np.int32)
+    targets = np.where(tokens % 4 == 2, -7, tokens + 1).astype(np.int32)    # a path ends behind every fourth token
+    cu, granted = torch.empty(5, dtype=torch.int32, device="cuda"), torch.empty(4, dtype=torch.int32, device="cuda")
+    slots, pos = torch.empty(T, dtype=torch.int64, device="cuda"), torch.empty(T, dtype=torch.int32, device="cuda")
+    first = np.concatenate([[0], np.cumsum(counts)])
+
+    def step(want_granted):
+        num, path, new = (torch.full(n, 9, dtype=torch.int32, device="cuda") for n in ((4,), (4, P), (4, P)))
+        paging.reserve(tables, lens, _dev(np.array(counts, np.int32)), ring, slots, pos, cu, granted=granted)
+        assert granted.tolist() == [c if w else 0 for c, w in zip(counts, want_granted)]
+        own = torch.arange(T, dtype=torch.int64, device="cuda") + (NB - 5) * 16 if scratch else slots
+        before, was = (kc.clone(), vc.clone()), lens.tolist()
+        tree.accept(kc, vc, _dev(tokens), _dev(parents), _dev(targets), cu, own, num, path, new,
+                    out_slots=slots, seq_lens=lens)
+        paths, news = oracle.accept(tokens, parents, targets, first.tolist(), P)
+        paths = [p if w else [] for p, w in zip(paths, want_granted)]
+        pad = lambda a: a + [-1] * (P - len(a))                                          # noqa: E731
+        assert num.tolist() == [len(p) for p in paths] and path.tolist() == [pad(p) for p in paths]
+        assert new.tolist() == [pad(n if w else []) for n, w in zip(news, want_granted)]
+        assert lens.tolist() == [a + len(p) for a, p in zip(was, paths)]
+        for old, now in zip(before, (kc, vc)):
+            want = old.clone()
+            for i, p in enumerate(paths):
+                for j, c in enumerate(p):
+                    a, b = int(own[first[i] + c]), int(slots[first[i] + j])
+                    want[:, b // 16, :, b % 16] = old[:, a // 16, :, a % 16]
+            assert torch.equal(now, want)
+
+    step([True, True, False, False])
+    ring2 = paging.free_list(paging.free_ids(ring) + list(range(10, 20)), capacity=20)
+    ring.copy_(ring2)
+    step([True] * 4)
+    assert lens[2] > 16 and lens[3] > 0 and _status() == 0
+
+
 # ---- through the model --------------------------------------------------------------------------------
 @pytest.fixture(scope="module")
 def model():

@@ -57,7 +57,10 @@ __global__ void __launch_bounds__(kThreads, 8) accept_kernel(const __grid_consta
   int32_t* s_path = reinterpret_cast<int32_t*>(s_move + 2 * p.deep);
   if (tid < 32) {
     int count = 0;
-    if (n > 0) {
+    // lengths count cached tokens: where they are kept here, a tree whose first node or place has no slot was
+    // not run (a sequence's new tokens have slots all or none), so it emits nothing
+    const bool run = n > 0 && !(p.seq_lens && (p.slots[first] < 0 || p.out_slots[first] < 0));
+    if (run) {
       const int32_t* parent = staged ? s_parent : p.parents + first;
       const int32_t* token = staged ? s_token : p.tokens + first;
       const int32_t* target = staged ? s_target : p.targets + first;

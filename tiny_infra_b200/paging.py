@@ -84,7 +84,8 @@ def reserve(block_tables: torch.Tensor, seq_lens: torch.Tensor, counts: torch.Te
     Unassigned (negative) entries of ``block_tables`` that the new tokens fall in take blocks from the
     front of ``ring``, sequence by sequence.  The first sequence that needs more than what is left gets
     none, nor does any later one that needs a block; ``granted`` [B] receives each one's tokens, its
-    count or 0.  A sequence that would pass its row's end, and one whose row an earlier sequence has, get
+    count or 0.  What the step computes for tokens that were not granted means nothing (they have no K
+    and V): their rows are to be left out, as ``tree.accept`` does where it keeps the lengths.  A sequence that would pass its row's end, and one whose row an earlier sequence has, get
     none and raise TI_DEVERR_BAD_INPUT.
 
     ``cu_seqlens`` [B + 1] receives the counts' running sum, granted or not.  ``slot_mapping`` int64 and

@@ -112,7 +112,7 @@ def accept(key_cache: torch.Tensor, value_cache: torch.Tensor, tokens: torch.Ten
     first later node whose parent is c and whose token (``tokens``) is that one, until there is none or
     the path is as long as ``path`` is wide.
 
-    ``num`` [B] receives the path's length (0: the tree has no nodes), ``path`` [B, P] its nodes and
+    ``num`` [B] receives the path's length (0: the tree has no nodes, or was not run), ``path`` [B, P] its nodes and
     ``out_tokens`` [B, P] the draws at them, the sequence's new tokens: those of the guesses that held
     and the one behind them (-1 behind the path).  All int32; parents and tokens as ``paging.reserve``
     takes them.
@@ -122,7 +122,10 @@ def accept(key_cache: torch.Tensor, value_cache: torch.Tensor, tokens: torch.Ten
     otherwise slots that hold none of the call's nodes; distinct either way), in every layer of ``key_cache`` / ``value_cache``
     [layers, num_blocks, KVH, block_size, D] (or of one layer).  Negative slots are skipped; slots
     outside the pool too, raising TI_DEVERR_BAD_INPUT.  ``seq_lens[row_index[i]]`` (default row i)
-    advances by the path's length.  At most 1024 places."""
+    advances by the path's length; where ``seq_lens`` is given, a tree whose node 0 or place 0 has a
+    negative slot (``paging.reserve`` did not grant it room) counts as not run: its path is empty, its
+    length stays.  Without ``seq_lens`` it is walked all the same, and leaving out what was not granted is
+    the caller's part.  At most 1024 places."""
     out_slots = slot_mapping if out_slots is None else out_slots
     dev = _device(key_cache, value_cache, tokens, parents, targets, cu_seqlens, slot_mapping, num, path,
                   out_tokens, out_slots, seq_lens, row_index)
