@@ -618,6 +618,30 @@ def test_sample_far_from_the_top():
     _check_draw(x[:6, :20000], np.array([1e-4, 1e-30, 1e3, 1e30, 30.0, 1e-2]), u[:6], None, None, None, torch.float32)
 
 
+@pytest.mark.parametrize("rows,vocab", [(1, 151936), (40, 151936), (256, 151936), (700, 9000)])
+def test_sample_min_p_same_bits_every_run(rows, vocab):
+    """Several CTAs a row and one: tokens and log probabilities repeat.  Half of the rows have one likely token
+    and 2000 of weights around 2^-54, whose sum is lost or not by the order in which it is taken, and
+    which the likely one's log probability is."""
+    from tiny_infra_b200 import sampler
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    x = torch.randn(rows, vocab, generator=gen, device="cuda") * 2
+    r = slice(0, None, 2)
+    x[r] = torch.where(torch.rand(x[r].shape, generator=gen, device="cuda") < 2000 / vocab, -37.4 + 0.1 * x[r], -80.0)
+    x[r, vocab // 3] = 0.0
+    t, u = torch.ones(rows, device="cuda"), torch.rand(rows, generator=gen, device="cuda")
+    m = torch.full((rows,), 0.01, device="cuda")
+    m[r] = 1e-20
+    first = None
+    for _ in range(40):
+        lp = torch.zeros(rows, device="cuda")
+        tok = sampler.sample(x, t, u, min_ps=m, logprobs=lp)
+        if first is None:
+            first = tok, lp
+        assert torch.equal(tok, first[0]) and torch.equal(lp, first[1])
+    assert (first[1][r] <= 0).all() and (first[1][r] > -2.0 ** -40).all() and _status() == 0
+
+
 def test_sample_frequencies():
     """A grid of uniforms draws each token as often as its probability says."""
     probs = np.array([0.5, 0.25, 0.125, 0.0625, 0.0625])

@@ -379,21 +379,25 @@ __device__ __forceinline__ void draw_by_radix(Shared& sh, const T* row, int V, c
 
 // ---- rank 0: the three places from the collected tokens and the sums above them ----------------------
 // The list's tokens lie in sh.intervals intervals; all: the sum of top-k's weights (k = 0), at_least: of the
-// weights >= least.
+// weights >= least; below 0: those sums are the list's own, taken here in its order (the tokens were collected
+// in any order, and a sum in that order would have other last bits on every run).
 __device__ __forceinline__ void finish(Shared& sh, const u64* collected, int n, const Weights& w, int k, float top_p, double least, double u,
                                        double all, double at_least, bool want_logp, int& token, double& logp) {
   const int tid = threadIdx.x;
   sort_list(sh.list, collected, n);
   auto value = [&](int i) { return value_of((uint32_t)(sh.list[i] >> 32)); };
   double base = 0;
+  int heavy = 0;                                   // the list's tokens of weight >= least
 #pragma unroll 1
   for (int i0 = 0; i0 < n; i0 += kThreads) {
     const int i = i0 + tid;
-    const double c = block_scan(i < n ? w.exact(value(i)) : 0.0, sh.scan_d);
+    const double e = i < n ? w.exact(value(i)) : 0.0, c = block_scan(e, sh.scan_d);
     if (i < n) sh.cum[i] = base + c;
-    __syncthreads();
+    heavy += __syncthreads_count(i < n && e >= least);
     base = sh.cum[min(n, i0 + kThreads) - 1];
   }
+  if (at_least < 0.0) at_least = heavy > 0 ? sh.cum[heavy - 1] : 0.0;
+  if (all < 0.0) all = at_least;
   // from here on every thread finds the same, by binary searches
   auto first = [&](int lo, int hi, auto&& test) {    // the first of [lo, hi) that passes, else hi
     while (lo < hi) {
@@ -656,21 +660,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         sh.k_high = INFINITY;
       }
       __syncthreads();
-      // min-p's sum, from the collected
-      double m = 0;
-      if (least > 0.0 || all == 0.0)
-        for (int i = tid; i < n; i += kThreads) {
-          const double e = w.exact(value_of((uint32_t)(collected[i] >> 32)));
-          m += e >= least ? e : 0.0;
-        }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
-      if (lane == 0) sh.part[warp][0] = m;
-      __syncthreads();
-      m = 0;
-      for (int i = 0; i < kWarps; ++i) m += sh.part[i][0];
-      __syncthreads();
-      finish(sh, collected, n, w, k, top_p, least, u, sum_all ? all : m, m, p.logprobs != nullptr, token, logp);
+      finish(sh, collected, n, w, k, top_p, least, u, sum_all ? all : -1.0, -1.0, p.logprobs != nullptr, token, logp);
       done = true;
       if (ctas > 1) cluster_wait_acquire();
     } else {
