@@ -513,7 +513,9 @@ int ti_release_blocks(int32_t* block_tables, int64_t bt_stride, int num_rows, in
  * behind cu_seqlens[num_seqs] are left as they were.  At most 16 query heads per kv head, head_dim 64
  * or 128, block_size 16, at most 4096 sequences.  The workspace (ti_tree_attention_workspace_bytes,
  * 16-byte aligned) holds counters in its first 4096 bytes, which must be zero before its first call and
- * which every call leaves zero; calls that share it must not overlap on the GPU.
+ * which every call leaves zero (one that raised TI_DEVERR_PREFILL_WAIT may not, which later calls do not
+ * mind, but replays of the same captured call do: zero them in the graph); calls that share it must not
+ * overlap on the GPU.
  *
  * ti_tree_accept: the path from node 0 to the first later node c with parents[c] = the current one and
  * tokens[c] = targets[current], and on, for at most max_path (<= 1024) nodes.  num [num_seqs] = its

@@ -81,6 +81,30 @@ def test_attention_on_two_streams_and_in_two_graphs():
     assert _status() == 0
 
 
+def test_attention_behind_a_call_that_ended_early():
+    """Words that a call whose waits gave up has left in the workspace are not taken for halves of joins."""
+    from tiny_infra_b200 import tree
+    rng = np.random.default_rng(13)
+    d = _device_scene(_scene(rng, 14, 2, 64, torch.bfloat16, [4000, 2100, 333], [9, 30, 2]))
+    _attend(d)
+    want = d["out"].clone(), d["lse"].clone()
+    for left in (1, -1):
+        torch.cuda.synchronize()
+        for ws in tree._ws._buf.values():
+            ws[:4096].view(torch.int32).fill_(left)
+        for x in (d["q"], d["k"]):
+            x.neg_()                                 # (the same scores, from parts written anew)
+        d["v"].mul_(2)
+        d["out"].zero_()
+        _attend(d)
+        assert torch.equal(d["out"], want[0] * 2) and torch.equal(d["lse"], want[1])
+        d["v"].div_(2)
+    for ws in tree._ws._buf.values():
+        ws[:4096].zero_()
+    torch.cuda.synchronize()
+    assert _status() == 0
+
+
 def test_attention_replayed_with_other_lengths():
     """A captured call reads lengths, tables and masks when it runs: sequences grow and shrink, some to
     nothing, between replays."""

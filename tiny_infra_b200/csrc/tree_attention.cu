@@ -61,7 +61,10 @@ constexpr int kMaxGroup = 16;
 constexpr int kMaxSeqs = 4096;
 constexpr int kRing = 16;                // items on their way: more than chunks on theirs
 constexpr int kCtas = 148;               // most CTAs of a launch (one per SM)
-constexpr size_t kCounterBytes = 4096;  // one counter per CTA and slot
+// One word per CTA and slot.  It holds the number of the call whose first half of a join is in memory; the second
+// half's CTA sets it back to 0.  A call that ends early (a wait gave up) leaves words of its own number
+// behind, which mean nothing to the calls that follow.
+constexpr size_t kCounterBytes = 4096;
 
 struct Params {
   void* out;
@@ -73,6 +76,7 @@ struct Params {
   unsigned* counters;
   int seqs, tokens, rows, cols, NH, KVH, group, mask_words;
   float scale_log2;
+  unsigned call;                         // not 0; another one for each call
 };
 
 template <int HD>
@@ -796,12 +800,12 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
             const bool is_right = i != left;
             unsigned* counter = p.counters + (it.first + right) * kTiles + x;
             // the other half is there: nothing has to be written; else this half goes to memory, and the
-            // counter says whether the other one has come meanwhile
+            // word says whether the other one has come meanwhile
             bar_sync(2 + x, 128);                  // (the word below has been read by all)
             if (quad == 0 && lane == 0) {
               unsigned there;
               asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(there) : "l"(counter) : "memory");
-              s_flag[x] = (int)there;
+              s_flag[x] = there == p.call;
             }
             bar_sync(2 + x, 128);
             bool second = s_flag[x] != 0;
@@ -825,8 +829,8 @@ attention_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
               bar_sync(2 + x, 128);
               if (quad == 0 && lane == 0) {
                 unsigned old;
-                asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(old) : "l"(counter) : "memory");
-                s_flag[x] = (int)old;
+                asm volatile("atom.exch.acq_rel.gpu.global.b32 %0, [%1], %2;" : "=r"(old) : "l"(counter), "r"(p.call) : "memory");
+                s_flag[x] = old == p.call;
               }
               bar_sync(2 + x, 128);
               second = s_flag[x] != 0;
@@ -976,7 +980,10 @@ extern "C" int ti_tree_attention(void* out, int64_t out_tok_stride, float* lse, 
                  context_lens, cu_seqlens, mask_words ? masks : nullptr,
                  reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + tree::kCounterBytes),
                  static_cast<unsigned*>(workspace), num_seqs, num_tokens, num_rows, max_blocks_per_seq, num_heads,
-                 num_kv_heads, group, mask_words, 1.4426950408889634f / sqrtf((float)head_dim)};
+                 num_kv_heads, group, mask_words, 1.4426950408889634f / sqrtf((float)head_dim), 0};
+  static std::atomic<unsigned> calls{0};
+  do p.call = calls.fetch_add(1, std::memory_order_relaxed) + 1;
+  while (p.call == 0);
   CUtensorMap km, vm;
   const cuuint64_t dims[2] = {(cuuint64_t)head_dim, (cuuint64_t)(num_blocks * num_kv_heads * block_size)};
   const cuuint64_t strides[1] = {(cuuint64_t)head_dim * 2};
