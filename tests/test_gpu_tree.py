@@ -618,6 +618,22 @@ def test_sample_far_from_the_top():
     _check_draw(x[:6, :20000], np.array([1e-4, 1e-30, 1e3, 1e30, 30.0, 1e-2]), u[:6], None, None, None, torch.float32)
 
 
+def test_sample_infinite_temperature():
+    """Every finite value is equally likely, -inf and NaN still never drawn; by all ways to a token."""
+    rng = np.random.default_rng(14)
+    n = 12
+    for vocab, scale in ((700, 1.0), (30011, 1.0), (30011, 1e38), (30011, 0.0)):
+        x = np.clip(rng.standard_normal((n, vocab)) * scale, -3e38, 3e38)
+        x[:, ::3] = -np.inf
+        x[:, 1::11] = np.nan
+        x[0, 5:] = -np.inf
+        u, inf = rng.random(n), np.full(n, np.inf)
+        for k, p, m in ((None, None, None), (None, np.full(n, 0.6), None), (np.full(n, 20), np.full(n, 0.9), None),
+                        (np.full(n, 600), np.full(n, 0.5), None), (None, None, np.full(n, 0.3)),
+                        (None, np.full(n, 0.7), np.full(n, 1.0))):
+            _check_draw(torch.from_numpy(x), inf, u, k, p, m, torch.float32)
+
+
 @pytest.mark.parametrize("rows,vocab", [(1, 151936), (40, 151936), (256, 151936), (700, 9000)])
 def test_sample_min_p_same_bits_every_run(rows, vocab):
     """Several CTAs a row and one: tokens and log probabilities repeat.  Half of the rows have one likely token

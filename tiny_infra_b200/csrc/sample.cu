@@ -465,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   if (k <= 0 || k >= V) k = 0;
   const float top_p = p.top_ps ? p.top_ps[r] : 1.f;
   const float min_p = p.min_ps ? p.min_ps[r] : 0.f;
-  const double least = min_p > 0.f ? fmin((double)min_p, 1.0) : 0.0;
+  const double least = min_p > 0.f && temp < INFINITY ? fmin((double)min_p, 1.0) : 0.0;   // (at inf all are as likely)
   const double u = fmin(fmax((double)p.uniforms[r], 0.0), 1.0 - 1.0 / 16777216.0);
   const int share = (int)((((int64_t)(V + 7) / 8 + ctas - 1) / ctas) * 8);
   const int j0 = (int)min((int64_t)V, (int64_t)rank * share), j1 = min(V, j0 + share);
@@ -569,8 +569,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     }
     return;
   }
-  const Weights w{best, 1.0 / (double)temp, 1.4426950408889634 / (double)temp,
-                  (unsigned)__double2hiint(-1000.0 / 1.4426950408889634 * (double)temp)};
+  // (an infinite one as 1e250: every finite value then weighs 1, and -inf still nothing rather than NaN)
+  const double t = fmin((double)temp, 1e250);
+  const Weights w{best, 1.0 / t, 1.4426950408889634 / t, (unsigned)__double2hiint(-1000.0 / 1.4426950408889634 * t)};
   auto collect = [&](float x, int j) {
     const int slot = atomicAdd(&sh.count, 1);
     if (slot < kList) sh.list[slot] = ((u64)key_of(x) << 32) | (uint32_t)~(uint32_t)j;
@@ -617,7 +618,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     float low = bound;
     if (by_weight) {
       // a little below the value whose weight is m; the weights themselves decide later
-      const double v = (double)best + log(least) * (double)temp;
+      const double v = (double)best + log(least) * t;
       const float f = (float)(v - 1e-6 * (fabs(v) + fabs((double)best)));
       low = fmaxf(low, f);
     }
