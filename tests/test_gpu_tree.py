@@ -634,6 +634,24 @@ def test_sample_infinite_temperature():
             _check_draw(torch.from_numpy(x), inf, u, k, p, m, torch.float32)
 
 
+def test_sample_thin_ties_of_a_huge_vocabulary():
+    """One likely token and four million of equal weights near 2^-41, of which a draw near the end takes one: its
+    place from the formula (a running sum in 64 bits would lose part of each weight).  With top-p behind it too."""
+    n, u = 1 << 22, 1 - 2.0 ** -21
+    x = torch.full((2, n), -28.4, dtype=torch.float64)
+    x[:, 5] = 0.0
+    tok, lp = _draw(x, np.ones(2), np.array([u, 0.5]), None, None, None, torch.float32)
+    w = np.exp(float(np.float32(-28.4)))
+    # the likely token first, then the others by index: place 1 + q has the sum 1 + (q + 1) w
+    q = int(np.floor(u * (n - 1) - (1 - u) / w))
+    assert abs(int(tok[0]) - (q if q < 5 else q + 1)) <= 1 and tok[1] == 5
+    assert abs(lp[0] - (np.log(w) - np.log1p((n - 1) * w))) < 2.0 ** -18
+    tok, _ = _draw(x, np.ones(2), np.array([u, 0.5]), None, np.full(2, 1 - 2.0 ** -22), None, torch.float32)
+    kept = np.floor((1 - 2.0 ** -22) * (n - 1) - 2.0 ** -22 / w) + 1             # tokens behind the likely one
+    q = int(np.floor(u * kept - (1 - u) / w))
+    assert abs(int(tok[0]) - (q if q < 5 else q + 1)) <= 1 and tok[1] == 5 and _status() == 0
+
+
 @pytest.mark.parametrize("rows,vocab", [(1, 151936), (40, 151936), (256, 151936), (700, 9000)])
 def test_sample_min_p_same_bits_every_run(rows, vocab):
     """Several CTAs a row and one: tokens and log probabilities repeat.  Half of the rows have one likely token

@@ -52,8 +52,9 @@ constexpr int kFew = 256;                // collected tokens that are ranked rat
 constexpr int kList = 4096;              // collected tokens (a power of two)
 constexpr int kGroups = 128;             // of 4 threads
 constexpr int kBins = 4096;
-constexpr double kOctaves = 40.0;        // range of the histogram below the maximum; 2^-40 * 2^24 tokens still
-                                         // is less than the 2^-24 that a float uniform can tell from 1
+constexpr double kOctaves = 40.0;        // range of the histogram below the maximum; what is below it is in the last
+                                         // bin, whose tokens are collected (or, if too many, placed by the
+                                         // radix selects) when a place can lie there
 
 struct Params {
   const void* logits;
@@ -63,7 +64,6 @@ struct Params {
   int32_t* tokens;
   float* logprobs;
   int vocab;
-  double unit;                           // fixed-point units of a weight of 1 (ties)
   float quanta;                          // units of a bin's largest weight in its sum (a row's fit 32 bits)
 };
 
@@ -332,15 +332,38 @@ __device__ void find(Shared& sh, const T* row, int V, uint32_t low, const Weight
 }
 
 template <typename T>
-__device__ __forceinline__ void draw_by_radix(Shared& sh, const T* row, int V, const Weights& w, double unit, int k,
+__device__ __forceinline__ void draw_by_radix(Shared& sh, const T* row, int V, const Weights& w, int k,
                                            float top_p, double least, double u, int& token, double& logp) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint32_t low = key_of(-INFINITY);
   if (k > 0 && k < V) {
-    find<T, true>(sh, row, V, 0, w, unit, (u64)(k - 1));
+    find<T, true>(sh, row, V, 0, w, 0.0, (u64)(k - 1));
     low = sh.key;
     __syncthreads();
   }
+  // fixed-point units of a weight of 1: as many as keep the whole sum between 2^61 and 2^62, so that the
+  // roundings of 2^24 weights move it by 2^-38 at most, whether it is the many tokens or the likely one
+  double about = 0;
+  {
+    uint32_t last = 0;
+    double weight = 0;
+    scan(row, 0, V, [&](float x, int) {
+      const uint32_t key = key_of(x);
+      if (key < low) return;
+      if (key != last) {
+        last = key;
+        weight = w.exact(value_of(key));
+      }
+      about += weight;
+    });
+    for (int o = 16; o > 0; o >>= 1) about += __shfl_xor_sync(0xffffffffu, about, o);
+    __syncthreads();
+    if (lane == 0) sh.scan_d[warp] = about;
+    __syncthreads();
+    about = 0;
+    for (int i = 0; i < kWarps; ++i) about += sh.scan_d[i];
+  }
+  const double unit = scalbn(1.0, 61 - ilogb(about));
   u64 sum[2] = {0, 0}, weight = 0;
   uint32_t last = 0;
   bool heavy = false;
@@ -931,7 +954,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   }
   if (!done && rank == 0) {
     __syncthreads();
-    draw_by_radix(sh, row, V, w, p.unit, k, top_p, least, u, token, logp);
+    draw_by_radix(sh, row, V, w, k, top_p, least, u, token, logp);
   }
   if (writer) {
     p.tokens[r] = token;
@@ -988,7 +1011,7 @@ extern "C" int ti_sample_ex(const void* logits, int64_t ld, int dtype, int rows,
   int bits = 0;
   while ((1 << bits) < vocab) ++bits;
   const sample::Params p{logits, ld, temperatures, top_ps, min_ps, uniforms, top_ks, out_tokens, logprobs, vocab,
-                         (double)(1ull << std::min(44, 62 - bits)), (float)(1 << std::min(14, 31 - bits))};
+                         (float)(1 << std::min(14, 31 - bits))};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (dtype == TI_DTYPE_BF16) return sample::launch<__nv_bfloat16>(p, rows, s);
   if (dtype == TI_DTYPE_FP16) return sample::launch<__half>(p, rows, s);
