@@ -981,7 +981,8 @@ static int launch(const Params& p, int rows, cudaStream_t s) {
   // end of the launch (256 rows of 151936, two CTAs each instead of one: mixed 126 us instead of 172, all
   // open 206 instead of 214, all top-k 20 53 instead of 39; with four, mixed 140, open 252; 256 rows of 32000
   // gain nothing).  Pairs of which one CTA leaves where a row does not need it are no way out: the GPU keeps
-  // its place until the pair ends (open 347, all top-k 20 71)
+  // its place until the pair ends (open 347, all top-k 20 71).  Measured at these two sizes only: where between
+  // them the border lies is a guess, and rows that all ask for few tokens would be better off without it
   unsigned ctas = 1;
   while (ctas < (unsigned)kCluster) {
     const int64_t next = (int64_t)rows * ctas * 2;

@@ -11,8 +11,9 @@
 //   S = Q K^T   M 128, N 64, into TMEM; freed as soon as the softmax warps have it in registers;
 //   softmax     one row per thread, a running max that is kept until a row's grows by more than 2^8
 //               (then O is rescaled in TMEM), P = 2^(s - m) back into TMEM as the sum of two values of the
-//               pool's type, P and what its rounding left (17 bits in all for bf16, 22 for fp16, as in the
-//               decode and prefill attention over the same pool); the sum is taken before that rounding;
+//               pool's type, P and what its rounding left (17 bits in all for bf16, 22 for fp16; the
+//               prefill attention over the same pool does so too, and for bf16 the decode attention); the
+//               sum is taken before that rounding;
 //   O += P V    twice, A from TMEM, V in place as an MN-major operand; fp32 O in TMEM.
 // O and both parts of P fill 384 of the 512 columns for three tiles of 64 dims (and for two of 128); the
 // scores have two buffers of 64, which the CTA's jobs (a tile's chunk each) take in turn: a buffer is free
@@ -25,24 +26,25 @@
 // pairs by whichever CTA of a pair comes second: no CTA waits for another, the joins of a long sequence
 // go on side by side, and their order does not depend on who comes when.
 //
-// Bound: 32 trees of 64 nodes behind 2048 to 8192 tokens (14 heads over 2, D = 64) take 94 us.  Their
-// exponentials alone would take 37 (8 clocks a warp instruction), the MMAs 28; a chunk of three tiles takes
-// 2450 clocks, of which the exponential unit is busy for 1536 (two tiles: 1900 and 1024; four tiles as two
-// and two instead of three and one take 104 us): the softmax warps of a scheduler do not hide each other's
-// trips to tensor memory and barriers.  8 trees of up to 16 nodes behind 16384 to 32768 tokens (32 heads over
-// 8, D = 128): 136 to 171 us, 0.9 to 0.72 of measured copy.
-// Weights in two parts instead of one: 111 us instead of 100 for the former, 156 instead of 139 for the
-// latter (calls in a row on three pools in turn), for an error against 64 bits that is the output's own
-// rounding alone.
-// Measured on the way: one warp for all MMAs, which then wait for each other's operands, 313 us instead of
-// 194 in the latter case; one warp for all TMA boxes 155 instead of 136.  Small batches are a chain of
-// dependent trips: 11.7 us in a graph for 4 trees of up to 8 nodes, with the memset of the counters.
+// Bound: 32 trees of 64 nodes behind 2048 to 8192 tokens (14 heads over 2, D = 64) take 111 us as calls in a
+// row.  Their exponentials alone would take 37 (8 clocks a warp instruction), the MMAs 42; a chunk of three
+// tiles takes 2820 clocks, of which the exponential unit is busy for 1536 (two tiles: 2330 and 1024, one: 1040;
+// four tiles as two and two instead of three and one take 120 us): the softmax warps of a scheduler do not
+// hide each other's trips to tensor memory and barriers.  8 trees of up to 16 nodes behind 16384 to 32768
+// tokens (32 heads over 8, D = 128): 156 us in a row, 190 to 196 between other work, 0.79 and 0.63 of
+// measured copy; a chunk there takes 1320 clocks.  Weights in one part took 100 and 139 us in a row, at 1.3
+// times the error against 64 bits; in two parts the error is the output's own rounding alone.
+// Measured on the way, with weights in one part: one warp for all MMAs, which then wait for each other's
+// operands, 313 us instead of 194 in the latter case; one warp for all TMA boxes 155 instead of 136.  Small
+// batches are a chain of dependent trips: 11.8 us in a graph for 4 trees of up to 8 nodes, with the memset
+// of the counters.
 //
 // Values that a node does not see: scores are replaced, so keys may hold anything.  V is multiplied by a
 // weight of 0, which a NaN or infinity would survive: in chunks that reach past the cached tokens or hold
 // an absent block the first slot's threads zero V's rows behind the end and those blocks, and any
 // non-finite elements of drafts; rows that do see such a draft add its values at the end (rare, from the
-// pool).
+// pool).  An infinite value of a cached token, which every node sees, makes that dim NaN or infinite (the
+// second part of a weight may be 0), as in the prefill attention.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>

@@ -3,7 +3,7 @@
 // A unit is up to kTiles query tiles (128 rows of (node, query head)) of one sequence and kv head, which
 // share their keys' way through the chip; it costs `width` jobs for each chunk of 64 keys and kUnitJobs
 // more.  A tree of more tiles has units of kTiles and one of what is left for each kv head (a chunk of three
-// tiles takes 2450 clocks, of two 1900, of one 820, so 3 + 1 is less than 2 + 2).  All units lie on one
+// tiles takes 2820 clocks, of two 2330, of one 1040, so 3 + 1 is less than 2 + 2).  All units lie on one
 // line, in order of sequence, full ones first, kv head and tiles; CTA c takes the line's piece [c per,
 // (c + 1) per), cut at whole chunks.  The pieces of a unit lie in consecutive CTAs.
 //

@@ -97,7 +97,8 @@ def reserve(block_tables: torch.Tensor, seq_lens: torch.Tensor, counts: torch.Te
     within its tree (negative: a root), an earlier one.  A token's position then goes by its depth, and
     row t of ``masks`` (int32 [tokens, words], bit b of word w: node 32 w + b) receives its ancestors
     and itself, as ``tree.attention`` takes them.  A tree with more nodes than bits raises
-    TI_DEVERR_BAD_INPUT and loses the bits.
+    TI_DEVERR_BAD_INPUT and loses the bits.  Each token walks up to its root, a dependent load per ancestor,
+    again for every four words of ``masks``: trees of up to some hundred levels are what this is for.
 
     ``seq_lens`` is not advanced; blocks reserved once stay in the row.  At most 4096 sequences, 32768 table
     rows with ``row_index``.  Calls that share a ring or a table follow one another."""

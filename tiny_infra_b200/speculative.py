@@ -3,14 +3,15 @@
 ``TreeDecoder.step`` takes a tree per slot -- node 0 the sequence's last token, every other node a guess
 for the token behind its parent, from whatever drafts the caller has -- runs the model over all nodes,
 draws a token at each from the model's own distribution, and keeps the path that the draws confirm.  What
-it emits is distributed as one token at a time would be; a step emits one token more than the guesses
-that held.
+it emits is distributed as one token at a time drawn by ``sampler.sample`` with the slot's own parameters
+would be (the batcher's rules for a whole batch's top-k and top-p, ``sampler.SamplingParams``, are not
+applied); a step emits one token more than the guesses that held.
 
 Per step: the host assigns blocks (``KVCacheManager.plan_tokens``, the reference's order),
 ``paging.reserve`` makes slots, positions and masks from the lengths on the device, the layers run with
 ``tree.attention``, ``sampler.sample`` draws at every node, ``tree.accept`` moves the kept nodes' K and V
 behind the cached tokens and advances ``seq_len``.  Blocks behind what was kept stay assigned and serve
-the next step.
+the next step.  A step copies its small inputs to the device and waits for its tokens at the end.
 """
 from __future__ import annotations
 
