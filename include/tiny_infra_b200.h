@@ -550,7 +550,7 @@ int ti_tree_accept(void* key_cache, void* value_cache, int num_layers, int64_t n
  * vocab: all), of these the shortest whose probability exceeds top_ps[r] (>= 1: all), of these those
  * with exp(z - max z) >= min(min_ps[r], 1).  out_tokens[r] = the first whose cumulative probability
  * among the kept exceeds uniforms[r]; logprobs[r] = ln of its probability among them.  Temperature <= 0
- * or NaN: the first of the largest, 0.  NaN counts as -inf, which is never drawn; without any other value
+ * or NaN: the first of the largest, 0; infinite: every finite value equally likely.  NaN counts as -inf, which is never drawn; without any other value
  * -1 and -inf.  +inf: equally likely, all others impossible.  top_ks, top_ps, min_ps, logprobs may be
  * NULL.  At most 2^24 tokens. */
 int ti_sample_ex(const void* logits, int64_t ld, int dtype, int rows, int vocab,
